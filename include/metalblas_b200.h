@@ -244,6 +244,86 @@ int mb_autotune_cache_save(const char *path);
 void mb_autotune_cache_clear(void);
 int64_t mb_autotune_cache_size(void);
 
+/* ---------------------------------------------------------------------------
+ * int8 products with scales, and tokens sorted by expert.  The reference has
+ * no counterpart of the functions down to mb_last_error_string.
+ *
+ * Float element types are MB_F32, MB_F16 and MB_BF16 throughout; row strides
+ * (ld) are in elements, columns are contiguous unless a stride is named.
+ * Sums are held in fp32 (the products' in exact 32-bit integers) and results
+ * round once; every result repeats bit for bit. */
+
+/* q[r, c] = rint(127 x[r, c] / amax_r), scale[r] = amax_r / 127 with amax_r the
+ * largest |x| of row r.  A row of zeros has scale 0; a row that holds an
+ * infinity or a NaN has scale NaN and q 0. */
+int mb_quantize(int32_t dtype, int64_t rows, int64_t cols, const void *x, int64_t ldx, int8_t *q, int64_t ldq,
+                float *scale, void *stream);
+
+/* C[m, n] = (sum_k A[m, k] B_e[k, n]) scale_a[m] scale_b[e, n] + bias[n] for
+ * int8 A and B; out_dtype is a float type.
+ *   groups == 0: one B for every row; offsets unused.
+ *   groups >= 1: `groups` matrices B, sB apart; offsets is a device array of
+ *     groups + 1 ascending row numbers starting at 0; rows
+ *     offsets[e] .. offsets[e+1]-1 use B_e, rows at or past offsets[groups] are
+ *     set to zero.  Values outside 0..M are taken as the nearest of the two.
+ * Operands with a unit stride, a 16-byte aligned base and 16-byte multiples in
+ * the other strides are read in place; others are copied into the workspace
+ * first.  K <= 131071, so that no sum leaves 32 bits. */
+typedef struct mb_scaled_desc {
+    int32_t out_dtype, bias_dtype;       /* bias_dtype: out_dtype or MB_F32      */
+    int64_t M, N, K, groups;
+    const int8_t *A, *B;
+    void *C;
+    int64_t a_rs, a_cs, b_rs, b_cs, sB;  /* element strides; sB: from B_e to B_e+1 */
+    int64_t c_rs, c_cs;
+    const float *scale_a, *scale_b;
+    int64_t scale_a_s;                   /* scale_a[m * scale_a_s]; 0: one scale  */
+    int64_t scale_b_s, scale_b_g;        /* scale_b[e * scale_b_g + n * scale_b_s] */
+    const void *bias;                    /* N values, bias_s apart, or null       */
+    int64_t bias_s;
+    const int32_t *offsets;
+    int32_t tile_n, split_k, swap_ab, cta_pair;  /* 0: chosen; see mb_scaled_plan  */
+    void *workspace;
+    int64_t workspace_bytes;
+} mb_scaled_desc;
+
+void mb_scaled_desc_init(mb_scaled_desc *d);
+int mb_scaled_gemm(const mb_scaled_desc *d, void *stream);
+/* Bytes of scratch mb_scaled_gemm needs for this descriptor (0 for operands
+ * read in place).  The contents need not be kept or cleared. */
+int64_t mb_scaled_workspace_size(const mb_scaled_desc *d);
+/* One line on the plan the descriptor gets; its length, or a negative status. */
+int mb_scaled_plan(const mb_scaled_desc *d, char *buf, int buflen);
+
+/* Entries 0..n-1 by ids (int32, or int64 with ids64), stable; ids outside
+ * 0..experts-1 last.  order[slot] = entry, position[entry] = slot,
+ * offsets[e] = first slot of expert e, offsets[experts] = entries kept.
+ * experts <= 1024, n < 2^31. */
+int mb_expert_sort(int32_t ids64, int64_t n, int64_t experts, const void *ids, int32_t *order, int32_t *position,
+                   int32_t *offsets, void *stream);
+
+/* The functions below take position [tokens, k] and `kept` (the address of
+ * offsets[experts]) of an mb_expert_sort: rows [0, *kept) of a sorted buffer of
+ * tokens * k rows hold entries, rows past it zeros. */
+/* sorted[position[t, j]] = x[t]. */
+int mb_expert_gather(int32_t dtype, int64_t tokens, int64_t k, int64_t cols, const void *x, int64_t ldx,
+                     const int32_t *position, const int32_t *kept, void *sorted, int64_t lds, void *stream);
+/* The same rows quantized as by mb_quantize (dropped rows: q 0, scale 0). */
+int mb_expert_gather_quantize(int32_t dtype, int64_t tokens, int64_t k, int64_t cols, const void *x, int64_t ldx,
+                              const int32_t *position, const int32_t *kept, int8_t *q, int64_t ldq, float *scale,
+                              void *stream);
+/* out[t] = sum_j weights[t, j] sorted[position[t, j]], j ascending; weights
+ * [tokens, k] of weights_dtype (dtype or MB_F32), or null for ones. */
+int mb_expert_combine(int32_t dtype, int32_t weights_dtype, int64_t tokens, int64_t k, int64_t cols,
+                      const void *sorted, int64_t lds, const void *weights, const int32_t *position,
+                      const int32_t *kept, void *out, int64_t ldo, void *stream);
+/* dsorted[position[t, j]] = weights[t, j] dout[t] (zero rows for dropped
+ * entries), dweights[t, j] = <dout[t], sorted[position[t, j]]> (zero likewise). */
+int mb_expert_combine_backward(int32_t dtype, int32_t weights_dtype, int64_t tokens, int64_t k, int64_t cols,
+                               const void *dout, int64_t ldd, const void *sorted, int64_t lds, const void *weights,
+                               const int32_t *position, const int32_t *kept, void *dsorted, int64_t ldds,
+                               void *dweights, void *stream);
+
 /* Text of the last error raised on this thread. */
 const char *mb_last_error_string(void);
 

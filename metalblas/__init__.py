@@ -18,4 +18,16 @@ from metalblas_b200 import (  # noqa: F401
     outer,
     vdot,
 )
+from metalblas_b200 import (  # noqa: F401
+    ExpertOrder,
+    expert_combine,
+    expert_combine_backward,
+    expert_gather,
+    expert_gather_backward,
+    expert_gather_quantize,
+    expert_sort,
+    grouped_scaled_mm,
+    quantize,
+    scaled_mm,
+)
 from metalblas_b200 import __all__  # noqa: F401

@@ -22,6 +22,18 @@ from .dispatch import (
     outer,
     vdot,
 )
+# This package's own operators, which the reference does not have (``__all__`` is the
+# reference's list of names).
+from .experts import (  # noqa: F401
+    ExpertOrder,
+    expert_combine,
+    expert_combine_backward,
+    expert_gather,
+    expert_gather_backward,
+    expert_gather_quantize,
+    expert_sort,
+)
+from .quantized import grouped_scaled_mm, quantize, scaled_mm  # noqa: F401
 
 __all__ = [
     "matmul", "gemm", "addmm", "bmm", "baddbmm", "addbmm",

@@ -39,6 +39,9 @@ EXPORTS = (
     "mb_autotune_record", "mb_autotune_lookup", "mb_autotune_cache_load", "mb_autotune_cache_save",
     "mb_autotune_cache_clear", "mb_autotune_cache_size", "mb_peak_probe",
     "mb_gemm_peer", "mb_ipc_get_handle", "mb_ipc_open", "mb_ipc_close",
+    "mb_quantize", "mb_scaled_desc_init", "mb_scaled_gemm", "mb_scaled_workspace_size", "mb_scaled_plan",
+    "mb_expert_sort", "mb_expert_gather", "mb_expert_gather_quantize", "mb_expert_combine",
+    "mb_expert_combine_backward",
 )
 
 MB_MAX_PEERS = 7
@@ -86,6 +89,25 @@ def peer_targets(addrs, mc=None) -> PeerTargets:
         t.C[i] = int(a)
     t.mc_C = int(mc) if mc else None
     return t
+
+
+class ScaledDesc(ctypes.Structure):
+    """Mirror of ``mb_scaled_desc`` (field order and C types must match)."""
+
+    _fields_ = [
+        ("out_dtype", ctypes.c_int32), ("bias_dtype", ctypes.c_int32),
+        ("M", ctypes.c_int64), ("N", ctypes.c_int64), ("K", ctypes.c_int64), ("groups", ctypes.c_int64),
+        ("A", ctypes.c_void_p), ("B", ctypes.c_void_p), ("C", ctypes.c_void_p),
+        ("a_rs", ctypes.c_int64), ("a_cs", ctypes.c_int64),
+        ("b_rs", ctypes.c_int64), ("b_cs", ctypes.c_int64), ("sB", ctypes.c_int64),
+        ("c_rs", ctypes.c_int64), ("c_cs", ctypes.c_int64),
+        ("scale_a", ctypes.c_void_p), ("scale_b", ctypes.c_void_p),
+        ("scale_a_s", ctypes.c_int64), ("scale_b_s", ctypes.c_int64), ("scale_b_g", ctypes.c_int64),
+        ("bias", ctypes.c_void_p), ("bias_s", ctypes.c_int64), ("offsets", ctypes.c_void_p),
+        ("tile_n", ctypes.c_int32), ("split_k", ctypes.c_int32), ("swap_ab", ctypes.c_int32),
+        ("cta_pair", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64),
+    ]
 
 
 class PlanOverride(ctypes.Structure):
@@ -160,8 +182,31 @@ def load():
         lib.mb_ipc_open.restype = ctypes.c_int
         lib.mb_ipc_close.argtypes = [V]
         lib.mb_ipc_close.restype = ctypes.c_int
+        _bind_ops(lib)
         _lib = lib
         return lib
+
+
+def _bind_ops(lib) -> None:
+    """Signatures of the int8 products with scales and the expert routing (a library built
+    before they existed lacks them: it still loads, so that the package's builder can run)."""
+    if not hasattr(lib, "mb_scaled_gemm"):
+        return
+    V, I64, I32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32
+    S = ctypes.POINTER(ScaledDesc)
+    lib.mb_scaled_desc_init.argtypes, lib.mb_scaled_desc_init.restype = [S], None
+    lib.mb_scaled_workspace_size.argtypes, lib.mb_scaled_workspace_size.restype = [S], I64
+    for name, args in (
+            ("mb_quantize", [I32, I64, I64, V, I64, V, I64, V, V]),
+            ("mb_scaled_gemm", [S, V]),
+            ("mb_scaled_plan", [S, ctypes.c_char_p, ctypes.c_int]),
+            ("mb_expert_sort", [I32, I64, I64, V, V, V, V, V]),
+            ("mb_expert_gather", [I32, I64, I64, I64, V, I64, V, V, V, I64, V]),
+            ("mb_expert_gather_quantize", [I32, I64, I64, I64, V, I64, V, V, V, I64, V, V]),
+            ("mb_expert_combine", [I32, I32, I64, I64, I64, V, I64, V, V, V, V, I64, V]),
+            ("mb_expert_combine_backward", [I32, I32, I64, I64, I64, V, I64, V, I64, V, V, V, V, I64, V, V])):
+        fn = getattr(lib, name)
+        fn.argtypes, fn.restype = args, ctypes.c_int
 
 
 _fast = None

@@ -1,7 +1,8 @@
 """Build the sm_100a shared library in-tree (nvcc, no JIT cache).
 
-The library is one CUDA translation unit (``csrc/mb_abi.cu``) exporting the C ABI
-declared in ``include/metalblas_b200.h``; a small torch C++ extension
+The library is two CUDA translation units, compiled side by side: ``csrc/mb_abi.cu``
+(the products of one element type) and ``csrc/mb_ops.cu`` (int8 products with scales,
+expert routing), exporting the C ABI declared in ``include/metalblas_b200.h``; a small torch C++ extension
 (``csrc/fastpath.cpp``) holds the per-thread descriptor cache of repeated calls.  It links the CUDA runtime statically
 so it does not depend on which libcudart torch happened to load, and reaches the
 driver (for cuTensorMapEncodeTiled) through cudaGetDriverEntryPoint, so it needs
@@ -19,7 +20,7 @@ import sys
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(PKG_DIR)
-SRC = os.path.join(PKG_DIR, "csrc", "mb_abi.cu")
+UNITS = ("mb_abi", "mb_ops")
 LIB = os.path.join(PKG_DIR, "libmetalblas_b200.so")
 ARCH = "-gencode=arch=compute_100a,code=sm_100a"
 
@@ -44,22 +45,56 @@ def up_to_date() -> bool:
     return all(os.path.getmtime(s) <= t for s in sources())
 
 
+def _run(procs) -> str:
+    """Wait for every (command, process); raise with the output of the first that failed."""
+    said, bad = "", None
+    for cmd, p in procs:
+        out = p.communicate()[0]
+        said += out
+        if p.returncode != 0 and bad is None:
+            bad = "nvcc failed:\n" + " ".join(cmd) + "\n" + out
+    if bad:
+        raise RuntimeError(bad)
+    return said
+
+
+def _units_of(src: str, seen=None) -> set:
+    """The source files of one unit: the file and what it includes from this repository."""
+    seen = set() if seen is None else seen
+    if src in seen:
+        return seen
+    seen.add(src)
+    with open(src) as f:
+        for line in f:
+            if line.startswith('#include "'):
+                _units_of(os.path.normpath(os.path.join(os.path.dirname(src), line.split('"')[1])), seen)
+    return seen
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
+    """Compile the units whose sources are newer than their objects (all with
+    ``force``), at the same time, and link the library."""
     if not force and up_to_date():
         return LIB
-    cmd = [
-        nvcc_path(), "-std=c++17", "-O3", ARCH, "-lineinfo",
-        "-Xcompiler", "-fPIC", "-shared", "-cudart", "static",
-        "-I", os.path.join(REPO, "include"),
-        "-o", LIB + ".tmp", SRC,
-    ]
+    obj_dir = os.path.join(PKG_DIR, "_build")
+    os.makedirs(obj_dir, exist_ok=True)
+    base = [nvcc_path(), "-std=c++17", "-O3", ARCH, "-lineinfo", "-Xcompiler", "-fPIC"]
     if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
+        base.insert(1, "-Xptxas=-v")
+    procs, objs = [], []
+    for unit in UNITS:
+        src, obj = os.path.join(PKG_DIR, "csrc", unit + ".cu"), os.path.join(obj_dir, unit + ".o")
+        objs.append(obj)
+        if not force and os.path.exists(obj) and all(os.path.getmtime(f) <= os.path.getmtime(obj)
+                                                     for f in _units_of(src) | {__file__}):
+            continue
+        cmd = base + ["-I", os.path.join(REPO, "include"), "-c", "-o", obj, src]
+        procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    said = _run(procs)
+    cmd = base + ["-shared", "-cudart", "static", "-o", LIB + ".tmp", *objs]
+    said += _run([(cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True))])
     if verbose:
-        sys.stderr.write(res.stdout + res.stderr)
+        sys.stderr.write(said)
     os.replace(LIB + ".tmp", LIB)
     return LIB
 

@@ -1,6 +1,6 @@
 // C ABI of metalblas_b200: validation, the sm_100a plan (tile table), TMA
-// descriptor construction and kernel launches.  One translation unit so that
-// the device status word has a single definition.
+// descriptor construction and kernel launches of the products of one element
+// type (mb_ops.cu holds the int8 products with scales and the expert routing).
 //
 // Plan rules (B200 replacement of the reference's planners):
 //  * M==1 or N==1 with a unit-stride matrix -> GEMV kernels, oriented like
@@ -30,7 +30,7 @@
 #include <string>
 #include <unordered_map>
 
-#include "../../include/metalblas_b200.h"
+#include "mb_host.cuh"
 #include "mb_common.cuh"
 #include "simt_gemm.cuh"
 #include "gemv.cuh"
@@ -40,45 +40,12 @@
 #include "pack.cuh"
 
 using namespace mb;
+using namespace mb::host;
 
 namespace {
 
-thread_local std::string g_err;
-
-int fail(int code, const char *fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  g_err = buf;
-  return code;
-}
-
-int cuda_check(cudaError_t e, const char *what) {
-  if (e == cudaSuccess) return MB_OK;
-  return fail(MB_ERR_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
-}
-
-int elem_size(int dt) {
-  switch (dt) {
-    case MB_F32: return 4;
-    case MB_F16: case MB_BF16: return 2;
-    case MB_C64: return 8;
-    case MB_C32: return 4;
-    case MB_I8: case MB_U8: return 1;
-    case MB_I16: return 2;
-    case MB_I32: return 4;
-    case MB_I64: return 8;
-  }
-  return 0;
-}
 bool acc_is_8byte(int dt) { return dt == MB_C64 || dt == MB_C32 || dt == MB_I64; }
 bool is_tc_dtype(int dt) { return dt == MB_BF16 || dt == MB_F16 || dt == MB_I8 || dt == MB_U8; }
-
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
-bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 struct DevInfo {
   int sms = 148;
@@ -140,16 +107,6 @@ std::string tune_key(const mb_gemm_desc *d) {
 
 bool has_overrides(const mb_gemm_desc *d) {
   return d->backend != MB_BACKEND_AUTO || d->tile_n || d->split_k || d->swap_ab || d->cta_pair || d->stream_k;
-}
-
-unsigned long long wait_timeout_ns() {
-  static unsigned long long v = [] {
-    const char *s = getenv("METALBLAS_WAIT_TIMEOUT_MS");
-    long long ms = s ? atoll(s) : 2000;
-    if (ms <= 0) ms = 2000;
-    return (unsigned long long)ms * 1000000ull;
-  }();
-  return v;
 }
 
 // A strided 2-D operand: element (r, c) at base[r*rs + c*cs].  Extent-1
@@ -1120,47 +1077,12 @@ EpiScalars make_epi(const mb_gemm_desc *d) {
 }
 
 // --------------------------------------------------------------------------- launches
-// Programmatic dependent launch for the GEMV and tcgen05 kernels (see
-// pdl_trigger / pdl_wait in mb_common.cuh); METALBLAS_PDL=0 launches them
-// with plain stream order.
 // Split-K of thin tiles reduced inside a thread-block cluster (rank 0's shared
 // memory) instead of through the workspace (METALBLAS_CLUSTER_SPLIT=0: off).
 const bool g_csplit = [] {
   const char *s = getenv("METALBLAS_CLUSTER_SPLIT");
   return !(s && s[0] == '0');
 }();
-
-const bool g_pdl = [] {
-  const char *s = getenv("METALBLAS_PDL");
-  return !(s && s[0] == '0');
-}();
-
-template <class... KArgs, class... Args>
-int launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster_x,
-               const char *what, Args &&...args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  int n = 0;
-  if (cluster_x > 1) {
-    attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = cluster_x;
-    attr[n].val.clusterDim.y = 1;
-    attr[n].val.clusterDim.z = 1;
-    ++n;
-  }
-  if (g_pdl) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n].val.programmaticStreamSerializationAllowed = 1;
-    ++n;
-  }
-  cfg.attrs = attr;
-  cfg.numAttrs = n;
-  return cuda_check(cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...), what);
-}
 
 template <class T>
 int launch_simt(const Op &o, const EpiScalars &e, cudaStream_t st, const int *gate = nullptr) {
@@ -1248,49 +1170,6 @@ int launch_gemv(const Plan &pl, const EpiScalars &e, void *ws, cudaStream_t st) 
     }
   }
   return cuda_check(cudaGetLastError(), "gemv launch");
-}
-
-PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void *p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-  });
-  return fn;
-}
-
-CUtensorMapDataType tma_dtype(int dt) {
-  switch (dt) {
-    case MB_BF16: return CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    case MB_F16: return CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    case MB_F32: return CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
-    default: return CU_TENSOR_MAP_DATA_TYPE_UINT8;
-  }
-}
-
-// 3-D tiled map {inner, outer, batch} with SWIZZLE_128B.
-int encode_map(CUtensorMap *m, int dt, const void *base, int64_t inner, int64_t outer, int64_t batch,
-               int64_t outer_stride_el, int64_t batch_stride_el, int box_inner, int box_outer,
-               CUtensorMapSwizzle swz = CU_TENSOR_MAP_SWIZZLE_128B) {
-  auto enc = get_encode();
-  if (!enc) return fail(MB_ERR_LAUNCH, "cuTensorMapEncodeTiled unavailable");
-  const int esz = elem_size(dt);
-  cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)std::max<int64_t>(batch, 1)};
-  int64_t ostr = outer_stride_el * esz;
-  int64_t bstr = batch_stride_el * esz;
-  if (batch <= 1 || bstr == 0) bstr = round_up(std::max<int64_t>(ostr * outer, 16), 16);
-  cuuint64_t strides[2] = {(cuuint64_t)ostr, (cuuint64_t)bstr};
-  cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer, 1};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = enc(m, tma_dtype(dt), 3, const_cast<void *>(base), dims, strides, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(MB_ERR_LAUNCH, "cuTensorMapEncodeTiled failed (%d)", (int)r);
-  return MB_OK;
 }
 
 template <class T, int BN, int PAIR, class TO = T, bool PEER = false>
@@ -1739,6 +1618,15 @@ int plan_for(const mb_gemm_desc *d, Plan &pl, Op &o, int &sms, bool query = fals
 
 }  // namespace
 
+int mb::host::device_sms() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return 148;
+  }
+  return num_sms(dev);
+}
+
 // =========================================================================== C ABI
 extern "C" {
 
@@ -2163,12 +2051,15 @@ int mb_device_status(void) {
   int v = 0;
   rc = cuda_check(cudaMemcpyFromSymbol(&v, g_mb_status, sizeof(int)), "read status");
   if (rc) return rc;
+  if (v == 0) rc = ops_status_read(&v);
+  if (rc) return rc;
   return v;
 }
 
 void mb_device_status_clear(void) {
   int z = 0;
   cudaMemcpyToSymbol(g_mb_status, &z, sizeof(int));
+  ops_status_clear();
 }
 
 int mb_debug_wait_timeout(int64_t limit_us, void *stream) {

@@ -149,8 +149,8 @@ template <> struct EpiOps<int32_t> : EpiOpsInt<int32_t> {};
 template <> struct EpiOps<int64_t> : EpiOpsInt<int64_t> {};
 
 // Device status word: set to a non-zero mb_status when a bounded wait gives up.
-// (The library is one translation unit, so this is its only definition.)
-__device__ int g_mb_status = 0;
+// Each translation unit has its own; mb_device_status reports either.
+static __device__ int g_mb_status = 0;
 
 __device__ __forceinline__ uint64_t globaltimer_ns() {
   uint64_t t;

@@ -1447,7 +1447,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) tc_gemm_kernel(const __grid_co
 }
 
 // Debug kernel for the bounded-wait path: waits on a barrier nobody arrives at.
-__global__ void wait_timeout_kernel(unsigned long long timeout_ns) {
+static __global__ void wait_timeout_kernel(unsigned long long timeout_ns) {
   __shared__ __align__(8) uint64_t bar;
   __shared__ int abort_flag;
   if (threadIdx.x == 0) {
