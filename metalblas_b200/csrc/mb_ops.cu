@@ -3,13 +3,16 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
+#include <cmath>
 #include <cstring>
 
 #include "mb_host.cuh"
 #include "mb_common.cuh"
 #include "quantize.cuh"
 #include "experts.cuh"
-#include "scaled_gemm.cuh"
+#include "pack.cuh"
+#include "scaled_tc.cuh"
 
 using namespace mb;
 using namespace mb::host;
@@ -53,6 +56,223 @@ int check_route(int64_t T, int64_t k, int64_t H, const int32_t *position, const 
   return MB_OK;
 }
 
+
+// ------------------------------------------------------------- int8 products with scales
+int scaled_check(const mb_scaled_desc *d) {
+  if (!d) return fail(MB_ERR_INVALID, "null descriptor");
+  if (!is_float(d->out_dtype)) return fail(MB_ERR_UNSUPPORTED, "out_dtype %d is not fp32, fp16 or bf16", d->out_dtype);
+  if (d->M < 0 || d->N < 0 || d->K < 0 || d->groups < 0) return fail(MB_ERR_INVALID, "negative extent");
+  if (d->M > 0x7fffff00ll || d->N > 0x7fffff00ll) return fail(MB_ERR_INVALID, "M and N must stay below 2^31");
+  if (d->K > 131071) return fail(MB_ERR_INVALID, "K = %lld: sums of more than 131071 int8 products can leave 32 bits", (long long)d->K);
+  if (d->groups > 1024) return fail(MB_ERR_INVALID, "more than 1024 groups");
+  if (d->M == 0 || d->N == 0) return MB_OK;
+  if (!d->C || !d->scale_a || !d->scale_b) return fail(MB_ERR_INVALID, "null C, scale_a or scale_b");
+  if (d->K > 0 && (!d->A || !d->B)) return fail(MB_ERR_INVALID, "null A or B");
+  if (d->groups > 0 && !d->offsets) return fail(MB_ERR_INVALID, "groups need offsets");
+  if (d->bias && d->bias_dtype != d->out_dtype && d->bias_dtype != MB_F32)
+    return fail(MB_ERR_INVALID, "bias must have the output's type or fp32");
+  return MB_OK;
+}
+
+
+struct SgPlan {
+  bool empty = false;
+  int bn = 0, pair = 1, split = 1, swap = 0;
+  int w_mn = 0;                       // weights are read with N contiguous
+  int pk_a = 0, pk_b = 0;             // operand copied into the workspace first
+  int64_t a_rs = 0, w_ld = 0, sB = 0; // strides of the operands as read
+  int64_t a_off = 0, b_off = 0, ws_bytes = 0;
+  int64_t units = 0;                  // at most
+};
+
+// TMA reads a matrix in place when `cs` is 1, the base lies on 16 bytes and rows
+// (and groups) are a multiple of 16 bytes apart.
+bool tma_rows(const void *p, int64_t rows, int64_t cols, int64_t &rs, int64_t cs, int64_t groups, int64_t gs) {
+  if (cols > 1 && cs != 1) return false;
+  if (rows <= 1) rs = round_up(std::max<int64_t>(cols, 1), 16);  // never used to step
+  return aligned16(p) && rs > 0 && rs % 16 == 0 && (groups <= 1 || (gs >= 0 && gs % 16 == 0));
+}
+
+// One tile shape's time in SM cycles.  Per 128-byte K-block an SM is bound by
+// its operands' way into shared memory, at the rates of tc_gemm.cuh's tile
+// table (45 B/clk alone, 35 on a CTA pair, 30.5 for the 512-wide pair tile); a
+// product with few rows is bound by the weights' way from HBM, 22.4 B/clk per SM
+// over the chip and 31 for one SM.
+struct SgCost {
+  double t;
+  int split;
+};
+SgCost sg_cost(const mb_scaled_desc *d, int swap, int bn, int pair, int sms, int force_split) {
+  const double M = (double)d->M, kb = (double)ceil_div(d->K, 128);
+  const double active = d->groups ? std::min<double>((double)d->groups, M) : 1.0;
+  const double rows = M / active;
+  const int trows = swap ? bn : 128 * pair;
+  // groups do not end on tile boundaries: half a tile more each
+  const double tiles_r = d->groups && rows > trows / 2 ? M / trows + 0.5 * active : active * std::ceil(rows / trows);
+  const double tiles_c = (double)ceil_div(d->N, swap ? 128 : bn);
+  const double units = tiles_r * tiles_c;
+  const double kbc = bn > 256 ? 1611.0 : pair == 2 ? (128.0 + bn / 2.0) * 128.0 / 35.0 : (128.0 + bn) * 128.0 / 45.0;
+  const double epi = (bn > 256 ? 12.0 : 4.0) * bn;
+  int split = 1;
+  if (pair == 1 && bn <= 128) {
+    if (force_split) split = force_split;
+    else
+      while (split < 8 && units * split * 2 <= sms && kb / (split * 2) >= 4) split *= 2;
+  }
+  const double slots = (double)sms / (pair * split);
+  const double waves = std::ceil(units / slots);
+  const double compute = waves * (std::ceil(kb / split) * kbc + epi + (split > 1 ? 1500.0 : 0.0));
+  const double busy = std::min<double>(sms, units * pair * split);
+  const double bytes = active * (double)d->N * (double)d->K + M * (double)d->K + M * (double)d->N * elem_size(d->out_dtype);
+  return {std::max(compute, bytes / std::min(22.4 * sms, 31.0 * busy)), split};
+}
+
+int sg_plan(const mb_scaled_desc *d, SgPlan &pl) {
+  if (d->M == 0 || d->N == 0) { pl.empty = true; return MB_OK; }
+  if (d->K == 0) return MB_OK;
+  const int64_t E = std::max<int64_t>(d->groups, 1);
+  const int64_t nB = d->groups > 1 && d->sB == 0 ? 1 : E;  // distinct weight matrices
+  // tokens: K contiguous
+  pl.a_rs = d->a_rs;
+  if (!tma_rows(d->A, d->M, d->K, pl.a_rs, d->a_cs, 1, 0)) {
+    pl.pk_a = 1;
+    pl.a_rs = round_up(d->K, 16);
+  }
+  // weights: K or N contiguous, as they come; without a unit stride copied with K contiguous
+  pl.w_ld = d->b_cs;
+  pl.sB = d->sB;
+  if (!tma_rows(d->B, d->N, d->K, pl.w_ld, d->b_rs, nB, d->sB)) {
+    pl.w_ld = d->b_rs;
+    pl.w_mn = 1;
+    if (!tma_rows(d->B, d->K, d->N, pl.w_ld, d->b_cs, nB, d->sB)) {
+      pl.pk_b = 1;
+      pl.w_mn = d->b_cs == 1 && d->b_rs != 1;
+      pl.w_ld = round_up(pl.w_mn ? d->N : d->K, 16);
+      pl.sB = pl.w_ld * (pl.w_mn ? d->K : d->N);
+    }
+  }
+  int64_t at = 0;
+  if (pl.pk_a) { pl.a_off = at; at = round_up(at + d->M * pl.a_rs, 256); }
+  if (pl.pk_b) { pl.b_off = at; at = round_up(at + nB * pl.sB, 256); }
+  pl.ws_bytes = at;
+
+  const int sms = device_sms();
+  static const struct { int swap, bn, pair; } tiles[] = {{1, 16, 1},  {1, 32, 1},  {1, 64, 1},  {1, 128, 1},
+                                                         {0, 128, 1}, {0, 256, 1}, {0, 256, 2}, {0, 512, 2}};
+  double best = 1e300;
+  for (const auto &c : tiles) {
+    if (d->tile_n && d->tile_n != c.bn) continue;
+    if (d->cta_pair && d->cta_pair != c.pair) continue;
+    if (d->swap_ab && (d->swap_ab > 0) != (c.swap == 1)) continue;
+    if (d->split_k > 1 && (c.pair != 1 || c.bn > 128)) continue;
+    const SgCost cost = sg_cost(d, c.swap, c.bn, c.pair, sms, d->split_k);
+    if (cost.t < best) {
+      best = cost.t;
+      pl.swap = c.swap; pl.bn = c.bn; pl.pair = c.pair; pl.split = cost.split;
+    }
+  }
+  if (!pl.bn) return fail(MB_ERR_INVALID, "no tile has tile_n %d, split_k %d, swap_ab %d, cta_pair %d", d->tile_n, d->split_k, d->swap_ab, d->cta_pair);
+  if (pl.split != 1 && pl.split != 2 && pl.split != 4 && pl.split != 8)
+    return fail(MB_ERR_INVALID, "split_k must be 1, 2, 4 or 8");
+  if (pl.split > ceil_div(d->K, 128)) return fail(MB_ERR_INVALID, "split_k %d exceeds the K-blocks", pl.split);
+  const int64_t trows = pl.swap ? pl.bn : 128 * pl.pair;
+  pl.units = (ceil_div(d->M, trows) + (d->groups ? std::min(E, d->M) : 0)) * ceil_div(d->N, pl.swap ? 128 : pl.bn);
+  if (pl.units >= (1ll << 31)) return fail(MB_ERR_INVALID, "too many tiles");
+  return MB_OK;
+}
+
+template <int BN, int PAIR, bool SWAP, class TO>
+int sg_launch_tile(const SgPlan &pl, sg::SgParams &p, cudaStream_t st) {
+  using C_ = sg::SgCfg<BN, PAIR, SWAP, TO>;
+  p.split = pl.split;
+  p.stages = C_::stages(pl.split);
+  p.tiles_c = (int)ceil_div(p.N, C_::TCOLS);
+  auto kern = sg::scaled_gemm_kernel<BN, PAIR, SWAP, TO>;
+  constexpr int smem_max = C_::CAN_SPLIT ? std::max(C_::smem_bytes(1), std::max(C_::smem_bytes(2), std::max(C_::smem_bytes(4), C_::smem_bytes(8))))
+                                         : C_::smem_bytes(1);
+  static_assert(smem_max <= tc::SMEM_LIMIT, "shared memory");
+  static std::atomic<bool> attr_done[64];
+  int dev = 0;
+  int rc = cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
+  if (rc) return rc;
+  if (dev < 0 || dev >= 64 || !attr_done[dev].load(std::memory_order_acquire)) {
+    rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_max), "cudaFuncSetAttribute");
+    if (rc) return rc;
+    if (dev >= 0 && dev < 64) attr_done[dev].store(true, std::memory_order_release);
+  }
+  const int csize = PAIR == 2 ? 2 : pl.split;
+  const int64_t clusters = std::min<int64_t>(pl.units, device_sms() / csize);
+  return launch_pdl(kern, dim3((unsigned)(clusters * csize)), dim3(tc::NUM_THREADS), C_::smem_bytes(pl.split), st, csize,
+                    "scaled_gemm", p);
+}
+
+int sg_pack(const void *src, void *dst, int64_t rows, int64_t cols, int64_t rs, int64_t cs, int64_t bs, int64_t batches,
+            int64_t ld, cudaStream_t st) {
+  PackArgs a{src, dst, rows, cols, rs, cs, bs, batches, ld};
+  const int64_t cap = (int64_t)device_sms() * 16;
+  if (cs == 1) {
+    const int64_t n = batches * rows * ceil_div(cols, 16);
+    pack_rows16_kernel<uint8_t><<<(unsigned)std::min<int64_t>(ceil_div(n, 256), cap), 256, 0, st>>>(a);
+  } else {
+    const int64_t tiles = batches * ceil_div(rows, 32) * ceil_div(cols, 32);
+    pack_matrix_kernel<uint8_t><<<(unsigned)std::min<int64_t>(tiles, cap), dim3(32, 8), 0, st>>>(a);
+  }
+  return cuda_check(cudaGetLastError(), "scaled_gemm: operand copy");
+}
+
+template <class TO>
+int sg_launch(const mb_scaled_desc *d, const SgPlan &pl, cudaStream_t st) {
+  sg::SgParams p;
+  memset(&p, 0, sizeof(p));
+  p.M = (int)d->M; p.N = (int)d->N; p.groups = (int)std::max<int64_t>(d->groups, 1);
+  p.offsets = d->groups ? d->offsets : nullptr;
+  p.one_b = d->groups > 1 && d->sB == 0;
+  p.kb_total = (int)ceil_div(d->K, 128);
+  p.C = d->C; p.c_rs = d->c_rs; p.c_cs = d->c_cs;
+  constexpr int OSZ = sizeof(TO);
+  p.c_vec = (d->c_cs == 1 || d->N == 1) && aligned16(d->C) && (d->M == 1 || (d->c_rs * OSZ) % 16 == 0);
+  p.scale_a = d->scale_a; p.scale_b = d->scale_b;
+  p.sa_s = d->scale_a_s; p.sb_s = d->scale_b_s; p.sb_g = d->scale_b_g;
+  p.bias = d->bias; p.bias_s = d->bias_s; p.bias_f32 = d->bias_dtype == MB_F32;
+  p.timeout_ns = wait_timeout_ns();
+  if (d->K == 0) {
+    const int64_t blocks = std::min<int64_t>(ceil_div(d->M * d->N, 256), (int64_t)device_sms() * 16);
+    return launch_pdl(sg::scaled_empty_kernel<TO>, dim3((unsigned)blocks), dim3(256), 0, st, 1, "scaled_gemm", p);
+  }
+  const int64_t nB = p.one_b ? 1 : p.groups;
+  const void *A = d->A, *B = d->B;
+  int rc = MB_OK;
+  if (pl.pk_a) {
+    A = static_cast<char *>(d->workspace) + pl.a_off;
+    rc = sg_pack(d->A, const_cast<void *>(A), d->M, d->K, d->a_rs, d->a_cs, 0, 1, pl.a_rs, st);
+  }
+  if (!rc && pl.pk_b) {
+    B = static_cast<char *>(d->workspace) + pl.b_off;
+    rc = pl.w_mn ? sg_pack(d->B, const_cast<void *>(B), d->K, d->N, d->b_rs, d->b_cs, d->sB, nB, pl.w_ld, st)
+                 : sg_pack(d->B, const_cast<void *>(B), d->N, d->K, d->b_cs, d->b_rs, d->sB, nB, pl.w_ld, st);
+  }
+  if (rc) return rc;
+  // boxes of 128 bytes along the contiguous dimension
+  CUtensorMap *ta = pl.swap ? &p.tmB : &p.tmA, *tw = pl.swap ? &p.tmA : &p.tmB;
+  const int w_rows = pl.swap ? 128 : std::min(pl.bn, 256) / pl.pair;  // channels per box
+  rc = encode_map(ta, MB_I8, A, d->K, d->M, 1, pl.a_rs, 0, 128, pl.swap ? pl.bn : 128);
+  if (!rc)
+    rc = pl.w_mn ? encode_map(tw, MB_I8, B, d->N, d->K, nB, pl.w_ld, pl.sB, 128, 128)
+                 : encode_map(tw, MB_I8, B, d->K, d->N, nB, pl.w_ld, pl.sB, 128, w_rows);
+  if (rc) return rc;
+  (pl.swap ? p.a_mn : p.b_mn) = pl.w_mn;
+  if (pl.swap) {
+    switch (pl.bn) {
+      case 16: return sg_launch_tile<16, 1, true, TO>(pl, p, st);
+      case 32: return sg_launch_tile<32, 1, true, TO>(pl, p, st);
+      case 64: return sg_launch_tile<64, 1, true, TO>(pl, p, st);
+      default: return sg_launch_tile<128, 1, true, TO>(pl, p, st);
+    }
+  }
+  if (pl.pair == 1) return pl.bn == 128 ? sg_launch_tile<128, 1, false, TO>(pl, p, st) : sg_launch_tile<256, 1, false, TO>(pl, p, st);
+  return pl.bn == 256 ? sg_launch_tile<256, 2, false, TO>(pl, p, st) : sg_launch_tile<512, 2, false, TO>(pl, p, st);
+}
+
 }  // namespace
 
 extern "C" {
@@ -82,46 +302,33 @@ void mb_scaled_desc_init(mb_scaled_desc *d) {
   if (d) memset(d, 0, sizeof(*d));
 }
 
-static int scaled_check(const mb_scaled_desc *d) {
-  if (!d) return fail(MB_ERR_INVALID, "null descriptor");
-  if (!is_float(d->out_dtype)) return fail(MB_ERR_UNSUPPORTED, "out_dtype %d is not fp32, fp16 or bf16", d->out_dtype);
-  if (d->M < 0 || d->N < 0 || d->K < 0 || d->groups < 0) return fail(MB_ERR_INVALID, "negative extent");
-  if (d->M > 0x7fffff00ll || d->N > 0x7fffff00ll) return fail(MB_ERR_INVALID, "M and N must stay below 2^31");
-  if (d->K > 131071) return fail(MB_ERR_INVALID, "K = %lld: sums of more than 131071 int8 products can leave 32 bits", (long long)d->K);
-  if (d->groups > 1024) return fail(MB_ERR_INVALID, "more than 1024 groups");
-  if (d->M == 0 || d->N == 0) return MB_OK;
-  if (!d->C || !d->scale_a || !d->scale_b) return fail(MB_ERR_INVALID, "null C, scale_a or scale_b");
-  if (d->K > 0 && (!d->A || !d->B)) return fail(MB_ERR_INVALID, "null A or B");
-  if (d->groups > 0 && !d->offsets) return fail(MB_ERR_INVALID, "groups need offsets");
-  if (d->bias && d->bias_dtype != d->out_dtype && d->bias_dtype != MB_F32)
-    return fail(MB_ERR_INVALID, "bias must have the output's type or fp32");
-  return MB_OK;
+int64_t mb_scaled_workspace_size(const mb_scaled_desc *d) {
+  SgPlan pl;
+  if (scaled_check(d) || sg_plan(d, pl)) return 0;
+  return pl.ws_bytes;
 }
 
-int64_t mb_scaled_workspace_size(const mb_scaled_desc *d) { return 0; }
-
 int mb_scaled_plan(const mb_scaled_desc *d, char *buf, int buflen) {
-  const int rc = scaled_check(d);
+  SgPlan pl;
+  int rc = scaled_check(d);
+  if (!rc) rc = sg_plan(d, pl);
   if (rc) return -rc;
-  return snprintf(buf, buf ? (size_t)std::max(buflen, 0) : 0, "simple");
+  const size_t room = buf ? (size_t)std::max(buflen, 0) : 0;
+  if (pl.bn == 0) return snprintf(buf, room, pl.empty ? "empty" : "no sum");
+  return snprintf(buf, room, "%s bn=%d pair=%d split=%d a_mn=%d b_mn=%d pack_a=%d pack_b=%d ws=%lld",
+                  pl.swap ? "channels" : "tokens", pl.bn, pl.pair, pl.split, 0, pl.w_mn, pl.pk_a, pl.pk_b,
+                  (long long)pl.ws_bytes);
 }
 
 int mb_scaled_gemm(const mb_scaled_desc *d, void *stream) {
-  const int rc = scaled_check(d);
-  if (rc || d->M == 0 || d->N == 0) return rc;
+  SgPlan pl;
+  int rc = scaled_check(d);
+  if (!rc) rc = sg_plan(d, pl);
+  if (rc || pl.empty) return rc;
+  if (pl.ws_bytes > 0 && (!d->workspace || d->workspace_bytes < pl.ws_bytes))
+    return fail(MB_ERR_WORKSPACE, "workspace of %lld bytes required", (long long)pl.ws_bytes);
   return by_float(d->out_dtype, [&](auto *tag) {
-    using T = std::remove_pointer_t<decltype(tag)>;
-    ScaledParams p{};
-    p.M = d->M; p.N = d->N; p.K = d->K; p.groups = (int)std::max<int64_t>(d->groups, 1);
-    p.A = d->A; p.B = d->B; p.C = d->C;
-    p.a_rs = d->a_rs; p.a_cs = d->a_cs; p.b_rs = d->b_rs; p.b_cs = d->b_cs; p.sB = d->sB;
-    p.c_rs = d->c_rs; p.c_cs = d->c_cs;
-    p.scale_a = d->scale_a; p.scale_b = d->scale_b;
-    p.sa_s = d->scale_a_s; p.sb_s = d->scale_b_s; p.sb_g = d->scale_b_g;
-    p.bias = d->bias; p.bias_s = d->bias_s; p.bias_f32 = d->bias_dtype == MB_F32;
-    p.offsets = d->groups ? d->offsets : nullptr;
-    return launch_pdl(scaled_simple_kernel<T>, dim3((unsigned)(device_sms() * 8)), dim3(256), 0, (cudaStream_t)stream, 1,
-                      "scaled_gemm", p);
+    return sg_launch<std::remove_pointer_t<decltype(tag)>>(d, pl, (cudaStream_t)stream);
   });
 }
 

@@ -156,7 +156,7 @@ __device__ __forceinline__ float split_load(const SplitArgs &a, const float *src
 // dst[b][r][c] = split(src(b, r, c)) through a shared-memory tile, so both the
 // source read (along whichever of r / c is contiguous) and the destination rows
 // are coalesced.  Block 32 x 8, grid-stride over tiles.
-__global__ void __launch_bounds__(256) split_tf32_kernel(const SplitArgs a) {
+static __global__ void __launch_bounds__(256) split_tf32_kernel(const SplitArgs a) {
   // 32 rows x 128 columns per tile; each thread then splits 4 consecutive
   // columns of a row and writes them with one 16-byte store per part
   __shared__ float tile[32][129];

@@ -77,8 +77,8 @@ struct SgCfg {
   static constexpr int STAGING_WARP = SWAP ? 0 : 32 * RB;
   static constexpr int VEC_WARP = 32 * 8;               // a chunk's column scales and biases
   static constexpr bool CAN_SPLIT = PAIR == 1 && BN <= 128;
-  static constexpr int piece_bytes() { return 64 * BN; }  // 32 lanes x BN / 2 columns x 4 bytes
-  static constexpr int red_bytes(int split) { return CAN_SPLIT ? (split - 1) * (8 / split) * piece_bytes() : 0; }
+  static constexpr int PIECE_BYTES = 64 * BN;   // 32 lanes x BN / 2 columns x 4 bytes
+  static __host__ __device__ constexpr int red_bytes(int split) { return CAN_SPLIT ? (split - 1) * (8 / split) * PIECE_BYTES : 0; }
   static constexpr int fixed_bytes(int split) {
     return 1024 + NUM_EPI_WARPS * (STAGING_WARP + VEC_WARP) + red_bytes(split) + BAR_BYTES + TABLE_BYTES;
   }
@@ -377,9 +377,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
     // With split ranks: the piece of the tile this warp holds, the rank that
     // finishes it, and where its sums go there.
     const int piece = q * 2 + half, per_rank = 8 / split;
-    const uint32_t owner = (uint32_t)(piece / per_rank);
-    const uint32_t red_u32 = smem_u32(red) + (uint32_t)(piece % per_rank) * C_::piece_bytes() + (uint32_t)lane * 16u;
-    const uint32_t red_step = (uint32_t)(per_rank * C_::piece_bytes());  // from one source rank to the next
+    const int owner = piece / per_rank, me = (int)rank;
+    const uint32_t red_u32 = smem_u32(red) + (uint32_t)(piece % per_rank) * C_::PIECE_BYTES + (uint32_t)lane * 16u;
+    const uint32_t red_step = (uint32_t)(per_rank * C_::PIECE_BYTES);  // from one source rank to the next
     uint32_t rphase = 0;
     bool first = true;
 
@@ -390,10 +390,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
       if (!all(wait_x(tfull_bar(abuf), aphase))) break;
       tc_fence_after();
       const uint32_t tbase = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(abuf * B_::ACC_COLS + half * WCOLS);
-      if (split > 1 && owner != rank) {
+      if (split > 1 && owner != me) {
         // what this CTA sent for the last unit has been read
         if (!first && !all(mbar_wait_cluster(red_free, rphase ^ 1u, abort_flag, p.timeout_ns))) break;
-        const uint32_t dst = mapa_shared(red_u32 + (rank - (rank > owner ? 1u : 0u)) * red_step, owner);
+        const uint32_t dst = mapa_shared(red_u32 + (uint32_t)(me - (me > owner ? 1 : 0)) * red_step, (uint32_t)owner);
 #pragma unroll 1
         for (int c = 0; c < WCOLS; c += CH) {
           uint32_t r[32];
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
         tc_fence_before();
         __syncwarp();
         if (lane == 0) release_tmem(abuf);
-        mbar_arrive_cluster(mapa_shared(red_full, owner));
+        mbar_arrive_cluster(mapa_shared(red_full, (uint32_t)owner));
       } else {
         if (split > 1 && !all(mbar_wait_cluster(red_full, rphase, abort_flag, p.timeout_ns))) break;
         const int row = (PAIR == 2 ? (int)rank * BM : 0) + q * 32 + lane;   // UMMA row of this lane
@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
         }
         if (split > 1) {
           __syncwarp();
-          if (lane < split && lane != (int)rank) mbar_arrive_cluster(mapa_shared(red_free, lane));
+          if (lane < split && lane != me) mbar_arrive_cluster(mapa_shared(red_free, (uint32_t)lane));
         }
       }
       rphase ^= 1u;

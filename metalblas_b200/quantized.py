@@ -17,7 +17,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .dispatch import FLOATS, _stream_of, _workspace
+from .dispatch import FLOATS, _stream_of
 
 MAX_K = 131071       # 127 or 128 squared times more would leave 32 bits
 MAX_GROUPS = 1024
@@ -118,8 +118,9 @@ def _product(a2, b, sa, sb, M, N, K, groups, offsets, bias, out_dtype, c, overri
     stream = _stream_of(c.device)
     need = lib.mb_scaled_workspace_size(_byref(d))
     if need > 0:
-        ws = _workspace(c.device, stream, need)
-        d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
+        # copies of operands that cannot be read in place; the allocator keeps it on this stream
+        ws = torch.empty(need, dtype=torch.uint8, device=c.device)
+        d.workspace, d.workspace_bytes = ws.data_ptr(), need
     _lib.raise_for(lib.mb_scaled_gemm(_byref(d), stream), "mb_scaled_gemm")
 
 

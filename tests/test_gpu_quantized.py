@@ -356,6 +356,47 @@ def test_on_another_stream_and_in_a_graph():
     assert torch.equal(y1, mb.scaled_mm(q0, w, s0, sb))
 
 
+# ------------------------------------------------------------------------------ every plan
+PLANS = [(bn, split, 1, 0) for bn in (16, 32, 64, 128) for split in (1, 2, 4, 8)] + \
+        [(128, split, -1, 0) for split in (1, 2, 4, 8)] + [(256, 0, -1, 1), (256, 0, -1, 2), (512, 0, -1, 2)]
+
+
+@pytest.mark.parametrize("plan", PLANS)
+def test_every_tile_and_split_gives_the_same_bits(plan):
+    """(tile_n, split, swap, pair) as given, over ragged tiles and, for the splits, more units
+    than clusters, so that each cluster hands its partial sums over several times."""
+    g = gen(41)
+    for M, K, N in ((1, 1040, 260), (130, 1040, 515), (300, 1296, 1000), (40, 1024, 30000)):
+        a, sa, sb = ints((M, K), g), scales((M,), g), scales((N,), g)
+        bias = torch.randn(N, generator=g).to(DEV)
+        for w in (ints((N, K), g).t(), ints((K, (N + 15) // 16 * 16), g)[:, :N]):
+            y = mb.scaled_mm(a, w, sa, sb, bias=bias, out_dtype=torch.float32, _plan=plan)
+            check_product(y, a, w, sa, sb, bias)
+            assert torch.equal(y, mb.scaled_mm(a, w, sa, sb, bias=bias, out_dtype=torch.float32))
+
+
+@pytest.mark.parametrize("plan", PLANS)
+def test_every_tile_and_split_by_group(plan):
+    g = gen(42)
+    K = 1040
+    for counts, extra, N in (([3, 0, 17, 130, 1, 0, 40], 5, 390), ([2, 1] * 30, 0, 1040), ([0, 600, 1, 300], 77, 515)):
+        M, E = sum(counts) + extra, len(counts)
+        a, sa, sb, off = ints((M, K), g), scales((M,), g), scales((E, N), g), offsets_of(counts)
+        w = ints((E, N, K), g).transpose(1, 2)
+        for out_dtype in (torch.bfloat16, torch.float32):
+            y = mb.grouped_scaled_mm(a, w, sa, sb, off, out_dtype=out_dtype, _plan=plan,
+                                     out=torch.full((M, N), float("nan"), dtype=out_dtype, device=DEV))
+            check_grouped(y, a, w, sa, sb, off)
+
+
+def test_forced_plans_that_do_not_exist_are_refused():
+    g = gen(43)
+    a, w, sa, sb = ints((64, 256), g), ints((128, 256), g).t(), scales((64,), g), scales((128,), g)
+    for plan in ((48, 0, 0, 0), (512, 0, 0, 1), (16, 0, -1, 0), (0, 3, 0, 0), (0, 4, 0, 0), (256, 2, 0, 0)):
+        with pytest.raises(ValueError):
+            mb.scaled_mm(a, w, sa, sb, _plan=plan)
+
+
 # ------------------------------------------------------------------------------ refusals
 def test_refusals():
     z = lambda *s, dt=torch.int8: torch.zeros(*s, dtype=dt, device=DEV)  # noqa: E731
