@@ -44,6 +44,7 @@ bool rows16(const void *p, int64_t ld, int esz) { return aligned16(p) && (ld * e
 
 int check_rows(int dt, int64_t rows, int64_t cols, int64_t ld, const void *p, const char *what) {
   if (rows < 0 || cols < 0) return fail(MB_ERR_INVALID, "%s: negative extent", what);
+  if (cols > (1ll << 30)) return fail(MB_ERR_INVALID, "%s: %lld columns", what, (long long)cols);
   if (rows > 1 && ld < cols) return fail(MB_ERR_INVALID, "%s: row stride %lld below %lld columns", what, (long long)ld, (long long)cols);
   if (rows > 0 && cols > 0 && !p) return fail(MB_ERR_INVALID, "%s: null pointer", what);
   return MB_OK;
@@ -56,6 +57,32 @@ int check_route(int64_t T, int64_t k, int64_t H, const int32_t *position, const 
   return MB_OK;
 }
 
+
+// Threads of a block that share a token: short rows would leave most of a block idle.
+int route_lanes(int64_t H, int esz) {
+  const int64_t vecs = ceil_div(H * esz, 16);
+  return vecs <= 64 ? 32 : vecs <= 512 ? 128 : 256;
+}
+dim3 route_grid(int64_t T, int64_t H, int esz, int lanes, bool whole_rows) {
+  const int64_t y = whole_rows ? 1 : std::min<int64_t>(ceil_div(ceil_div(H * esz, 16) + 1, lanes), 64);
+  return dim3((unsigned)ceil_div(T, kRouteThreads / lanes), (unsigned)y);
+}
+
+template <class T>
+int launch_quantize(const RouteParams &p, cudaStream_t st, const char *what) {
+  constexpr int V = Vec<T>::V;
+  const bool al = rows16(p.src, p.ld_src, sizeof(T));
+  const int q_vec = reinterpret_cast<uintptr_t>(p.dst) % V == 0 && p.ld_dst % V == 0;
+  // up to four vectors of a row per thread stay in registers
+  const int64_t vecs = ceil_div(p.H, V);
+  auto go = [&](auto kern, int tpr) {
+    const int threads = std::max(tpr, 256);
+    return launch_pdl(kern, dim3((unsigned)ceil_div(p.T, threads / tpr)), dim3(threads), 0, st, 1, what, p, q_vec);
+  };
+  if (vecs <= 128) return al ? go(quantize_rows_kernel<T, true, 32>, 32) : go(quantize_rows_kernel<T, false, 32>, 32);
+  if (vecs <= 512) return al ? go(quantize_rows_kernel<T, true, 128>, 128) : go(quantize_rows_kernel<T, false, 128>, 128);
+  return al ? go(quantize_rows_kernel<T, true, 512>, 512) : go(quantize_rows_kernel<T, false, 512>, 512);
+}
 
 // ------------------------------------------------------------- int8 products with scales
 int scaled_check(const mb_scaled_desc *d) {
@@ -289,12 +316,9 @@ int mb_quantize(int32_t dtype, int64_t rows, int64_t cols, const void *x, int64_
   return by_float(dtype, [&](auto *tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     RouteParams p{};
-    p.T = rows; p.H = cols; p.k = 1;
+    p.T = (int)rows; p.H = (int)cols; p.k = 1;
     p.src = x; p.ld_src = ldx; p.dst = q; p.ld_dst = ldq; p.scale = scale;
-    constexpr int V = 16 / sizeof(T);
-    const bool vec = rows16(x, ldx, sizeof(T)) && cols % V == 0;
-    return launch_pdl(vec ? quantize_rows_kernel<T, V> : quantize_rows_kernel<T, 1>, dim3((unsigned)rows), dim3(256), 0,
-                      (cudaStream_t)stream, 1, "quantize", p);
+    return launch_quantize<T>(p, (cudaStream_t)stream, "quantize");
   });
 }
 
@@ -339,13 +363,20 @@ int mb_expert_sort(int32_t ids64, int64_t n, int64_t experts, const void *ids, i
     return fail(MB_ERR_INVALID, "expert_sort: %lld experts (1 to %d)", (long long)experts, kMaxExperts);
   if (!offsets || (n > 0 && (!ids || !order || !position))) return fail(MB_ERR_INVALID, "expert_sort: null pointer");
   SortParams p{ids, (int)n, (int)experts, order, position, offsets};
-  const int W = (int)std::max<int64_t>(1, std::min<int64_t>(32, ceil_div(n, 32)));
-  const size_t smem = (size_t)W * (experts + 1) * 4;
+  // a warp per 256 entries (what its lanes hold at once), a thread per expert
+  // for the scan, and a cluster of blocks past 8192 entries
+  const int W = (int)std::max<int64_t>(std::min<int64_t>(32, ceil_div(n, 32 * kSortBatch)), ceil_div(experts, 32));
+  int ranks = 1;
+  while (ranks < 8 && n > (int64_t)ranks * 32 * 32 * kSortBatch) ranks *= 2;
+  const int threads = std::min(W, 32) * 32;
+  const size_t smem = ((size_t)(threads / 32 + 1) * (experts + 1) + 32) * 4;
   auto kern = ids64 ? expert_sort_kernel<long long> : expert_sort_kernel<int>;
-  const int rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
-                            "cudaFuncSetAttribute");
-  if (rc) return rc;
-  return launch_pdl(kern, dim3(1), dim3(W * 32), smem, (cudaStream_t)stream, 1, "expert_sort", p);
+  if (smem > 48 * 1024) {
+    const int rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+                              "cudaFuncSetAttribute");
+    if (rc) return rc;
+  }
+  return launch_pdl(kern, dim3(ranks), dim3(threads), smem, (cudaStream_t)stream, ranks, "expert_sort", p);
 }
 
 int mb_expert_gather(int32_t dtype, int64_t tokens, int64_t k, int64_t cols, const void *x, int64_t ldx,
@@ -358,13 +389,13 @@ int mb_expert_gather(int32_t dtype, int64_t tokens, int64_t k, int64_t cols, con
   return by_float(dtype, [&](auto *tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     RouteParams p{};
-    p.T = tokens; p.H = cols; p.k = (int)k; p.position = position; p.kept = kept;
+    p.T = (int)tokens; p.H = (int)cols; p.k = (int)k; p.position = position; p.kept = kept;
     p.src = x; p.ld_src = ldx; p.dst = sorted; p.ld_dst = lds;
-    constexpr int V = 16 / sizeof(T);
-    const bool vec = rows16(x, ldx, sizeof(T)) && rows16(sorted, lds, sizeof(T)) && cols % V == 0;
-    const dim3 grid((unsigned)tokens, (unsigned)std::min<int64_t>(ceil_div(cols, 256 * (vec ? V : 1)), 16));
-    return launch_pdl(vec ? expert_gather_kernel<T, V> : expert_gather_kernel<T, 1>, grid, dim3(256), 0,
-                      (cudaStream_t)stream, 1, "expert_gather", p);
+    const bool al = rows16(x, ldx, sizeof(T)) && rows16(sorted, lds, sizeof(T));
+    const int lanes = route_lanes(cols, sizeof(T));
+    return launch_pdl(al ? expert_gather_kernel<T, true> : expert_gather_kernel<T, false>,
+                      route_grid(tokens, cols, sizeof(T), lanes, false), dim3(kRouteThreads), 0, (cudaStream_t)stream, 1,
+                      "expert_gather", p, lanes);
   });
 }
 
@@ -380,12 +411,9 @@ int mb_expert_gather_quantize(int32_t dtype, int64_t tokens, int64_t k, int64_t 
   return by_float(dtype, [&](auto *tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     RouteParams p{};
-    p.T = tokens; p.H = cols; p.k = (int)k; p.position = position; p.kept = kept;
+    p.T = (int)tokens; p.H = (int)cols; p.k = (int)k; p.position = position; p.kept = kept;
     p.src = x; p.ld_src = ldx; p.dst = q; p.ld_dst = ldq; p.scale = scale;
-    constexpr int V = 16 / sizeof(T);
-    const bool vec = rows16(x, ldx, sizeof(T)) && cols % V == 0;
-    return launch_pdl(vec ? quantize_rows_kernel<T, V> : quantize_rows_kernel<T, 1>, dim3((unsigned)tokens), dim3(256),
-                      0, (cudaStream_t)stream, 1, "expert_gather_quantize", p);
+    return launch_quantize<T>(p, (cudaStream_t)stream, "expert_gather_quantize");
   });
 }
 
@@ -402,15 +430,15 @@ int mb_expert_combine(int32_t dtype, int32_t weights_dtype, int64_t tokens, int6
   return by_float(dtype, [&](auto *tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     RouteParams p{};
-    p.T = tokens; p.H = cols; p.k = (int)k; p.position = position; p.kept = kept;
+    p.T = (int)tokens; p.H = (int)cols; p.k = (int)k; p.position = position; p.kept = kept;
     p.src = sorted; p.ld_src = lds; p.w = weights; p.dst = out; p.ld_dst = ldo;
-    constexpr int V = 16 / sizeof(T);
-    const bool vec = rows16(sorted, lds, sizeof(T)) && rows16(out, ldo, sizeof(T)) && cols % V == 0;
-    const dim3 grid((unsigned)tokens, (unsigned)std::min<int64_t>(ceil_div(cols, 256 * (vec ? V : 1)), 16));
+    const bool al = rows16(sorted, lds, sizeof(T)) && rows16(out, ldo, sizeof(T));
+    const int lanes = route_lanes(cols, sizeof(T));
     const bool f32 = weights_dtype == MB_F32;
-    auto kern = vec ? (f32 ? expert_combine_kernel<T, float, V> : expert_combine_kernel<T, T, V>)
-                    : (f32 ? expert_combine_kernel<T, float, 1> : expert_combine_kernel<T, T, 1>);
-    return launch_pdl(kern, grid, dim3(256), 0, (cudaStream_t)stream, 1, "expert_combine", p);
+    auto kern = al ? (f32 ? expert_combine_kernel<T, float, true> : expert_combine_kernel<T, T, true>)
+                   : (f32 ? expert_combine_kernel<T, float, false> : expert_combine_kernel<T, T, false>);
+    return launch_pdl(kern, route_grid(tokens, cols, sizeof(T), lanes, false), dim3(kRouteThreads), 0,
+                      (cudaStream_t)stream, 1, "expert_combine", p, lanes);
   });
 }
 
@@ -430,17 +458,16 @@ int mb_expert_combine_backward(int32_t dtype, int32_t weights_dtype, int64_t tok
   return by_float(dtype, [&](auto *tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     RouteParams p{};
-    p.T = tokens; p.H = cols; p.k = (int)k; p.position = position; p.kept = kept;
+    p.T = (int)tokens; p.H = (int)cols; p.k = (int)k; p.position = position; p.kept = kept;
     p.src = dout; p.ld_src = ldd; p.src2 = sorted; p.ld_src2 = lds; p.w = weights;
     p.dst = dsorted; p.ld_dst = ldds; p.dst2 = dweights;
-    constexpr int V = 16 / sizeof(T);
-    const bool vec = rows16(dout, ldd, sizeof(T)) && rows16(sorted, lds, sizeof(T)) &&
-                     rows16(dsorted, ldds, sizeof(T)) && cols % V == 0;
+    const bool al = rows16(dout, ldd, sizeof(T)) && rows16(sorted, lds, sizeof(T)) && rows16(dsorted, ldds, sizeof(T));
+    const int lanes = route_lanes(cols, sizeof(T));
     const bool f32 = weights_dtype == MB_F32;
-    auto kern = vec ? (f32 ? expert_combine_backward_kernel<T, float, V> : expert_combine_backward_kernel<T, T, V>)
-                    : (f32 ? expert_combine_backward_kernel<T, float, 1> : expert_combine_backward_kernel<T, T, 1>);
-    return launch_pdl(kern, dim3((unsigned)tokens), dim3(256), 0, (cudaStream_t)stream, 1, "expert_combine_backward",
-                      p);
+    auto kern = al ? (f32 ? expert_combine_backward_kernel<T, float, true> : expert_combine_backward_kernel<T, T, true>)
+                   : (f32 ? expert_combine_backward_kernel<T, float, false> : expert_combine_backward_kernel<T, T, false>);
+    return launch_pdl(kern, route_grid(tokens, cols, sizeof(T), lanes, true), dim3(kRouteThreads), 0,
+                      (cudaStream_t)stream, 1, "expert_combine_backward", p, lanes);
   });
 }
 

@@ -15,29 +15,66 @@
 // shows NaN.  |q| <= 127 always.
 #pragma once
 #include "mb_common.cuh"
+#include "pack.cuh"
 
 namespace mb {
 
 template <class T> __device__ __forceinline__ float to_f32(T v) { return Elem<T>::load(v, false); }
 
-// V consecutive elements: one 16-byte load, or one element.
-template <class T, int V> struct Vec {
-  static_assert(V * sizeof(T) == 16, "16-byte vectors");
+// 16 bytes of a row.
+template <class T> struct Vec {
+  static constexpr int V = 16 / (int)sizeof(T);
   union { uint4 q; T t[V]; } u;
-  __device__ __forceinline__ void load(const T *p) { u.q = *reinterpret_cast<const uint4 *>(p); }
-  __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<uint4 *>(p) = u.q; }
-  __device__ __forceinline__ void zero() { u.q = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ Vec() {}
   __device__ __forceinline__ float f(int i) const { return to_f32(u.t[i]); }
   __device__ __forceinline__ void set(int i, float v) { u.t[i] = Elem<T>::store(v); }
+  __device__ __forceinline__ void zero() { u.q = make_uint4(0, 0, 0, 0); }
 };
-template <class T> struct Vec<T, 1> {
-  T t;
-  __device__ __forceinline__ void load(const T *p) { t = *p; }
-  __device__ __forceinline__ void store(T *p) const { *p = t; }
-  __device__ __forceinline__ void zero() { t = Elem<T>::store(0.f); }
-  __device__ __forceinline__ float f(int) const { return to_f32(t); }
-  __device__ __forceinline__ void set(int, float v) { t = Elem<T>::store(v); }
-};
+
+// Elements c .. c+V-1 of a row of H, zeros outside it.  AL: rows start on 16
+// bytes and c is a multiple of V.  Otherwise the 16 bytes are cut out of the
+// one or two aligned words that hold them: the second word is read only when it
+// holds some of them, so nothing past the row's last word is touched, and the
+// neighbouring thread's copy of it comes from L1.
+template <class T, bool AL>
+__device__ __forceinline__ Vec<T> load_vec(const T *row, int c, int H) {
+  constexpr int V = Vec<T>::V;
+  Vec<T> v;
+  if (c >= 0 && c + V <= H) {
+    if constexpr (AL) {
+      v.u.q = *reinterpret_cast<const uint4 *>(row + c);
+    } else {
+      const uintptr_t a = reinterpret_cast<uintptr_t>(row + c);
+      const uint32_t off = (uint32_t)(a & 15);
+      const uint4 *w = reinterpret_cast<const uint4 *>(a - off);
+      v.u.q = w[0];
+      if (off) v.u.q = bytes_at(v.u.q, w[1], off);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v.u.t[i] = (c + i >= 0 && c + i < H) ? row[c + i] : Elem<T>::store(0.f);
+  }
+  return v;
+}
+
+// The first column of a row's vectors: 0 when the row starts on 16 bytes, else
+// the column (<= 0) whose address does, so that whole vectors can be stored.
+template <class T, bool AL> __device__ __forceinline__ int frame(const T *row) {
+  if constexpr (AL) return 0;
+  return -(int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+}
+// Store to c .. c+V-1 (c on the row's frame), the part inside the row only.
+template <class T>
+__device__ __forceinline__ void store_vec(T *row, int c, int H, const Vec<T> &v) {
+  constexpr int V = Vec<T>::V;
+  if (c >= 0 && c + V <= H) {
+    *reinterpret_cast<uint4 *>(row + c) = v.u.q;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (c + i >= 0 && c + i < H) row[c + i] = v.u.t[i];
+  }
+}
 
 // |x| of a row as ordered bits: NaN above infinity above every finite value,
 // so an integer maximum never loses a NaN.
