@@ -209,8 +209,16 @@ def _bind_ops(lib) -> None:
         fn.argtypes, fn.restype = args, ctypes.c_int
 
 
+# What csrc/fastops.h calls, in its order.
+_FAST_OPS = ("mb_quantize", "mb_scaled_gemm", "mb_scaled_workspace_size", "mb_expert_sort", "mb_expert_gather",
+             "mb_expert_gather_quantize", "mb_expert_combine", "mb_expert_combine_backward")
 _fast = None
 _fast_tried = False
+
+
+def fast_op(name):
+    """A function of the host fast path's operators, or one that never serves a call."""
+    return getattr(fast(), name, None) or (lambda *a: None)
 
 
 def fast():
@@ -236,6 +244,8 @@ def fast():
                 raise RuntimeError("_mbfast was built against a different mb_gemm_desc; rebuild the package")
             fn = ctypes.cast(lib.mb_gemm, ctypes.c_void_p).value
             mod.set_gemm(fn)
+            if hasattr(mod, "set_ops") and hasattr(lib, "mb_scaled_gemm"):
+                mod.set_ops([ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _FAST_OPS])
         _fast = mod
         _fast_tried = True
         return _fast

@@ -3,7 +3,7 @@
 The library is two CUDA translation units, compiled side by side: ``csrc/mb_abi.cu``
 (the products of one element type) and ``csrc/mb_ops.cu`` (int8 products with scales,
 expert routing), exporting the C ABI declared in ``include/metalblas_b200.h``; a small torch C++ extension
-(``csrc/fastpath.cpp``) holds the per-thread descriptor cache of repeated calls.  It links the CUDA runtime statically
+(``csrc/fastpath.cpp``) holds the host fast paths.  The library links the CUDA runtime statically
 so it does not depend on which libcudart torch happened to load, and reaches the
 driver (for cuTensorMapEncodeTiled) through cudaGetDriverEntryPoint, so it needs
 no libcuda at link time.
@@ -115,7 +115,7 @@ def build_fastpath(force: bool = False, verbose: bool = False) -> str:
     import torch
     import torch.utils.cpp_extension as ce
     out = fast_lib_path()
-    srcs = [FAST_SRC, os.path.join(REPO, "include", "metalblas_b200.h"), __file__]
+    srcs = [*_units_of(FAST_SRC), __file__]
     if not force and os.path.exists(out) and all(os.path.getmtime(s) <= os.path.getmtime(out) for s in srcs):
         return out
     cuda_home = os.environ.get("CUDA_HOME", "/usr/local/cuda")

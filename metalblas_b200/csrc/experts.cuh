@@ -52,12 +52,12 @@ template <class I>
 __global__ void __launch_bounds__(1024) expert_sort_kernel(const SortParams p) {
   extern __shared__ int sm[];  // next[W][E + 1], total[E + 1], warp sums[32]
   const int W = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int B = p.E + 1;
+  const int B = p.E + 1, S = B | 1;  // an odd pitch spreads a column over the banks
   const int rank = blockIdx.x, ranks = gridDim.x;
-  int *total = sm + W * B, *sums = total + B;
-  int *h = sm + warp * B;
+  int *total = sm + W * S, *sums = total + B;
+  int *h = sm + warp * S;
   const I *ids = static_cast<const I *>(p.ids);
-  for (int i = threadIdx.x; i < W * B; i += blockDim.x) sm[i] = 0;
+  for (int i = threadIdx.x; i < W * S; i += blockDim.x) sm[i] = 0;
   pdl_trigger();
   pdl_wait();
   const int step = 32 * kSortBatch;
@@ -85,15 +85,18 @@ __global__ void __launch_bounds__(1024) expert_sort_kernel(const SortParams p) {
       if (e[b] >= 0) atomicAdd(h + e[b], 1);
   }
   __syncthreads();
-  // down the block: each cell becomes the number of that expert's entries in the warps before
-  for (int x = threadIdx.x; x < B; x += blockDim.x) {
-    int at = 0;
-    for (int w = 0; w < W; ++w) {
-      const int c = sm[w * B + x];
-      sm[w * B + x] = at;
-      at += c;
+  // down the block: each cell becomes the number of that expert's entries in the
+  // warps before (a warp scans a column, a lane per warp)
+  for (int x = warp; x < B; x += W) {
+    const int c = lane < W ? sm[lane * S + x] : 0;
+    int upto = c;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += o;
     }
-    total[x] = at;
+    if (lane < W) sm[lane * S + x] = upto - c;
+    if (lane == 31) total[x] = upto;
   }
   __syncthreads();
   if (ranks > 1)
@@ -173,20 +176,34 @@ struct RouteParams {
 // token, so that short rows still fill warps and long ones have a block; a
 // token's columns are shared out over blockIdx.y as well.
 constexpr int kRouteThreads = 256;
-constexpr int kEntries = 8;  // entries of a token worked on at a time
+// A token's entries are worked on NE (2 or 8) at a time: the rows of a batch are
+// in flight together, and a batch wider than k would be spent on nothing (k = 2
+// with batches of 8: combine 84 us, 2.4 TB/s, at 8192 tokens of 4096 bf16).
 
-// Slots of entries j0 .. j0+7 of token t: -1 for none (past k, or a number that
+// Slots of entries j0 .. j0+NE-1 of token t: -1 for none (past k, or a number that
 // is no row of the buffer).
-__device__ __forceinline__ void load_slots(const RouteParams &p, int t, int j0, int (&slot)[kEntries]) {
+template <int NE>
+__device__ __forceinline__ void load_slots(const RouteParams &p, int t, int j0, int (&slot)[NE]) {
   const int n = p.T * p.k;
 #pragma unroll
-  for (int j = 0; j < kEntries; ++j) {
+  for (int j = 0; j < NE; ++j) {
     const int s = j0 + j < p.k ? p.position[(int64_t)t * p.k + j0 + j] : -1;
     slot[j] = s < n ? s : -1;
   }
 }
 
-template <class T, bool AL>
+template <class T> __device__ __forceinline__ T *row_of(void *base, int64_t r, int64_t ld) {
+  return static_cast<T *>(base) + r * ld;
+}
+template <class T> __device__ __forceinline__ const T *row_of(const void *base, int64_t r, int64_t ld) {
+  return static_cast<const T *>(base) + r * ld;
+}
+
+// In the kernels below a vector that sticks out of its row (the row's end, or its
+// start where rows are not aligned) takes a plain loop over its elements, kept
+// apart so that the vectors inside are loaded without a branch between them.
+
+template <class T, int NE, bool AL>
 __global__ void __launch_bounds__(kRouteThreads) expert_gather_kernel(const RouteParams p, int lanes) {
   constexpr int V = Vec<T>::V;
   pdl_trigger();
@@ -194,31 +211,37 @@ __global__ void __launch_bounds__(kRouteThreads) expert_gather_kernel(const Rout
   const int t = blockIdx.x * (kRouteThreads / lanes) + threadIdx.x / lanes;
   if (t >= p.T) return;
   const int kept = p.kept ? *p.kept : 0;
-  const T *x = static_cast<const T *>(p.src) + t * p.ld_src;
+  const T *x = row_of<T>(p.src, t, p.ld_src);
   const int v0 = blockIdx.y * lanes + threadIdx.x % lanes, dv = gridDim.y * lanes;
-  for (int j0 = 0; j0 < p.k; j0 += kEntries) {
-    int slot[kEntries];
+  for (int j0 = 0; j0 < p.k; j0 += NE) {
+    int slot[NE];
     load_slots(p, t, j0, slot);
     for (int c = v0 * V; c < p.H + (AL ? 0 : V); c += dv * V) {
       Vec<T> v;
-      if constexpr (AL) v = load_vec<T, AL>(x, c, p.H);
+      const bool in = c + V <= p.H;
+      if (AL && in) v = load16<T, AL>(x + c);
 #pragma unroll
-      for (int j = 0; j < kEntries; ++j) {
+      for (int j = 0; j < NE; ++j) {
         if (slot[j] < 0) continue;
-        T *d = static_cast<T *>(p.dst) + slot[j] * p.ld_dst;
+        T *d = row_of<T>(p.dst, slot[j], p.ld_dst);
         const int cc = c + frame<T, AL>(d);
-        if constexpr (!AL) v = load_vec<T, AL>(x, cc, p.H);
-        Vec<T> o = v;
-        if (slot[j] >= kept) o.zero();
-        store_vec(d, cc, p.H, o);
+        if (AL ? in : (cc >= 0 && cc + V <= p.H)) {
+          if constexpr (!AL) v = load16<T, AL>(x + cc);
+          Vec<T> o = v;
+          if (slot[j] >= kept) o.zero();
+          *reinterpret_cast<uint4 *>(d + cc) = o.u.q;
+        } else {
+#pragma unroll 1
+          for (int i = max(cc, 0); i < min(cc + V, p.H); ++i) d[i] = slot[j] < kept ? x[i] : Elem<T>::store(0.f);
+        }
       }
     }
   }
 }
 
-// The k rows of a token are fetched together (eight 16-byte loads in flight per
+// The rows of a token are fetched together (NE 16-byte loads in flight per
 // thread) and summed in order.
-template <class T, class TW, bool AL>
+template <class T, class TW, int NE, bool AL>
 __global__ void __launch_bounds__(kRouteThreads) expert_combine_kernel(const RouteParams p, int lanes) {
   constexpr int V = Vec<T>::V;
   pdl_trigger();
@@ -227,102 +250,175 @@ __global__ void __launch_bounds__(kRouteThreads) expert_combine_kernel(const Rou
   if (t >= p.T) return;
   const int kept = p.kept ? *p.kept : 0;
   const TW *w = static_cast<const TW *>(p.w);
-  T *out = static_cast<T *>(p.dst) + t * p.ld_dst;
+  T *out = row_of<T>(p.dst, t, p.ld_dst);
   const int c0 = frame<T, AL>(out);
   const int v0 = blockIdx.y * lanes + threadIdx.x % lanes, dv = gridDim.y * lanes;
-  for (int c = c0 + v0 * V; c < p.H; c += dv * V) {
-    float acc[V];
+  int slot[NE];
+  float wj[NE];
+  auto entries = [&](int j0) {
+    load_slots(p, t, j0, slot);
 #pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] = 0.f;
-    for (int j0 = 0; j0 < p.k; j0 += kEntries) {
-      int slot[kEntries];
-      float wj[kEntries];
-      load_slots(p, t, j0, slot);
-      Vec<T> v[kEntries];
-#pragma unroll
-      for (int j = 0; j < kEntries; ++j) {
-        const bool live = slot[j] >= 0 && slot[j] < kept;
-        wj[j] = live ? (w ? to_f32(w[(int64_t)t * p.k + j0 + j]) : 1.f) : 0.f;
-        if (live) v[j] = load_vec<T, AL>(static_cast<const T *>(p.src) + slot[j] * p.ld_src, c, p.H);
-        else v[j].zero();
-      }
-#pragma unroll
-      for (int j = 0; j < kEntries; ++j)
-#pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = fmaf(wj[j], v[j].f(i), acc[i]);
+    for (int j = 0; j < NE; ++j) {
+      if (slot[j] >= kept) slot[j] = -1;
+      wj[j] = slot[j] < 0 ? 0.f : w ? to_f32(w[(int64_t)t * p.k + j0 + j]) : 1.f;
     }
-    Vec<T> o;
+  };
+  if (p.k <= NE) entries(0);
+  for (int c = c0 + v0 * V; c < p.H; c += dv * V) {
+    if (c >= 0 && c + V <= p.H) {
+      float acc[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) o.set(i, acc[i]);
-    store_vec(out, c, p.H, o);
+      for (int i = 0; i < V; ++i) acc[i] = 0.f;
+      for (int j0 = 0; j0 < p.k; j0 += NE) {
+        if (p.k > NE) entries(j0);
+        Vec<T> v[NE];
+#pragma unroll
+        for (int j = 0; j < NE; ++j) {
+          v[j].zero();
+          if (slot[j] >= 0) v[j] = load16<T, AL>(row_of<T>(p.src, slot[j], p.ld_src) + c);
+        }
+#pragma unroll
+        for (int j = 0; j < NE; ++j)
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[i] = fmaf(wj[j], v[j].f(i), acc[i]);
+      }
+      Vec<T> o;
+#pragma unroll
+      for (int i = 0; i < V; ++i) o.set(i, acc[i]);
+      *reinterpret_cast<uint4 *>(out + c) = o.u.q;
+    } else {
+#pragma unroll 1
+      for (int i = max(c, 0); i < min(c + V, p.H); ++i) {
+        float acc = 0.f;
+        for (int j = 0; j < p.k; ++j) {
+          const int s = p.position[(int64_t)t * p.k + j];
+          if (s < 0 || s >= kept || s >= p.T * p.k) continue;
+          acc = fmaf(w ? to_f32(w[(int64_t)t * p.k + j]) : 1.f, to_f32(row_of<T>(p.src, s, p.ld_src)[i]), acc);
+        }
+        out[i] = Elem<T>::store(acc);
+      }
+    }
   }
 }
 
 // src = dout, src2 = y, dst = dy, dst2 = dw.  A token's lanes see its whole rows
-// (blockIdx.y unused), so that the dot products are summed here.
-template <class T, class TW, bool AL>
+// (blockIdx.y unused), so that the dot products are summed here: by thread along
+// the row, then over lanes and warps in a fixed order.  With aligned rows dout is
+// read once for the NE entries of a batch; otherwise every entry has a vector
+// frame of its own (its row of dy's) and is worked on alone.
+template <class T, class TW, int NE, bool AL>
 __global__ void __launch_bounds__(kRouteThreads) expert_combine_backward_kernel(const RouteParams p, int lanes) {
   constexpr int V = Vec<T>::V;
-  __shared__ float part[kRouteThreads / 32][kEntries];
+  __shared__ float part[kRouteThreads / 32][NE];
   pdl_trigger();
   pdl_wait();
   const int per = kRouteThreads / lanes, tb = threadIdx.x / lanes, tl = threadIdx.x % lanes;
   const int t = blockIdx.x * per + tb;
   const int kept = p.kept ? *p.kept : 0;
   const TW *w = static_cast<const TW *>(p.w);
-  const T *dout = static_cast<const T *>(p.src) + t * p.ld_src;
-  for (int j0 = 0; j0 < p.k; j0 += kEntries) {
-    int slot[kEntries];
-    float wj[kEntries], dot[kEntries];
-#pragma unroll
-    for (int j = 0; j < kEntries; ++j) {
-      slot[j] = -1;
-      dot[j] = 0.f;
+  const T *dout = row_of<T>(p.src, t, p.ld_src);
+  // one entry's elements i0 .. i1-1, one at a time; their share of its dot product
+  auto by_element = [&](int s, float ws, int i0, int i1) {
+    float sum = 0.f;
+    T *dy = row_of<T>(p.dst, s, p.ld_dst);
+    const T *y = row_of<T>(p.src2, s, p.ld_src2);
+#pragma unroll 1
+    for (int i = i0; i < i1; ++i) {
+      const float d = to_f32(dout[i]);
+      dy[i] = Elem<T>::store(s < kept ? ws * d : 0.f);
+      if (s < kept) sum = fmaf(d, to_f32(y[i]), sum);
     }
-    if (t < p.T) {
-      load_slots(p, t, j0, slot);
+    return sum;
+  };
+  auto warp_sum = [](float v) {
 #pragma unroll
-      for (int j = 0; j < kEntries; ++j)
-        wj[j] = slot[j] >= 0 && slot[j] < kept ? to_f32(w[(int64_t)t * p.k + j0 + j]) : 0.f;
-      for (int c = tl * V; c < p.H + (AL ? 0 : V); c += lanes * V) {
-        Vec<T> d, y[kEntries];
-        if constexpr (AL) d = load_vec<T, AL>(dout, c, p.H);
+    for (int m = 16; m; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+    return v;
+  };
+  for (int j0 = 0; j0 < p.k; j0 += NE) {
+    int slot[NE];
+    float wj[NE];
 #pragma unroll
-        for (int j = 0; j < kEntries; ++j) {
-          if (slot[j] >= 0 && slot[j] < kept) {
-            const int cc = c + frame<T, AL>(static_cast<T *>(p.dst) + slot[j] * p.ld_dst);
-            y[j] = load_vec<T, AL>(static_cast<const T *>(p.src2) + slot[j] * p.ld_src2, cc, p.H);
-          } else {
-            y[j].zero();
-          }
-        }
+    for (int j = 0; j < NE; ++j) slot[j] = -1;
+    if (t < p.T) load_slots(p, t, j0, slot);
 #pragma unroll
-        for (int j = 0; j < kEntries; ++j) {
-          if (slot[j] < 0) continue;
-          T *dy = static_cast<T *>(p.dst) + slot[j] * p.ld_dst;
-          const int cc = c + frame<T, AL>(dy);
-          Vec<T> o;
-          o.zero();
-          if (slot[j] < kept) {
-            if constexpr (!AL) d = load_vec<T, AL>(dout, cc, p.H);
+    for (int j = 0; j < NE; ++j)
+      wj[j] = slot[j] >= 0 && slot[j] < kept ? to_f32(w[(int64_t)t * p.k + j0 + j]) : 0.f;
+    if constexpr (AL) {
+      float dot[NE];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-              dot[j] = fmaf(d.f(i), y[j].f(i), dot[j]);
-              o.set(i, wj[j] * d.f(i));
+      for (int j = 0; j < NE; ++j) dot[j] = 0.f;
+      if (t < p.T) {
+        for (int c = tl * V; c < p.H; c += lanes * V) {
+          if (c + V <= p.H) {
+            const Vec<T> d = load16<T, AL>(dout + c);
+            Vec<T> y[NE];
+#pragma unroll
+            for (int j = 0; j < NE; ++j) {
+              y[j].zero();
+              if (slot[j] >= 0 && slot[j] < kept) y[j] = load16<T, AL>(row_of<T>(p.src2, slot[j], p.ld_src2) + c);
             }
+#pragma unroll
+            for (int j = 0; j < NE; ++j) {
+              if (slot[j] < 0) continue;
+              Vec<T> o;
+              o.zero();
+              if (slot[j] < kept) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                  dot[j] = fmaf(d.f(i), y[j].f(i), dot[j]);
+                  o.set(i, wj[j] * d.f(i));
+                }
+              }
+              *reinterpret_cast<uint4 *>(row_of<T>(p.dst, slot[j], p.ld_dst) + c) = o.u.q;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < NE; ++j)
+              if (slot[j] >= 0) dot[j] += by_element(slot[j], wj[j], c, p.H);
           }
-          store_vec(dy, cc, p.H, o);
         }
       }
-    }
 #pragma unroll
-    for (int j = 0; j < kEntries; ++j) {
+      for (int j = 0; j < NE; ++j) {
+        dot[j] = warp_sum(dot[j]);
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5][j] = dot[j];
+      }
+    } else {
+#pragma unroll 1
+      for (int j = 0; j < NE; ++j) {
+        const int s = t < p.T && j0 + j < p.k ? p.position[(int64_t)t * p.k + j0 + j] : -1;
+        float dot = 0.f;
+        if (s >= 0 && s < p.T * p.k) {
+          T *dy = row_of<T>(p.dst, s, p.ld_dst);
+          const T *y = row_of<T>(p.src2, s, p.ld_src2);
+          const float ws = s < kept ? to_f32(w[(int64_t)t * p.k + j0 + j]) : 0.f;
+          const int c0 = frame<T, AL>(dy);
+#pragma unroll 2
+          for (int c = c0 + tl * V; c < p.H; c += lanes * V) {
+            if (c >= 0 && c + V <= p.H) {
+              Vec<T> o;
+              o.zero();
+              if (s < kept) {
+                const Vec<T> d = load16<T, AL>(dout + c), yv = load16<T, AL>(y + c);
 #pragma unroll
-      for (int m = 16; m; m >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], m);
-      if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5][j] = dot[j];
+                for (int i = 0; i < V; ++i) {
+                  dot = fmaf(d.f(i), yv.f(i), dot);
+                  o.set(i, ws * d.f(i));
+                }
+              }
+              *reinterpret_cast<uint4 *>(dy + c) = o.u.q;
+            } else {
+              dot += by_element(s, ws, max(c, 0), min(c + V, p.H));
+            }
+          }
+        }
+        dot = warp_sum(dot);
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5][j] = dot;
+      }
     }
     __syncthreads();
-    if (t < p.T && tl < kEntries && j0 + tl < p.k) {
+    if (t < p.T && tl < NE && j0 + tl < p.k) {
       float sum = 0.f;
       for (int i = 0; i < lanes / 32; ++i) sum += part[tb * (lanes / 32) + i][tl];
       static_cast<TW *>(p.dst2)[(int64_t)t * p.k + j0 + tl] = Elem<TW>::store(sum);
@@ -334,10 +430,12 @@ __global__ void __launch_bounds__(kRouteThreads) expert_combine_backward_kernel(
 // Rows to int8 (see quantize.cuh): row t of src goes to the k slots of token t,
 // or, with position == null, to row t.  TPR threads hold a row's vectors, up to
 // HELD each, in registers between the maximum and the rounding; longer rows are
-// read again (from L2).
+// read again (from L2).  Two vectors a thread and at most 32 registers keep 2048
+// threads, 64 KB of loads, on an SM: with four the compiler took 80 registers and
+// 512-thread blocks ran one to an SM (16384 x 8192 bf16: 174 us).
 template <class T, bool AL, int TPR>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) quantize_rows_kernel(const RouteParams p, int q_vec) {
-  constexpr int V = Vec<T>::V, HELD = 4, THREADS = TPR < 256 ? 256 : TPR;
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, 2048 / (TPR < 256 ? 256 : TPR)) quantize_rows_kernel(const RouteParams p, int q_vec) {
+  constexpr int V = Vec<T>::V, HELD = 2, THREADS = TPR < 256 ? 256 : TPR;
   __shared__ uint32_t part[THREADS / 32];
   pdl_trigger();
   pdl_wait();
@@ -374,8 +472,10 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) quantize_rows_kernel(co
   const int kept = p.kept ? *p.kept : 0, k = p.position ? p.k : 1;
   auto put = [&](int c, const Vec<T> &a) {
     union { int8_t b[V]; uint32_t w[V / 4]; } q;
+    float f[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) q.b[i] = rq.dead ? 0 : (int8_t)rq.q(a.f(i));
+    for (int i = 0; i < V; ++i) f[i] = a.f(i);
+    rq.q(f, q.w);
     for (int j = 0; j < k; ++j) {
       int64_t s = t;
       bool zero = false;

@@ -21,6 +21,7 @@
 #include <unordered_map>
 
 #include "../../include/metalblas_b200.h"
+#include "fastops.h"
 
 namespace {
 
@@ -182,4 +183,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("try_mm_new", &try_mm_new);
   m.def("try_bmm_new", &try_bmm_new);
   m.def("desc_size", &desc_size);
+  fastops::bind(m);
 }

@@ -6,6 +6,7 @@
 #include <atomic>
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 #include "mb_host.cuh"
 #include "mb_common.cuh"
@@ -64,8 +65,11 @@ int route_lanes(int64_t H, int esz) {
   return vecs <= 64 ? 32 : vecs <= 512 ? 128 : 256;
 }
 dim3 route_grid(int64_t T, int64_t H, int esz, int lanes, bool whole_rows) {
-  const int64_t y = whole_rows ? 1 : std::min<int64_t>(ceil_div(ceil_div(H * esz, 16) + 1, lanes), 64);
-  return dim3((unsigned)ceil_div(T, kRouteThreads / lanes), (unsigned)y);
+  const int64_t x = ceil_div(T, kRouteThreads / lanes);
+  // with few tokens a row is shared out as far as its vectors go
+  int64_t y = whole_rows ? 1 : std::min<int64_t>(ceil_div(ceil_div(H * esz, 16) + 1, lanes), 64);
+  y = std::min<int64_t>(y, std::max<int64_t>(1, ceil_div(16 * (int64_t)device_sms(), x)));
+  return dim3((unsigned)x, (unsigned)y);
 }
 
 template <class T>
@@ -73,15 +77,17 @@ int launch_quantize(const RouteParams &p, cudaStream_t st, const char *what) {
   constexpr int V = Vec<T>::V;
   const bool al = rows16(p.src, p.ld_src, sizeof(T));
   const int q_vec = reinterpret_cast<uintptr_t>(p.dst) % V == 0 && p.ld_dst % V == 0;
-  // up to four vectors of a row per thread stay in registers
+  // up to two vectors of a row per thread stay in registers
   const int64_t vecs = ceil_div(p.H, V);
-  auto go = [&](auto kern, int tpr) {
-    const int threads = std::max(tpr, 256);
-    return launch_pdl(kern, dim3((unsigned)ceil_div(p.T, threads / tpr)), dim3(threads), 0, st, 1, what, p, q_vec);
+  auto go = [&](auto tpr_) {
+    constexpr int TPR = decltype(tpr_)::value, threads = TPR < 256 ? 256 : TPR;
+    auto kern = al ? quantize_rows_kernel<T, true, TPR> : quantize_rows_kernel<T, false, TPR>;
+    return launch_pdl(kern, dim3((unsigned)ceil_div(p.T, threads / TPR)), dim3(threads), 0, st, 1, what, p, q_vec);
   };
-  if (vecs <= 128) return al ? go(quantize_rows_kernel<T, true, 32>, 32) : go(quantize_rows_kernel<T, false, 32>, 32);
-  if (vecs <= 512) return al ? go(quantize_rows_kernel<T, true, 128>, 128) : go(quantize_rows_kernel<T, false, 128>, 128);
-  return al ? go(quantize_rows_kernel<T, true, 512>, 512) : go(quantize_rows_kernel<T, false, 512>, 512);
+  if (vecs <= 64) return go(std::integral_constant<int, 32>());
+  if (vecs <= 256) return go(std::integral_constant<int, 128>());
+  if (vecs <= 512) return go(std::integral_constant<int, 256>());
+  return vecs <= 1024 ? go(std::integral_constant<int, 512>()) : go(std::integral_constant<int, 1024>());
 }
 
 // ------------------------------------------------------------- int8 products with scales
@@ -363,13 +369,14 @@ int mb_expert_sort(int32_t ids64, int64_t n, int64_t experts, const void *ids, i
     return fail(MB_ERR_INVALID, "expert_sort: %lld experts (1 to %d)", (long long)experts, kMaxExperts);
   if (!offsets || (n > 0 && (!ids || !order || !position))) return fail(MB_ERR_INVALID, "expert_sort: null pointer");
   SortParams p{ids, (int)n, (int)experts, order, position, offsets};
-  // a warp per 256 entries (what its lanes hold at once), a thread per expert
-  // for the scan, and a cluster of blocks past 8192 entries
-  const int W = (int)std::max<int64_t>(std::min<int64_t>(32, ceil_div(n, 32 * kSortBatch)), ceil_div(experts, 32));
+  // A warp per 32 entries up to a block's 32 warps and a cluster of 8 blocks (the
+  // scattered stores of `order` bind one SM: 8000 entries on one block 11.4 us),
+  // and a thread per expert for the scan.
+  const int W = (int)std::max<int64_t>(std::min<int64_t>(32, ceil_div(n, 32)), ceil_div(experts, 32));
   int ranks = 1;
-  while (ranks < 8 && n > (int64_t)ranks * 32 * 32 * kSortBatch) ranks *= 2;
+  while (ranks < 8 && n > (int64_t)ranks * 1024) ranks *= 2;
   const int threads = std::min(W, 32) * 32;
-  const size_t smem = ((size_t)(threads / 32 + 1) * (experts + 1) + 32) * 4;
+  const size_t smem = ((size_t)(threads / 32) * ((experts + 1) | 1) + experts + 1 + 32) * 4;
   auto kern = ids64 ? expert_sort_kernel<long long> : expert_sort_kernel<int>;
   if (smem > 48 * 1024) {
     const int rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
@@ -393,7 +400,9 @@ int mb_expert_gather(int32_t dtype, int64_t tokens, int64_t k, int64_t cols, con
     p.src = x; p.ld_src = ldx; p.dst = sorted; p.ld_dst = lds;
     const bool al = rows16(x, ldx, sizeof(T)) && rows16(sorted, lds, sizeof(T));
     const int lanes = route_lanes(cols, sizeof(T));
-    return launch_pdl(al ? expert_gather_kernel<T, true> : expert_gather_kernel<T, false>,
+    auto kern = k <= 2 ? (al ? expert_gather_kernel<T, 2, true> : expert_gather_kernel<T, 2, false>)
+                       : (al ? expert_gather_kernel<T, 8, true> : expert_gather_kernel<T, 8, false>);
+    return launch_pdl(kern,
                       route_grid(tokens, cols, sizeof(T), lanes, false), dim3(kRouteThreads), 0, (cudaStream_t)stream, 1,
                       "expert_gather", p, lanes);
   });
@@ -435,8 +444,12 @@ int mb_expert_combine(int32_t dtype, int32_t weights_dtype, int64_t tokens, int6
     const bool al = rows16(sorted, lds, sizeof(T)) && rows16(out, ldo, sizeof(T));
     const int lanes = route_lanes(cols, sizeof(T));
     const bool f32 = weights_dtype == MB_F32;
-    auto kern = al ? (f32 ? expert_combine_kernel<T, float, true> : expert_combine_kernel<T, T, true>)
-                   : (f32 ? expert_combine_kernel<T, float, false> : expert_combine_kernel<T, T, false>);
+    auto pick = [&](auto ne) {
+      constexpr int NE = decltype(ne)::value;
+      return al ? (f32 ? expert_combine_kernel<T, float, NE, true> : expert_combine_kernel<T, T, NE, true>)
+                : (f32 ? expert_combine_kernel<T, float, NE, false> : expert_combine_kernel<T, T, NE, false>);
+    };
+    auto kern = k <= 2 ? pick(std::integral_constant<int, 2>()) : pick(std::integral_constant<int, 8>());
     return launch_pdl(kern, route_grid(tokens, cols, sizeof(T), lanes, false), dim3(kRouteThreads), 0,
                       (cudaStream_t)stream, 1, "expert_combine", p, lanes);
   });
@@ -464,8 +477,12 @@ int mb_expert_combine_backward(int32_t dtype, int32_t weights_dtype, int64_t tok
     const bool al = rows16(dout, ldd, sizeof(T)) && rows16(sorted, lds, sizeof(T)) && rows16(dsorted, ldds, sizeof(T));
     const int lanes = route_lanes(cols, sizeof(T));
     const bool f32 = weights_dtype == MB_F32;
-    auto kern = al ? (f32 ? expert_combine_backward_kernel<T, float, true> : expert_combine_backward_kernel<T, T, true>)
-                   : (f32 ? expert_combine_backward_kernel<T, float, false> : expert_combine_backward_kernel<T, T, false>);
+    auto pick = [&](auto ne) {
+      constexpr int NE = decltype(ne)::value;
+      return al ? (f32 ? expert_combine_backward_kernel<T, float, NE, true> : expert_combine_backward_kernel<T, T, NE, true>)
+                : (f32 ? expert_combine_backward_kernel<T, float, NE, false> : expert_combine_backward_kernel<T, T, NE, false>);
+    };
+    auto kern = k <= 2 ? pick(std::integral_constant<int, 2>()) : pick(std::integral_constant<int, 8>());
     return launch_pdl(kern, route_grid(tokens, cols, sizeof(T), lanes, true), dim3(kRouteThreads), 0,
                       (cudaStream_t)stream, 1, "expert_combine_backward", p, lanes);
   });

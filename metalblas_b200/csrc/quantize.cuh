@@ -15,7 +15,6 @@
 // shows NaN.  |q| <= 127 always.
 #pragma once
 #include "mb_common.cuh"
-#include "pack.cuh"
 
 namespace mb {
 
@@ -31,29 +30,42 @@ template <class T> struct Vec {
   __device__ __forceinline__ void zero() { u.q = make_uint4(0, 0, 0, 0); }
 };
 
-// Elements c .. c+V-1 of a row of H, zeros outside it.  AL: rows start on 16
-// bytes and c is a multiple of V.  Otherwise the 16 bytes are cut out of the
-// one or two aligned words that hold them: the second word is read only when it
-// holds some of them, so nothing past the row's last word is touched, and the
-// neighbouring thread's copy of it comes from L1.
+// 16 bytes starting `off` bytes into the 32 bytes a:b, without branches.
+__device__ __forceinline__ uint4 cut16(const uint4 &a, const uint4 &b, uint32_t off) {
+  const bool two = off & 8, one = off & 4;
+  const uint32_t x0 = two ? a.z : a.x, x1 = two ? a.w : a.y, x2 = two ? b.x : a.z, x3 = two ? b.y : a.w,
+                 x4 = two ? b.z : b.x, x5 = two ? b.w : b.y;
+  const uint32_t y0 = one ? x1 : x0, y1 = one ? x2 : x1, y2 = one ? x3 : x2, y3 = one ? x4 : x3, y4 = one ? x5 : x4;
+  const uint32_t sh = (off & 3) * 8;
+  return make_uint4(__funnelshift_r(y0, y1, sh), __funnelshift_r(y1, y2, sh), __funnelshift_r(y2, y3, sh),
+                    __funnelshift_r(y3, y4, sh));
+}
+
+// The V elements at p.  AL: on a 16-byte boundary.  Otherwise they are cut out of
+// the one or two aligned words that hold them: the second word is read only
+// when it holds some of them, so no word without an element of the row is
+// touched, and the neighbouring thread's copy of it comes from L1.
+template <class T, bool AL>
+__device__ __forceinline__ Vec<T> load16(const T *p) {
+  Vec<T> v;
+  if constexpr (AL) {
+    v.u.q = *reinterpret_cast<const uint4 *>(p);
+  } else {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+    const uint32_t off = (uint32_t)(a & 15);
+    const uint4 *w = reinterpret_cast<const uint4 *>(a - off);
+    v.u.q = cut16(w[0], w[off ? 1 : 0], off);
+  }
+  return v;
+}
+// Elements c .. c+V-1 of a row of H, zeros outside it.
 template <class T, bool AL>
 __device__ __forceinline__ Vec<T> load_vec(const T *row, int c, int H) {
   constexpr int V = Vec<T>::V;
+  if (c >= 0 && c + V <= H) return load16<T, AL>(row + c);
   Vec<T> v;
-  if (c >= 0 && c + V <= H) {
-    if constexpr (AL) {
-      v.u.q = *reinterpret_cast<const uint4 *>(row + c);
-    } else {
-      const uintptr_t a = reinterpret_cast<uintptr_t>(row + c);
-      const uint32_t off = (uint32_t)(a & 15);
-      const uint4 *w = reinterpret_cast<const uint4 *>(a - off);
-      v.u.q = w[0];
-      if (off) v.u.q = bytes_at(v.u.q, w[1], off);
-    }
-  } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) v.u.t[i] = (c + i >= 0 && c + i < H) ? row[c + i] : Elem<T>::store(0.f);
-  }
+  for (int i = 0; i < V; ++i) v.u.t[i] = (c + i >= 0 && c + i < H) ? row[c + i] : Elem<T>::store(0.f);
   return v;
 }
 
@@ -62,18 +74,6 @@ __device__ __forceinline__ Vec<T> load_vec(const T *row, int c, int H) {
 template <class T, bool AL> __device__ __forceinline__ int frame(const T *row) {
   if constexpr (AL) return 0;
   return -(int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
-}
-// Store to c .. c+V-1 (c on the row's frame), the part inside the row only.
-template <class T>
-__device__ __forceinline__ void store_vec(T *row, int c, int H, const Vec<T> &v) {
-  constexpr int V = Vec<T>::V;
-  if (c >= 0 && c + V <= H) {
-    *reinterpret_cast<uint4 *>(row + c) = v.u.q;
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (c + i >= 0 && c + i < H) row[c + i] = v.u.t[i];
-  }
 }
 
 // |x| of a row as ordered bits: NaN above infinity above every finite value,
@@ -91,17 +91,35 @@ struct RowQuant {
     // a row whose 127 x or 127 / amax would leave fp32's range is moved by a
     // power of two first (exact, and the same for x and amax)
     pre = m > 0x1p120f ? 0x1p-64f : (m < 0x1p-100f ? 0x1p64f : 1.f);
-    amax = m * pre;
-    inv = __fdiv_rn(127.f, amax);
+    amax = dead ? 1.f : m * pre;
+    inv = dead ? 0.f : __fdiv_rn(127.f, amax);
   }
-  __device__ __forceinline__ int q(float x) const {
-    // x * inv is within 2e-5 of the quotient (two roundings of a value <= 127);
-    // only a result that near to a half needs the quotient itself.
-    x *= pre;
-    const float t = x * inv;
-    float r = rintf(t);
-    if (fabsf(t - r) > 0.4999f) r = rintf(__fdiv_rn(x * 127.f, amax));
-    return (int)r;
+  // N elements at once.  x * inv is within 2e-5 of the quotient (two roundings
+  // of a value of at most 127), so only a result that near to a half needs the
+  // quotient itself: it is looked for once per N elements, and found for about
+  // one element in 25000.  Adding 1.5 * 2^23 rounds to an integer, halves to
+  // even, and leaves it in the low bits; conversions run at a quarter of that
+  // rate or less, and bf16 rows were bound by them (2.6 TB/s at 16384 x 8192).
+  template <int N>
+  __device__ __forceinline__ void q(const float (&x)[N], uint32_t (&out)[N / 4]) const {
+    constexpr float kMagic = 12582912.f;
+    float r[N], worst = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float t = x[i] * pre * inv;
+      r[i] = t + kMagic;
+      worst = fmaxf(worst, fabsf(t - (r[i] - kMagic)));
+    }
+    if (worst > 0.49997f) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) r[i] = __fdiv_rn(x[i] * pre * 127.f, amax) + kMagic;
+    }
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint32_t lo = __byte_perm(__float_as_uint(r[4 * i]), __float_as_uint(r[4 * i + 1]), 0x0040);
+      const uint32_t hi = __byte_perm(__float_as_uint(r[4 * i + 2]), __float_as_uint(r[4 * i + 3]), 0x0040);
+      out[i] = dead ? 0u : __byte_perm(lo, hi, 0x5410);
+    }
   }
 };
 

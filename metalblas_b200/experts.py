@@ -21,10 +21,17 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .dispatch import FLOATS, _stream_of
+from .dispatch import FLOATS, _plain, _stream_of
 from .quantized import _int8_rows, _ld, _on_device, _rows
 
 MAX_EXPERTS = 1024
+
+# The host fast path (csrc/fastops.h): the result of a plain call, or None.
+_try_sort = _lib.fast_op("try_sort")
+_try_gather = _lib.fast_op("try_gather")
+_try_gather_quantize = _lib.fast_op("try_gather_quantize")
+_try_combine = _lib.fast_op("try_combine")
+_try_combine_backward = _lib.fast_op("try_combine_backward")
 
 
 class ExpertOrder(NamedTuple):
@@ -40,10 +47,15 @@ class ExpertOrder(NamedTuple):
     offsets: torch.Tensor
 
 
-@_on_device
 def expert_sort(experts, num_experts):
     """``ExpertOrder`` of ``experts [T, k]`` (int32 or int64): entries by expert, those of one
     expert in their own order; numbers outside ``0 .. num_experts-1`` mark dropped entries."""
+    fast = _try_sort(experts, num_experts)
+    return ExpertOrder(*fast) if fast is not None else _sort(experts, num_experts)
+
+
+@_on_device
+def _sort(experts, num_experts):
     if experts.dtype not in (torch.int32, torch.int64):
         raise NotImplementedError(f"expert numbers must be int32 or int64, got {experts.dtype}")
     assert experts.dim() == 2, f"experts must be [tokens, k], got {tuple(experts.shape)}"
@@ -81,13 +93,14 @@ def _check_weights(weights, pos, dtype):
         f"weights have shape {tuple(weights.shape)}, expected {tuple(pos.shape)}"
     if weights.dtype is not dtype and weights.dtype is not torch.float32:
         raise NotImplementedError(f"weights must be {dtype} or fp32, got {weights.dtype}")
-    return weights.contiguous()
+    return _plain(weights).contiguous()
 
 
 def _kept(off):
     return off.data_ptr() + 4 * (off.numel() - 1)
 
 
+@_on_device
 def _gather(x, order):
     assert x.dim() == 2, f"x must be [T, cols], got {tuple(x.shape)}"
     pos, off = _check_order(order, x.device)
@@ -101,6 +114,7 @@ def _gather(x, order):
     return out
 
 
+@_on_device
 def _combine(rows, weights, order):
     assert rows.dim() == 2, f"rows must be [T * k, cols], got {tuple(rows.shape)}"
     pos, off = _check_order(order, rows.device)
@@ -143,24 +157,30 @@ class _Combine(torch.autograd.Function):
         return (*expert_combine_backward(grad, rows, weights, ExpertOrder(*order)), None, None, None)
 
 
-@_on_device
 def expert_gather(x, order):
     """The rows of ``x [T, cols]`` in ``order``: ``[T * k, cols]``, zero rows for dropped entries."""
+    out = _try_gather(x, order.position, order.offsets)
+    if out is not None:
+        return out
     if x.requires_grad and torch.is_grad_enabled():
         return _Gather.apply(x, *order)
     return _gather(x, order)
 
 
-@_on_device
 def expert_gather_backward(grad, order):
     """Gradient of ``expert_gather`` by x: each token's rows of ``grad [T * k, cols]`` summed."""
-    return _combine(grad, None, order)
+    out = _try_combine(grad, None, order.position, order.offsets)
+    return out if out is not None else _combine(grad, None, order)
 
 
-@_on_device
 def expert_gather_quantize(x, order):
     """``quantize(expert_gather(x, order))`` without the rows in between: int8 ``[T * k, cols]``
     and fp32 ``[T * k]``; dropped entries have q 0 and scale 0."""
+    return _try_gather_quantize(x, order.position, order.offsets) or _gather_quantize(x, order)
+
+
+@_on_device
+def _gather_quantize(x, order):
     assert x.dim() == 2, f"x must be [T, cols], got {tuple(x.shape)}"
     pos, off = _check_order(order, x.device)
     T, k = pos.shape
@@ -175,11 +195,13 @@ def expert_gather_quantize(x, order):
     return q, scale
 
 
-@_on_device
 def expert_combine(rows, weights, order):
     """``out[t] = sum_j weights[t, j] * rows[position[t, j]]``: ``[T, cols]`` from the experts'
     ``rows [T * k, cols]``, dropped entries left out, summed in fp32 in the order of j.
     ``weights [T, k]`` have the rows' type or fp32; None stands for ones."""
+    out = _try_combine(rows, weights, order.position, order.offsets)
+    if out is not None:
+        return out
     if torch.is_grad_enabled():
         if weights is None:
             if rows.requires_grad:
@@ -190,11 +212,16 @@ def expert_combine(rows, weights, order):
     return _combine(rows, weights, order)
 
 
-@_on_device
 def expert_combine_backward(grad, rows, weights, order):
     """Gradients of ``expert_combine`` by rows and by weights: ``drows[position[t, j]] =
     weights[t, j] * grad[t]`` (zero for dropped entries) and ``dweights[t, j] = <grad[t],
     rows[position[t, j]]>`` (zero likewise), in the types of rows and weights."""
+    return _try_combine_backward(grad, rows, weights, order.position, order.offsets) or \
+        _combine_backward(grad, rows, weights, order)
+
+
+@_on_device
+def _combine_backward(grad, rows, weights, order):
     pos, off = _check_order(order, grad.device)
     T, k = pos.shape
     H = grad.shape[-1]

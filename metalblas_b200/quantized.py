@@ -17,12 +17,15 @@ import ctypes
 import torch
 
 from . import _lib
-from .dispatch import FLOATS, _stream_of
+from .dispatch import FLOATS, _plain, _stream_of
 
 MAX_K = 131071       # 127 or 128 squared times more would leave 32 bits
 MAX_GROUPS = 1024
 
 _byref = ctypes.byref
+# The host fast path (csrc/fastops.h): the result of a plain call, or None.
+_try_quantize = _lib.fast_op("try_quantize")
+_try_scaled = _lib.fast_op("try_scaled")
 
 
 def _on_device(fn):
@@ -39,6 +42,7 @@ def _on_device(fn):
 
 def _rows(x):
     """x with its last dimension contiguous and rows that do not overlap."""
+    x = _plain(x)
     if x.stride(-1) == 1 or x.shape[-1] <= 1:
         if x.dim() < 2 or x.shape[0] <= 1 or x.stride(0) >= x.shape[1]:
             return x
@@ -57,7 +61,6 @@ def _int8_rows(rows, cols, device):
     return q if pitch == cols else q[:, :cols]
 
 
-@_on_device
 def quantize(x):
     """Rows of ``x [..., cols]`` (fp32, fp16 or bf16) as ``(q, scale)``: int8 ``q`` of x's
     shape and fp32 ``scale`` of its leading dimensions, with ``x ~ q * scale[..., None]``.
@@ -67,6 +70,11 @@ def quantize(x):
     rows of a 2-D ``q`` start on 16-byte boundaries: with a number of columns that is no
     multiple of 16, ``q`` is a view of a wider matrix.
     """
+    return _try_quantize(x) or _quantize(x)
+
+
+@_on_device
+def _quantize(x):
     if x.dtype not in FLOATS:
         raise NotImplementedError(f"quantize takes fp32, fp16 or bf16, got {x.dtype}")
     assert x.dim() >= 1, "quantize takes rows"
@@ -93,7 +101,7 @@ def _scale(s, shape, name, device):
         assert all(a in (1, b) for a, b in zip(s.shape[::-1], shape[::-1])), \
             f"{name} has shape {tuple(s.shape)}, not {tuple(shape)}"
         s = s.expand(shape)
-    return s
+    return _plain(s)
 
 
 def _product(a2, b, sa, sb, M, N, K, groups, offsets, bias, out_dtype, c, overrides):
@@ -128,6 +136,8 @@ def _check_int8(a, b):
     if a.dtype is not torch.int8 or b.dtype is not torch.int8:
         raise NotImplementedError(f"int8 operands expected, got {a.dtype} and {b.dtype}")
     assert a.device == b.device, "operands on different devices"
+    if a.is_neg() or b.is_neg():
+        raise NotImplementedError("int8 operands with a lazy negation")
     if a.shape[-1] > MAX_K:
         raise ValueError(f"K = {a.shape[-1]}: sums of more than {MAX_K} int8 products can leave 32 bits")
 
@@ -147,13 +157,13 @@ def _check_out(out_dtype, out, shape, device):
 
 def _check_bias(bias, N, out_dtype, device):
     if bias is None:
-        return
+        return None
     assert bias.device == device and tuple(bias.shape) == (N,), f"bias has shape {tuple(bias.shape)}, not ({N},)"
     if bias.dtype is not out_dtype and bias.dtype is not torch.float32:
         raise NotImplementedError(f"bias must be {out_dtype} or fp32, got {bias.dtype}")
+    return _plain(bias)
 
 
-@_on_device
 def scaled_mm(a, b, scale_a, scale_b, *, bias=None, out_dtype=None, out=None, _plan=None):
     """``(a @ b) * scale_a[..., None] * scale_b + bias`` for int8 ``a [..., K]`` and ``b [K, N]``.
 
@@ -166,6 +176,15 @@ def scaled_mm(a, b, scale_a, scale_b, *, bias=None, out_dtype=None, out=None, _p
     a 16-byte aligned base and pitch, as is ``a`` with contiguous aligned rows; other layouts
     are copied into scratch in every call.
     """
+    if out is None and _plan is None:
+        c = _try_scaled(a, b, scale_a, scale_b, None, bias, out_dtype or torch.bfloat16)
+        if c is not None:
+            return c
+    return _scaled_mm(a, b, scale_a, scale_b, bias, out_dtype, out, _plan)
+
+
+@_on_device
+def _scaled_mm(a, b, scale_a, scale_b, bias, out_dtype, out, _plan):
     assert b.dim() == 2 and a.dim() >= 1, "scaled_mm takes a [..., K] and b [K, N]"
     _check_int8(a, b)
     K, N = b.shape
@@ -173,7 +192,7 @@ def scaled_mm(a, b, scale_a, scale_b, *, bias=None, out_dtype=None, out=None, _p
     lead = a.shape[:-1]
     dev = a.device
     out_dtype = _check_out(out_dtype, out, (*lead, N), dev)
-    _check_bias(bias, N, out_dtype, dev)
+    bias = _check_bias(bias, N, out_dtype, dev)
     sa = _scale(scale_a, lead, "scale_a", dev)
     sb = _scale(scale_b, (N,), "scale_b", dev)
     M = lead.numel()
@@ -186,7 +205,6 @@ def scaled_mm(a, b, scale_a, scale_b, *, bias=None, out_dtype=None, out=None, _p
     return out
 
 
-@_on_device
 def grouped_scaled_mm(a, b, scale_a, scale_b, offsets, *, out_dtype=None, out=None, _plan=None):
     """``scaled_mm`` with a weight matrix per group of rows.
 
@@ -196,6 +214,15 @@ def grouped_scaled_mm(a, b, scale_a, scale_b, offsets, *, out_dtype=None, out=No
     ascending row numbers starting at 0 (``expert_sort``'s): the host never reads it, empty
     groups cost nothing, and E is at most 1024.
     """
+    if out is None and _plan is None:
+        c = _try_scaled(a, b, scale_a, scale_b, offsets, None, out_dtype or torch.bfloat16)
+        if c is not None:
+            return c
+    return _grouped_scaled_mm(a, b, scale_a, scale_b, offsets, out_dtype, out, _plan)
+
+
+@_on_device
+def _grouped_scaled_mm(a, b, scale_a, scale_b, offsets, out_dtype, out, _plan):
     assert a.dim() == 2 and b.dim() == 3, "grouped_scaled_mm takes a [M, K] and b [E, K, N]"
     _check_int8(a, b)
     M, K = a.shape
