@@ -60,8 +60,9 @@ int check_route(int64_t T, int64_t k, int64_t H, const int32_t *position, const 
 
 
 // Threads of a block that share a token: short rows would leave most of a block idle.
-int route_lanes(int64_t H, int esz) {
+int route_lanes(int64_t H, int esz, bool whole_warps) {
   const int64_t vecs = ceil_div(H * esz, 16);
+  if (!whole_warps && vecs <= 16) return 16;
   return vecs <= 64 ? 32 : vecs <= 512 ? 128 : 256;
 }
 dim3 route_grid(int64_t T, int64_t H, int esz, int lanes, bool whole_rows) {
@@ -70,6 +71,44 @@ dim3 route_grid(int64_t T, int64_t H, int esz, int lanes, bool whole_rows) {
   int64_t y = whole_rows ? 1 : std::min<int64_t>(ceil_div(ceil_div(H * esz, 16) + 1, lanes), 64);
   y = std::min<int64_t>(y, std::max<int64_t>(1, ceil_div(16 * (int64_t)device_sms(), x)));
   return dim3((unsigned)x, (unsigned)y);
+}
+
+constexpr size_t sort_smem(int warps, int64_t experts) {
+  return ((size_t)warps * ((experts + 1) | 1) + experts + 1 + 32) * 4;
+}
+// Sets the sort kernel up on the current device, once: its largest shared memory,
+// and whether the device runs clusters of 16 of its largest blocks (past the
+// portable 8).
+template <class I>
+int sort_setup(int &max_ranks) {
+  static std::atomic<int> ranks[64];
+  int dev = 0;
+  int rc = cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
+  if (rc) return rc;
+  const bool keep = dev >= 0 && dev < 64;
+  if (keep && (max_ranks = ranks[dev].load(std::memory_order_acquire)) > 0) return MB_OK;
+  auto kern = expert_sort_kernel<I>;
+  const size_t smem = sort_smem(32, kMaxExperts);
+  rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "cudaFuncSetAttribute");
+  if (rc) return rc;
+  max_ranks = 8;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kSortRanks);
+  cfg.blockDim = dim3(1024);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute a[1];
+  a[0].id = cudaLaunchAttributeClusterDimension;
+  a[0].val.clusterDim.x = kSortRanks;
+  a[0].val.clusterDim.y = a[0].val.clusterDim.z = 1;
+  cfg.attrs = a;
+  cfg.numAttrs = 1;
+  int clusters = 0;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+      cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) == cudaSuccess && clusters > 0)
+    max_ranks = kSortRanks;
+  (void)cudaGetLastError();
+  if (keep) ranks[dev].store(max_ranks, std::memory_order_release);
+  return MB_OK;
 }
 
 template <class T>
@@ -369,20 +408,25 @@ int mb_expert_sort(int32_t ids64, int64_t n, int64_t experts, const void *ids, i
     return fail(MB_ERR_INVALID, "expert_sort: %lld experts (1 to %d)", (long long)experts, kMaxExperts);
   if (!offsets || (n > 0 && (!ids || !order || !position))) return fail(MB_ERR_INVALID, "expert_sort: null pointer");
   SortParams p{ids, (int)n, (int)experts, order, position, offsets};
-  // A warp per 32 entries up to a block's 32 warps and a cluster of 8 blocks (the
-  // scattered stores of `order` bind one SM: 8000 entries on one block 11.4 us),
-  // and a thread per expert for the scan.
-  const int W = (int)std::max<int64_t>(std::min<int64_t>(32, ceil_div(n, 32)), ceil_div(experts, 32));
+  int max_ranks = 0;
+  const int rc = ids64 ? sort_setup<long long>(max_ranks) : sort_setup<int>(max_ranks);
+  if (rc) return rc;
+  // Blocks of few warps and many of them: a 32-warp block costs 2 us to start and
+  // to step through its barriers, a cluster barrier 1 us, a warp's round of 32
+  // entries 0.1 us, and the scattered stores of `order` bind an SM.  Up to 512
+  // entries one block (4.1 us at 256 experts), then 256 entries a block up to 16
+  // blocks, then 8 warps a block until a warp holds 256 entries.  Measured
+  // against 1 to 16 blocks and 32 to 256 entries a warp: 1024 entries 4.5 us
+  // (4.3 at best), 8192 5.2 (one block 14.7), 65536 10.9 (8 blocks 16.6).
   int ranks = 1;
-  while (ranks < 8 && n > (int64_t)ranks * 1024) ranks *= 2;
-  const int threads = std::min(W, 32) * 32;
-  const size_t smem = ((size_t)(threads / 32) * ((experts + 1) | 1) + experts + 1 + 32) * 4;
+  if (n > 512)
+    while (ranks < max_ranks && n > (int64_t)ranks * 256) ranks *= 2;
+  int64_t W = std::min<int64_t>(8, ceil_div(n, 64 * ranks));
+  W = std::max(W, ceil_div(n, (int64_t)ranks * 32 * kSortBatch));  // the batch that lanes hold, while warps last
+  W = std::min<int64_t>(32, std::max(W, ceil_div(experts, 32)));   // a thread per expert in the scan
+  const int threads = (int)std::max<int64_t>(W, 1) * 32;
+  const size_t smem = sort_smem(threads / 32, experts);
   auto kern = ids64 ? expert_sort_kernel<long long> : expert_sort_kernel<int>;
-  if (smem > 48 * 1024) {
-    const int rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
-                              "cudaFuncSetAttribute");
-    if (rc) return rc;
-  }
   return launch_pdl(kern, dim3(ranks), dim3(threads), smem, (cudaStream_t)stream, ranks, "expert_sort", p);
 }
 
@@ -399,7 +443,7 @@ int mb_expert_gather(int32_t dtype, int64_t tokens, int64_t k, int64_t cols, con
     p.T = (int)tokens; p.H = (int)cols; p.k = (int)k; p.position = position; p.kept = kept;
     p.src = x; p.ld_src = ldx; p.dst = sorted; p.ld_dst = lds;
     const bool al = rows16(x, ldx, sizeof(T)) && rows16(sorted, lds, sizeof(T));
-    const int lanes = route_lanes(cols, sizeof(T));
+    const int lanes = route_lanes(cols, sizeof(T), false);
     auto kern = k <= 2 ? (al ? expert_gather_kernel<T, 2, true> : expert_gather_kernel<T, 2, false>)
                        : (al ? expert_gather_kernel<T, 8, true> : expert_gather_kernel<T, 8, false>);
     return launch_pdl(kern,
@@ -442,7 +486,7 @@ int mb_expert_combine(int32_t dtype, int32_t weights_dtype, int64_t tokens, int6
     p.T = (int)tokens; p.H = (int)cols; p.k = (int)k; p.position = position; p.kept = kept;
     p.src = sorted; p.ld_src = lds; p.w = weights; p.dst = out; p.ld_dst = ldo;
     const bool al = rows16(sorted, lds, sizeof(T)) && rows16(out, ldo, sizeof(T));
-    const int lanes = route_lanes(cols, sizeof(T));
+    const int lanes = route_lanes(cols, sizeof(T), false);
     const bool f32 = weights_dtype == MB_F32;
     auto pick = [&](auto ne) {
       constexpr int NE = decltype(ne)::value;
@@ -475,7 +519,7 @@ int mb_expert_combine_backward(int32_t dtype, int32_t weights_dtype, int64_t tok
     p.src = dout; p.ld_src = ldd; p.src2 = sorted; p.ld_src2 = lds; p.w = weights;
     p.dst = dsorted; p.ld_dst = ldds; p.dst2 = dweights;
     const bool al = rows16(dout, ldd, sizeof(T)) && rows16(sorted, lds, sizeof(T)) && rows16(dsorted, ldds, sizeof(T));
-    const int lanes = route_lanes(cols, sizeof(T));
+    const int lanes = route_lanes(cols, sizeof(T), true);
     const bool f32 = weights_dtype == MB_F32;
     auto pick = [&](auto ne) {
       constexpr int NE = decltype(ne)::value;

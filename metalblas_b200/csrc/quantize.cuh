@@ -41,6 +41,21 @@ __device__ __forceinline__ uint4 cut16(const uint4 &a, const uint4 &b, uint32_t 
                     __funnelshift_r(y3, y4, sh));
 }
 
+// 16 bytes that are read once, zeros where `on` is false.  As volatile assembly a
+// batch of these is issued as written, ahead of its uses; left to itself the
+// compiler interleaved loads and sums to save registers, two or three in flight
+// (combine of 4096 tokens x 8 x 4096 bf16: 72 us, 4.2 TB/s).
+__device__ __forceinline__ uint4 load_once(const void *p, bool on) {
+  uint4 v;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+      "mov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
+      "@q ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+      : "l"(p), "r"((uint32_t)on));
+  return v;
+}
+
 // The V elements at p.  AL: on a 16-byte boundary.  Otherwise they are cut out of
 // the one or two aligned words that hold them: the second word is read only
 // when it holds some of them, so no word without an element of the row is
