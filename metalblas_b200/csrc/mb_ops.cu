@@ -6,6 +6,7 @@
 #include <atomic>
 #include <cmath>
 #include <cstring>
+#include <map>
 #include <type_traits>
 
 #include "mb_host.cuh"
@@ -14,6 +15,7 @@
 #include "experts.cuh"
 #include "pack.cuh"
 #include "scaled_tc.cuh"
+#include "scaled_gemv.cuh"
 
 using namespace mb;
 using namespace mb::host;
@@ -149,6 +151,7 @@ int scaled_check(const mb_scaled_desc *d) {
 
 struct SgPlan {
   bool empty = false;
+  bool gemv = false;                  // up to four rows: one pass over the weights
   int bn = 0, pair = 1, split = 1, swap = 0;
   int w_mn = 0;                       // weights are read with N contiguous
   int pk_a = 0, pk_b = 0;             // operand copied into the workspace first
@@ -199,6 +202,17 @@ SgCost sg_cost(const mb_scaled_desc *d, int swap, int bn, int pair, int sms, int
   return {std::max(compute, bytes / std::min(22.4 * sms, 31.0 * busy)), split};
 }
 
+// The single-pass kernel's weight rows of a block, at most, and its shared memory.
+int64_t gemv_max_rows(const mb_scaled_desc *d) {
+  const int64_t total = (d->groups ? d->M : 1) * d->N;
+  return ceil_div(total, (int64_t)device_sms() * sg::GEMV_BLOCKS_PER_SM) + 1;
+}
+int64_t gemv_smem(const mb_scaled_desc *d) {
+  const int64_t mr = d->groups ? 1 : d->M;
+  return d->M * round_up(d->K, 16) + gemv_max_rows(d) * mr * 4;
+}
+constexpr int kGemvSmem = 96 * 1024;  // two blocks to an SM
+
 int sg_plan(const mb_scaled_desc *d, SgPlan &pl) {
   if (d->M == 0 || d->N == 0) { pl.empty = true; return MB_OK; }
   if (d->K == 0) return MB_OK;
@@ -229,6 +243,12 @@ int sg_plan(const mb_scaled_desc *d, SgPlan &pl) {
   pl.ws_bytes = at;
 
   const int sms = device_sms();
+  const bool forced = d->tile_n || d->cta_pair || d->split_k || d->swap_ab;
+  if (!forced && d->M <= (d->groups ? sg::GEMV_GROUPED_ROWS : sg::GEMV_ROWS) && !pl.pk_a && !pl.pk_b && !pl.w_mn &&
+      gemv_smem(d) <= kGemvSmem) {
+    pl.gemv = true;
+    return MB_OK;
+  }
   static const struct { int swap, bn, pair; } tiles[] = {{1, 16, 1},  {1, 32, 1},  {1, 64, 1},  {1, 128, 1},
                                                          {0, 128, 1}, {0, 256, 1}, {0, 256, 2}, {0, 512, 2}};
   double best = 1e300;
@@ -253,6 +273,41 @@ int sg_plan(const mb_scaled_desc *d, SgPlan &pl) {
   return MB_OK;
 }
 
+// Lets a kernel use `bytes` of dynamic shared memory; once per kernel and device.
+template <class K>
+int allow_smem(K *kern, int bytes) {
+  static std::mutex mu;
+  static std::map<std::pair<const void *, int>, int> done;
+  thread_local std::pair<const void *, int> last{nullptr, -1};
+  int dev = 0;
+  int rc = cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
+  if (rc) return rc;
+  const std::pair<const void *, int> key{reinterpret_cast<const void *>(kern), dev};
+  if (key == last) return MB_OK;
+  std::lock_guard<std::mutex> lk(mu);
+  int &have = done[key];
+  if (have < bytes) {
+    rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute");
+    if (rc) return rc;
+    have = bytes;
+  }
+  last = key;
+  return MB_OK;
+}
+
+template <int MR, bool GROUPED, class TO>
+int gemv_launch(const mb_scaled_desc *d, const SgPlan &pl, const sg::SgParams &p, cudaStream_t st) {
+  sg::GemvArgs g{};
+  g.A = d->A; g.B = d->B; g.a_rs = pl.a_rs; g.b_rs = pl.w_ld; g.sB = pl.sB;
+  g.K = (int)d->K;
+  g.max_rows = (int)gemv_max_rows(d);
+  auto kern = sg::scaled_gemv_kernel<MR, GROUPED, TO>;
+  const int rc = allow_smem(kern, kGemvSmem);
+  if (rc) return rc;
+  return launch_pdl(kern, dim3((unsigned)(device_sms() * sg::GEMV_BLOCKS_PER_SM)), dim3(sg::GEMV_THREADS),
+                    (size_t)gemv_smem(d), st, 1, "scaled_gemm", p, g);
+}
+
 template <int BN, int PAIR, bool SWAP, class TO>
 int sg_launch_tile(const SgPlan &pl, sg::SgParams &p, cudaStream_t st) {
   using C_ = sg::SgCfg<BN, PAIR, SWAP, TO>;
@@ -263,15 +318,8 @@ int sg_launch_tile(const SgPlan &pl, sg::SgParams &p, cudaStream_t st) {
   constexpr int smem_max = C_::CAN_SPLIT ? std::max(C_::smem_bytes(1), std::max(C_::smem_bytes(2), std::max(C_::smem_bytes(4), C_::smem_bytes(8))))
                                          : C_::smem_bytes(1);
   static_assert(smem_max <= tc::SMEM_LIMIT, "shared memory");
-  static std::atomic<bool> attr_done[64];
-  int dev = 0;
-  int rc = cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
+  const int rc = allow_smem(kern, smem_max);
   if (rc) return rc;
-  if (dev < 0 || dev >= 64 || !attr_done[dev].load(std::memory_order_acquire)) {
-    rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_max), "cudaFuncSetAttribute");
-    if (rc) return rc;
-    if (dev >= 0 && dev < 64) attr_done[dev].store(true, std::memory_order_release);
-  }
   const int csize = PAIR == 2 ? 2 : pl.split;
   const int64_t clusters = std::min<int64_t>(pl.units, device_sms() / csize);
   return launch_pdl(kern, dim3((unsigned)(clusters * csize)), dim3(tc::NUM_THREADS), C_::smem_bytes(pl.split), st, csize,
@@ -310,6 +358,10 @@ int sg_launch(const mb_scaled_desc *d, const SgPlan &pl, cudaStream_t st) {
   if (d->K == 0) {
     const int64_t blocks = std::min<int64_t>(ceil_div(d->M * d->N, 256), (int64_t)device_sms() * 16);
     return launch_pdl(sg::scaled_empty_kernel<TO>, dim3((unsigned)blocks), dim3(256), 0, st, 1, "scaled_gemm", p);
+  }
+  if (pl.gemv) {
+    if (d->groups) return gemv_launch<1, true, TO>(d, pl, p, st);
+    return d->M == 1 ? gemv_launch<1, false, TO>(d, pl, p, st) : gemv_launch<2, false, TO>(d, pl, p, st);
   }
   const int64_t nB = p.one_b ? 1 : p.groups;
   const void *A = d->A, *B = d->B;
@@ -383,6 +435,7 @@ int mb_scaled_plan(const mb_scaled_desc *d, char *buf, int buflen) {
   if (!rc) rc = sg_plan(d, pl);
   if (rc) return -rc;
   const size_t room = buf ? (size_t)std::max(buflen, 0) : 0;
+  if (pl.gemv) return snprintf(buf, room, "rows in one pass over the weights");
   if (pl.bn == 0) return snprintf(buf, room, pl.empty ? "empty" : "no sum");
   return snprintf(buf, room, "%s bn=%d pair=%d split=%d a_mn=%d b_mn=%d pack_a=%d pack_b=%d ws=%lld",
                   pl.swap ? "channels" : "tokens", pl.bn, pl.pair, pl.split, 0, pl.w_mn, pl.pk_a, pl.pk_b,

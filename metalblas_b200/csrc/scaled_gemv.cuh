@@ -1,0 +1,188 @@
+// The int8 product with scales (scaled_tc.cuh) for very few rows: a decode
+// step's one or two tokens, or a few rows spread over experts.
+//
+// Such a product is one pass over the weights and nothing else, so the work is
+// cut to put the same number of weight bytes on every SM: the weight rows to
+// read are numbered through and shared out evenly over two blocks per SM, and a
+// block's rows, as steps of 512 bytes, evenly over its warps; a warp runs
+// through whole rows but for the first and the last of its share.  The
+// tensor-core kernel hands out 128 channels at a time, which leaves 36 of 148
+// SMs idle at N = 14336, and starts later (TMEM, pipeline).  Measured on B200,
+// one row: K x N = 4096 x 14336 12.9 us against 14.3, 8192 x 28672 39.4
+// (5.96 TB/s) against 47.9.  With four rows the dp4a work and the rows' reads from shared
+// memory bind it (17.6 us against 14.6), so it takes two at most.
+//
+// By group (GROUPED) every row of A is a product of its own with its group's
+// weights: a decode step's rows nearly always have an expert each, and rows that
+// share one find its weights in L2.
+//
+// A lane multiplies its 16 weight bytes by dp4a with the rows of A, which lie in
+// shared memory, padded with zeros to whole vectors.  A run's 32-bit sums are
+// added into shared memory with integer atomics: the sum is exact, so their
+// order does not matter.  The block then applies the scales in the tensor-core
+// kernel's order; results have the same bits.
+#pragma once
+#include "quantize.cuh"
+#include "scaled_tc.cuh"
+
+namespace mb {
+namespace sg {
+
+constexpr int GEMV_ROWS = 2;          // rows of A, one weight matrix
+constexpr int GEMV_GROUPED_ROWS = 8;  // rows of A, weights by group
+constexpr int GEMV_THREADS = 512;
+constexpr int GEMV_BLOCKS_PER_SM = 2;
+constexpr int GEMV_BATCH = 8;         // 512-byte steps in flight per warp: 128 KB an SM
+
+struct GemvArgs {
+  const int8_t *A, *B;   // K contiguous, 16-byte aligned rows
+  int64_t a_rs, b_rs, sB;
+  int K;
+  int max_rows;          // weight rows of a block, at most
+};
+
+template <int MR, bool GROUPED, class TO>
+__global__ void __launch_bounds__(GEMV_THREADS, GEMV_BLOCKS_PER_SM)
+scaled_gemv_kernel(const __grid_constant__ SgParams p, const GemvArgs g) {
+  static_assert(!GROUPED || MR == 1, "a row of A at a time");
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const int vecs = (g.K + 15) / 16;
+  const int staged = GROUPED ? p.M : MR;
+  uint4 *xs = reinterpret_cast<uint4 *>(smem_raw);                // [staged][vecs]
+  int *acc = reinterpret_cast<int *>(xs + (int64_t)staged * vecs);  // [max_rows][MR]
+  __shared__ int group_of[GEMV_GROUPED_ROWS];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr int W = GEMV_THREADS / 32;
+  const int per_row = (g.K + 511) / 512;
+
+  // this block's weight rows and this warp's steps of them, for `total` rows in all
+  int64_t r0 = 0;
+  int rows = 0, row = 0, k = 0, left = 0;
+  auto share = [&](int64_t total) {
+    r0 = total * blockIdx.x / gridDim.x;
+    rows = (int)(total * (blockIdx.x + 1) / gridDim.x - r0);
+    const int64_t steps = (int64_t)rows * per_row;
+    const int64_t s0 = steps * warp / W;
+    left = (int)(steps * (warp + 1) / W - s0);
+    row = (int)(s0 / per_row);
+    k = (int)(s0 - (int64_t)row * per_row);
+  };
+  uint4 w[GEMV_BATCH];
+  // steps k .. k+run-1 of the weight row at src, from step b of them
+  auto fetch = [&](const int8_t *src, int run, int b) {
+    const int v0 = (k + b) * 32 + lane, stop = min((k + run) * 32, vecs);
+#pragma unroll
+    for (int i = 0; i < GEMV_BATCH; ++i) w[i] = load_once(src + (int64_t)(v0 + i * 32) * 16, v0 + i * 32 < stop);
+  };
+
+  for (int i = tid; i < g.max_rows * MR; i += GEMV_THREADS) acc[i] = 0;
+  if (tid < GEMV_GROUPED_ROWS) group_of[tid] = 0;
+  if constexpr (!GROUPED) {
+    // The weights' way into L2 may begin while the previous kernel ends.
+    share(p.N);
+    const int bytes = g.K & ~15;
+    if (bytes)
+      for (int i = tid; i < rows; i += GEMV_THREADS) prefetch_l2_bulk(g.B + (r0 + i) * g.b_rs, (uint32_t)bytes);
+  }
+  pdl_trigger();
+  pdl_wait();
+  if constexpr (!GROUPED) {
+    if (left > 0) fetch(g.B + (r0 + row) * g.b_rs, min(left, per_row - k), 0);
+  }
+  for (int i = tid; i < staged * vecs; i += GEMV_THREADS) {
+    const int m = i / vecs, v = i - m * vecs;
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (m < p.M) {
+      const int8_t *src = g.A + m * g.a_rs;
+      if (v * 16 + 16 <= g.K) {
+        x = *reinterpret_cast<const uint4 *>(src + v * 16);
+      } else {
+        int8_t b[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) b[j] = v * 16 + j < g.K ? src[v * 16 + j] : 0;
+        x = *reinterpret_cast<uint4 *>(b);
+      }
+    }
+    xs[i] = x;
+  }
+  __syncthreads();
+  int live = p.M;  // rows that belong to a group
+  if constexpr (GROUPED) {
+    // a row's group: the number of groups that end at or before it (p.groups: none)
+    for (int e = tid; e < p.groups; e += GEMV_THREADS) {
+      const int end = p.offsets[e + 1];
+      for (int m = 0; m < p.M; ++m)
+        if (end <= m) atomicAdd(group_of + m, 1);
+    }
+    __syncthreads();
+    while (live > 0 && group_of[live - 1] >= p.groups) --live;
+    share((int64_t)live * p.N);
+  }
+  int m0 = 0;
+  int64_t n = r0 + row;
+  if constexpr (GROUPED) {
+    m0 = (int)(n / p.N);
+    n -= (int64_t)m0 * p.N;
+  }
+  bool fetched = !GROUPED;  // the first batch is on its way
+  while (left > 0) {
+    const int run = min(left, per_row - k);
+    const int e = GROUPED ? min(group_of[m0], p.groups - 1) : 0;
+    const int8_t *src = g.B + (p.one_b ? 0 : e) * g.sB + n * g.b_rs;
+    const uint4 *x0 = xs + (GROUPED ? (int64_t)m0 * vecs : 0);
+    int s[MR];
+#pragma unroll
+    for (int m = 0; m < MR; ++m) s[m] = 0;
+    for (int b = 0; b < run; b += GEMV_BATCH) {
+      if (!fetched) fetch(src, run, b);
+      fetched = false;
+      const int v0 = (k + b) * 32 + lane;
+#pragma unroll
+      for (int i = 0; i < GEMV_BATCH; ++i) {
+        const int v = min(v0 + i * 32, vecs - 1);  // past the end w is zero
+#pragma unroll
+        for (int m = 0; m < MR; ++m) {
+          const uint4 x = x0[m * vecs + v];
+          s[m] = __dp4a((int)w[i].x, (int)x.x, s[m]);
+          s[m] = __dp4a((int)w[i].y, (int)x.y, s[m]);
+          s[m] = __dp4a((int)w[i].z, (int)x.z, s[m]);
+          s[m] = __dp4a((int)w[i].w, (int)x.w, s[m]);
+        }
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+      const int sum = __reduce_add_sync(0xffffffffu, s[m]);
+      if (lane == m) atomicAdd(acc + row * MR + m, sum);
+    }
+    left -= run;
+    k = 0;
+    ++row;
+    if (++n == p.N && GROUPED) {
+      n = 0;
+      ++m0;
+    }
+  }
+  __syncthreads();
+  TO *C = static_cast<TO *>(p.C);
+  for (int i = tid; i < rows * MR; i += GEMV_THREADS) {
+    int64_t m = i / rows, c = r0 + i - m * rows;  // rows of A outside, so that channels are stored in runs
+    const int sum = acc[(i - (int)m * rows) * MR + (int)m];
+    if constexpr (GROUPED) {
+      m = c / p.N;
+      c -= m * p.N;
+    }
+    if (m >= p.M) continue;
+    const int e = GROUPED ? min(group_of[m], p.groups - 1) : 0;
+    float v = scaled_sum(sum, p.scale_a[m * p.sa_s], p.scale_b[e * p.sb_g + c * p.sb_s]);
+    if (p.bias) v = __fadd_rn(v, bias_at<TO>(p, c));
+    C[m * p.c_rs + c * p.c_cs] = Elem<TO>::store(v);
+  }
+  // rows of no group
+  for (int64_t m = live; m < p.M; ++m)
+    for (int64_t c = (int64_t)blockIdx.x * GEMV_THREADS + tid; c < p.N; c += (int64_t)gridDim.x * GEMV_THREADS)
+      C[m * p.c_rs + c * p.c_cs] = Elem<TO>::store(0.f);
+}
+
+}  // namespace sg
+}  // namespace mb

@@ -122,6 +122,12 @@ template <class TO> __device__ __forceinline__ float bias_at(const SgParams &p, 
   return Elem<TO>::load(static_cast<const TO *>(p.bias)[n * p.bias_s], false);
 }
 
+// The value of a sum.  The roundings are spelled out: contracted to a fused
+// multiply-add in one kernel and not in another, they would differ in the last bit.
+__device__ __forceinline__ float scaled_sum(int sum, float scale_a, float scale_b) {
+  return __fmul_rn(__fmul_rn(__int2float_rn(sum), scale_a), scale_b);
+}
+
 // 4 consecutive results as the words of a staged row.
 template <class TO> __device__ __forceinline__ void pack4(const float *v, uint32_t *w) {
   if constexpr (sizeof(TO) == 4) {
@@ -460,8 +466,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
             const int64_t m0 = t.r0 + half * WCOLS + c;
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
-              float v = __int2float_rn((int)r[j]) * vec[j] * rs;
-              if (p.bias) v += rb;
+              float v = scaled_sum((int)r[j], vec[j], rs);
+              if (p.bias) v = __fadd_rn(v, rb);
               if (m0 + j < t.rend && n < p.N) C[(m0 + j) * p.c_rs + n * p.c_cs] = Elem<TO>::store(v);
             }
           } else {
@@ -479,11 +485,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
               for (int g = 0; g < EPC / 4; ++g) {
                 const int j = ch * EPC + g * 4;
                 const float4 s4 = *reinterpret_cast<const float4 *>(vec + j);
-                float v[4] = {__int2float_rn((int)r[j]) * rs * s4.x, __int2float_rn((int)r[j + 1]) * rs * s4.y,
-                              __int2float_rn((int)r[j + 2]) * rs * s4.z, __int2float_rn((int)r[j + 3]) * rs * s4.w};
+                float v[4] = {scaled_sum((int)r[j], rs, s4.x), scaled_sum((int)r[j + 1], rs, s4.y),
+                              scaled_sum((int)r[j + 2], rs, s4.z), scaled_sum((int)r[j + 3], rs, s4.w)};
                 if (p.bias) {
                   const float4 b4 = *reinterpret_cast<const float4 *>(vec + 32 + j);
-                  v[0] += b4.x; v[1] += b4.y; v[2] += b4.z; v[3] += b4.w;
+                  v[0] = __fadd_rn(v[0], b4.x); v[1] = __fadd_rn(v[1], b4.y);
+                  v[2] = __fadd_rn(v[2], b4.z); v[3] = __fadd_rn(v[3], b4.w);
                 }
                 pack4<TO>(v, w + (sizeof(TO) == 4 ? 0 : 2 * g));
               }
@@ -545,8 +552,8 @@ __global__ void __launch_bounds__(256) scaled_empty_kernel(const SgParams p) {
     }
     float v = 0.f;
     if (e < p.groups) {
-      v = 0.f * p.scale_a[m * p.sa_s] * p.scale_b[e * p.sb_g + n * p.sb_s];
-      if (p.bias) v += bias_at<TO>(p, n);
+      v = scaled_sum(0, p.scale_a[m * p.sa_s], p.scale_b[e * p.sb_g + n * p.sb_s]);
+      if (p.bias) v = __fadd_rn(v, bias_at<TO>(p, n));
     }
     static_cast<TO *>(p.C)[m * p.c_rs + n * p.c_cs] = Elem<TO>::store(v);
   }
