@@ -168,11 +168,11 @@ bool tma_rows(const void *p, int64_t rows, int64_t cols, int64_t &rs, int64_t cs
   return aligned16(p) && rs > 0 && rs % 16 == 0 && (groups <= 1 || (gs >= 0 && gs % 16 == 0));
 }
 
-// One tile shape's time in SM cycles.  Per 128-byte K-block an SM is bound by
-// its operands' way into shared memory, at the rates of tc_gemm.cuh's tile
-// table (45 B/clk alone, 35 on a CTA pair, 30.5 for the 512-wide pair tile); a
-// product with few rows is bound by the weights' way from HBM, 22.4 B/clk per SM
-// over the chip and 31 for one SM.
+// One tile shape's time in SM cycles, from what the kernel measured on B200.  Per
+// 128-byte K-block an SM is bound by its operands' way into shared memory: 51
+// B/clk, 35 on a CTA pair, 30.5 for the 512-wide pair tile (from L2 or HBM alike);
+// the chip's HBM adds 22.4 B/clk per SM.  Splitting K costs a cluster's exchange:
+// 0.7 us at 16 columns (of a half per rank), 3.5 us at 128, again for each doubling.
 struct SgCost {
   double t;
   int split;
@@ -184,22 +184,21 @@ SgCost sg_cost(const mb_scaled_desc *d, int swap, int bn, int pair, int sms, int
   const int trows = swap ? bn : 128 * pair;
   // groups do not end on tile boundaries: half a tile more each
   const double tiles_r = d->groups && rows > trows / 2 ? M / trows + 0.5 * active : active * std::ceil(rows / trows);
-  const double tiles_c = (double)ceil_div(d->N, swap ? 128 : bn);
-  const double units = tiles_r * tiles_c;
-  const double kbc = bn > 256 ? 1611.0 : pair == 2 ? (128.0 + bn / 2.0) * 128.0 / 35.0 : (128.0 + bn) * 128.0 / 45.0;
-  const double epi = (bn > 256 ? 12.0 : 4.0) * bn;
-  int split = 1;
-  if (pair == 1 && bn <= 128) {
-    if (force_split) split = force_split;
-    else
-      while (split < 8 && units * split * 2 <= sms && kb / (split * 2) >= 4) split *= 2;
-  }
-  const double slots = (double)sms / (pair * split);
-  const double waves = std::ceil(units / slots);
-  const double compute = waves * (std::ceil(kb / split) * kbc + epi + (split > 1 ? 1500.0 : 0.0));
-  const double busy = std::min<double>(sms, units * pair * split);
+  const double units = tiles_r * (double)ceil_div(d->N, swap ? 128 : bn);
+  const double kbc = bn > 256 ? 1611.0 : pair == 2 ? (128.0 + bn / 2.0) * 128.0 / 35.0 : (128.0 + bn) * 128.0 / 51.0;
+  const double epi = (bn > 256 ? 12.0 : swap ? 8.0 : 4.0) * bn;
   const double bytes = active * (double)d->N * (double)d->K + M * (double)d->K + M * (double)d->N * elem_size(d->out_dtype);
-  return {std::max(compute, bytes / std::min(22.4 * sms, 31.0 * busy)), split};
+  SgCost best{1e300, 1};
+  for (int split = 1, log2 = 0; split <= 8; split *= 2, ++log2) {
+    if (force_split ? split != force_split : (split > 1 && (pair == 2 || bn > 128 || kb < split))) continue;
+    // clusters of 4 and 8 leave SMs over in some GPCs
+    const double slots = std::floor((double)sms / (pair * split) * (split >= 4 ? 0.9 : 1.0));
+    const double waves = std::ceil(units / slots);
+    const double compute = waves * (std::ceil(kb / split) * kbc + epi + log2 * (600.0 + 45.0 * bn));
+    const double t = std::max(compute, bytes / (22.4 * sms)) * (1.0 + 0.01 * log2);
+    if (t < best.t) best = {t, split};
+  }
+  return best;
 }
 
 // The single-pass kernel's weight rows of a block, at most, and its shared memory.
@@ -257,7 +256,7 @@ int sg_plan(const mb_scaled_desc *d, SgPlan &pl) {
     if (d->cta_pair && d->cta_pair != c.pair) continue;
     if (d->swap_ab && (d->swap_ab > 0) != (c.swap == 1)) continue;
     if (d->split_k > 1 && (c.pair != 1 || c.bn > 128)) continue;
-    const SgCost cost = sg_cost(d, c.swap, c.bn, c.pair, sms, d->split_k);
+    const SgCost cost = sg_cost(d, c.swap, c.bn, c.pair, sms, d->split_k);  // (an impossible split: never less)
     if (cost.t < best) {
       best = cost.t;
       pl.swap = c.swap; pl.bn = c.bn; pl.pair = c.pair; pl.split = cost.split;
@@ -347,6 +346,7 @@ int sg_launch(const mb_scaled_desc *d, const SgPlan &pl, cudaStream_t st) {
   p.M = (int)d->M; p.N = (int)d->N; p.groups = (int)std::max<int64_t>(d->groups, 1);
   p.offsets = d->groups ? d->offsets : nullptr;
   p.one_b = d->groups > 1 && d->sB == 0;
+  p.K = (int)d->K;
   p.kb_total = (int)ceil_div(d->K, 128);
   p.C = d->C; p.c_rs = d->c_rs; p.c_cs = d->c_cs;
   constexpr int OSZ = sizeof(TO);
@@ -385,6 +385,10 @@ int sg_launch(const mb_scaled_desc *d, const SgPlan &pl, cudaStream_t st) {
                  : encode_map(tw, MB_I8, B, d->K, d->N, nB, pl.w_ld, pl.sB, 128, w_rows);
   if (rc) return rc;
   (pl.swap ? p.a_mn : p.b_mn) = pl.w_mn;
+  if (pl.swap && !d->groups && !pl.w_mn) {
+    p.w = static_cast<const int8_t *>(B);
+    p.w_ld = pl.w_ld;
+  }
   if (pl.swap) {
     switch (pl.bn) {
       case 16: return sg_launch_tile<16, 1, true, TO>(pl, p, st);

@@ -27,8 +27,8 @@
 //   group's end masked (a TMA store could only clip at the tensor's end).
 // SWAP = true: UMMA rows are 128 channels, columns 16..128 tokens: with few
 //   rows per group the product is a stream of weights, and this form loads the
-//   fewest other bytes per weight byte.  Lanes hold channels, so each token's
-//   store is a run of 32 channels.
+//   fewest other bytes per weight byte.  Lanes hold channels; the staged rows
+//   are tokens all the same.
 //
 // split > 1 (few units): the CTAs of a cluster share one unit, each a range of
 // K.  Eight epilogue warps hold eight pieces of the tile; piece i is finished
@@ -54,7 +54,9 @@ struct SgParams {
   const int *offsets;      // null: one group of all M rows
   int a_mn, b_mn;          // operand is MN-major in global memory
   int one_b;               // every group has the same B
-  int kb_total, stages, split;
+  int K, kb_total, stages, split;
+  const int8_t *w;         // SWAP, one group, K contiguous: the weights and their pitch
+  int64_t w_ld;
   int tiles_c;             // channel tiles
   void *C;
   int64_t c_rs, c_cs;
@@ -74,7 +76,7 @@ struct SgCfg {
   static constexpr int TCOLS = SWAP ? BM : BN;          // channels per tile
   static constexpr int STAGE_BYTES = B::A_BYTES + B::B_BYTES;
   static constexpr int RB = 32 * (int)sizeof(TO);       // bytes of a staged row
-  static constexpr int STAGING_WARP = SWAP ? 0 : 32 * RB;
+  static constexpr int STAGING_WARP = (SWAP && BN < 64 ? BN / 2 : 32) * RB;  // rows a warp stores at a time
   static constexpr int VEC_WARP = 32 * 8;               // a chunk's column scales and biases
   static constexpr bool CAN_SPLIT = PAIR == 1 && BN <= 128;
   static constexpr int PIECE_BYTES = 64 * BN;   // 32 lanes x BN / 2 columns x 4 bytes
@@ -193,8 +195,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
     }
     mbar_init(drain_bar, 1);
     if (split > 1) {
-      // every lane of each sending warp; lane 0 of each finishing warp
-      mbar_init(red_full, (split - 1) * (8 / split) * 32);
+      // lane 0 of each sending warp; lane 0 of each finishing warp
+      mbar_init(red_full, (split - 1) * (8 / split));
       mbar_init(red_free, (split - 1) * (8 / split));
     }
     *abort_flag = 0;
@@ -205,6 +207,19 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
   if (warp == 1) {
     tmem_alloc_g<PAIR>(smem_u32(tmem_slot), B_::TMEM_COLS);
     tmem_relinquish_g<PAIR>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (csize > 1) cluster_sync_all();  // every CTA's barriers are initialised before any remote arrival
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  // One group: this CTA's first unit is known, and its weights' way into L2 (as
+  // much of them as the ring holds) may begin while the previous kernel ends.
+  if (SWAP && p.w && threadIdx.x >= 64 && threadIdx.x < 64 + BM) {
+    const int64_t n = (int64_t)(cid % p.tiles_c) * C_::TCOLS + (threadIdx.x - 64);
+    const int k0 = split > 1 ? (int)((int64_t)rank * p.kb_total / split) * BK : 0;
+    const int bytes = (min(p.K, k0 + stages * BK) - k0) & ~15;
+    if (n < p.N && bytes > 0) prefetch_l2_bulk(p.w + n * p.w_ld + k0, (uint32_t)bytes);
   }
   pdl_wait();
   // The unit table: row0[e] and first_unit[e] for e <= groups.
@@ -241,11 +256,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
     }
     if (threadIdx.x == NUM_THREADS - 1) first_unit[G] = at;
   }
-  tc_fence_before();
   __syncthreads();
-  if (csize > 1) cluster_sync_all();  // every CTA's barriers are initialised before any remote arrival
-  tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
   const int num_units = first_unit[G];
 
   if (warp == 0) {
@@ -393,10 +404,39 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
     uint32_t aphase = 0;
     for (int u = cid; u < num_units; u += ncl) {
       const Tile t = unit_tile<C_::TROWS, C_::TCOLS>(first_unit, row0, G, p.tiles_c, u);
+      // The scales are on their way while the accumulator fills: this lane's row (a
+      // token, or a channel when swapped) and, a column per lane, the first columns.
+      const int row = (PAIR == 2 ? (int)rank * BM : 0) + q * 32 + lane;   // UMMA row of this lane
+      const int64_t m = t.r0 + row, n = t.c0 + row;
+      const bool finish = split == 1 || owner == me;
+      float rs = 0.f, rb = 0.f, cs_next = 0.f, cb_next = 0.f;
+      auto load_cols = [&](int c) {
+        const int64_t col = (SWAP ? t.r0 : t.c0) + half * WCOLS + c + lane;
+        cs_next = cb_next = 0.f;
+        if constexpr (SWAP) {
+          if (lane < CH && col < t.rend) cs_next = p.scale_a[col * p.sa_s];
+        } else {
+          if (lane < CH && col < p.N) {
+            cs_next = p.scale_b[t.e * p.sb_g + col * p.sb_s];
+            if (p.bias) cb_next = bias_at<TO>(p, col);
+          }
+        }
+      };
+      if (finish) {
+        if constexpr (SWAP) {
+          if (n < p.N) {
+            rs = p.scale_b[t.e * p.sb_g + n * p.sb_s];
+            if (p.bias) rb = bias_at<TO>(p, n);
+          }
+        } else {
+          if (m < t.rend) rs = p.scale_a[m * p.sa_s];
+        }
+        load_cols(0);
+      }
       if (!all(wait_x(tfull_bar(abuf), aphase))) break;
       tc_fence_after();
       const uint32_t tbase = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(abuf * B_::ACC_COLS + half * WCOLS);
-      if (split > 1 && owner != me) {
+      if (!finish) {
         // what this CTA sent for the last unit has been read
         if (!first && !all(mbar_wait_cluster(red_free, rphase ^ 1u, abort_flag, p.timeout_ns))) break;
         const uint32_t dst = mapa_shared(red_u32 + (uint32_t)(me - (me > owner ? 1 : 0)) * red_step, (uint32_t)owner);
@@ -410,38 +450,19 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
             st_cluster_v4(dst + (uint32_t)((c + j) >> 2) * 512u, r[j], r[j + 1], r[j + 2], r[j + 3]);
         }
         tc_fence_before();
-        __syncwarp();
-        if (lane == 0) release_tmem(abuf);
-        mbar_arrive_cluster(mapa_shared(red_full, (uint32_t)owner));
+        __syncwarp();  // the lanes' stores come before lane 0's release
+        if (lane == 0) {
+          mbar_arrive_cluster(mapa_shared(red_full, (uint32_t)owner));
+          release_tmem(abuf);
+        }
       } else {
         if (split > 1 && !all(mbar_wait_cluster(red_full, rphase, abort_flag, p.timeout_ns))) break;
-        const int row = (PAIR == 2 ? (int)rank * BM : 0) + q * 32 + lane;   // UMMA row of this lane
-        // this lane's row: a token, or a channel when swapped
-        const int64_t m = t.r0 + row, n = t.c0 + row;
-        float rs = 0.f, rb = 0.f;
-        if constexpr (SWAP) {
-          if (n < p.N) {
-            rs = p.scale_b[t.e * p.sb_g + n * p.sb_s];
-            if (p.bias) rb = bias_at<TO>(p, n);
-          }
-        } else {
-          if (m < t.rend) rs = p.scale_a[m * p.sa_s];
-        }
 #pragma unroll 1
         for (int c = 0; c < WCOLS; c += CH) {
           uint32_t r[32];
           tmem_ld<CH>(tbase + c, r);
-          // the columns' scales (and biases), one column per lane
-          const int64_t col = (SWAP ? t.r0 : t.c0) + half * WCOLS + c + lane;
-          float cs = 0.f, cb = 0.f;
-          if constexpr (SWAP) {
-            if (lane < CH && col < t.rend) cs = p.scale_a[col * p.sa_s];
-          } else {
-            if (lane < CH && col < p.N) {
-              cs = p.scale_b[t.e * p.sb_g + col * p.sb_s];
-              if (p.bias) cb = bias_at<TO>(p, col);
-            }
-          }
+          const float cs = cs_next, cb = cb_next;
+          if (c + CH < WCOLS) load_cols(c + CH);
           __syncwarp();  // the last step's reads of vec and of the staging rows are done
           vec[lane] = cs;
           if constexpr (!SWAP) vec[32 + lane] = cb;
@@ -462,21 +483,28 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
               }
             }
           }
+          constexpr int EPC = 16 / (int)sizeof(TO);   // elements per 16-byte chunk
+          constexpr int NCH = C_::RB / 16;            // chunks per staged row
+          auto chunk_addr = [&](int rr, int ch) {
+            // Written by rows (a lane a row), rows 8 (16-bit) or 4 apart would share
+            // banks; written by columns (swapped) they lie as they are.
+            const int x = SWAP ? 0 : NCH == 4 ? (rr >> 1) & 3 : rr & 7;
+            return stg + (uint32_t)(rr * C_::RB) + ((uint32_t)(ch ^ x) << 4);
+          };
           if constexpr (SWAP) {
-            const int64_t m0 = t.r0 + half * WCOLS + c;
+            TO *col = reinterpret_cast<TO *>(staging + ew * C_::STAGING_WARP) + lane;
 #pragma unroll
-            for (int j = 0; j < CH; ++j) {
-              float v = scaled_sum((int)r[j], vec[j], rs);
-              if (p.bias) v = __fadd_rn(v, rb);
-              if (m0 + j < t.rend && n < p.N) C[(m0 + j) * p.c_rs + n * p.c_cs] = Elem<TO>::store(v);
+            for (int j = 0; j < CH; j += 4) {
+              const float4 s4 = *reinterpret_cast<const float4 *>(vec + j);
+              const float sc[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                float v = scaled_sum((int)r[j + i], sc[i], rs);
+                if (p.bias) v = __fadd_rn(v, rb);
+                col[(j + i) * 32] = Elem<TO>::store(v);
+              }
             }
           } else {
-            constexpr int EPC = 16 / (int)sizeof(TO);   // elements per 16-byte chunk
-            constexpr int NCH = C_::RB / 16;            // chunks per staged row
-            auto chunk_addr = [&](int rr, int ch) {     // conflict-free: rows 8 (16-bit) or 4 apart share banks
-              const int x = NCH == 4 ? (rr >> 1) & 3 : rr & 7;
-              return stg + (uint32_t)(rr * C_::RB) + ((uint32_t)(ch ^ x) << 4);
-            };
             static_assert(CH == 32, "whole staged rows");
 #pragma unroll
             for (int ch = 0; ch < NCH; ++ch) {
@@ -498,14 +526,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
                            "r"(w[1]), "r"(w[2]), "r"(w[3])
                            : "memory");
             }
-            __syncwarp();
+          }
+          __syncwarp();
+          {
+            // the staged rows (tokens) in 16-byte chunks, whole rows by neighbouring lanes
             const int ch = lane % NCH, rr0 = lane / NCH;
-            const int64_t mw = t.r0 + (PAIR == 2 ? (int)rank * BM : 0) + q * 32;   // the warp's first row
-            const int64_t nn = t.c0 + half * WCOLS + c + ch * EPC;
+            const int64_t mw = SWAP ? t.r0 + half * WCOLS + c : t.r0 + (PAIR == 2 ? (int)rank * BM : 0) + q * 32;
+            const int64_t nn = (SWAP ? t.c0 + q * 32 : t.c0 + half * WCOLS + c) + ch * EPC;
+            constexpr int ROWS = SWAP ? CH : 32, PASS = 32 / NCH;
 #pragma unroll
-            for (int i = 0; i < NCH; ++i) {
-              const int rr = i * (32 / NCH) + rr0;
-              if (mw + rr >= t.rend || nn >= p.N) continue;
+            for (int i = 0; i < (ROWS + PASS - 1) / PASS; ++i) {
+              const int rr = i * PASS + rr0;
+              if (rr >= ROWS || mw + rr >= t.rend || nn >= p.N) continue;
               const uint4 v = ld_shared_v4(chunk_addr(rr, ch));
               TO *dst = C + (mw + rr) * p.c_rs;
               if (p.c_vec && nn + EPC <= p.N) {
