@@ -168,11 +168,14 @@ bool tma_rows(const void *p, int64_t rows, int64_t cols, int64_t &rs, int64_t cs
   return aligned16(p) && rs > 0 && rs % 16 == 0 && (groups <= 1 || (gs >= 0 && gs % 16 == 0));
 }
 
-// One tile shape's time in SM cycles, from what the kernel measured on B200.  Per
-// 128-byte K-block an SM is bound by its operands' way into shared memory: 51
-// B/clk, 35 on a CTA pair, 30.5 for the 512-wide pair tile (from L2 or HBM alike);
-// the chip's HBM adds 22.4 B/clk per SM.  Splitting K costs a cluster's exchange:
-// 0.7 us at 16 columns (of a half per rank), 3.5 us at 128, again for each doubling.
+// One tile shape's time in SM cycles, fitted to the kernel's times on B200 (8192 x
+// 512..8192 x 8192, 16384 x 4096 x 4096 and the thin shapes of 4 to 256 rows).  A tile
+// takes its 128-byte K-blocks, bound by the operands' way into shared memory (59
+// B/clk, 64 for 128 x 256, 47 on each SM of a pair, 36 for the 512-wide pair
+// tile), plus a hand-over, but never less than its epilogue, which runs beside
+// the next tile's K-blocks; the 512-wide tile fills TMEM alone, so its epilogue
+// is all hand-over.  The chip's HBM gives 22.4 B/clk per SM.  Splitting K costs a
+// cluster's exchange: 0.7 us at 16 columns, 3.5 us at 128, again for each doubling.
 struct SgCost {
   double t;
   int split;
@@ -185,16 +188,22 @@ SgCost sg_cost(const mb_scaled_desc *d, int swap, int bn, int pair, int sms, int
   // groups do not end on tile boundaries: half a tile more each
   const double tiles_r = d->groups && rows > trows / 2 ? M / trows + 0.5 * active : active * std::ceil(rows / trows);
   const double units = tiles_r * (double)ceil_div(d->N, swap ? 128 : bn);
-  const double kbc = bn > 256 ? 1611.0 : pair == 2 ? (128.0 + bn / 2.0) * 128.0 / 35.0 : (128.0 + bn) * 128.0 / 51.0;
-  const double epi = (bn > 256 ? 12.0 : swap ? 8.0 : 4.0) * bn;
-  const double bytes = active * (double)d->N * (double)d->K + M * (double)d->K + M * (double)d->N * elem_size(d->out_dtype);
+  const double out = elem_size(d->out_dtype) == 4 ? 1.3 : 1.0;
+  const bool wide = bn > 256;
+  const double kbc = wide ? 1330.0 : pair == 2 ? 700.0 : bn == 256 ? 770.0 : (128.0 + bn) * 128.0 / 59.0;
+  const double hand = wide ? 8000.0 * out : pair == 2 ? 1500.0 : bn == 256 ? 1200.0 : 500.0 + 4.0 * bn;
+  const double epi = wide ? 0.0 : (pair == 2 ? 7000.0 : (swap ? 25.0 : bn == 256 ? 22.0 : 28.0) * bn) * out;
+  // a group's weights read for a second tile of its rows come from L2, mostly
+  const double again = d->groups ? 0.4 * std::min(1.0, tiles_r / active - 1.0) : 0.0;
+  const double bytes = active * (double)d->N * (double)d->K * (1.0 + again) + M * (double)d->K +
+                       M * (double)d->N * elem_size(d->out_dtype);
   SgCost best{1e300, 1};
   for (int split = 1, log2 = 0; split <= 8; split *= 2, ++log2) {
     if (force_split ? split != force_split : (split > 1 && (pair == 2 || bn > 128 || kb < split))) continue;
     // clusters of 4 and 8 leave SMs over in some GPCs
     const double slots = std::floor((double)sms / (pair * split) * (split >= 4 ? 0.9 : 1.0));
     const double waves = std::ceil(units / slots);
-    const double compute = waves * (std::ceil(kb / split) * kbc + epi + log2 * (600.0 + 45.0 * bn));
+    const double compute = waves * std::max(std::ceil(kb / split) * kbc + hand + log2 * (500.0 + 40.0 * bn), epi);
     const double t = std::max(compute, bytes / (22.4 * sms)) * (1.0 + 0.01 * log2);
     if (t < best.t) best = {t, split};
   }
@@ -385,6 +394,9 @@ int sg_launch(const mb_scaled_desc *d, const SgPlan &pl, cudaStream_t st) {
                  : encode_map(tw, MB_I8, B, d->K, d->N, nB, pl.w_ld, pl.sB, 128, w_rows);
   if (rc) return rc;
   (pl.swap ? p.a_mn : p.b_mn) = pl.w_mn;
+  if (!pl.swap && p.c_vec && (d->M == 1 || d->c_rs >= d->N))
+    p.c_tma = encode_map(&p.tmC, d->out_dtype, d->C, d->N, d->M, 1, d->M == 1 ? round_up(d->N, 16) : d->c_rs, 0, 32, 32,
+                         OSZ == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B) == MB_OK;
   if (pl.swap && !d->groups && !pl.w_mn) {
     p.w = static_cast<const int8_t *>(B);
     p.w_ld = pl.w_ld;

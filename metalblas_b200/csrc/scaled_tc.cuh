@@ -23,8 +23,8 @@
 //
 // SWAP = false: UMMA rows are tokens (128, or 256 on a CTA pair), columns are
 //   channels: the compute-bound form.  A warp stages 32 rows x 32 columns in
-//   shared memory and writes whole rows with 16-byte stores, rows past the
-//   group's end masked (a TMA store could only clip at the tensor's end).
+//   shared memory and stores them as one TMA box; rows that end with a group
+//   inside C (a box could only clip at the tensor's end) go out by 16-byte stores.
 // SWAP = true: UMMA rows are 128 channels, columns 16..128 tokens: with few
 //   rows per group the product is a stream of weights, and this form loads the
 //   fewest other bytes per weight byte.  Lanes hold channels; the staged rows
@@ -49,6 +49,7 @@ constexpr int BAR_BYTES = 512;
 
 struct SgParams {
   CUtensorMap tmA, tmB;    // UMMA-A and UMMA-B operands, {inner, outer, group}
+  CUtensorMap tmC;         // C, boxes of 32 x 32, for c_tma
   int M, N;                // tokens, channels
   int groups;
   const int *offsets;      // null: one group of all M rows
@@ -60,6 +61,7 @@ struct SgParams {
   int tiles_c;             // channel tiles
   void *C;
   int64_t c_rs, c_cs;
+  int c_tma;               // C has a tensor map
   int c_vec;               // c_cs == 1 and rows on 16-byte boundaries
   const float *scale_a, *scale_b;
   int64_t sa_s, sb_s, sb_g;
@@ -128,6 +130,25 @@ template <class TO> __device__ __forceinline__ float bias_at(const SgParams &p, 
 // multiply-add in one kernel and not in another, they would differ in the last bit.
 __device__ __forceinline__ float scaled_sum(int sum, float scale_a, float scale_b) {
   return __fmul_rn(__fmul_rn(__int2float_rn(sum), scale_a), scale_b);
+}
+
+// Four sums of one row, two to an instruction: the same roundings.
+__device__ __forceinline__ void scaled_sums(const int *sum, float scale_a, const float4 &scale_b, float *v) {
+  auto mul2 = [](float2 a, float2 b) {
+    float2 o;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<unsigned long long &>(o))
+        : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
+    return o;
+  };
+  const float2 sa = make_float2(scale_a, scale_a);
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const float2 f = make_float2(__int2float_rn(sum[i]), __int2float_rn(sum[i + 1]));
+    const float2 o = mul2(mul2(f, sa), i ? make_float2(scale_b.z, scale_b.w) : make_float2(scale_b.x, scale_b.y));
+    v[i] = o.x;
+    v[i + 1] = o.y;
+  }
 }
 
 // 4 consecutive results as the words of a staged row.
@@ -506,25 +527,44 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
             }
           } else {
             static_assert(CH == 32, "whole staged rows");
+            uint32_t w[NCH][4];
+            auto convert = [&](auto with_bias) {
 #pragma unroll
-            for (int ch = 0; ch < NCH; ++ch) {
-              uint32_t w[4];
-#pragma unroll
-              for (int g = 0; g < EPC / 4; ++g) {
-                const int j = ch * EPC + g * 4;
+              for (int j = 0; j < 32; j += 4) {
                 const float4 s4 = *reinterpret_cast<const float4 *>(vec + j);
-                float v[4] = {scaled_sum((int)r[j], rs, s4.x), scaled_sum((int)r[j + 1], rs, s4.y),
-                              scaled_sum((int)r[j + 2], rs, s4.z), scaled_sum((int)r[j + 3], rs, s4.w)};
-                if (p.bias) {
+                float v[4];
+                scaled_sums(reinterpret_cast<const int *>(r) + j, rs, s4, v);
+                if constexpr (decltype(with_bias)::value) {
                   const float4 b4 = *reinterpret_cast<const float4 *>(vec + 32 + j);
                   v[0] = __fadd_rn(v[0], b4.x); v[1] = __fadd_rn(v[1], b4.y);
                   v[2] = __fadd_rn(v[2], b4.z); v[3] = __fadd_rn(v[3], b4.w);
                 }
-                pack4<TO>(v, w + (sizeof(TO) == 4 ? 0 : 2 * g));
+                pack4<TO>(v, &w[j / EPC][sizeof(TO) == 4 ? 0 : j % 8 / 2]);
               }
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(chunk_addr(lane, ch)), "r"(w[0]),
-                           "r"(w[1]), "r"(w[2]), "r"(w[3])
+            };
+            if (p.bias) convert(std::true_type());
+            else convert(std::false_type());
+            if (p.c_tma) {  // the last step's store has read the staging rows
+              if (lane == 0) bulk_wait_read0();
+              __syncwarp();
+            }
+#pragma unroll
+            for (int ch = 0; ch < NCH; ++ch)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(chunk_addr(lane, ch)), "r"(w[ch][0]),
+                           "r"(w[ch][1]), "r"(w[ch][2]), "r"(w[ch][3])
                            : "memory");
+            // 32 rows of the group (or up to the end of C, where the store clips)
+            // go out as one box; the rows before another group's by hand.
+            const int64_t mw = t.r0 + (PAIR == 2 ? (int)rank * BM : 0) + q * 32;
+            if (p.c_tma && (mw + 32 <= t.rend || t.rend == p.M)) {
+              const int64_t nn = t.c0 + half * WCOLS + c;
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0 && mw < t.rend && nn < p.N) {
+                tma_store_3d(&p.tmC, stg, (int)nn, (int)mw, 0);
+                bulk_commit();
+              }
+              continue;
             }
           }
           __syncwarp();
@@ -560,6 +600,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
       first = false;
       if (++abuf == B_::NACC) { abuf = 0; aphase ^= 1u; }
     }
+    if (!SWAP && lane == 0) bulk_wait0();  // this warp's stores have been made
+    __syncwarp();
   }
 
   tc_fence_before();
