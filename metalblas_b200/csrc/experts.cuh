@@ -479,12 +479,14 @@ __global__ void __launch_bounds__(kRouteThreads) expert_combine_backward_kernel(
 // Rows to int8 (see quantize.cuh): row t of src goes to the k slots of token t,
 // or, with position == null, to row t.  TPR threads hold a row's vectors, up to
 // HELD each, in registers between the maximum and the rounding; longer rows are
-// read again (from L2).  Two vectors a thread and at most 32 registers keep 2048
-// threads, 64 KB of loads, on an SM: with four the compiler took 80 registers and
-// 512-thread blocks ran one to an SM (16384 x 8192 bf16: 174 us).
-template <class T, bool AL, int TPR>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, 2048 / (TPR < 256 ? 256 : TPR)) quantize_rows_kernel(const RouteParams p, int q_vec) {
-  constexpr int V = Vec<T>::V, HELD = 2, THREADS = TPR < 256 ? 256 : TPR;
+// read again (from L2).  It is bound by how much of its loads an SM can keep in
+// flight between the barriers and roundings, and by HBM behind that: 16384 x 8192
+// bf16 72.8 us (5.5 TB/s) with four vectors a thread, 87 with two and twice the
+// threads, 79 with eight and half of them; copies into shared memory ahead of a
+// persistent block gave 79.
+template <class T, bool AL, int TPR, int HELD>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, (HELD > 4 ? 768 : HELD > 2 ? 1280 : 2048) / (TPR < 256 ? 256 : TPR)) quantize_rows_kernel(const RouteParams p, int q_vec) {
+  constexpr int V = Vec<T>::V, THREADS = TPR < 256 ? 256 : TPR;
   __shared__ uint32_t part[THREADS / 32];
   pdl_trigger();
   pdl_wait();
@@ -492,11 +494,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, 2048 / (TPR < 256 ? 256
   const bool row = t < p.T;
   const T *x = static_cast<const T *>(p.src) + t * p.ld_src;
   Vec<T> v[HELD];
-  uint32_t m = 0;
-  auto largest = [&](const Vec<T> &a) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) m = max(m, abs_bits(a.f(i)));
-  };
+  MaxAbs<T> largest;
   if (row) {
 #pragma unroll
     for (int g = 0; g < HELD; ++g) {
@@ -505,10 +503,16 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, 2048 / (TPR < 256 ? 256
       else v[g].zero();
     }
 #pragma unroll
-    for (int g = 0; g < HELD; ++g) largest(v[g]);
-    for (int c = (HELD * TPR + tl) * V; c < p.H; c += TPR * V) largest(load_vec<T, AL>(x, c, p.H));
+    for (int g = 0; g < HELD; ++g) largest.add(v[g]);
+    for (int c = (HELD * TPR + tl) * V; c < p.H; c += TPR * V) largest.add(load_vec<T, AL>(x, c, p.H));
   }
-  m = __reduce_max_sync(0xffffffffu, m);
+  uint32_t m = largest.bits();
+  if constexpr (TPR < 32) {
+#pragma unroll
+    for (int d = TPR / 2; d; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+  } else {
+    m = __reduce_max_sync(0xffffffffu, m);
+  }
   if constexpr (TPR > 32) {
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
     __syncthreads();
@@ -517,7 +521,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, 2048 / (TPR < 256 ? 256
     for (int i = 0; i < TPR / 32; ++i) m = max(m, part[w0 + i]);
   }
   if (!row) return;
-  const RowQuant rq(m);
+  const RowQuant<T> rq(m);
   const int kept = p.kept ? *p.kept : 0, k = p.position ? p.k : 1;
   auto put = [&](int c, const Vec<T> &a) {
     union { int8_t b[V]; uint32_t w[V / 4]; } q;
@@ -558,7 +562,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, 2048 / (TPR < 256 ? 256
       if (s < 0 || s >= (int64_t)p.T * p.k) continue;
       zero = s >= kept;
     }
-    p.scale[s] = zero ? 0.f : rq.scale;
+    p.scale[s] = zero ? 0.f : RowQuant<T>::scale(m);
   }
 }
 

@@ -113,22 +113,54 @@ int sort_setup(int &max_ranks) {
   return MB_OK;
 }
 
+// Lets a kernel use `bytes` of dynamic shared memory; once per kernel and device.
+template <class K>
+int allow_smem(K *kern, int bytes) {
+  static std::mutex mu;
+  static std::map<std::pair<const void *, int>, int> done;
+  thread_local std::pair<const void *, int> last{nullptr, -1};
+  int dev = 0;
+  int rc = cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
+  if (rc) return rc;
+  const std::pair<const void *, int> key{reinterpret_cast<const void *>(kern), dev};
+  if (key == last) return MB_OK;
+  std::lock_guard<std::mutex> lk(mu);
+  int &have = done[key];
+  if (have < bytes) {
+    rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute");
+    if (rc) return rc;
+    have = bytes;
+  }
+  last = key;
+  return MB_OK;
+}
+
 template <class T>
 int launch_quantize(const RouteParams &p, cudaStream_t st, const char *what) {
   constexpr int V = Vec<T>::V;
   const bool al = rows16(p.src, p.ld_src, sizeof(T));
   const int q_vec = reinterpret_cast<uintptr_t>(p.dst) % V == 0 && p.ld_dst % V == 0;
-  // up to two vectors of a row per thread stay in registers
   const int64_t vecs = ceil_div(p.H, V);
-  auto go = [&](auto tpr_) {
-    constexpr int TPR = decltype(tpr_)::value, threads = TPR < 256 ? 256 : TPR;
-    auto kern = al ? quantize_rows_kernel<T, true, TPR> : quantize_rows_kernel<T, false, TPR>;
+  auto go = [&](auto tpr_, auto held_) {
+    constexpr int TPR = decltype(tpr_)::value, HELD = decltype(held_)::value, threads = TPR < 256 ? 256 : TPR;
+    auto kern = al ? quantize_rows_kernel<T, true, TPR, HELD> : quantize_rows_kernel<T, false, TPR, HELD>;
     return launch_pdl(kern, dim3((unsigned)ceil_div(p.T, threads / TPR)), dim3(threads), 0, st, 1, what, p, q_vec);
   };
-  if (vecs <= 64) return go(std::integral_constant<int, 32>());
-  if (vecs <= 256) return go(std::integral_constant<int, 128>());
-  if (vecs <= 512) return go(std::integral_constant<int, 256>());
-  return vecs <= 1024 ? go(std::integral_constant<int, 512>()) : go(std::integral_constant<int, 1024>());
+  using std::integral_constant;
+  // Threads to a row and vectors they hold, by the row's vectors, measured on B200
+  // with 2, 4 and 8 held: many rows want them held by few threads (16384 x 4096
+  // bf16 41.5 us by 128, 44.3 by 256; 8192 x 14336 70 us by 256, 88 by 512), few
+  // rows want many threads (1024 x 4096 3.9 us by 256, 4.5 by 128).
+  if (vecs <= 16) return go(integral_constant<int, 8>(), integral_constant<int, 2>());
+  if (vecs <= 64) return go(integral_constant<int, 32>(), integral_constant<int, 2>());
+  if (vecs <= 128) return go(integral_constant<int, 32>(), integral_constant<int, 4>());
+  if (vecs <= 256) return go(integral_constant<int, 128>(), integral_constant<int, 2>());
+  if (vecs <= 512 && p.T < 4096) return go(integral_constant<int, 256>(), integral_constant<int, 2>());
+  if (vecs <= 512) return go(integral_constant<int, 128>(), integral_constant<int, 4>());
+  if (vecs <= 1024) return go(integral_constant<int, 256>(), integral_constant<int, 4>());
+  if (vecs <= 2048 && p.T < 512) return go(integral_constant<int, 512>(), integral_constant<int, 4>());
+  if (vecs <= 2048) return go(integral_constant<int, 256>(), integral_constant<int, 8>());
+  return go(integral_constant<int, 512>(), integral_constant<int, 8>());
 }
 
 // ------------------------------------------------------------- int8 products with scales
@@ -278,28 +310,6 @@ int sg_plan(const mb_scaled_desc *d, SgPlan &pl) {
   const int64_t trows = pl.swap ? pl.bn : 128 * pl.pair;
   pl.units = (ceil_div(d->M, trows) + (d->groups ? std::min(E, d->M) : 0)) * ceil_div(d->N, pl.swap ? 128 : pl.bn);
   if (pl.units >= (1ll << 31)) return fail(MB_ERR_INVALID, "too many tiles");
-  return MB_OK;
-}
-
-// Lets a kernel use `bytes` of dynamic shared memory; once per kernel and device.
-template <class K>
-int allow_smem(K *kern, int bytes) {
-  static std::mutex mu;
-  static std::map<std::pair<const void *, int>, int> done;
-  thread_local std::pair<const void *, int> last{nullptr, -1};
-  int dev = 0;
-  int rc = cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
-  if (rc) return rc;
-  const std::pair<const void *, int> key{reinterpret_cast<const void *>(kern), dev};
-  if (key == last) return MB_OK;
-  std::lock_guard<std::mutex> lk(mu);
-  int &have = done[key];
-  if (have < bytes) {
-    rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute");
-    if (rc) return rc;
-    have = bytes;
-  }
-  last = key;
   return MB_OK;
 }
 

@@ -4,17 +4,21 @@
 //   amax_r = max_c |x[r, c]|,  scale_r = amax_r / 127,
 //   q[r, c] = rint(127 x[r, c] / amax_r)            (halves to even)
 //
-// The quotient is taken as 127 x over amax, not as x over the rounded scale:
-// for bf16 and fp16 the product 127 x is exact in fp32, and a quotient of two
-// such numbers that is not a half differs from the nearest half by more than
-// an fp32 rounding, so q is the value of the real-number formula, halves
-// included.  (For fp32 x the product rounds once.)
+// The quotient is taken as 127 x over amax, not as x over the rounded scale, and
+// 127 / amax is held as a sum hi + lo of two fp32 numbers, so that
+// fma(x, hi, x lo) is the quotient rounded once to fp32.  For bf16 and fp16 x a
+// quotient that is a half comes out exactly, and one that is not differs from the
+// nearest half by more (2^-19 of it) than that rounding: q is the value of the
+// real-number formula, halves included.  (For fp32 x the product y = 127 x rounds
+// once, and hi + lo stands for 1 / amax.)
 //
 // A row of zeros has scale 0 and q 0.  A row that holds an infinity or a NaN
 // has no scale: it gets scale NaN and q 0, so whatever is computed from it
 // shows NaN.  |q| <= 127 always.
 #pragma once
 #include "mb_common.cuh"
+
+#include <type_traits>
 
 namespace mb {
 
@@ -91,49 +95,97 @@ template <class T, bool AL> __device__ __forceinline__ int frame(const T *row) {
   return -(int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
 }
 
-// |x| of a row as ordered bits: NaN above infinity above every finite value,
-// so an integer maximum never loses a NaN.
-__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+// The largest |x| of a row, as ordered bits: NaN above infinity above every finite
+// value, so an integer maximum never loses a NaN.  16-bit types are compared two
+// to a word, as they come.
+template <class T> struct MaxAbs {
+  uint32_t m = 0;
+  __device__ __forceinline__ void add(const Vec<T> &v) {
+    const uint32_t w[4] = {v.u.q.x, v.u.q.y, v.u.q.z, v.u.q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 2) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+      else m = max(m, w[i] & 0x7fffffffu);
+    }
+  }
+  // As fp32 bits.
+  __device__ __forceinline__ uint32_t bits() const {
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t h = max(m & 0xffffu, m >> 16);
+      if constexpr (std::is_same_v<T, __half>) return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
+      return h << 16;
+    }
+    return m;
+  }
+};
 
-// How a row's elements become integers.
-struct RowQuant {
-  float amax, inv, pre, scale;
+// Two fp32 at a time: the same roundings as one by one.
+__device__ __forceinline__ unsigned long long &bits64(float2 &v) { return reinterpret_cast<unsigned long long &>(v); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 o;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(bits64(o)) : "l"(bits64(a)), "l"(bits64(b)));
+  return o;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 o;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(bits64(o)) : "l"(bits64(a)), "l"(bits64(b)));
+  return o;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 o;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(bits64(o)) : "l"(bits64(a)), "l"(bits64(b)), "l"(bits64(c)));
+  return o;
+}
+
+// How the elements of a row of T become integers.
+template <class T> struct RowQuant {
+  static constexpr bool kLong = sizeof(T) == 4;  // fp32: y = 127 x
+  float hi, lo, pre;
   bool dead;  // zero or non-finite row: q = 0
   __device__ __forceinline__ explicit RowQuant(uint32_t bits) {
+    constexpr float kTop = kLong ? 1.f : 127.f;
     const float m = __uint_as_float(bits);
     dead = bits == 0 || bits >= 0x7f800000u;
-    scale = bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __fdiv_rn(m, 127.f);
-    // a row whose 127 x or 127 / amax would leave fp32's range is moved by a
-    // power of two first (exact, and the same for x and amax)
-    pre = m > 0x1p120f ? 0x1p-64f : (m < 0x1p-100f ? 0x1p64f : 1.f);
-    amax = dead ? 1.f : m * pre;
-    inv = dead ? 0.f : __fdiv_rn(127.f, amax);
+    // a row whose 127 x or 127 / amax would leave fp32's range (lo included) is
+    // moved by a power of two first: exact, and the same for x and amax
+    pre = m > 0x1p90f ? 0x1p-96f : (m < 0x1p-60f ? 0x1p80f : 1.f);
+    const float amax = dead ? 1.f : m * pre;
+    // an approximate quotient serves as hi: lo makes up for what it is off, to
+    // 2^-42 of the sum (three IEEE divisions by every thread of a row were a
+    // third of the kernel's instructions)
+    hi = __fdividef(kTop, amax);
+    lo = fmaf(-hi, amax, kTop) * (hi * (1.f / kTop));
   }
-  // N elements at once.  x * inv is within 2e-5 of the quotient (two roundings
-  // of a value of at most 127), so only a result that near to a half needs the
-  // quotient itself: it is looked for once per N elements, and found for about
-  // one element in 25000.  Adding 1.5 * 2^23 rounds to an integer, halves to
-  // even, and leaves it in the low bits; conversions run at a quarter of that
-  // rate or less, and bf16 rows were bound by them (2.6 TB/s at 16384 x 8192).
+  __device__ static __forceinline__ float scale(uint32_t bits) {
+    return bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __fdiv_rn(__uint_as_float(bits), 127.f);
+  }
+  // N elements at once.  Adding 1.5 * 2^23 rounds to an integer, halves to even,
+  // and leaves it in the low bits.  No division and no branch per element: bf16
+  // significands over each other give halves so often (every other group of 256
+  // elements has one) that deciding them apart took two thirds of all
+  // instructions (16384 x 8192 bf16: 204 a vector of eight, 119 us).
   template <int N>
-  __device__ __forceinline__ void q(const float (&x)[N], uint32_t (&out)[N / 4]) const {
+  __device__ __forceinline__ void q(float (&x)[N], uint32_t (&out)[N / 4]) const {
     constexpr float kMagic = 12582912.f;
-    float r[N], worst = 0.f;
+    if (pre != 1.f) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float t = x[i] * pre * inv;
-      r[i] = t + kMagic;
-      worst = fmaxf(worst, fabsf(t - (r[i] - kMagic)));
+      for (int i = 0; i < N; ++i) x[i] *= pre;
     }
-    if (worst > 0.49997f) {
+    uint32_t r[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) r[i] = __fdiv_rn(x[i] * pre * 127.f, amax) + kMagic;
+    for (int i = 0; i < N; i += 2) {
+      float2 y = make_float2(x[i], x[i + 1]);
+      if constexpr (kLong) y = mul2(y, make_float2(127.f, 127.f));
+      const float2 t = fma2(y, make_float2(hi, hi), mul2(y, make_float2(lo, lo)));
+      const float2 s = add2(t, make_float2(kMagic, kMagic));
+      r[i] = __float_as_uint(s.x);
+      r[i + 1] = __float_as_uint(s.y);
     }
 #pragma unroll
     for (int i = 0; i < N / 4; ++i) {
-      const uint32_t lo = __byte_perm(__float_as_uint(r[4 * i]), __float_as_uint(r[4 * i + 1]), 0x0040);
-      const uint32_t hi = __byte_perm(__float_as_uint(r[4 * i + 2]), __float_as_uint(r[4 * i + 3]), 0x0040);
-      out[i] = dead ? 0u : __byte_perm(lo, hi, 0x5410);
+      const uint32_t a = __byte_perm(r[4 * i], r[4 * i + 1], 0x0040);
+      const uint32_t b = __byte_perm(r[4 * i + 2], r[4 * i + 3], 0x0040);
+      out[i] = dead ? 0u : __byte_perm(a, b, 0x5410);
     }
   }
 };

@@ -37,7 +37,7 @@ def plain_sort(ids, E):
 
 
 SORTS = [(1, 1, 1), (1, 2, 8), (3, 1, 4), (16, 2, 8), (33, 4, 60), (100, 8, 64), (257, 3, 128), (5, 8, 1024),
-         (1000, 2, 7), (4097, 1, 256), (3000, 8, 512), (20000, 4, 16)]
+         (1000, 2, 7), (4097, 1, 256), (3000, 8, 512), (20000, 4, 16), (40000, 4, 70)]
 
 
 @pytest.mark.parametrize("T,k,E", SORTS)

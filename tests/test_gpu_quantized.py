@@ -48,7 +48,8 @@ def plain_quantize(x):
 
 @pytest.mark.parametrize("dtype", FLOATS)
 @pytest.mark.parametrize("rows,cols", [(1, 1), (1, 7), (3, 16), (5, 33), (17, 129), (2, 2048), (64, 4096), (7, 4100),
-                                       (3, 16384), (2, 40000), (1000, 64), (1, 100001)])
+                                       (3, 16384), (2, 40000), (1000, 64), (1, 100001), (4099, 4096), (4096, 2056),
+                                       (600, 14336), (300, 1000), (70, 8200)])
 def test_quantize_is_the_formula(rows, cols, dtype):
     x = torch.randn(rows, cols, generator=gen(rows + cols)).to(dtype).to(DEV)
     q, s = mb.quantize(x)
