@@ -344,18 +344,26 @@ int sg_launch_tile(const SgPlan &pl, sg::SgParams &p, cudaStream_t st) {
                     "scaled_gemm", p);
 }
 
-int sg_pack(const void *src, void *dst, int64_t rows, int64_t cols, int64_t rs, int64_t cs, int64_t bs, int64_t batches,
-            int64_t ld, cudaStream_t st) {
-  PackArgs a{src, dst, rows, cols, rs, cs, bs, batches, ld};
+// Copies the operands that need it (rows of neither: null).  Rows go sixteen
+// bytes a thread; a matrix without a unit stride through tiles.
+int sg_pack(const PackArgs *a, const PackArgs *b, cudaStream_t st) {
   const int64_t cap = (int64_t)device_sms() * 16;
-  if (cs == 1) {
-    const int64_t n = batches * rows * ceil_div(cols, 16);
-    pack_rows16_kernel<uint8_t><<<(unsigned)std::min<int64_t>(ceil_div(n, 256), cap), 256, 0, st>>>(a);
-  } else {
-    const int64_t tiles = batches * ceil_div(rows, 32) * ceil_div(cols, 32);
-    pack_matrix_kernel<uint8_t><<<(unsigned)std::min<int64_t>(tiles, cap), dim3(32, 8), 0, st>>>(a);
+  for (const PackArgs **m : {&a, &b}) {
+    if (!*m || (*m)->cs == 1) continue;
+    const int64_t tiles = (*m)->batch * ceil_div((*m)->rows, 32) * ceil_div((*m)->cols, 32);
+    pack_matrix_kernel<uint8_t><<<(unsigned)std::min<int64_t>(tiles, cap), dim3(32, 8), 0, st>>>(**m);
+    const int rc = cuda_check(cudaGetLastError(), "scaled_gemm: operand copy");
+    if (rc) return rc;
+    *m = nullptr;
   }
-  return cuda_check(cudaGetLastError(), "scaled_gemm: operand copy");
+  auto blocks = [&](const PackArgs *m) {
+    return m ? std::min<int64_t>(ceil_div(m->batch * m->rows * ceil_div(m->cols, 16), 256), cap) : 0;
+  };
+  const int64_t na = blocks(a), nb = blocks(b);
+  if (na + nb == 0) return MB_OK;
+  const PackArgs none{};
+  return launch_pdl(sg::scaled_pack_kernel, dim3((unsigned)(na + nb)), dim3(256), 0, st, 1, "scaled_gemm: operand copy",
+                    a ? *a : none, b ? *b : none, (int)na);
 }
 
 template <class TO>
@@ -384,16 +392,17 @@ int sg_launch(const mb_scaled_desc *d, const SgPlan &pl, cudaStream_t st) {
   }
   const int64_t nB = p.one_b ? 1 : p.groups;
   const void *A = d->A, *B = d->B;
-  int rc = MB_OK;
+  PackArgs pa{}, pb{};
   if (pl.pk_a) {
     A = static_cast<char *>(d->workspace) + pl.a_off;
-    rc = sg_pack(d->A, const_cast<void *>(A), d->M, d->K, d->a_rs, d->a_cs, 0, 1, pl.a_rs, st);
+    pa = PackArgs{d->A, const_cast<void *>(A), d->M, d->K, d->a_rs, d->a_cs, 0, 1, pl.a_rs};
   }
-  if (!rc && pl.pk_b) {
+  if (pl.pk_b) {
     B = static_cast<char *>(d->workspace) + pl.b_off;
-    rc = pl.w_mn ? sg_pack(d->B, const_cast<void *>(B), d->K, d->N, d->b_rs, d->b_cs, d->sB, nB, pl.w_ld, st)
-                 : sg_pack(d->B, const_cast<void *>(B), d->N, d->K, d->b_cs, d->b_rs, d->sB, nB, pl.w_ld, st);
+    pb = pl.w_mn ? PackArgs{d->B, const_cast<void *>(B), d->K, d->N, d->b_rs, d->b_cs, d->sB, nB, pl.w_ld}
+                 : PackArgs{d->B, const_cast<void *>(B), d->N, d->K, d->b_cs, d->b_rs, d->sB, nB, pl.w_ld};
   }
+  int rc = sg_pack(pl.pk_a ? &pa : nullptr, pl.pk_b ? &pb : nullptr, st);
   if (rc) return rc;
   // boxes of 128 bytes along the contiguous dimension
   CUtensorMap *ta = pl.swap ? &p.tmB : &p.tmA, *tw = pl.swap ? &p.tmA : &p.tmB;

@@ -35,6 +35,7 @@
 // by cluster rank i * split / 8, and the other ranks send it their s32 partial
 // sums through distributed shared memory.
 #pragma once
+#include "pack.cuh"
 #include "tc_gemm.cuh"
 
 namespace mb {
@@ -611,6 +612,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
     tc_fence_after();
     tmem_dealloc_g<PAIR>(tmem_base, B_::TMEM_COLS);
   }
+}
+
+// Operands that TMA cannot read in place, copied to aligned rows: A's rows by the
+// first `split` blocks, B's by the others, in one launch.
+__global__ static void __launch_bounds__(256) scaled_pack_kernel(const PackArgs a, const PackArgs b, int split) {
+  pdl_trigger();
+  pdl_wait();
+  if ((int)blockIdx.x < split) pack_rows16<uint8_t>(a, blockIdx.x, split);
+  else pack_rows16<uint8_t>(b, blockIdx.x - split, gridDim.x - split);
 }
 
 // K = 0: the sum is empty.
