@@ -238,40 +238,61 @@ template <class T> __device__ __forceinline__ const T *row_of(const void *base, 
   return static_cast<const T *>(base) + r * ld;
 }
 
-// In the kernels below a vector that sticks out of its row (the row's end, or its
-// start where rows are not aligned) takes a plain loop over its elements, kept
-// apart so that the vectors inside are loaded without a branch between them.
+// AL below: every row starts on 16 bytes and holds whole vectors.
+//
+// The elements of a row that no whole vector of its frame holds: the first `head`
+// ones and those from `tail` on, fewer than two vectors of them.  The kernels
+// below give them a lane each after the vectors; taken by the vectors' own
+// threads, one by one, they cost more than the row (combine of 8192 x 8 x 4099
+// bf16: 243 us).
+struct Edges {
+  int head, tail, H;
+  __device__ __forceinline__ Edges(int frame, int H_, int V) : H(H_) {
+    head = frame < 0 ? min(V + frame, H) : 0;
+    tail = max(head, frame + (H - frame) / V * V);
+  }
+  __device__ __forceinline__ int count() const { return head + H - tail; }
+  __device__ __forceinline__ int column(int e) const { return e < head ? e : tail + e - head; }
+};
 
 template <class T, int NE, bool AL>
 __global__ void __launch_bounds__(kRouteThreads) expert_gather_kernel(const RouteParams p, int lanes) {
   constexpr int V = Vec<T>::V;
   pdl_trigger();
   pdl_wait();
-  const int t = blockIdx.x * (kRouteThreads / lanes) + threadIdx.x / lanes;
+  const int t = blockIdx.x * (kRouteThreads / lanes) + threadIdx.x / lanes, tl = threadIdx.x % lanes;
   if (t >= p.T) return;
   const int kept = p.kept ? *p.kept : 0;
   const T *x = row_of<T>(p.src, t, p.ld_src);
-  const int v0 = blockIdx.y * lanes + threadIdx.x % lanes, dv = gridDim.y * lanes;
+  const int v0 = blockIdx.y * lanes + tl, dv = gridDim.y * lanes;
   for (int j0 = 0; j0 < p.k; j0 += NE) {
     int slot[NE];
     load_slots(p, t, j0, slot);
     for (int c = v0 * V; c < p.H + (AL ? 0 : V); c += dv * V) {
       Vec<T> v;
-      const bool in = c + V <= p.H;
-      if (AL && in) v = load16<T, AL>(x + c);
+      if constexpr (AL) v = load16<T, AL>(x + c);
 #pragma unroll
       for (int j = 0; j < NE; ++j) {
         if (slot[j] < 0) continue;
         T *d = row_of<T>(p.dst, slot[j], p.ld_dst);
         const int cc = c + frame<T, AL>(d);
-        if (AL ? in : (cc >= 0 && cc + V <= p.H)) {
-          if constexpr (!AL) v = load16<T, AL>(x + cc);
-          Vec<T> o = v;
-          if (slot[j] >= kept) o.zero();
-          *reinterpret_cast<uint4 *>(d + cc) = o.u.q;
-        } else {
-#pragma unroll 1
-          for (int i = max(cc, 0); i < min(cc + V, p.H); ++i) d[i] = slot[j] < kept ? x[i] : Elem<T>::store(0.f);
+        if (!AL && (cc < 0 || cc + V > p.H)) continue;
+        if constexpr (!AL) v = load16<T, AL>(x + cc);
+        Vec<T> o = v;
+        if (slot[j] >= kept) o.zero();
+        *reinterpret_cast<uint4 *>(d + cc) = o.u.q;
+      }
+    }
+    if constexpr (!AL) {
+      if (blockIdx.y) continue;
+#pragma unroll
+      for (int j = 0; j < NE; ++j) {
+        if (slot[j] < 0) continue;
+        T *d = row_of<T>(p.dst, slot[j], p.ld_dst);
+        const Edges g(frame<T, AL>(d), p.H, V);
+        for (int e = tl; e < g.count(); e += lanes) {
+          const int c = g.column(e);
+          d[c] = slot[j] < kept ? x[c] : Elem<T>::store(0.f);
         }
       }
     }
@@ -285,13 +306,13 @@ __global__ void __launch_bounds__(kRouteThreads) expert_combine_kernel(const Rou
   constexpr int V = Vec<T>::V;
   pdl_trigger();
   pdl_wait();
-  const int t = blockIdx.x * (kRouteThreads / lanes) + threadIdx.x / lanes;
+  const int t = blockIdx.x * (kRouteThreads / lanes) + threadIdx.x / lanes, tl = threadIdx.x % lanes;
   if (t >= p.T) return;
   const int kept = p.kept ? *p.kept : 0;
   const TW *w = static_cast<const TW *>(p.w);
   T *out = row_of<T>(p.dst, t, p.ld_dst);
   const int c0 = frame<T, AL>(out);
-  const int v0 = blockIdx.y * lanes + threadIdx.x % lanes, dv = gridDim.y * lanes;
+  const int v0 = blockIdx.y * lanes + tl, dv = gridDim.y * lanes;
   int slot[NE];
   float wj[NE];
   auto entries = [&](int j0) {
@@ -303,49 +324,54 @@ __global__ void __launch_bounds__(kRouteThreads) expert_combine_kernel(const Rou
     }
   };
   if (p.k <= NE) entries(0);
-  for (int c = c0 + v0 * V; c < p.H; c += dv * V) {
-    if (c >= 0 && c + V <= p.H) {
-      float acc[V];
+  for (int c = c0 + v0 * V; AL ? c < p.H : c + V <= p.H; c += dv * V) {
+    if (!AL && c < 0) continue;
+    float acc[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] = 0.f;
-      for (int j0 = 0; j0 < p.k; j0 += NE) {
-        if (p.k > NE) entries(j0);
-        Vec<T> v[NE];
-        uint4 next[AL ? 1 : NE];
+    for (int i = 0; i < V; ++i) acc[i] = 0.f;
+    for (int j0 = 0; j0 < p.k; j0 += NE) {
+      if (p.k > NE) entries(j0);
+      Vec<T> v[NE];
+      uint4 next[AL ? 1 : NE];
 #pragma unroll
-        for (int j = 0; j < NE; ++j) {
-          const T *y = row_of<T>(p.src, max(slot[j], 0), p.ld_src) + c;
-          const uint32_t off = AL ? 0u : (uint32_t)(reinterpret_cast<uintptr_t>(y) & 15);
-          const char *word = reinterpret_cast<const char *>(y) - off;
-          v[j].u.q = load_once(word, slot[j] >= 0);
-          if constexpr (!AL) next[j] = load_once(word + 16, slot[j] >= 0 && off);
-        }
-        if constexpr (!AL) {
-#pragma unroll
-          for (int j = 0; j < NE; ++j)
-            v[j].u.q = cut16(v[j].u.q, next[j],
-                             (uint32_t)reinterpret_cast<uintptr_t>(row_of<T>(p.src, max(slot[j], 0), p.ld_src) + c) & 15);
-        }
+      for (int j = 0; j < NE; ++j) {
+        const T *y = row_of<T>(p.src, max(slot[j], 0), p.ld_src) + c;
+        const uint32_t off = AL ? 0u : (uint32_t)(reinterpret_cast<uintptr_t>(y) & 15);
+        const char *word = reinterpret_cast<const char *>(y) - off;
+        v[j].u.q = load_once<!AL>(word, slot[j] >= 0);
+        if constexpr (!AL) next[j] = load_once<true>(word + 16, slot[j] >= 0 && off);
+      }
+      if constexpr (!AL) {
 #pragma unroll
         for (int j = 0; j < NE; ++j)
-#pragma unroll
-          for (int i = 0; i < V; ++i) acc[i] = fmaf(wj[j], v[j].f(i), acc[i]);
+          v[j].u.q = cut16(v[j].u.q, next[j],
+                           (uint32_t)reinterpret_cast<uintptr_t>(row_of<T>(p.src, max(slot[j], 0), p.ld_src) + c) & 15);
       }
-      Vec<T> o;
 #pragma unroll
-      for (int i = 0; i < V; ++i) o.set(i, acc[i]);
-      *reinterpret_cast<uint4 *>(out + c) = o.u.q;
-    } else {
-#pragma unroll 1
-      for (int i = max(c, 0); i < min(c + V, p.H); ++i) {
-        float acc = 0.f;
-        for (int j = 0; j < p.k; ++j) {
-          const int s = p.position[(int64_t)t * p.k + j];
-          if (s < 0 || s >= kept || s >= p.T * p.k) continue;
-          acc = fmaf(w ? to_f32(w[(int64_t)t * p.k + j]) : 1.f, to_f32(row_of<T>(p.src, s, p.ld_src)[i]), acc);
-        }
-        out[i] = Elem<T>::store(acc);
+      for (int j = 0; j < NE; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = fmaf(wj[j], v[j].f(i), acc[i]);
+    }
+    Vec<T> o;
+#pragma unroll
+    for (int i = 0; i < V; ++i) o.set(i, acc[i]);
+    *reinterpret_cast<uint4 *>(out + c) = o.u.q;
+  }
+  if constexpr (!AL) {
+    if (blockIdx.y) return;
+    const Edges g(c0, p.H, V);
+    for (int e = tl; e < g.count(); e += lanes) {
+      const int c = g.column(e);
+      float acc = 0.f;
+      for (int j0 = 0; j0 < p.k; j0 += NE) {
+        if (p.k > NE) entries(j0);
+        float y[NE];
+#pragma unroll
+        for (int j = 0; j < NE; ++j) y[j] = slot[j] >= 0 ? to_f32(row_of<T>(p.src, slot[j], p.ld_src)[c]) : 0.f;
+#pragma unroll
+        for (int j = 0; j < NE; ++j) acc = fmaf(wj[j], y[j], acc);
       }
+      out[c] = Elem<T>::store(acc);
     }
   }
 }
@@ -366,16 +392,17 @@ __global__ void __launch_bounds__(kRouteThreads) expert_combine_backward_kernel(
   const int kept = p.kept ? *p.kept : 0;
   const TW *w = static_cast<const TW *>(p.w);
   const T *dout = row_of<T>(p.src, t, p.ld_src);
-  // one entry's elements i0 .. i1-1, one at a time; their share of its dot product
-  auto by_element = [&](int s, float ws, int i0, int i1) {
-    float sum = 0.f;
+  // The edge elements of entry slot s with weight ws; returns their share of its dot product.
+  auto edges = [&](int s, float ws, int frame_) {
     T *dy = row_of<T>(p.dst, s, p.ld_dst);
     const T *y = row_of<T>(p.src2, s, p.ld_src2);
-#pragma unroll 1
-    for (int i = i0; i < i1; ++i) {
-      const float d = to_f32(dout[i]);
-      dy[i] = Elem<T>::store(s < kept ? ws * d : 0.f);
-      if (s < kept) sum = fmaf(d, to_f32(y[i]), sum);
+    const Edges g(frame_, p.H, V);
+    float sum = 0.f;
+    for (int e = tl; e < g.count(); e += lanes) {
+      const int c = g.column(e);
+      const float d = to_f32(dout[c]);
+      dy[c] = Elem<T>::store(s < kept ? ws * d : 0.f);
+      if (s < kept) sum = fmaf(d, to_f32(y[c]), sum);
     }
     return sum;
   };
@@ -399,32 +426,26 @@ __global__ void __launch_bounds__(kRouteThreads) expert_combine_backward_kernel(
       for (int j = 0; j < NE; ++j) dot[j] = 0.f;
       if (t < p.T) {
         for (int c = tl * V; c < p.H; c += lanes * V) {
-          if (c + V <= p.H) {
-            const Vec<T> d = load16<T, AL>(dout + c);
-            Vec<T> y[NE];
+          const Vec<T> d = load16<T, AL>(dout + c);
+          Vec<T> y[NE];
 #pragma unroll
-            for (int j = 0; j < NE; ++j) {
-              y[j].zero();
-              if (slot[j] >= 0 && slot[j] < kept) y[j] = load16<T, AL>(row_of<T>(p.src2, slot[j], p.ld_src2) + c);
-            }
+          for (int j = 0; j < NE; ++j) {
+            y[j].zero();
+            if (slot[j] >= 0 && slot[j] < kept) y[j] = load16<T, AL>(row_of<T>(p.src2, slot[j], p.ld_src2) + c);
+          }
 #pragma unroll
-            for (int j = 0; j < NE; ++j) {
-              if (slot[j] < 0) continue;
-              Vec<T> o;
-              o.zero();
-              if (slot[j] < kept) {
+          for (int j = 0; j < NE; ++j) {
+            if (slot[j] < 0) continue;
+            Vec<T> o;
+            o.zero();
+            if (slot[j] < kept) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                  dot[j] = fmaf(d.f(i), y[j].f(i), dot[j]);
-                  o.set(i, wj[j] * d.f(i));
-                }
+              for (int i = 0; i < V; ++i) {
+                dot[j] = fmaf(d.f(i), y[j].f(i), dot[j]);
+                o.set(i, wj[j] * d.f(i));
               }
-              *reinterpret_cast<uint4 *>(row_of<T>(p.dst, slot[j], p.ld_dst) + c) = o.u.q;
             }
-          } else {
-#pragma unroll
-            for (int j = 0; j < NE; ++j)
-              if (slot[j] >= 0) dot[j] += by_element(slot[j], wj[j], c, p.H);
+            *reinterpret_cast<uint4 *>(row_of<T>(p.dst, slot[j], p.ld_dst) + c) = o.u.q;
           }
         }
       }
@@ -443,24 +464,22 @@ __global__ void __launch_bounds__(kRouteThreads) expert_combine_backward_kernel(
           const T *y = row_of<T>(p.src2, s, p.ld_src2);
           const float ws = s < kept ? to_f32(w[(int64_t)t * p.k + j0 + j]) : 0.f;
           const int c0 = frame<T, AL>(dy);
-#pragma unroll 2
-          for (int c = c0 + tl * V; c < p.H; c += lanes * V) {
-            if (c >= 0 && c + V <= p.H) {
-              Vec<T> o;
-              o.zero();
-              if (s < kept) {
-                const Vec<T> d = load16<T, AL>(dout + c), yv = load16<T, AL>(y + c);
+#pragma unroll 4
+          for (int c = c0 + tl * V; c + V <= p.H; c += lanes * V) {
+            if (c < 0) continue;
+            Vec<T> o;
+            o.zero();
+            if (s < kept) {
+              const Vec<T> d = load16<T, AL>(dout + c), yv = load16<T, AL>(y + c);
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                  dot = fmaf(d.f(i), yv.f(i), dot);
-                  o.set(i, ws * d.f(i));
-                }
+              for (int i = 0; i < V; ++i) {
+                dot = fmaf(d.f(i), yv.f(i), dot);
+                o.set(i, ws * d.f(i));
               }
-              *reinterpret_cast<uint4 *>(dy + c) = o.u.q;
-            } else {
-              dot += by_element(s, ws, max(c, 0), min(c + V, p.H));
             }
+            *reinterpret_cast<uint4 *>(dy + c) = o.u.q;
           }
+          dot += edges(s, ws, c0);
         }
         dot = warp_sum(dot);
         if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5][j] = dot;

@@ -530,7 +530,7 @@ int mb_expert_gather(int32_t dtype, int64_t tokens, int64_t k, int64_t cols, con
     RouteParams p{};
     p.T = (int)tokens; p.H = (int)cols; p.k = (int)k; p.position = position; p.kept = kept;
     p.src = x; p.ld_src = ldx; p.dst = sorted; p.ld_dst = lds;
-    const bool al = rows16(x, ldx, sizeof(T)) && rows16(sorted, lds, sizeof(T));
+    const bool al = rows16(x, ldx, sizeof(T)) && rows16(sorted, lds, sizeof(T)) && cols % Vec<T>::V == 0;
     const int lanes = route_lanes(cols, sizeof(T), false);
     auto kern = k <= 2 ? (al ? expert_gather_kernel<T, 2, true> : expert_gather_kernel<T, 2, false>)
                        : (al ? expert_gather_kernel<T, 8, true> : expert_gather_kernel<T, 8, false>);
@@ -573,7 +573,7 @@ int mb_expert_combine(int32_t dtype, int32_t weights_dtype, int64_t tokens, int6
     RouteParams p{};
     p.T = (int)tokens; p.H = (int)cols; p.k = (int)k; p.position = position; p.kept = kept;
     p.src = sorted; p.ld_src = lds; p.w = weights; p.dst = out; p.ld_dst = ldo;
-    const bool al = rows16(sorted, lds, sizeof(T)) && rows16(out, ldo, sizeof(T));
+    const bool al = rows16(sorted, lds, sizeof(T)) && rows16(out, ldo, sizeof(T)) && cols % Vec<T>::V == 0;
     const int lanes = route_lanes(cols, sizeof(T), false);
     const bool f32 = weights_dtype == MB_F32;
     auto pick = [&](auto ne) {
@@ -606,7 +606,8 @@ int mb_expert_combine_backward(int32_t dtype, int32_t weights_dtype, int64_t tok
     p.T = (int)tokens; p.H = (int)cols; p.k = (int)k; p.position = position; p.kept = kept;
     p.src = dout; p.ld_src = ldd; p.src2 = sorted; p.ld_src2 = lds; p.w = weights;
     p.dst = dsorted; p.ld_dst = ldds; p.dst2 = dweights;
-    const bool al = rows16(dout, ldd, sizeof(T)) && rows16(sorted, lds, sizeof(T)) && rows16(dsorted, ldds, sizeof(T));
+    const bool al = rows16(dout, ldd, sizeof(T)) && rows16(sorted, lds, sizeof(T)) &&
+                    rows16(dsorted, ldds, sizeof(T)) && cols % Vec<T>::V == 0;
     const int lanes = route_lanes(cols, sizeof(T), true);
     const bool f32 = weights_dtype == MB_F32;
     auto pick = [&](auto ne) {
