@@ -236,7 +236,8 @@ SgCost sg_cost(const mb_scaled_desc *d, int swap, int bn, int pair, int sms, int
     const double slots = std::floor((double)sms / (pair * split) * (split >= 4 ? 0.9 : 1.0));
     const double waves = std::ceil(units / slots);
     const double compute = waves * std::max(std::ceil(kb / split) * kbc + hand + log2 * (500.0 + 40.0 * bn), epi);
-    const double t = std::max(compute, bytes / (22.4 * sms)) * (1.0 + 0.01 * log2);
+    const double hbm = bytes / (22.4 * sms);
+    const double t = std::max(compute, hbm) + 0.15 * std::min(compute, hbm);  // they overlap, not quite
     if (t < best.t) best = {t, split};
   }
   return best;
