@@ -215,9 +215,12 @@ struct RouteParams {
 // token, so that short rows still fill warps and long ones have a block; a
 // token's columns are shared out over blockIdx.y as well.
 constexpr int kRouteThreads = 256;
-// A token's entries are worked on NE (2 or 8) at a time: the rows of a batch are
-// in flight together, and a batch wider than k would be spent on nothing (k = 2
-// with batches of 8: combine 84 us, 2.4 TB/s, at 8192 tokens of 4096 bf16).
+// A token's entries are worked on NE (2, 4 or 8) at a time: the rows of a batch
+// are in flight together, a batch wider than k is spent on nothing (k = 2 in
+// batches of 8: combine of 8192 tokens of 4096 bf16 84 us against 36), and a
+// batch's registers cost threads.  Measured at k = 8: combine of aligned bf16 rows
+// 95.7 us in eights and 102 in fours, of fp32 rows 219 and 190, of unaligned bf16
+// rows 170 and 159; its gradient 191 and 183.
 
 // Slots of entries j0 .. j0+NE-1 of token t: -1 for none (past k, or a number that
 // is no row of the buffer).
@@ -430,8 +433,7 @@ __global__ void __launch_bounds__(kRouteThreads) expert_combine_backward_kernel(
           Vec<T> y[NE];
 #pragma unroll
           for (int j = 0; j < NE; ++j) {
-            y[j].zero();
-            if (slot[j] >= 0 && slot[j] < kept) y[j] = load16<T, AL>(row_of<T>(p.src2, slot[j], p.ld_src2) + c);
+            y[j].u.q = load_once(row_of<T>(p.src2, max(slot[j], 0), p.ld_src2) + c, slot[j] >= 0 && slot[j] < kept);
           }
 #pragma unroll
           for (int j = 0; j < NE; ++j) {

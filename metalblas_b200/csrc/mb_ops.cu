@@ -534,7 +534,9 @@ int mb_expert_gather(int32_t dtype, int64_t tokens, int64_t k, int64_t cols, con
     const bool al = rows16(x, ldx, sizeof(T)) && rows16(sorted, lds, sizeof(T)) && cols % Vec<T>::V == 0;
     const int lanes = route_lanes(cols, sizeof(T), false);
     auto kern = k <= 2 ? (al ? expert_gather_kernel<T, 2, true> : expert_gather_kernel<T, 2, false>)
-                       : (al ? expert_gather_kernel<T, 8, true> : expert_gather_kernel<T, 8, false>);
+                       : (al ? expert_gather_kernel<T, 4, true> : expert_gather_kernel<T, 4, false>);
+    if constexpr (sizeof(T) == 2)
+      if (k > 4 && al) kern = expert_gather_kernel<T, 8, true>;
     return launch_pdl(kern,
                       route_grid(tokens, cols, sizeof(T), lanes, false), dim3(kRouteThreads), 0, (cudaStream_t)stream, 1,
                       "expert_gather", p, lanes);
@@ -582,7 +584,9 @@ int mb_expert_combine(int32_t dtype, int32_t weights_dtype, int64_t tokens, int6
       return al ? (f32 ? expert_combine_kernel<T, float, NE, true> : expert_combine_kernel<T, T, NE, true>)
                 : (f32 ? expert_combine_kernel<T, float, NE, false> : expert_combine_kernel<T, T, NE, false>);
     };
-    auto kern = k <= 2 ? pick(std::integral_constant<int, 2>()) : pick(std::integral_constant<int, 8>());
+    auto kern = k <= 2 ? pick(std::integral_constant<int, 2>()) : pick(std::integral_constant<int, 4>());
+    if constexpr (sizeof(T) == 2)
+      if (k > 4 && al) kern = f32 ? expert_combine_kernel<T, float, 8, true> : expert_combine_kernel<T, T, 8, true>;
     return launch_pdl(kern, route_grid(tokens, cols, sizeof(T), lanes, false), dim3(kRouteThreads), 0,
                       (cudaStream_t)stream, 1, "expert_combine", p, lanes);
   });
@@ -616,7 +620,7 @@ int mb_expert_combine_backward(int32_t dtype, int32_t weights_dtype, int64_t tok
       return al ? (f32 ? expert_combine_backward_kernel<T, float, NE, true> : expert_combine_backward_kernel<T, T, NE, true>)
                 : (f32 ? expert_combine_backward_kernel<T, float, NE, false> : expert_combine_backward_kernel<T, T, NE, false>);
     };
-    auto kern = k <= 2 ? pick(std::integral_constant<int, 2>()) : pick(std::integral_constant<int, 8>());
+    auto kern = k <= 2 ? pick(std::integral_constant<int, 2>()) : pick(std::integral_constant<int, 4>());
     return launch_pdl(kern, route_grid(tokens, cols, sizeof(T), lanes, true), dim3(kRouteThreads), 0,
                       (cudaStream_t)stream, 1, "expert_combine_backward", p, lanes);
   });
