@@ -265,7 +265,8 @@ int mb_quantize(int32_t dtype, int64_t rows, int64_t cols, const void *x, int64_
  *   groups >= 1: `groups` matrices B, sB apart; offsets is a device array of
  *     groups + 1 ascending row numbers starting at 0; rows
  *     offsets[e] .. offsets[e+1]-1 use B_e, rows at or past offsets[groups] are
- *     set to zero.  Values outside 0..M are taken as the nearest of the two.
+ *     set to zero.  Values outside 0..M are taken as the nearest of the two; if
+ *     they are not ascending, every row is set to zero.
  * Operands with a unit stride, a 16-byte aligned base and 16-byte multiples in
  * the other strides are read in place; others are copied into the workspace
  * first.  K <= 131071, so that no sum leaves 32 bits. */
@@ -298,7 +299,7 @@ int mb_scaled_plan(const mb_scaled_desc *d, char *buf, int buflen);
 /* Entries 0..n-1 by ids (int32, or int64 with ids64), stable; ids outside
  * 0..experts-1 last.  order[slot] = entry, position[entry] = slot,
  * offsets[e] = first slot of expert e, offsets[experts] = entries kept.
- * experts <= 1024, n < 2^31. */
+ * experts <= 1024, n < 2^31 - 2^16. */
 int mb_expert_sort(int32_t ids64, int64_t n, int64_t experts, const void *ids, int32_t *order, int32_t *position,
                    int32_t *offsets, void *stream);
 

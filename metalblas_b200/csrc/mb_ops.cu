@@ -6,7 +6,6 @@
 #include <atomic>
 #include <cmath>
 #include <cstring>
-#include <map>
 #include <type_traits>
 
 #include "mb_host.cuh"
@@ -55,7 +54,7 @@ int check_rows(int dt, int64_t rows, int64_t cols, int64_t ld, const void *p, co
 
 int check_route(int64_t T, int64_t k, int64_t H, const int32_t *position, const int32_t *kept) {
   if (T < 0 || k < 0 || H < 0) return fail(MB_ERR_INVALID, "negative extent");
-  if (k && T > 0x7fffffffll / k) return fail(MB_ERR_INVALID, "tokens * k must stay below 2^31");
+  if (T > 0x7fff0000ll || (k && T > 0x7fff0000ll / k)) return fail(MB_ERR_INVALID, "tokens * k must stay below 2^31 - 2^16");
   if (T * k > 0 && (!position || !kept)) return fail(MB_ERR_INVALID, "null position or kept");
   return MB_OK;
 }
@@ -114,25 +113,17 @@ int sort_setup(int &max_ranks) {
 }
 
 // Lets a kernel use `bytes` of dynamic shared memory; once per kernel and device.
-template <class K>
-int allow_smem(K *kern, int bytes) {
-  static std::mutex mu;
-  static std::map<std::pair<const void *, int>, int> done;
-  thread_local std::pair<const void *, int> last{nullptr, -1};
+template <auto Kernel>
+int allow_smem(int bytes) {
+  static std::atomic<bool> done[64];
   int dev = 0;
   int rc = cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
   if (rc) return rc;
-  const std::pair<const void *, int> key{reinterpret_cast<const void *>(kern), dev};
-  if (key == last) return MB_OK;
-  std::lock_guard<std::mutex> lk(mu);
-  int &have = done[key];
-  if (have < bytes) {
-    rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute");
-    if (rc) return rc;
-    have = bytes;
-  }
-  last = key;
-  return MB_OK;
+  const bool keep = dev >= 0 && dev < 64;
+  if (keep && done[dev].load(std::memory_order_acquire)) return MB_OK;
+  rc = cuda_check(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute");
+  if (!rc && keep) done[dev].store(true, std::memory_order_release);
+  return rc;
 }
 
 template <class T>
@@ -168,7 +159,7 @@ int scaled_check(const mb_scaled_desc *d) {
   if (!d) return fail(MB_ERR_INVALID, "null descriptor");
   if (!is_float(d->out_dtype)) return fail(MB_ERR_UNSUPPORTED, "out_dtype %d is not fp32, fp16 or bf16", d->out_dtype);
   if (d->M < 0 || d->N < 0 || d->K < 0 || d->groups < 0) return fail(MB_ERR_INVALID, "negative extent");
-  if (d->M > 0x7fffff00ll || d->N > 0x7fffff00ll) return fail(MB_ERR_INVALID, "M and N must stay below 2^31");
+  if (d->M > 0x7fff0000ll || d->N > 0x7fff0000ll) return fail(MB_ERR_INVALID, "M and N must stay below 2^31 - 2^16");
   if (d->K > 131071) return fail(MB_ERR_INVALID, "K = %lld: sums of more than 131071 int8 products can leave 32 bits", (long long)d->K);
   if (d->groups > 1024) return fail(MB_ERR_INVALID, "more than 1024 groups");
   if (d->M == 0 || d->N == 0) return MB_OK;
@@ -320,8 +311,8 @@ int gemv_launch(const mb_scaled_desc *d, const SgPlan &pl, const sg::SgParams &p
   g.A = d->A; g.B = d->B; g.a_rs = pl.a_rs; g.b_rs = pl.w_ld; g.sB = pl.sB;
   g.K = (int)d->K;
   g.max_rows = (int)gemv_max_rows(d);
-  auto kern = sg::scaled_gemv_kernel<MR, GROUPED, TO>;
-  const int rc = allow_smem(kern, kGemvSmem);
+  constexpr auto kern = sg::scaled_gemv_kernel<MR, GROUPED, TO>;
+  const int rc = allow_smem<kern>(kGemvSmem);
   if (rc) return rc;
   return launch_pdl(kern, dim3((unsigned)(device_sms() * sg::GEMV_BLOCKS_PER_SM)), dim3(sg::GEMV_THREADS),
                     (size_t)gemv_smem(d), st, 1, "scaled_gemm", p, g);
@@ -333,11 +324,11 @@ int sg_launch_tile(const SgPlan &pl, sg::SgParams &p, cudaStream_t st) {
   p.split = pl.split;
   p.stages = C_::stages(pl.split);
   p.tiles_c = (int)ceil_div(p.N, C_::TCOLS);
-  auto kern = sg::scaled_gemm_kernel<BN, PAIR, SWAP, TO>;
+  constexpr auto kern = sg::scaled_gemm_kernel<BN, PAIR, SWAP, TO>;
   constexpr int smem_max = C_::CAN_SPLIT ? std::max(C_::smem_bytes(1), std::max(C_::smem_bytes(2), std::max(C_::smem_bytes(4), C_::smem_bytes(8))))
                                          : C_::smem_bytes(1);
   static_assert(smem_max <= tc::SMEM_LIMIT, "shared memory");
-  const int rc = allow_smem(kern, smem_max);
+  const int rc = allow_smem<kern>(smem_max);
   if (rc) return rc;
   const int csize = PAIR == 2 ? 2 : pl.split;
   const int64_t clusters = std::min<int64_t>(pl.units, device_sms() / csize);
@@ -445,7 +436,7 @@ int mb_quantize(int32_t dtype, int64_t rows, int64_t cols, const void *x, int64_
   if (rc) return rc;
   if (rows == 0) return MB_OK;
   if (!scale) return fail(MB_ERR_INVALID, "quantize: null scale");
-  if (rows > 0x7fffffff) return fail(MB_ERR_INVALID, "quantize: more than 2^31 - 1 rows");
+  if (rows > 0x7fff0000ll) return fail(MB_ERR_INVALID, "quantize: more than 2^31 - 2^16 rows");
   return by_float(dtype, [&](auto *tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     RouteParams p{};

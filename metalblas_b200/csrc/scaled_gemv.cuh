@@ -109,12 +109,18 @@ scaled_gemv_kernel(const __grid_constant__ SgParams p, const GemvArgs g) {
   int live = p.M;  // rows that belong to a group
   if constexpr (GROUPED) {
     // a row's group: the number of groups that end at or before it (p.groups: none)
+    // (offsets that are not ascending: none for any row)
+    int wrong = 0;
     for (int e = tid; e < p.groups; e += GEMV_THREADS) {
       const int end = p.offsets[e + 1];
+      wrong |= e && min(max(end, 0), p.M) < min(max(p.offsets[e], 0), p.M);
       for (int m = 0; m < p.M; ++m)
         if (end <= m) atomicAdd(group_of + m, 1);
     }
-    __syncthreads();
+    if (__syncthreads_or(wrong)) {
+      if (tid < p.M) group_of[tid] = p.groups;
+      __syncthreads();
+    }
     while (live > 0 && group_of[live - 1] >= p.groups) --live;
     share((int64_t)live * p.N);
   }

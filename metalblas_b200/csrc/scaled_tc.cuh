@@ -254,12 +254,20 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
       first_unit[1] = (p.M + C_::TROWS - 1) / C_::TROWS * p.tiles_c;
     }
   } else {
-    for (int e = threadIdx.x; e <= G; e += NUM_THREADS) row0[e] = min(max(p.offsets[e], 0), p.M);
+    for (int e = threadIdx.x; e <= G; e += NUM_THREADS) row0[e] = e ? min(max(p.offsets[e], 0), p.M) : 0;
     __syncthreads();
+    // Offsets that are not ascending name no groups: every row comes out as zeros
+    // (and no count below can leave the range the host has checked).
+    int wrong = 0;
+    for (int e = threadIdx.x; e < G; e += NUM_THREADS) wrong |= row0[e + 1] < row0[e];
+    if (__syncthreads_or(wrong)) {
+      for (int e = threadIdx.x; e <= G; e += NUM_THREADS) row0[e] = 0;
+      __syncthreads();
+    }
     // each thread sums `per` consecutive groups, then a scan over threads
     const int per = (G + NUM_THREADS - 1) / NUM_THREADS;
     const int e0 = min(G, (int)threadIdx.x * per), e1 = min(G, e0 + per);
-    auto units_of = [&](int e) { return (max(row0[e + 1] - row0[e], 0) + C_::TROWS - 1) / C_::TROWS * p.tiles_c; };
+    auto units_of = [&](int e) { return (row0[e + 1] - row0[e] + C_::TROWS - 1) / C_::TROWS * p.tiles_c; };
     int sum = 0;
     for (int e = e0; e < e1; ++e) sum += units_of(e);
     int upto = sum;

@@ -212,7 +212,8 @@ def grouped_scaled_mm(a, b, scale_a, scale_b, offsets, *, out_dtype=None, out=No
     ``b [E, K, N]`` and scaled by ``scale_a [M]`` and ``scale_b [E, N]``; rows at or past
     ``offsets[E]`` come out as zeros.  ``offsets`` is an int32 device tensor of ``E + 1``
     ascending row numbers starting at 0 (``expert_sort``'s): the host never reads it, empty
-    groups cost nothing, and E is at most 1024.
+    groups cost nothing, and E is at most 1024.  Numbers that are not ascending name no groups:
+    every row comes out as zeros.
     """
     if out is None and _plan is None:
         c = _try_scaled(a, b, scale_a, scale_b, offsets, None, out_dtype or torch.bfloat16)

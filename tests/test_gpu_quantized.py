@@ -321,6 +321,17 @@ def test_grouped_offsets_outside_the_rows_stay_inside():
     assert bool((room[M:] == 9).all())
 
 
+@pytest.mark.parametrize("M", [6, 40, 700])
+def test_grouped_offsets_that_are_not_ascending_name_no_groups(M):
+    g = gen(26)
+    K, N = 64, 80
+    a, w, sa, sb = ints((M, K), g), ints((4, N, K), g).transpose(1, 2), scales((M,), g), scales((4, N), g)
+    for off in ([0, M, 0, M, 2], [0, 5, 3, M, M], [0, -1 << 31, M, (1 << 31) - 1, 1]):
+        off = torch.tensor(off, dtype=torch.int32, device=DEV)
+        y = mb.grouped_scaled_mm(a, w, sa, sb, off, out=torch.full((M, N), 3.0, device=DEV))
+        assert bool((y == 0).all())
+
+
 def test_grouped_equals_dense():
     g = gen(24)
     counts = [70, 3, 200]
