@@ -174,7 +174,8 @@ int scaled_check(const mb_scaled_desc *d) {
 
 struct SgPlan {
   bool empty = false;
-  bool gemv = false;                  // up to four rows: one pass over the weights
+  bool gemv = false;                  // one row, or few by group: one pass over the weights
+  int thin = 0;                       // two to sixteen rows: the same; blocks per SM
   int bn = 0, pair = 1, split = 1, swap = 0;
   int w_mn = 0;                       // weights are read with N contiguous
   int pk_a = 0, pk_b = 0;             // operand copied into the workspace first
@@ -244,6 +245,11 @@ int64_t gemv_smem(const mb_scaled_desc *d) {
   return d->M * round_up(d->K, 16) + gemv_max_rows(d) * mr * 4;
 }
 constexpr int kGemvSmem = 96 * 1024;  // two blocks to an SM
+int64_t thin_max_rows(const mb_scaled_desc *d, int per_sm) { return ceil_div(d->N, (int64_t)device_sms() * per_sm); }
+int64_t thin_smem(const mb_scaled_desc *d, int per_sm) {
+  return (d->M > 8 ? 16 : 8) * (int64_t)(sg::thin_pitch((int)d->K) + 4 * sg::thin_sums((int)thin_max_rows(d, per_sm)));
+}
+constexpr int kThinSmem = 216 * 1024;
 
 int sg_plan(const mb_scaled_desc *d, SgPlan &pl) {
   if (d->M == 0 || d->N == 0) { pl.empty = true; return MB_OK; }
@@ -276,10 +282,21 @@ int sg_plan(const mb_scaled_desc *d, SgPlan &pl) {
 
   const int sms = device_sms();
   const bool forced = d->tile_n || d->cta_pair || d->split_k || d->swap_ab;
-  if (!forced && d->M <= (d->groups ? sg::GEMV_GROUPED_ROWS : sg::GEMV_ROWS) && !pl.pk_a && !pl.pk_b && !pl.w_mn &&
-      gemv_smem(d) <= kGemvSmem) {
-    pl.gemv = true;
-    return MB_OK;
+  if (!forced && !pl.pk_a && !pl.pk_b && !pl.w_mn) {
+    // Few rows: one of the single-pass kernels of scaled_gemv.cuh, by the weights'
+    // bytes.  The MMA one starts first (4 x 2048 x 1536 3.5 us, tcgen05 5.1; 4 x 4096 x
+    // 4096 6.0 and 8.8; 16 x 4096 x 4096 7.5 and 8.7) but streams at 4.5 TB/s (4 x 4096 x
+    // 14336 14.7 and 14.0; 16 rows 17.3 and 14.3); the dp4a one streams two rows
+    // faster (2 x 4096 x 14336 13.4, MMA 14.7) and starts later (2 x 2048 x 1536 4.2, 3.3).
+    const int64_t weights = d->K * d->N, small = (d->M > 8 || d->M == 2 ? 20ll : 40ll) << 20;
+    if (!d->groups && d->M > 1 && d->M <= sg::THIN_ROWS && weights <= small) {
+      pl.thin = thin_smem(d, 2) <= kThinSmem / 2 ? 2 : thin_smem(d, 1) <= kThinSmem ? 1 : 0;
+      if (pl.thin) return MB_OK;
+    }
+    if (d->M <= (d->groups ? sg::GEMV_GROUPED_ROWS : sg::GEMV_ROWS) && gemv_smem(d) <= kGemvSmem) {
+      pl.gemv = true;
+      return MB_OK;
+    }
   }
   static const struct { int swap, bn, pair; } tiles[] = {{1, 16, 1},  {1, 32, 1},  {1, 64, 1},  {1, 128, 1},
                                                          {0, 128, 1}, {0, 256, 1}, {0, 256, 2}, {0, 512, 2}};
@@ -316,6 +333,19 @@ int gemv_launch(const mb_scaled_desc *d, const SgPlan &pl, const sg::SgParams &p
   if (rc) return rc;
   return launch_pdl(kern, dim3((unsigned)(device_sms() * sg::GEMV_BLOCKS_PER_SM)), dim3(sg::GEMV_THREADS),
                     (size_t)gemv_smem(d), st, 1, "scaled_gemm", p, g);
+}
+
+template <bool MANY, class TO>
+int thin_launch(const mb_scaled_desc *d, const SgPlan &pl, const sg::SgParams &p, cudaStream_t st) {
+  sg::GemvArgs g{};
+  g.A = d->A; g.B = d->B; g.a_rs = pl.a_rs; g.b_rs = pl.w_ld;
+  g.K = (int)d->K;
+  g.max_rows = (int)thin_max_rows(d, pl.thin);
+  constexpr auto kern = sg::scaled_thin_kernel<MANY, TO>;
+  const int rc = allow_smem<kern>(kThinSmem);
+  if (rc) return rc;
+  return launch_pdl(kern, dim3((unsigned)(device_sms() * pl.thin)), dim3(sg::THIN_THREADS), (size_t)thin_smem(d, pl.thin),
+                    st, 1, "scaled_gemm", p, g);
 }
 
 template <int BN, int PAIR, bool SWAP, class TO>
@@ -382,6 +412,7 @@ int sg_launch(const mb_scaled_desc *d, const SgPlan &pl, cudaStream_t st) {
     if (d->groups) return gemv_launch<1, true, TO>(d, pl, p, st);
     return d->M == 1 ? gemv_launch<1, false, TO>(d, pl, p, st) : gemv_launch<2, false, TO>(d, pl, p, st);
   }
+  if (pl.thin) return d->M > 8 ? thin_launch<true, TO>(d, pl, p, st) : thin_launch<false, TO>(d, pl, p, st);
   const int64_t nB = p.one_b ? 1 : p.groups;
   const void *A = d->A, *B = d->B;
   PackArgs pa{}, pb{};
@@ -463,6 +494,7 @@ int mb_scaled_plan(const mb_scaled_desc *d, char *buf, int buflen) {
   if (rc) return -rc;
   const size_t room = buf ? (size_t)std::max(buflen, 0) : 0;
   if (pl.gemv) return snprintf(buf, room, "rows in one pass over the weights");
+  if (pl.thin) return snprintf(buf, room, "rows in one pass over the weights, MMA, %d blocks an SM", pl.thin);
   if (pl.bn == 0) return snprintf(buf, room, pl.empty ? "empty" : "no sum");
   return snprintf(buf, room, "%s bn=%d pair=%d split=%d a_mn=%d b_mn=%d pack_a=%d pack_b=%d ws=%lld",
                   pl.swap ? "channels" : "tokens", pl.bn, pl.pair, pl.split, 0, pl.w_mn, pl.pk_a, pl.pk_b,

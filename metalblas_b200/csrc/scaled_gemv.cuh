@@ -190,5 +190,127 @@ scaled_gemv_kernel(const __grid_constant__ SgParams p, const GemvArgs g) {
       C[m * p.c_rs + c * p.c_cs] = Elem<TO>::store(0.f);
 }
 
+// Two to sixteen rows, one weight matrix: the same single balanced pass, with the
+// rows of A as the 16 rows of a warp-level int8 MMA and eight weight rows as its
+// columns.  A lane loads 16 consecutive bytes of one weight row, which serve as
+// the B words of two MMAs: the sum does not mind which bytes of K a position of
+// the instruction stands for, as long as A's words, read from shared memory the
+// same way, agree.  What counts here is that every SM reads the same bytes and
+// starts at once: the tcgen05 kernel, which hands out 128 channels at a time and
+// sets up TMEM and a pipeline first, took 8.8 us for 4 x 4096 x 4096 against 6.0.
+// Its eight-row reads stream at 4.5 TB/s, so products of more weights go there.
+//
+// A block's warps share K (KS slices) and pairs of eight weight rows.
+constexpr int THIN_ROWS = 16;
+constexpr int THIN_THREADS = 512;
+constexpr int THIN_KS = 8;                                  // slices of K
+constexpr int THIN_GS = THIN_THREADS / 32 / THIN_KS;        // warps that share out the pairs
+// Rows of A in shared memory, an odd number of 64 bytes apart (no bank conflicts).
+__host__ __device__ constexpr int thin_pitch(int K) { return (K + 127) / 128 * 128 + 64; }
+// Sums of a row of A in shared memory, 8 words modulo 32 apart.
+__host__ __device__ constexpr int thin_sums(int rows) { return (rows + 15) / 32 * 32 + 40; }
+
+__device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// MANY: more than eight rows of A.
+template <bool MANY, class TO>
+__global__ void __launch_bounds__(THIN_THREADS, 2) scaled_thin_kernel(const __grid_constant__ SgParams p, const GemvArgs g) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  constexpr int STAGED = MANY ? 16 : 8, BATCH = 4;
+  const int pitch = thin_pitch(g.K), vecs = (g.K + 15) / 16, chunks = (g.K + 63) / 64, sums = thin_sums(g.max_rows);
+  uint8_t *xs = smem_raw;                                          // [STAGED][pitch]
+  int *acc = reinterpret_cast<int *>(smem_raw + STAGED * pitch);   // [STAGED][sums]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t r0 = (int64_t)p.N * blockIdx.x / gridDim.x;
+  const int rows = (int)((int64_t)p.N * (blockIdx.x + 1) / gridDim.x - r0);
+  for (int i = tid; i < STAGED * sums; i += THIN_THREADS) acc[i] = 0;
+  {
+    const int bytes = g.K & ~15;
+    if (bytes)
+      for (int i = tid; i < rows; i += THIN_THREADS) prefetch_l2_bulk(g.B + (r0 + i) * g.b_rs, (uint32_t)bytes);
+  }
+  pdl_trigger();
+  pdl_wait();
+  const int ks = warp % THIN_KS, gs = warp / THIN_KS;
+  const int c0 = ks * chunks / THIN_KS, c1 = (ks + 1) * chunks / THIN_KS;
+  const int pairs = (rows + 15) / 16, wrow = lane >> 2, piece = lane & 3;
+  uint4 w[2][BATCH];
+  // chunks c .. c+BATCH-1 of both groups of a pair: this lane's row and 16 bytes
+  auto fetch = [&](int pair, int c) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = pair * 16 + h * 8 + wrow;
+      const int8_t *src = g.B + (r0 + row) * g.b_rs + piece * 16;
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i)
+        w[h][i] = load_once(src + (c + i) * 64, row < rows && c + i < c1 && (c + i) * 4 + piece < vecs);
+    }
+  };
+  if (gs < pairs && c0 < c1) fetch(gs, c0);
+  for (int i = tid; i < STAGED * (pitch / 16); i += THIN_THREADS) {
+    const int m = i / (pitch / 16), v = i - m * (pitch / 16);
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (m < p.M && v < vecs) {
+      const int8_t *src = g.A + m * g.a_rs;
+      if (v * 16 + 16 <= g.K) {
+        x = *reinterpret_cast<const uint4 *>(src + v * 16);
+      } else {
+        int8_t b[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) b[j] = v * 16 + j < g.K ? src[v * 16 + j] : 0;
+        x = *reinterpret_cast<uint4 *>(b);
+      }
+    }
+    *reinterpret_cast<uint4 *>(xs + m * pitch + v * 16) = x;
+  }
+  __syncthreads();
+  bool fetched = true;
+  for (int pair = gs; pair < pairs; pair += THIN_GS) {
+    int d[2][4] = {};
+    for (int c = c0; c < c1; c += BATCH) {
+      if (!fetched) fetch(pair, c);
+      fetched = false;
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        // past the slice w is zero; A's word is any that exists
+        const uint8_t *x = xs + wrow * pitch + min(c + i, chunks - 1) * 64 + piece * 16;
+        const uint4 lo = *reinterpret_cast<const uint4 *>(x);
+        uint4 hi = make_uint4(0, 0, 0, 0);
+        if constexpr (MANY) hi = *reinterpret_cast<const uint4 *>(x + 8 * pitch);
+        const uint32_t a0[4] = {lo.x, hi.x, lo.y, hi.y}, a1[4] = {lo.z, hi.z, lo.w, hi.w};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          mma_s8(d[h], a0, w[h][i].x, w[h][i].y);
+          mma_s8(d[h], a1, w[h][i].z, w[h][i].w);
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      int *s = acc + wrow * sums + pair * 16 + h * 8 + piece * 2;
+      atomicAdd(s, d[h][0]);
+      atomicAdd(s + 1, d[h][1]);
+      if constexpr (MANY) {
+        atomicAdd(s + 8 * sums, d[h][2]);
+        atomicAdd(s + 8 * sums + 1, d[h][3]);
+      }
+    }
+  }
+  __syncthreads();
+  TO *C = static_cast<TO *>(p.C);
+  for (int i = tid; i < p.M * rows; i += THIN_THREADS) {
+    const int m = i / rows, row = i - m * rows;
+    const int64_t n = r0 + row;
+    float v = scaled_sum(acc[m * sums + row], p.scale_a[m * p.sa_s], p.scale_b[n * p.sb_s]);
+    if (p.bias) v = __fadd_rn(v, bias_at<TO>(p, n));
+    C[m * p.c_rs + n * p.c_cs] = Elem<TO>::store(v);
+  }
+}
+
 }  // namespace sg
 }  // namespace mb

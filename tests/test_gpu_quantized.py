@@ -161,6 +161,23 @@ def test_scaled_mm_bias(M, K, N, out_dtype):
             check_product(y, a, w, sa, sb, bias)
 
 
+@pytest.mark.parametrize("M", [1, 2, 3, 7, 8, 9, 15, 16, 17])
+@pytest.mark.parametrize("K", [1, 15, 16, 63, 65, 500, 1040, 2050])
+def test_scaled_mm_few_rows(M, K):
+    """The single-pass kernels: rows of K bytes in aligned storage, few and many channels."""
+    g = gen(M * 3 + K)
+    room = (K + 15) // 16 * 16 + 32
+    A = ints((M, room), g)[:, :K]
+    for N in (1, 5, 148, 297, 2000, 40000 if K > 1000 else 601):
+        w, sa, sb = ints((N, room), g)[:, :K].t(), scales((M,), g), scales((N,), g)
+        bias = torch.randn(N, generator=g).to(DEV)
+        for out_dtype in (torch.bfloat16, torch.float32):
+            y = mb.scaled_mm(A, w, sa, sb, bias=bias if N % 2 else None, out_dtype=out_dtype)
+            check_product(y, A, w, sa, sb, bias if N % 2 else None)
+        assert torch.equal(y, mb.scaled_mm(A, w, sa, sb, bias=bias if N % 2 else None, out_dtype=torch.float32,
+                                           _plan=(16, 1, 1, 1)))
+
+
 def test_scaled_mm_extreme_values_are_exact():
     """The longest K of -128 * -128 and -128 * 127: no sum wraps."""
     K = 131071
