@@ -379,7 +379,7 @@ int sg_pack(const PackArgs *a, const PackArgs *b, cudaStream_t st) {
     *m = nullptr;
   }
   auto blocks = [&](const PackArgs *m) {
-    return m ? std::min<int64_t>(ceil_div(m->batch * m->rows * ceil_div(m->cols, 16), 256), cap) : 0;
+    return m ? std::min<int64_t>(ceil_div(m->batch * m->rows * ceil_div(m->cols, 512), 8), cap) : 0;
   };
   const int64_t na = blocks(a), nb = blocks(b);
   if (na + nb == 0) return MB_OK;

@@ -36,6 +36,7 @@
 // sums through distributed shared memory.
 #pragma once
 #include "pack.cuh"
+#include "quantize.cuh"
 #include "tc_gemm.cuh"
 
 namespace mb {
@@ -553,6 +554,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
             };
             if (p.bias) convert(std::true_type());
             else convert(std::false_type());
+            if (p.c_rs == 1 && p.c_cs != 1) {  // columns of C are contiguous: lanes hold rows
+              const int64_t r = t.r0 + row, n0 = t.c0 + half * WCOLS + c;
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (r < t.rend && n0 + j < p.N) C[r + (n0 + j) * p.c_cs] = reinterpret_cast<const TO *>(w)[j];
+              continue;
+            }
             if (p.c_tma) {  // the last step's store has read the staging rows
               if (lane == 0) bulk_wait_read0();
               __syncwarp();
@@ -564,39 +572,46 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
                            : "memory");
             // 32 rows of the group (or up to the end of C, where the store clips)
             // go out as one box; the rows before another group's by hand.
-            const int64_t mw = t.r0 + (PAIR == 2 ? (int)rank * BM : 0) + q * 32;
-            if (p.c_tma && (mw + 32 <= t.rend || t.rend == p.M)) {
+            const int64_t first_row = t.r0 + (PAIR == 2 ? (int)rank * BM : 0) + q * 32;
+            if (p.c_tma && (first_row + 32 <= t.rend || t.rend == p.M)) {
               const int64_t nn = t.c0 + half * WCOLS + c;
               fence_proxy_async_smem();
               __syncwarp();
-              if (lane == 0 && mw < t.rend && nn < p.N) {
-                tma_store_3d(&p.tmC, stg, (int)nn, (int)mw, 0);
+              if (lane == 0 && first_row < t.rend && nn < p.N) {
+                tma_store_3d(&p.tmC, stg, (int)nn, (int)first_row, 0);
                 bulk_commit();
               }
               continue;
             }
           }
           __syncwarp();
-          {
-            // the staged rows (tokens) in 16-byte chunks, whole rows by neighbouring lanes
+          constexpr int ROWS = SWAP ? CH : 32, PASS = 32 / NCH;
+          const int64_t mw = SWAP ? t.r0 + half * WCOLS + c : t.r0 + (PAIR == 2 ? (int)rank * BM : 0) + q * 32;
+          const int64_t nw = SWAP ? t.c0 + q * 32 : t.c0 + half * WCOLS + c;
+          const int live = (int)min((int64_t)ROWS, t.rend - mw);   // rows of the group among them
+          if (p.c_vec && nw + 32 <= p.N) {
+            // 16-byte chunks, whole rows by neighbouring lanes
             const int ch = lane % NCH, rr0 = lane / NCH;
-            const int64_t mw = SWAP ? t.r0 + half * WCOLS + c : t.r0 + (PAIR == 2 ? (int)rank * BM : 0) + q * 32;
-            const int64_t nn = (SWAP ? t.c0 + q * 32 : t.c0 + half * WCOLS + c) + ch * EPC;
-            constexpr int ROWS = SWAP ? CH : 32, PASS = 32 / NCH;
 #pragma unroll
             for (int i = 0; i < (ROWS + PASS - 1) / PASS; ++i) {
               const int rr = i * PASS + rr0;
-              if (rr >= ROWS || mw + rr >= t.rend || nn >= p.N) continue;
-              const uint4 v = ld_shared_v4(chunk_addr(rr, ch));
-              TO *dst = C + (mw + rr) * p.c_rs;
-              if (p.c_vec && nn + EPC <= p.N) {
-                *reinterpret_cast<uint4 *>(dst + nn) = v;
-              } else {
-                const TO *e = reinterpret_cast<const TO *>(&v);
-#pragma unroll
-                for (int j = 0; j < EPC; ++j)
-                  if (nn + j < p.N) dst[(nn + j) * p.c_cs] = e[j];
-              }
+              if (rr < live)
+                *reinterpret_cast<uint4 *>(C + (mw + rr) * p.c_rs + nw + ch * EPC) = ld_shared_v4(chunk_addr(rr, ch));
+            }
+          } else {
+            // rows that start anywhere: an element a lane, along whichever of rows
+            // and columns is contiguous in C
+            const uint8_t *own = staging + ew * C_::STAGING_WARP;
+            auto staged = [&](int rr, int col) {
+              return *reinterpret_cast<const TO *>(own + (chunk_addr(rr, col / EPC) - stg) + (col % EPC) * sizeof(TO));
+            };
+            if (p.c_rs == 1 && p.c_cs != 1) {
+#pragma unroll 4
+              for (int col = 0; col < 32; ++col)
+                if (lane < live && nw + col < p.N) C[mw + lane + (nw + col) * p.c_cs] = staged(lane, col);
+            } else if (nw + lane < p.N) {
+#pragma unroll 4
+              for (int rr = 0; rr < live; ++rr) C[(mw + rr) * p.c_rs + (nw + lane) * p.c_cs] = staged(rr, lane);
             }
           }
         }
@@ -623,12 +638,26 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
 }
 
 // Operands that TMA cannot read in place, copied to aligned rows: A's rows by the
-// first `split` blocks, B's by the others, in one launch.
+// first `split` blocks, B's by the others, in one launch.  A warp takes 512 bytes
+// of a row at a time, a lane 16 of them; the bytes past the row's end go to its
+// padding, which no tensor map covers.
+__device__ __forceinline__ void scaled_pack_rows(const PackArgs &a, int block, int blocks) {
+  const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+  const int64_t segs = (a.cols + 511) / 512, total = a.batch * a.rows * segs;
+  for (int64_t u = (int64_t)block * warps + (threadIdx.x >> 5); u < total; u += (int64_t)blocks * warps) {
+    const int64_t r = total < (1ll << 32) ? (uint32_t)u / (uint32_t)segs : u / segs;
+    const int64_t b = a.batch > 1 ? r / a.rows : 0;
+    const int c = (int)(u - r * segs) * 512 + lane * 16;
+    if (c >= (int)a.cols) continue;
+    const int8_t *src = static_cast<const int8_t *>(a.src) + b * a.bs + (r - b * a.rows) * a.rs;
+    *reinterpret_cast<uint4 *>(static_cast<int8_t *>(a.dst) + r * a.ld + c) = load_bytes16(src, c, (int)a.cols);
+  }
+}
 __global__ static void __launch_bounds__(256) scaled_pack_kernel(const PackArgs a, const PackArgs b, int split) {
   pdl_trigger();
   pdl_wait();
-  if ((int)blockIdx.x < split) pack_rows16<uint8_t>(a, blockIdx.x, split);
-  else pack_rows16<uint8_t>(b, blockIdx.x - split, gridDim.x - split);
+  if ((int)blockIdx.x < split) scaled_pack_rows(a, blockIdx.x, split);
+  else scaled_pack_rows(b, blockIdx.x - split, gridDim.x - split);
 }
 
 // K = 0: the sum is empty.
