@@ -18,6 +18,13 @@
 //
 // Sums have a fixed order and nothing is accumulated with floating-point
 // atomics, so results repeat bit for bit.
+//
+// All but the sort are bound by HBM: they move each row once, 16 bytes a thread,
+// with as many rows in flight as registers allow.  Measured on B200 at 8192
+// tokens x 8 experts each, 4096 bf16 columns (a copy moves 6.54 TB/s): gather
+// 104.5 us (5.8 TB/s), gather to int8 57.7 us (5.8), combine 95.5 us (6.3), its
+// gradient 184 us (6.2); the sort of those 65536 entries 11 us, of 32 entries
+// 2.2 us, where launch and latency are all there is.
 #pragma once
 #include "mb_common.cuh"
 #include "quantize.cuh"

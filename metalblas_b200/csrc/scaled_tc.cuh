@@ -34,6 +34,19 @@
 // K.  Eight epilogue warps hold eight pieces of the tile; piece i is finished
 // by cluster rank i * split / 8, and the other ranks send it their s32 partial
 // sums through distributed shared memory.
+//
+// What bounds it, measured on B200 (twice the bf16 GEMM rate 1650 TFLOP/s is
+// taken as the int8 rate, 6.54 TB/s is a copy's):
+//   8192^3 bf16 out                331 us, 3320 TOPS: the tensor pipe;
+//   4096^3                         48.6 us, 2830 TOPS: operands into shared memory,
+//                                  and 256 tiles over 74 pairs;
+//   16384 rows by 8 experts of 4096 x 14336   650 us, 2960 TOPS: the same, and
+//                                  tiles that end with their group;
+//   8192 x 512 x 8192              45 us: the epilogue (134 MB out);
+//   16 rows by 8 experts of 4096 x 14336      65.8 us, 6.2 TB/s: the weights' bytes;
+//   16 x 4096 x 14336              14.3 us, 4.1 TB/s: 112 tiles keep 112 SMs busy.
+// The tile is chosen by sg_cost (mb_ops.cu) from these times' model; TROWS, TCOLS
+// and split change no result.
 #pragma once
 #include "pack.cuh"
 #include "quantize.cuh"
