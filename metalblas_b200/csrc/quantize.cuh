@@ -45,6 +45,18 @@ __device__ __forceinline__ uint4 cut16(const uint4 &a, const uint4 &b, uint32_t 
                     __funnelshift_r(y3, y4, sh));
 }
 
+// Zeros all but the first n elements of v.
+template <class T> __device__ __forceinline__ void keep_first(Vec<T> &v, int n) {
+  if (n >= Vec<T>::V) return;
+  uint32_t *w = &v.u.q.x;
+  const int bytes = n * (int)sizeof(T);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int b = bytes - 4 * i;
+    w[i] = b >= 4 ? w[i] : (b <= 0 ? 0u : w[i] & ((1u << (8 * b)) - 1));
+  }
+}
+
 // 16 bytes that are read once, zeros where `on` is false.  As volatile assembly a
 // batch of these is issued as written, ahead of its uses; left to itself the
 // compiler interleaved loads and sums to save registers, two or three in flight
