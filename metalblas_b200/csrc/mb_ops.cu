@@ -367,8 +367,9 @@ int sg_launch_tile(const SgPlan &pl, sg::SgParams &p, cudaStream_t st) {
 }
 
 // Copies the operands that need it (rows of neither: null).  Rows go sixteen
-// bytes a thread; a matrix without a unit stride through tiles.
-int sg_pack(const PackArgs *a, const PackArgs *b, cudaStream_t st) {
+// bytes a thread, of groups with rows (offsets: as p.offsets, b's batches the
+// groups) alone; a matrix without a unit stride through tiles.
+int sg_pack(const PackArgs *a, const PackArgs *b, const int *offsets, int M, cudaStream_t st) {
   const int64_t cap = (int64_t)device_sms() * 16;
   for (const PackArgs **m : {&a, &b}) {
     if (!*m || (*m)->cs == 1) continue;
@@ -379,13 +380,13 @@ int sg_pack(const PackArgs *a, const PackArgs *b, cudaStream_t st) {
     *m = nullptr;
   }
   auto blocks = [&](const PackArgs *m) {
-    return m ? std::min<int64_t>(ceil_div(m->batch * m->rows * ceil_div(m->cols, 512), 8), cap) : 0;
+    return m ? std::min<int64_t>(ceil_div(m->batch * m->rows * ceil_div(m->cols, 512), 8), (int64_t)device_sms() * 4) : 0;
   };
   const int64_t na = blocks(a), nb = blocks(b);
   if (na + nb == 0) return MB_OK;
   const PackArgs none{};
   return launch_pdl(sg::scaled_pack_kernel, dim3((unsigned)(na + nb)), dim3(256), 0, st, 1, "scaled_gemm: operand copy",
-                    a ? *a : none, b ? *b : none, (int)na);
+                    a ? *a : none, b ? *b : none, (int)na, offsets, M);
 }
 
 template <class TO>
@@ -425,7 +426,7 @@ int sg_launch(const mb_scaled_desc *d, const SgPlan &pl, cudaStream_t st) {
     pb = pl.w_mn ? PackArgs{d->B, const_cast<void *>(B), d->K, d->N, d->b_rs, d->b_cs, d->sB, nB, pl.w_ld}
                  : PackArgs{d->B, const_cast<void *>(B), d->N, d->K, d->b_cs, d->b_rs, d->sB, nB, pl.w_ld};
   }
-  int rc = sg_pack(pl.pk_a ? &pa : nullptr, pl.pk_b ? &pb : nullptr, st);
+  int rc = sg_pack(pl.pk_a ? &pa : nullptr, pl.pk_b ? &pb : nullptr, p.one_b ? nullptr : p.offsets, p.M, st);
   if (rc) return rc;
   // boxes of 128 bytes along the contiguous dimension
   CUtensorMap *ta = pl.swap ? &p.tmB : &p.tmA, *tw = pl.swap ? &p.tmA : &p.tmB;

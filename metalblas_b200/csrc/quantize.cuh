@@ -110,18 +110,6 @@ __device__ __forceinline__ Vec<T> load_vec(const T *row, int c, int H) {
   return v;
 }
 
-// Bytes c .. c+15 of a row of n bytes that starts anywhere, zeros past its end.
-__device__ __forceinline__ uint4 load_bytes16(const int8_t *row, int c, int n) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(row + c);
-  const uint32_t off = (uint32_t)(a & 15);
-  const uint4 *w = reinterpret_cast<const uint4 *>(a - off);
-  if (c + 16 <= n) return cut16(w[0], w[off ? 1 : 0], off);
-  union { uint4 q; int8_t b[16]; } v;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v.b[i] = c + i < n ? row[c + i] : 0;
-  return v.q;
-}
-
 // The first column of a row's vectors: 0 when the row starts on 16 bytes, else
 // the column (<= 0) whose address does, so that whole vectors can be stored.
 template <class T, bool AL> __device__ __forceinline__ int frame(const T *row) {

@@ -653,24 +653,65 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
 // Operands that TMA cannot read in place, copied to aligned rows: A's rows by the
 // first `split` blocks, B's by the others, in one launch.  A warp takes 512 bytes
 // of a row at a time, a lane 16 of them; the bytes past the row's end go to its
-// padding, which no tensor map covers.
-__device__ __forceinline__ void scaled_pack_rows(const PackArgs &a, int block, int blocks) {
-  const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
-  const int64_t segs = (a.cols + 511) / 512, total = a.batch * a.rows * segs;
-  for (int64_t u = (int64_t)block * warps + (threadIdx.x >> 5); u < total; u += (int64_t)blocks * warps) {
-    const int64_t r = total < (1ll << 32) ? (uint32_t)u / (uint32_t)segs : u / segs;
-    const int64_t b = a.batch > 1 ? r / a.rows : 0;
-    const int c = (int)(u - r * segs) * 512 + lane * 16;
-    if (c >= (int)a.cols) continue;
-    const int8_t *src = static_cast<const int8_t *>(a.src) + b * a.bs + (r - b * a.rows) * a.rs;
-    *reinterpret_cast<uint4 *>(static_cast<int8_t *>(a.dst) + r * a.ld + c) = load_bytes16(src, c, (int)a.cols);
-  }
-}
-__global__ static void __launch_bounds__(256) scaled_pack_kernel(const PackArgs a, const PackArgs b, int split) {
+// padding, which no tensor map covers.  Weights of groups without rows (offsets:
+// of the groups; null: all have some) are left where they are: no unit reads them,
+// and copying them all was most of a call with few rows (4 rows, 128 groups of 431 x
+// 8192: 276 us, 26 now; 1024 x 4 rows, 32 groups of 4095 x 2048: 199, 190).
+__global__ static void __launch_bounds__(256) scaled_pack_kernel(const PackArgs pa, const PackArgs pb, int split,
+                                                                 const int *offsets, int M) {
+  __shared__ uint16_t used[1024];  // groups with rows
+  __shared__ int count[8];
   pdl_trigger();
   pdl_wait();
-  if ((int)blockIdx.x < split) scaled_pack_rows(a, blockIdx.x, split);
-  else scaled_pack_rows(b, blockIdx.x - split, gridDim.x - split);
+  const bool is_a = (int)blockIdx.x < split;
+  const PackArgs &a = is_a ? pa : pb;
+  const int block = is_a ? blockIdx.x : blockIdx.x - split, blocks = is_a ? split : gridDim.x - split;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int batch = (int)a.batch;
+  const bool some = !is_a && offsets;
+  if (some) {
+    const int groups = batch;
+    batch = 0;
+    for (int e0 = 0; e0 < groups; e0 += 256) {
+      const int e = e0 + threadIdx.x;
+      const bool has = e < groups && min(max(offsets[e + 1], 0), M) > (e ? min(max(offsets[e], 0), M) : 0);
+      const unsigned mask = __ballot_sync(0xffffffffu, has);
+      if (lane == 0) count[warp] = __popc(mask);
+      __syncthreads();
+      int at = batch + __popc(mask & ((1u << lane) - 1));
+      for (int w = 0; w < 8; ++w) {
+        at += w < warp ? count[w] : 0;
+        batch += count[w];
+      }
+      if (has) used[at] = (uint16_t)e;
+      __syncthreads();
+    }
+  }
+  const int64_t segs = (a.cols + 511) / 512, total = batch * a.rows * segs;
+  const int64_t step = (int64_t)blocks * 8;
+  for (int64_t u0 = (int64_t)block * 8 + warp; u0 < total; u0 += 4 * step) {
+    // four units' words on their way at a time; words without a byte of the row are not read
+    uint4 lo[4], hi[4];
+    uint32_t off[4];
+    int8_t *dst[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t u = u0 + i * step;
+      const bool small = total < (1ll << 32);
+      const int64_t r = small ? (uint32_t)u / (uint32_t)segs : u / segs;
+      const int64_t n = batch <= 1 ? 0 : small ? (uint32_t)r / (uint32_t)a.rows : r / a.rows;
+      const int c = (int)(u - r * segs) * 512 + lane * 16, left = u < total ? (int)a.cols - c : 0;
+      const int64_t b = some && left > 0 ? used[n] : n, row = r - n * a.rows;
+      const int8_t *src = static_cast<const int8_t *>(a.src) + b * a.bs + row * a.rs + c;
+      off[i] = (uint32_t)(reinterpret_cast<uintptr_t>(src) & 15);
+      lo[i] = load_once<true>(src - off[i], left > 0);
+      hi[i] = load_once<true>(src - off[i] + 16, off[i] && left > 16 - (int)off[i]);
+      dst[i] = left > 0 ? static_cast<int8_t *>(a.dst) + (b * a.rows + row) * a.ld + c : nullptr;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (dst[i]) *reinterpret_cast<uint4 *>(dst[i]) = cut16(lo[i], hi[i], off[i]);
+  }
 }
 
 // K = 0: the sum is empty.
