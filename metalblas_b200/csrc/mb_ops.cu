@@ -322,17 +322,27 @@ int sg_plan(const mb_scaled_desc *d, SgPlan &pl) {
   return MB_OK;
 }
 
-template <int MR, bool GROUPED, class TO>
-int gemv_launch(const mb_scaled_desc *d, const SgPlan &pl, const sg::SgParams &p, cudaStream_t st) {
+template <int MR, bool GROUPED, int ROWSTEPS, class TO>
+int gemv_launch_as(const mb_scaled_desc *d, const SgPlan &pl, const sg::SgParams &p, cudaStream_t st) {
   sg::GemvArgs g{};
   g.A = d->A; g.B = d->B; g.a_rs = pl.a_rs; g.b_rs = pl.w_ld; g.sB = pl.sB;
   g.K = (int)d->K;
   g.max_rows = (int)gemv_max_rows(d);
-  constexpr auto kern = sg::scaled_gemv_kernel<MR, GROUPED, TO>;
+  constexpr auto kern = sg::scaled_gemv_kernel<MR, GROUPED, ROWSTEPS, TO>;
   const int rc = allow_smem<kern>(kGemvSmem);
   if (rc) return rc;
   return launch_pdl(kern, dim3((unsigned)(device_sms() * sg::GEMV_BLOCKS_PER_SM)), dim3(sg::GEMV_THREADS),
                     (size_t)gemv_smem(d), st, 1, "scaled_gemm", p, g);
+}
+// Rows are taken whole when they are short and every warp has some.
+template <int MR, bool GROUPED, class TO>
+int gemv_launch(const mb_scaled_desc *d, const SgPlan &pl, const sg::SgParams &p, cudaStream_t st) {
+  const int64_t warps = (int64_t)device_sms() * sg::GEMV_BLOCKS_PER_SM * (sg::GEMV_THREADS / 32);
+  const bool whole = (d->groups ? d->M : 1) * d->N > warps;
+  if (whole && d->K <= 512) return gemv_launch_as<MR, GROUPED, 1, TO>(d, pl, p, st);
+  if (whole && d->K <= 1024) return gemv_launch_as<MR, GROUPED, 2, TO>(d, pl, p, st);
+  if (whole && d->K <= 2048) return gemv_launch_as<MR, GROUPED, 4, TO>(d, pl, p, st);
+  return gemv_launch_as<MR, GROUPED, 0, TO>(d, pl, p, st);
 }
 
 template <bool MANY, class TO>

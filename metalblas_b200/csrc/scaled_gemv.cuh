@@ -16,6 +16,12 @@
 // weights: a decode step's rows nearly always have an expert each, and rows that
 // share one find its weights in L2.
 //
+// Rows of up to 2048 bytes leave most of a warp's eight loads unused, and a row's
+// wait, sum and reduction follow one another.  So with more rows than warps a warp
+// takes several whole rows at a time (ROWSTEPS: the 512-byte steps of a row): one
+// row, K x N = 432 x 32768 4.3 us against 10.6, 1024 x 32768 6.9 against 12.0, 2048 x
+// 8192 4.0 against 6.4; eight rows with an expert each, 512 x 8192 10.1 against 23.0.
+//
 // A lane multiplies its 16 weight bytes by dp4a with the rows of A, which lie in
 // shared memory, padded with zeros to whole vectors.  A run's 32-bit sums are
 // added into shared memory with integer atomics: the sum is exact, so their
@@ -41,7 +47,8 @@ struct GemvArgs {
   int max_rows;          // weight rows of a block, at most
 };
 
-template <int MR, bool GROUPED, class TO>
+// ROWSTEPS: 1, 2 or 4, rows of at most as many steps, taken whole; 0: any rows.
+template <int MR, bool GROUPED, int ROWSTEPS, class TO>
 __global__ void __launch_bounds__(GEMV_THREADS, GEMV_BLOCKS_PER_SM)
 scaled_gemv_kernel(const __grid_constant__ SgParams p, const GemvArgs g) {
   static_assert(!GROUPED || MR == 1, "a row of A at a time");
@@ -61,6 +68,11 @@ scaled_gemv_kernel(const __grid_constant__ SgParams p, const GemvArgs g) {
   auto share = [&](int64_t total) {
     r0 = total * blockIdx.x / gridDim.x;
     rows = (int)(total * (blockIdx.x + 1) / gridDim.x - r0);
+    if constexpr (ROWSTEPS > 0) {
+      row = (int)((int64_t)rows * warp / W);
+      left = (int)((int64_t)rows * (warp + 1) / W) - row;  // rows
+      return;
+    }
     const int64_t steps = (int64_t)rows * per_row;
     const int64_t s0 = steps * warp / W;
     left = (int)(steps * (warp + 1) / W - s0);
@@ -75,6 +87,21 @@ scaled_gemv_kernel(const __grid_constant__ SgParams p, const GemvArgs g) {
     for (int i = 0; i < GEMV_BATCH; ++i) w[i] = load_once(src + (int64_t)(v0 + i * 32) * 16, v0 + i * 32 < stop);
   };
 
+  // whole rows: the next of them, `at` its A row, n its column
+  int n = 0, at = 0;
+  constexpr int RS = ROWSTEPS ? ROWSTEPS : 1, RB = GEMV_BATCH / RS;
+  // (N is more than a batch: rows are taken whole when there are more than warps)
+  auto fetch_rows = [&]() {
+#pragma unroll
+    for (int j = 0; j < RB; ++j) {
+      const int wrap = GROUPED && n + j >= p.N;
+      const int e = GROUPED && j < left ? min(group_of[at + wrap], p.groups - 1) : 0;
+      const int8_t *src = g.B + (p.one_b ? 0 : e) * g.sB + (n + j - (wrap ? p.N : 0)) * g.b_rs;
+#pragma unroll
+      for (int i = 0; i < RS; ++i) w[j * RS + i] = load_once(src + (i * 32 + lane) * 16, j < left && i * 32 + lane < vecs);
+    }
+  };
+
   for (int i = tid; i < g.max_rows * MR; i += GEMV_THREADS) acc[i] = 0;
   if (tid < GEMV_GROUPED_ROWS) group_of[tid] = 0;
   if constexpr (!GROUPED) {
@@ -87,7 +114,9 @@ scaled_gemv_kernel(const __grid_constant__ SgParams p, const GemvArgs g) {
   pdl_trigger();
   pdl_wait();
   if constexpr (!GROUPED) {
-    if (left > 0) fetch(g.B + (r0 + row) * g.b_rs, min(left, per_row - k), 0);
+    n = (int)r0 + row;
+    if constexpr (ROWSTEPS > 0) fetch_rows();
+    else if (left > 0) fetch(g.B + n * g.b_rs, min(left, per_row - k), 0);
   }
   for (int i = tid; i < staged * vecs; i += GEMV_THREADS) {
     const int m = i / vecs, v = i - m * vecs;
@@ -124,18 +153,56 @@ scaled_gemv_kernel(const __grid_constant__ SgParams p, const GemvArgs g) {
     while (live > 0 && group_of[live - 1] >= p.groups) --live;
     share((int64_t)live * p.N);
   }
-  int m0 = 0;
-  int64_t n = r0 + row;
   if constexpr (GROUPED) {
-    m0 = (int)(n / p.N);
-    n -= (int64_t)m0 * p.N;
+    const int64_t first = r0 + row;
+    at = (int)(first / p.N);
+    n = (int)(first - (int64_t)at * p.N);
   }
   bool fetched = !GROUPED;  // the first batch is on its way
-  while (left > 0) {
+  if constexpr (ROWSTEPS > 0) {
+    while (left > 0) {
+      if (!fetched) fetch_rows();
+      fetched = false;
+      int s[RB][MR];
+#pragma unroll
+      for (int j = 0; j < RB; ++j) {
+#pragma unroll
+        for (int m = 0; m < MR; ++m) s[j][m] = 0;
+        const uint4 *x0 = xs + (GROUPED ? min(at + (n + j >= p.N), p.M - 1) * vecs : 0);
+#pragma unroll
+        for (int i = 0; i < RS; ++i) {
+          const int v = min(i * 32 + lane, vecs - 1);
+#pragma unroll
+          for (int m = 0; m < MR; ++m) {
+            const uint4 x = x0[m * vecs + v];
+            s[j][m] = __dp4a((int)w[j * RS + i].x, (int)x.x, s[j][m]);
+            s[j][m] = __dp4a((int)w[j * RS + i].y, (int)x.y, s[j][m]);
+            s[j][m] = __dp4a((int)w[j * RS + i].z, (int)x.z, s[j][m]);
+            s[j][m] = __dp4a((int)w[j * RS + i].w, (int)x.w, s[j][m]);
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < RB; ++j)
+#pragma unroll
+        for (int m = 0; m < MR; ++m) {
+          const int sum = __reduce_add_sync(0xffffffffu, s[j][m]);
+          if (lane == 0 && j < left) acc[(row + j) * MR + m] = sum;
+        }
+      left -= RB;
+      row += RB;
+      n += RB;
+      if (GROUPED && n >= p.N) {
+        n -= p.N;
+        ++at;
+      }
+    }
+  }
+  while (ROWSTEPS == 0 && left > 0) {
     const int run = min(left, per_row - k);
-    const int e = GROUPED ? min(group_of[m0], p.groups - 1) : 0;
+    const int e = GROUPED ? min(group_of[at], p.groups - 1) : 0;
     const int8_t *src = g.B + (p.one_b ? 0 : e) * g.sB + n * g.b_rs;
-    const uint4 *x0 = xs + (GROUPED ? (int64_t)m0 * vecs : 0);
+    const uint4 *x0 = xs + (GROUPED ? (int64_t)at * vecs : 0);
     int s[MR];
 #pragma unroll
     for (int m = 0; m < MR; ++m) s[m] = 0;
@@ -166,7 +233,7 @@ scaled_gemv_kernel(const __grid_constant__ SgParams p, const GemvArgs g) {
     ++row;
     if (++n == p.N && GROUPED) {
       n = 0;
-      ++m0;
+      ++at;
     }
   }
   __syncthreads();

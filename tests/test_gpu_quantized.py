@@ -305,6 +305,44 @@ def test_grouped_many_experts():
     check_grouped(mb.grouped_scaled_mm(a, w, sa, sb, off, out_dtype=torch.float32), a, w, sa, sb, off)
 
 
+@pytest.mark.parametrize("K", [1, 17, 432, 512, 513, 1024, 1040, 2047, 2048, 2064])
+def test_few_rows_of_short_sums(K):
+    """More weight rows than warps: short rows are taken whole, several at a time."""
+    g = gen(K)
+    room = (K + 15) // 16 * 16
+    for N in (4800, 9473, 40001):
+        W, sb = ints((N, room), g)[:, :K].t(), scales((N,), g)
+        for M in (1, 2):
+            a, sa = ints((M, room), g)[:, :K], scales((M,), g)
+            check_product(mb.scaled_mm(a, W, sa, sb, out_dtype=torch.float32), a, W, sa, sb)
+    for counts, N in (([2, 0, 1], 1601), ([1, 1, 0, 3, 1, 1, 1], 613), ([0, 5], 3001)):
+        M = sum(counts)
+        W, sb = ints((len(counts), N, room), g)[:, :, :K].transpose(1, 2), scales((len(counts), N), g)
+        for extra in (0, 1):
+            if M + extra > 8:
+                continue
+            a, sa = ints((M + extra, room), g)[:, :K], scales((M + extra,), g)
+            y = mb.grouped_scaled_mm(a, W, sa, sb, offsets_of(counts), out_dtype=torch.float32)
+            check_grouped(y, a, W, sa, sb, offsets_of(counts))
+
+
+@pytest.mark.parametrize("K", [63, 700])
+def test_grouped_weights_off_16_bytes_few_used(K):
+    """Weights copied first, of the groups with rows alone: every group's place in turn."""
+    g = gen(K)
+    E, N = 600, 33
+    for layout in ("nk", "kn"):
+        W = ints((E, N, K), g).transpose(1, 2) if layout == "nk" else ints((E, K, N), g)
+        sb = scales((E, N), g)
+        for used in ([0], [599], [255, 256], list(range(0, 600, 7)), [3, 400, 599]):
+            counts = [0] * E
+            for i, e in enumerate(used):
+                counts[e] = 1 + i % 3
+            M = sum(counts)
+            a, sa, off = ints((M, K), g), scales((M,), g), offsets_of(counts)
+            check_grouped(mb.grouped_scaled_mm(a, W, sa, sb, off, out_dtype=torch.float32), a, W, sa, sb, off)
+
+
 def test_grouped_strides_and_broadcast_scales():
     g = gen(22)
     counts = [20, 0, 33]
