@@ -611,9 +611,37 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
               if (rr < live)
                 *reinterpret_cast<uint4 *>(C + (mw + rr) * p.c_rs + nw + ch * EPC) = ld_shared_v4(chunk_addr(rr, ch));
             }
+          } else if (p.c_cs == 1 && nw + 32 <= p.N) {
+            // Rows that start anywhere: the 16-byte chunks that lie whole in C, cut out of
+            // two staged ones, then the EPC elements before and after them by lanes of
+            // their own.  (An element a lane throughout: 5551 x 512 x 9315 bf16 85 us.)
+            const int ch = lane % NCH, rr0 = lane / NCH;
+            auto before = [&](const TO *row) {  // elements before the first whole chunk
+              return (int)((0 - (reinterpret_cast<uintptr_t>(row) / sizeof(TO))) % EPC);
+            };
+#pragma unroll
+            for (int i = 0; i < (ROWS + PASS - 1) / PASS; ++i) {
+              const int rr = i * PASS + rr0;
+              if (rr >= live) continue;
+              TO *dst = C + (mw + rr) * p.c_rs + nw;
+              const int sh = before(dst);
+              if (sh && ch == NCH - 1) continue;
+              *reinterpret_cast<uint4 *>(dst + sh + ch * EPC) =
+                  cut16(ld_shared_v4(chunk_addr(rr, ch)), ld_shared_v4(chunk_addr(rr, sh ? ch + 1 : ch)), sh * sizeof(TO));
+            }
+#pragma unroll
+            for (int i = 0; i < ROWS * EPC / 32; ++i) {
+              const int rr = i * (32 / EPC) + lane / EPC, j = lane % EPC;
+              if (rr >= live) continue;
+              TO *dst = C + (mw + rr) * p.c_rs + nw;
+              const int sh = before(dst), col = j < sh ? j : 32 - EPC + j;
+              if (sh)
+                dst[col] = *reinterpret_cast<const TO *>(staging + ew * C_::STAGING_WARP + (chunk_addr(rr, col / EPC) - stg) +
+                                                         (col % EPC) * sizeof(TO));
+            }
           } else {
-            // rows that start anywhere: an element a lane, along whichever of rows
-            // and columns is contiguous in C
+            // columns of C, the last ones of its rows, or any strides: an element a
+            // lane, along whichever of rows and columns is contiguous
             const uint8_t *own = staging + ew * C_::STAGING_WARP;
             auto staged = [&](int rr, int col) {
               return *reinterpret_cast<const TO *>(own + (chunk_addr(rr, col / EPC) - stg) + (col % EPC) * sizeof(TO));
@@ -651,13 +679,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
 }
 
 // Operands that TMA cannot read in place, copied to aligned rows: A's rows by the
-// first `split` blocks, B's by the others, in one launch.  A warp takes 512 bytes
-// of a row at a time, a lane 16 of them; the bytes past the row's end go to its
+// first `split` blocks, B's by the others, in one launch.  A lane takes 16 bytes of
+// a row at a time and the lanes run on through rows; the bytes past a row's end go to its
 // padding, which no tensor map covers.  Weights of groups without rows (offsets:
 // of the groups; null: all have some) are left where they are: no unit reads them,
 // and copying them all was most of a call with few rows (4 rows, 128 groups of 431 x
 // 8192: 276 us, 26 now; 1024 x 4 rows, 32 groups of 4095 x 2048: 199, 190).
-__global__ static void __launch_bounds__(256) scaled_pack_kernel(const PackArgs pa, const PackArgs pb, int split,
+__global__ static void __launch_bounds__(256, 4) scaled_pack_kernel(const PackArgs pa, const PackArgs pb, int split,
                                                                  const int *offsets, int M) {
   __shared__ uint16_t used[1024];  // groups with rows
   __shared__ int count[8];
@@ -687,26 +715,30 @@ __global__ static void __launch_bounds__(256) scaled_pack_kernel(const PackArgs 
       __syncthreads();
     }
   }
-  const int64_t segs = (a.cols + 511) / 512, total = batch * a.rows * segs;
-  const int64_t step = (int64_t)blocks * 8;
-  for (int64_t u0 = (int64_t)block * 8 + warp; u0 < total; u0 += 4 * step) {
-    // four units' words on their way at a time; words without a byte of the row are not read
+  // vectors numbered through the rows; a thread's are `step` apart: dn batches, dr rows, dc vectors
+  const int vecs = (int)((a.cols + 15) / 16), rows = (int)a.rows;
+  const int step = blocks * 256, at = block * 256 + threadIdx.x;
+  const int dc = step % vecs, dr = step / vecs % rows, dn = step / vecs / rows;
+  int c = at % vecs, r = at / vecs % rows, n = at / vecs / rows;
+  while (n < batch) {
+    // four words on their way at a time; those without a byte of the row are not read
     uint4 lo[4], hi[4];
     uint32_t off[4];
     int8_t *dst[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t u = u0 + i * step;
-      const bool small = total < (1ll << 32);
-      const int64_t r = small ? (uint32_t)u / (uint32_t)segs : u / segs;
-      const int64_t n = batch <= 1 ? 0 : small ? (uint32_t)r / (uint32_t)a.rows : r / a.rows;
-      const int c = (int)(u - r * segs) * 512 + lane * 16, left = u < total ? (int)a.cols - c : 0;
-      const int64_t b = some && left > 0 ? used[n] : n, row = r - n * a.rows;
-      const int8_t *src = static_cast<const int8_t *>(a.src) + b * a.bs + row * a.rs + c;
+      const bool on = n < batch;
+      const int64_t b = on ? (some ? used[n] : n) : 0;
+      const int8_t *src = static_cast<const int8_t *>(a.src) + b * a.bs + r * a.rs + c * 16;
       off[i] = (uint32_t)(reinterpret_cast<uintptr_t>(src) & 15);
-      lo[i] = load_once<true>(src - off[i], left > 0);
-      hi[i] = load_once<true>(src - off[i] + 16, off[i] && left > 16 - (int)off[i]);
-      dst[i] = left > 0 ? static_cast<int8_t *>(a.dst) + (b * a.rows + row) * a.ld + c : nullptr;
+      lo[i] = load_once<true>(src - off[i], on);
+      hi[i] = load_once<true>(src - off[i] + 16, on && off[i] && (int)a.cols - c * 16 > 16 - (int)off[i]);
+      dst[i] = on ? static_cast<int8_t *>(a.dst) + (b * rows + r) * a.ld + c * 16 : nullptr;
+      c += dc;
+      r += dr;
+      n += dn;
+      if (c >= vecs) { c -= vecs; ++r; }
+      if (r >= rows) { r -= rows; ++n; }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
