@@ -358,13 +358,16 @@ int thin_launch(const mb_scaled_desc *d, const SgPlan &pl, const sg::SgParams &p
                     st, 1, "scaled_gemm", p, g);
 }
 
-template <int BN, int PAIR, bool SWAP, class TO>
+template <int BN, int PAIR, bool SWAP, class TO, bool RUNS = false>
 int sg_launch_tile(const SgPlan &pl, sg::SgParams &p, cudaStream_t st) {
+  if constexpr (!SWAP && !RUNS) {
+    if (!p.c_vec && p.c_cs == 1) return sg_launch_tile<BN, PAIR, SWAP, TO, true>(pl, p, st);
+  }
   using C_ = sg::SgCfg<BN, PAIR, SWAP, TO>;
   p.split = pl.split;
   p.stages = C_::stages(pl.split);
   p.tiles_c = (int)ceil_div(p.N, C_::TCOLS);
-  constexpr auto kern = sg::scaled_gemm_kernel<BN, PAIR, SWAP, TO>;
+  constexpr auto kern = sg::scaled_gemm_kernel<BN, PAIR, SWAP, RUNS, TO>;
   constexpr int smem_max = C_::CAN_SPLIT ? std::max(C_::smem_bytes(1), std::max(C_::smem_bytes(2), std::max(C_::smem_bytes(4), C_::smem_bytes(8))))
                                          : C_::smem_bytes(1);
   static_assert(smem_max <= tc::SMEM_LIMIT, "shared memory");

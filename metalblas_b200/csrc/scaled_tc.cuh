@@ -166,6 +166,39 @@ __device__ __forceinline__ void scaled_sums(const int *sum, float scale_a, const
   }
 }
 
+// Moves the words x[0 .. W-1] up by `bytes` (0 to 15), with the last bytes of `before` in front.
+template <int W>
+__device__ __forceinline__ void shift_up(uint32_t *x, std::integral_constant<int, W>, const uint4 &before, uint32_t bytes) {
+  const uint32_t b[4] = {before.x, before.y, before.z, before.w};
+  const bool two = bytes & 8, one = bytes & 4;
+  uint32_t y[W + 2], z[W + 1];
+#pragma unroll
+  for (int k = -2; k < W; ++k) y[k + 2] = two ? (k < 2 ? b[(k + 2) & 3] : x[k < 2 ? 0 : k - 2]) : (k < 0 ? b[(k + 4) & 3] : x[k < 0 ? 0 : k]);
+#pragma unroll
+  for (int k = 0; k <= W; ++k) z[k] = one ? y[k] : y[k + 1];
+#pragma unroll
+  for (int k = 0; k < W; ++k) x[k] = __funnelshift_l(z[k], z[k + 1], (bytes & 3) * 8);
+}
+// Bytes past .. 15 (store_from) and 0 .. past-1 (store_up_to) of a 16-byte chunk, past a
+// multiple of TO's size and not 0, as 8, 4 and 2 bytes.
+template <class TO> __device__ __forceinline__ void store_from(char *chunk, const uint32_t *w, uint32_t past) {
+  if (past <= 8) *reinterpret_cast<uint2 *>(chunk + 8) = make_uint2(w[2], w[3]);
+  const uint32_t up4 = (past + 3) & ~3u;  // the first whole word
+  if (up4 & 4) *reinterpret_cast<uint32_t *>(chunk + up4) = up4 & 8 ? w[3] : w[1];
+  if constexpr (sizeof(TO) == 2) {
+    const uint32_t i = past >> 2, word = i & 2 ? (i & 1 ? w[3] : w[2]) : (i & 1 ? w[1] : w[0]);
+    if (past & 2) *reinterpret_cast<uint16_t *>(chunk + past) = (uint16_t)(word >> 16);
+  }
+}
+template <class TO> __device__ __forceinline__ void store_up_to(char *chunk, const uint32_t *w, uint32_t past) {
+  if (past & 8) *reinterpret_cast<uint2 *>(chunk) = make_uint2(w[0], w[1]);
+  if (past & 4) *reinterpret_cast<uint32_t *>(chunk + (past & 8)) = past & 8 ? w[2] : w[0];
+  if constexpr (sizeof(TO) == 2) {
+    const uint32_t i = past >> 2, word = i & 2 ? (i & 1 ? w[3] : w[2]) : (i & 1 ? w[1] : w[0]);
+    if (past & 2) *reinterpret_cast<uint16_t *>(chunk + (past & 12)) = (uint16_t)word;
+  }
+}
+
 // 4 consecutive results as the words of a staged row.
 template <class TO> __device__ __forceinline__ void pack4(const float *v, uint32_t *w) {
   if constexpr (sizeof(TO) == 4) {
@@ -180,7 +213,9 @@ template <class TO> __device__ __forceinline__ void pack4(const float *v, uint32
   }
 }
 
-template <int BN, int PAIR, bool SWAP, class TO>
+// RUNS: rows of C are contiguous but off 16 bytes (a kernel of its own: the shifts
+// cost the others 10% where the epilogue binds, 5551 x 512 x 9312 37.8 us).
+template <int BN, int PAIR, bool SWAP, bool RUNS, class TO>
 __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __grid_constant__ SgParams p) {
   using C_ = SgCfg<BN, PAIR, SWAP, TO>;
   using B_ = typename C_::B;
@@ -501,6 +536,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
         }
       } else {
         if (split > 1 && !all(mbar_wait_cluster(red_full, rphase, abort_flag, p.timeout_ns))) break;
+        static_assert(!(SWAP && RUNS), "lanes hold rows");
+        uint4 rest = make_uint4(0, 0, 0, 0);  // RUNS: the row's last chunk as converted
 #pragma unroll 1
         for (int c = 0; c < WCOLS; c += CH) {
           uint32_t r[32];
@@ -574,7 +611,27 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
                 if (r < t.rend && n0 + j < p.N) C[r + (n0 + j) * p.c_cs] = reinterpret_cast<const TO *>(w)[j];
               continue;
             }
-            if (p.c_tma) {  // the last step's store has read the staging rows
+            const int64_t nn = t.c0 + half * WCOLS + c;
+            if constexpr (RUNS) if (nn + 32 <= p.N) {
+              // A row that starts anywhere: its 32 elements move up to the 16-byte chunks of
+              // C that hold them, with the last chunk's rest before them.  What is left
+              // over at either end of the warp's columns goes out by itself.  (5551 x 512 x
+              // 9315 bf16 53 us; an element a lane 85, with chunks cut out of the staged
+              // rows 87: instructions bind it; rows of 9312 40.)
+              TO *own = C + m * p.c_rs + nn;
+              const uint32_t past = (uint32_t)(reinterpret_cast<uintptr_t>(own) & 15);
+              char *chunk = reinterpret_cast<char *>(own) - past;
+              const uint4 end = make_uint4(w[NCH - 1][0], w[NCH - 1][1], w[NCH - 1][2], w[NCH - 1][3]);
+              shift_up(&w[0][0], std::integral_constant<int, NCH * 4>(), rest, past);
+              if (c == 0 && past && m < t.rend) store_from<TO>(chunk, w[0], past);
+              if ((c + CH >= WCOLS || nn + 64 > p.N) && past && m < t.rend) {
+                uint32_t tail[4] = {0, 0, 0, 0};
+                shift_up(tail, std::integral_constant<int, 4>(), end, past);
+                store_up_to<TO>(chunk + 32 * sizeof(TO), tail, past);
+              }
+              rest = end;
+            }
+            if (!RUNS && p.c_tma) {  // the last step's store has read the staging rows
               if (lane == 0) bulk_wait_read0();
               __syncwarp();
             }
@@ -584,10 +641,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
                            "r"(w[ch][1]), "r"(w[ch][2]), "r"(w[ch][3])
                            : "memory");
             // 32 rows of the group (or up to the end of C, where the store clips)
-            // go out as one box; the rows before another group's by hand.
+            // go out as one box; the rows before another group's by hand, and so the
+            // columns before an end off 16 bytes: along them the store clips whole
+            // chunks alone, and wrote up to 14 bytes past a row of N = 33.
             const int64_t first_row = t.r0 + (PAIR == 2 ? (int)rank * BM : 0) + q * 32;
-            if (p.c_tma && (first_row + 32 <= t.rend || t.rend == p.M)) {
-              const int64_t nn = t.c0 + half * WCOLS + c;
+            if (!RUNS && p.c_tma && (first_row + 32 <= t.rend || t.rend == p.M) && (nn + 32 <= p.N || p.N % EPC == 0)) {
               fence_proxy_async_smem();
               __syncwarp();
               if (lane == 0 && first_row < t.rend && nn < p.N) {
@@ -602,7 +660,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
           const int64_t mw = SWAP ? t.r0 + half * WCOLS + c : t.r0 + (PAIR == 2 ? (int)rank * BM : 0) + q * 32;
           const int64_t nw = SWAP ? t.c0 + q * 32 : t.c0 + half * WCOLS + c;
           const int live = (int)min((int64_t)ROWS, t.rend - mw);   // rows of the group among them
-          if (p.c_vec && nw + 32 <= p.N) {
+          if (!RUNS && p.c_vec && nw + 32 <= p.N) {
             // 16-byte chunks, whole rows by neighbouring lanes
             const int ch = lane % NCH, rr0 = lane / NCH;
 #pragma unroll
@@ -611,33 +669,17 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
               if (rr < live)
                 *reinterpret_cast<uint4 *>(C + (mw + rr) * p.c_rs + nw + ch * EPC) = ld_shared_v4(chunk_addr(rr, ch));
             }
-          } else if (p.c_cs == 1 && nw + 32 <= p.N) {
-            // Rows that start anywhere: the 16-byte chunks that lie whole in C, cut out of
-            // two staged ones, then the EPC elements before and after them by lanes of
-            // their own.  (An element a lane throughout: 5551 x 512 x 9315 bf16 85 us.)
+          } else if (RUNS && nw + 32 <= p.N) {
+            // the staged chunks lie on 16 bytes of their rows; the first one of the
+            // warp's columns has been stored by its lane where it is not whole
             const int ch = lane % NCH, rr0 = lane / NCH;
-            auto before = [&](const TO *row) {  // elements before the first whole chunk
-              return (int)((0 - (reinterpret_cast<uintptr_t>(row) / sizeof(TO))) % EPC);
-            };
+            const TO *dst = C + (mw + rr0) * p.c_rs + nw;
 #pragma unroll
-            for (int i = 0; i < (ROWS + PASS - 1) / PASS; ++i) {
+            for (int i = 0; i < (ROWS + PASS - 1) / PASS; ++i, dst += PASS * p.c_rs) {
               const int rr = i * PASS + rr0;
-              if (rr >= live) continue;
-              TO *dst = C + (mw + rr) * p.c_rs + nw;
-              const int sh = before(dst);
-              if (sh && ch == NCH - 1) continue;
-              *reinterpret_cast<uint4 *>(dst + sh + ch * EPC) =
-                  cut16(ld_shared_v4(chunk_addr(rr, ch)), ld_shared_v4(chunk_addr(rr, sh ? ch + 1 : ch)), sh * sizeof(TO));
-            }
-#pragma unroll
-            for (int i = 0; i < ROWS * EPC / 32; ++i) {
-              const int rr = i * (32 / EPC) + lane / EPC, j = lane % EPC;
-              if (rr >= live) continue;
-              TO *dst = C + (mw + rr) * p.c_rs + nw;
-              const int sh = before(dst), col = j < sh ? j : 32 - EPC + j;
-              if (sh)
-                dst[col] = *reinterpret_cast<const TO *>(staging + ew * C_::STAGING_WARP + (chunk_addr(rr, col / EPC) - stg) +
-                                                         (col % EPC) * sizeof(TO));
+              const uintptr_t at = reinterpret_cast<uintptr_t>(dst);
+              if (rr < live && (c | ch || at % 16 == 0))
+                *reinterpret_cast<uint4 *>((at & ~uintptr_t(15)) + ch * 16) = ld_shared_v4(chunk_addr(rr, ch));
             }
           } else {
             // columns of C, the last ones of its rows, or any strides: an element a

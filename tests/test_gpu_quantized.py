@@ -343,6 +343,34 @@ def test_grouped_weights_off_16_bytes_few_used(K):
             check_grouped(mb.grouped_scaled_mm(a, W, sa, sb, off, out_dtype=torch.float32), a, W, sa, sb, off)
 
 
+@pytest.mark.parametrize("out_dtype", FLOATS)
+def test_rows_of_the_output_that_start_anywhere(out_dtype):
+    """Every start of a row against 16 bytes, every end; what lies around the rows stays."""
+    g = gen(31)
+    M, K = 150, 64
+    a, sa = ints((M, K), g), scales((M,), g)
+    off = offsets_of([70, 0, 45, 30])  # and five rows of no group
+    for N in (31, 32, 33, 63, 64, 100, 128, 129, 161, 255, 257, 300, 523):
+        w, sb = ints((N, K), g).t(), scales((N,), g)
+        W, SB = ints((4, N, K), g).transpose(1, 2), scales((4, N), g)
+        for start, pitch in ((0, N + 9), (1, N + 1), (3, N + 7), (4, N + 8), (6, N + 13), (7, N + 26)):
+            for plan in ((128, 1, -1, 1), (256, 1, -1, 1), (256, 1, -1, 2), (512, 1, -1, 2), (64, 1, 1, 1)):
+                room = torch.full((M + 1, pitch), 7.0, dtype=out_dtype, device=DEV).view(-1)
+                view = room[start:start + (M - 1) * pitch + N].as_strided((M, N), (pitch, 1), start)
+                kept = room.clone()
+                kept.as_strided((M, N), (pitch, 1), start).fill_(0)
+                mb.scaled_mm(a, w, sa, sb, out=view, _plan=plan)
+                check_product(view, a, w, sa, sb)
+                view_copy = room.clone()
+                view_copy.as_strided((M, N), (pitch, 1), start).fill_(0)
+                assert torch.equal(view_copy, kept)
+                mb.grouped_scaled_mm(a, W, sa, SB, off, out=view, _plan=plan)
+                check_grouped(view, a, W, sa, SB, off)
+                view_copy = room.clone()
+                view_copy.as_strided((M, N), (pitch, 1), start).fill_(0)
+                assert torch.equal(view_copy, kept)
+
+
 def test_grouped_strides_and_broadcast_scales():
     g = gen(22)
     counts = [20, 0, 33]
