@@ -192,14 +192,15 @@ bool tma_rows(const void *p, int64_t rows, int64_t cols, int64_t &rs, int64_t cs
   return aligned16(p) && rs > 0 && rs % 16 == 0 && (groups <= 1 || (gs >= 0 && gs % 16 == 0));
 }
 
-// One tile shape's time in SM cycles, fitted to the kernel's times on B200 (8192 x
-// 512..8192 x 8192, 16384 x 4096 x 4096 and the thin shapes of 4 to 256 rows).  A tile
-// takes its 128-byte K-blocks, bound by the operands' way into shared memory (59
-// B/clk, 64 for 128 x 256, 47 on each SM of a pair, 36 for the 512-wide pair
-// tile), plus a hand-over, but never less than its epilogue, which runs beside
-// the next tile's K-blocks; the 512-wide tile fills TMEM alone, so its epilogue
-// is all hand-over.  The chip's HBM gives 22.4 B/clk per SM.  Splitting K costs a
-// cluster's exchange: 0.7 us at 16 columns, 3.5 us at 128, again for each doubling.
+// One tile shape's time in SM cycles, up to what all have in common.  A tile takes
+// its 128-byte K-blocks and a hand-over; beside it runs the epilogue of the tile
+// before, so a wave takes the longer of the two, and the last wave both.  The
+// 512-wide pair tile fills TMEM alone: its epilogue is all hand-over.  The chip's
+// HBM gives 22.4 B/clk per SM.  Splitting K costs a cluster's exchange for each doubling.
+// The constants are fitted to times on B200 of every tile and split over 240 shapes (17
+// to 16000 rows, K of 128 to 12000, N of 256 to 15000, half as many with 4 to 128
+// groups), where the choice costs 2.4% over the best tile in the mean (7% with
+// a model that had the last wave's epilogue run beside the next).
 struct SgCost {
   double t;
   int split;
@@ -212,24 +213,25 @@ SgCost sg_cost(const mb_scaled_desc *d, int swap, int bn, int pair, int sms, int
   // groups do not end on tile boundaries: half a tile more each
   const double tiles_r = d->groups && rows > trows / 2 ? M / trows + 0.5 * active : active * std::ceil(rows / trows);
   const double units = tiles_r * (double)ceil_div(d->N, swap ? 128 : bn);
-  const double out = elem_size(d->out_dtype) == 4 ? 1.3 : 1.0;
+  const double out = elem_size(d->out_dtype) == 4 ? 1.15 : 1.0;
   const bool wide = bn > 256;
-  const double kbc = wide ? 1330.0 : pair == 2 ? 700.0 : bn == 256 ? 770.0 : (128.0 + bn) * 128.0 / 59.0;
-  const double hand = wide ? 8000.0 * out : pair == 2 ? 1500.0 : bn == 256 ? 1200.0 : 500.0 + 4.0 * bn;
-  const double epi = wide ? 0.0 : (pair == 2 ? 7000.0 : (swap ? 25.0 : bn == 256 ? 22.0 : 28.0) * bn) * out;
+  const double kbc = wide ? 1795.0 : pair == 2 ? 748.0 : bn == 256 ? 1133.0 : (128.0 + bn) * 128.0 / 46.5;
+  const double hand = wide ? 15660.0 * out : pair == 2 ? 1220.0 : bn == 256 ? 80.0 : 1480.0;
+  const double epi = wide ? 0.0 : (pair == 2 ? 10770.0 : (swap ? 33.0 : bn == 256 ? 16.4 : 9.4) * bn) * out;
   // a group's weights read for a second tile of its rows come from L2, mostly
-  const double again = d->groups ? 0.4 * std::min(1.0, tiles_r / active - 1.0) : 0.0;
+  const double again = d->groups ? 0.1 * std::min(1.0, tiles_r / active - 1.0) : 0.0;
   const double bytes = active * (double)d->N * (double)d->K * (1.0 + again) + M * (double)d->K +
                        M * (double)d->N * elem_size(d->out_dtype);
   SgCost best{1e300, 1};
   for (int split = 1, log2 = 0; split <= 8; split *= 2, ++log2) {
     if (force_split ? split != force_split : (split > 1 && (pair == 2 || bn > 128 || kb < split))) continue;
     // clusters of 4 and 8 leave SMs over in some GPCs
-    const double slots = std::floor((double)sms / (pair * split) * (split >= 4 ? 0.9 : 1.0));
+    const double slots = std::floor((double)sms / (pair * split) * (split == 8 ? 0.75 : split == 4 ? 0.9 : 1.0));
     const double waves = std::ceil(units / slots);
-    const double compute = waves * std::max(std::ceil(kb / split) * kbc + hand + log2 * (500.0 + 40.0 * bn), epi);
+    const double tile = std::ceil(kb / split) * kbc + hand + log2 * 1900.0;
+    const double compute = (waves - 1.0) * std::max(tile, epi) + tile + epi;
     const double hbm = bytes / (22.4 * sms);
-    const double t = std::max(compute, hbm) + 0.15 * std::min(compute, hbm);  // they overlap, not quite
+    const double t = std::max(compute, hbm) + 0.21 * std::min(compute, hbm);  // they overlap, not quite
     if (t < best.t) best = {t, split};
   }
   return best;
