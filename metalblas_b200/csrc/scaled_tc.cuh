@@ -42,10 +42,10 @@
 //                                  and 256 tiles over 74 pairs;
 //   16384 rows by 8 experts of 4096 x 14336   650 us, 2960 TOPS: the same, and
 //                                  tiles that end with their group;
-//   8192 x 512 x 8192              45 us: the epilogue (134 MB out);
+//   8192 x 512 x 8192              45 to 49 us: the epilogue (134 MB out);
 //   16 rows by 8 experts of 4096 x 14336      65.8 us, 6.2 TB/s: the weights' bytes;
 //   16 x 4096 x 14336              14.3 us, 4.1 TB/s: 112 tiles keep 112 SMs busy.
-// The tile is chosen by sg_cost (mb_ops.cu) from these times' model; TROWS, TCOLS
+// The tile is chosen by sg_cost (mb_ops.cu), a model of such times; TROWS, TCOLS
 // and split change no result.
 #pragma once
 #include "pack.cuh"
