@@ -758,10 +758,12 @@ __global__ static void __launch_bounds__(256, 4) scaled_pack_kernel(const PackAr
     }
   }
   // vectors numbered through the rows; a thread's are `step` apart: dn batches, dr rows, dc vectors
-  const int vecs = (int)((a.cols + 15) / 16), rows = (int)a.rows;
-  const int step = blocks * 256, at = block * 256 + threadIdx.x;
-  const int dc = step % vecs, dr = step / vecs % rows, dn = step / vecs / rows;
-  int c = at % vecs, r = at / vecs % rows, n = at / vecs / rows;
+  // (r + dr can pass 31 bits)
+  const uint32_t vecs = (uint32_t)((a.cols + 15) / 16), rows = (uint32_t)a.rows;
+  const uint32_t step = blocks * 256, at = block * 256 + threadIdx.x;
+  const uint32_t dc = step % vecs, dr = step / vecs % rows, dn = step / vecs / rows;
+  uint32_t c = at % vecs, r = at / vecs % rows;
+  int n = (int)(at / vecs / rows);
   while (n < batch) {
     // four words on their way at a time; those without a byte of the row are not read
     uint4 lo[4], hi[4];
@@ -771,14 +773,14 @@ __global__ static void __launch_bounds__(256, 4) scaled_pack_kernel(const PackAr
     for (int i = 0; i < 4; ++i) {
       const bool on = n < batch;
       const int64_t b = on ? (some ? used[n] : n) : 0;
-      const int8_t *src = static_cast<const int8_t *>(a.src) + b * a.bs + r * a.rs + c * 16;
+      const int8_t *src = static_cast<const int8_t *>(a.src) + b * a.bs + (int64_t)r * a.rs + c * 16;
       off[i] = (uint32_t)(reinterpret_cast<uintptr_t>(src) & 15);
       lo[i] = load_once<true>(src - off[i], on);
-      hi[i] = load_once<true>(src - off[i] + 16, on && off[i] && (int)a.cols - c * 16 > 16 - (int)off[i]);
-      dst[i] = on ? static_cast<int8_t *>(a.dst) + (b * rows + r) * a.ld + c * 16 : nullptr;
+      hi[i] = load_once<true>(src - off[i] + 16, on && off[i] && c * 16 + 16 - off[i] < (uint32_t)a.cols);
+      dst[i] = on ? static_cast<int8_t *>(a.dst) + (b * (int64_t)rows + r) * a.ld + c * 16 : nullptr;
       c += dc;
       r += dr;
-      n += dn;
+      n += (int)dn;
       if (c >= vecs) { c -= vecs; ++r; }
       if (r >= rows) { r -= rows; ++n; }
     }
