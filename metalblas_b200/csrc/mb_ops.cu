@@ -192,15 +192,14 @@ bool tma_rows(const void *p, int64_t rows, int64_t cols, int64_t &rs, int64_t cs
   return aligned16(p) && rs > 0 && rs % 16 == 0 && (groups <= 1 || (gs >= 0 && gs % 16 == 0));
 }
 
-// One tile shape's time in SM cycles, up to what all have in common.  A tile takes
-// its 128-byte K-blocks and a hand-over; beside it runs the epilogue of the tile
-// before, so a wave takes the longer of the two, and the last wave both.  The
-// 512-wide pair tile fills TMEM alone: its epilogue is all hand-over.  The chip's
-// HBM gives 22.4 B/clk per SM.  Splitting K costs a cluster's exchange for each doubling.
-// The constants are fitted to times on B200 of every tile and split over 240 shapes (17
-// to 16000 rows, K of 128 to 12000, N of 256 to 15000, half as many with 4 to 128
-// groups), where the choice costs 2.4% over the best tile in the mean (7% with
-// a model that had the last wave's epilogue run beside the next).
+// One tile shape's time in SM cycles.  A tile takes its 128-byte K-blocks and a
+// hand-over; beside it runs the epilogue of the tile before, so a wave takes the
+// longer of the two, and the last wave both.  The chip's HBM gives 22.4 B/clk per
+// SM.  Splitting K costs a cluster's exchange for each doubling.  The constants are
+// fitted to times on B200 of every tile and split over 240 shapes (17 to 16000
+// rows, K of 128 to 12000, N of 256 to 15000, half as many with 4 to 128 groups): the
+// choice costs 2% over the best tile in the mean (7% with a model that had the
+// last wave's epilogue run beside the next).  A 512-wide pair tile won in none.
 struct SgCost {
   double t;
   int split;
@@ -213,13 +212,12 @@ SgCost sg_cost(const mb_scaled_desc *d, int swap, int bn, int pair, int sms, int
   // groups do not end on tile boundaries: half a tile more each
   const double tiles_r = d->groups && rows > trows / 2 ? M / trows + 0.5 * active : active * std::ceil(rows / trows);
   const double units = tiles_r * (double)ceil_div(d->N, swap ? 128 : bn);
-  const double out = elem_size(d->out_dtype) == 4 ? 1.15 : 1.0;
-  const bool wide = bn > 256;
-  const double kbc = wide ? 1795.0 : pair == 2 ? 748.0 : bn == 256 ? 1133.0 : (128.0 + bn) * 128.0 / 46.5;
-  const double hand = wide ? 15660.0 * out : pair == 2 ? 1220.0 : bn == 256 ? 80.0 : 1480.0;
-  const double epi = wide ? 0.0 : (pair == 2 ? 10770.0 : (swap ? 33.0 : bn == 256 ? 16.4 : 9.4) * bn) * out;
+  const double kbc = pair == 2 ? 660.0 : bn == 256 ? 850.0 : (128.0 + bn) * 128.0 / (swap ? 46.5 : 49.5);
+  const double hand = pair == 2 ? 2560.0 : bn == 256 ? 2900.0 : 1200.0;
+  const double epi = pair == 2 ? 10400.0 : (swap ? 37.5 : bn == 256 ? 19.7 : 29.5) * bn;
+  const double start = pair == 2 ? 2600.0 : bn == 256 ? 2150.0 : swap ? 5100.0 : 2950.0;
   // a group's weights read for a second tile of its rows come from L2, mostly
-  const double again = d->groups ? 0.1 * std::min(1.0, tiles_r / active - 1.0) : 0.0;
+  const double again = d->groups ? 0.14 * std::min(1.0, tiles_r / active - 1.0) : 0.0;
   const double bytes = active * (double)d->N * (double)d->K * (1.0 + again) + M * (double)d->K +
                        M * (double)d->N * elem_size(d->out_dtype);
   SgCost best{1e300, 1};
@@ -228,10 +226,10 @@ SgCost sg_cost(const mb_scaled_desc *d, int swap, int bn, int pair, int sms, int
     // clusters of 4 and 8 leave SMs over in some GPCs
     const double slots = std::floor((double)sms / (pair * split) * (split == 8 ? 0.75 : split == 4 ? 0.9 : 1.0));
     const double waves = std::ceil(units / slots);
-    const double tile = std::ceil(kb / split) * kbc + hand + log2 * 1900.0;
-    const double compute = (waves - 1.0) * std::max(tile, epi) + tile + epi;
+    const double tile = std::ceil(kb / split) * kbc + hand + log2 * 1960.0;
+    const double compute = start + (waves - 1.0) * std::max(tile, epi) + tile + epi;
     const double hbm = bytes / (22.4 * sms);
-    const double t = std::max(compute, hbm) + 0.21 * std::min(compute, hbm);  // they overlap, not quite
+    const double t = std::max(compute, hbm) + 0.35 * std::min(compute, hbm);  // they overlap, not quite
     if (t < best.t) best = {t, split};
   }
   return best;
@@ -301,7 +299,7 @@ int sg_plan(const mb_scaled_desc *d, SgPlan &pl) {
     }
   }
   static const struct { int swap, bn, pair; } tiles[] = {{1, 16, 1},  {1, 32, 1},  {1, 64, 1},  {1, 128, 1},
-                                                         {0, 128, 1}, {0, 256, 1}, {0, 256, 2}, {0, 512, 2}};
+                                                         {0, 128, 1}, {0, 256, 1}, {0, 256, 2}};
   double best = 1e300;
   for (const auto &c : tiles) {
     if (d->tile_n && d->tile_n != c.bn) continue;
@@ -445,7 +443,7 @@ int sg_launch(const mb_scaled_desc *d, const SgPlan &pl, cudaStream_t st) {
   if (rc) return rc;
   // boxes of 128 bytes along the contiguous dimension
   CUtensorMap *ta = pl.swap ? &p.tmB : &p.tmA, *tw = pl.swap ? &p.tmA : &p.tmB;
-  const int w_rows = pl.swap ? 128 : std::min(pl.bn, 256) / pl.pair;  // channels per box
+  const int w_rows = pl.swap ? 128 : pl.bn / pl.pair;  // channels per box
   rc = encode_map(ta, MB_I8, A, d->K, d->M, 1, pl.a_rs, 0, 128, pl.swap ? pl.bn : 128);
   if (!rc)
     rc = pl.w_mn ? encode_map(tw, MB_I8, B, d->N, d->K, nB, pl.w_ld, pl.sB, 128, 128)
@@ -468,7 +466,7 @@ int sg_launch(const mb_scaled_desc *d, const SgPlan &pl, cudaStream_t st) {
     }
   }
   if (pl.pair == 1) return pl.bn == 128 ? sg_launch_tile<128, 1, false, TO>(pl, p, st) : sg_launch_tile<256, 1, false, TO>(pl, p, st);
-  return pl.bn == 256 ? sg_launch_tile<256, 2, false, TO>(pl, p, st) : sg_launch_tile<512, 2, false, TO>(pl, p, st);
+  return sg_launch_tile<256, 2, false, TO>(pl, p, st);
 }
 
 }  // namespace
