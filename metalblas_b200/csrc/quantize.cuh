@@ -62,6 +62,10 @@ template <class T> __device__ __forceinline__ void keep_first(Vec<T> &v, int n) 
 // compiler interleaved loads and sums to save registers, two or three in flight
 // (combine of 4096 tokens x 8 x 4096 bf16: 72 us, 4.2 TB/s).
 // KEEP: the neighbouring thread reads the same word, so it stays in L1.
+// The loads are ordinary (coherent) ones: a kernel launched with programmatic
+// serialization may be resident while the kernel before it still writes these
+// bytes, and pdl_wait orders ordinary loads only; the non-coherent form is for
+// memory that nobody writes as long as the kernel lives.
 template <bool KEEP = false>
 __device__ __forceinline__ uint4 load_once(const void *p, bool on) {
   uint4 v;
@@ -69,14 +73,14 @@ __device__ __forceinline__ uint4 load_once(const void *p, bool on) {
     asm volatile(
         "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %5, 0;\n\t"
         "mov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
-        "@q ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+        "@q ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
         : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
         : "l"(p), "r"((uint32_t)on));
   else
     asm volatile(
         "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %5, 0;\n\t"
         "mov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
-        "@q ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+        "@q ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
         : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
         : "l"(p), "r"((uint32_t)on));
   return v;
