@@ -12,8 +12,10 @@
 //    the B200 form of gemv_nt (metalblas/shaders/gemv_nt.h:16-101): one warp
 //    per row, 16-byte loads, a warp-shuffle reduction.
 // Orientation is chosen by the host like the reference's _dispatch_gemv
-// (metalblas/dispatch.py:49-70).  Loads of W use ld.global.nc with L1
-// no-allocate (W is streamed once); x is small and re-read from L1/L2.
+// (metalblas/dispatch.py:49-70).  Loads of W do not allocate in L1 (W is
+// streamed once); x is small and re-read from L1/L2.  All are coherent loads:
+// the kernel may be resident while the one before it still writes x or W, and
+// pdl_wait orders those only.
 #pragma once
 #include "mb_common.cuh"
 
@@ -48,14 +50,14 @@ struct VecLoad {
   static_assert(sizeof(T) * VEC == 16, "16-byte vectors");
   __device__ static __forceinline__ void load(const T *p, T (&out)[VEC]) {
     U x;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(x.u.x), "=r"(x.u.y), "=r"(x.u.z), "=r"(x.u.w) : "l"(p));
 #pragma unroll
     for (int i = 0; i < VEC; ++i) out[i] = x.v[i];
   }
   __device__ static __forceinline__ uint4 raw(const T *p) {
     uint4 q;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "l"(p));
     return q;
   }
@@ -400,7 +402,7 @@ __global__ void __launch_bounds__(NW * 32) gemv_rows_kernel(const GemvParams p) 
           T xv[VEC];
           const T *xp = X + kk;
           union { uint4 q; T v[VEC]; } xu;
-          xu.q = __ldg(reinterpret_cast<const uint4 *>(xp));
+          xu.q = *reinterpret_cast<const uint4 *>(xp);
 #pragma unroll
           for (int i = 0; i < VEC; ++i) xv[i] = xu.v[i];
 #pragma unroll
@@ -483,7 +485,7 @@ gemv_rows_smem_kernel(const GemvParams p) {
     __syncthreads();  // previous chunk fully consumed
     for (int i = threadIdx.x * VEC; i < kn; i += NW * 32 * VEC) {
       if (i + VEC <= kn) {
-        *reinterpret_cast<uint4 *>(&xs[i]) = __ldg(reinterpret_cast<const uint4 *>(X + kc + i));
+        *reinterpret_cast<uint4 *>(&xs[i]) = *reinterpret_cast<const uint4 *>(X + kc + i);
       } else {
         for (int j = 0; j < VEC && i + j < kn; ++j) xs[i + j] = X[kc + i + j];
       }

@@ -652,7 +652,7 @@ __device__ __forceinline__ void epi_real(const TcParams &p, int b, int m, int n0
     const T *row = (const T *)p.bias + (int64_t)b * p.bias_bs + (int64_t)m * p.bias_rs;
     if (BYTES % 16 == 0 && p.bias_cs == 1 && n0 + NC <= p.N && (reinterpret_cast<uintptr_t>(row + n0) & 15) == 0) {
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) u.q[i] = __ldg(reinterpret_cast<const uint4 *>(row + n0) + i);
+      for (int i = 0; i < NQ; ++i) u.q[i] = reinterpret_cast<const uint4 *>(row + n0)[i];
     } else {
 #pragma unroll
       for (int j = 0; j < NC; ++j) u.t[j] = (n0 + j < p.N) ? row[(int64_t)(n0 + j) * p.bias_cs] : T();

@@ -102,3 +102,31 @@ def test_quantize_then_product(rows, K, N, start):
         pause()
         return (y,)
     same_as_one_by_one(step)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("K,N", [(640, 1024), (2048, 260)])
+def test_products_with_one_row(dtype, K, N):
+    """The row, the matrix (in both orientations) and the bias of a product, each made by the
+    product before it."""
+    g = gen(K + N)
+    a = [torch.randn(1, 128, generator=g).to(dtype).to(DEV) for _ in range(ROUNDS)]
+    b = torch.randn(128, K, generator=g).to(dtype).to(DEV)
+    p = [torch.randn(K, 64, generator=g).to(dtype).to(DEV) for _ in range(4)]
+    q = torch.randn(64, N, generator=g).to(dtype).to(DEV)
+    x, w = torch.empty(1, K, dtype=dtype, device=DEV), torch.empty(K, N, dtype=dtype, device=DEV)
+    wt = torch.empty(N, K, dtype=dtype, device=DEV)
+
+    def step(i, pause):
+        mb.matmul(a[i], b, out=x)
+        pause()
+        mb.matmul(p[i % 4], q, out=w)
+        pause()
+        y = mb.matmul(x, w)
+        pause()
+        mb.matmul(q.t(), p[i % 4].t(), out=wt)
+        pause()
+        z = mb.matmul(x, wt.t())
+        pause()
+        return y, z, mb.addmm(y[0], p[i % 4], q)
+    same_as_one_by_one(step)

@@ -16,6 +16,9 @@ CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
 OPERATORS = ("quantize.cuh", "experts.cuh", "scaled_tc.cuh", "scaled_gemv.cuh")
 
 
+PRODUCTS = ("gemv.cuh", "tc_gemm.cuh")
+
+
 def code_of(name):
     with open(os.path.join(CSRC, name)) as f:
         return re.sub(r"//[^\n]*", "", f.read())
@@ -23,5 +26,11 @@ def code_of(name):
 
 @pytest.mark.parametrize("name", OPERATORS)
 def test_operators_load_coherently(name):
+    code = code_of(name)
+    assert "ld.global.nc" not in code and "__ldg" not in code
+
+
+@pytest.mark.parametrize("name", PRODUCTS)
+def test_products_load_coherently(name):
     code = code_of(name)
     assert "ld.global.nc" not in code and "__ldg" not in code
