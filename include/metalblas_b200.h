@@ -57,7 +57,7 @@ typedef enum mb_status {
     MB_ERR_UNSUPPORTED = 2,    /* dtype or layout not handled by the forced backend -> NotImplementedError */
     MB_ERR_LAUNCH = 3,         /* CUDA launch or driver error               -> RuntimeError */
     MB_ERR_DEVICE_TIMEOUT = 4, /* a bounded device-side wait ran out        -> RuntimeError */
-    MB_ERR_WORKSPACE = 5       /* workspace missing or too small            -> ValueError */
+    MB_ERR_WORKSPACE = 5       /* workspace missing, too small or unaligned -> ValueError */
 } mb_status;
 
 /*
@@ -291,7 +291,8 @@ typedef struct mb_scaled_desc {
 void mb_scaled_desc_init(mb_scaled_desc *d);
 int mb_scaled_gemm(const mb_scaled_desc *d, void *stream);
 /* Bytes of scratch mb_scaled_gemm needs for this descriptor (0 for operands
- * read in place).  The contents need not be kept or cleared. */
+ * read in place), on a 16-byte boundary.  The contents need not be kept or
+ * cleared. */
 int64_t mb_scaled_workspace_size(const mb_scaled_desc *d);
 /* One line on the plan the descriptor gets; its length, or a negative status. */
 int mb_scaled_plan(const mb_scaled_desc *d, char *buf, int buflen);

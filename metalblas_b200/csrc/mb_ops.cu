@@ -522,6 +522,8 @@ int mb_scaled_gemm(const mb_scaled_desc *d, void *stream) {
   if (rc || pl.empty) return rc;
   if (pl.ws_bytes > 0 && (!d->workspace || d->workspace_bytes < pl.ws_bytes))
     return fail(MB_ERR_WORKSPACE, "workspace of %lld bytes required", (long long)pl.ws_bytes);
+  if (pl.ws_bytes > 0 && !aligned16(d->workspace))  // operand copies are stored and loaded 16 bytes at a time
+    return fail(MB_ERR_WORKSPACE, "the workspace must start on a 16-byte boundary");
   return by_float(d->out_dtype, [&](auto *tag) {
     return sg_launch<std::remove_pointer_t<decltype(tag)>>(d, pl, (cudaStream_t)stream);
   });
