@@ -1584,6 +1584,20 @@ template <> struct IsTc<__nv_bfloat16> { static constexpr bool v = true; };
 template <> struct IsTc<int8_t> { static constexpr bool v = true; };
 template <> struct IsTc<uint8_t> { static constexpr bool v = true; };
 
+// The plan's scratch: present, large enough, and on a boundary its kernels can
+// use.  Tensor-core plans move partial sums and operand copies by 16 bytes; the
+// GEMV kernels hold tickets and single accumulators.
+int check_workspace(const mb_gemm_desc *d, const Plan &pl) {
+  if (pl.ws_bytes <= 0) return MB_OK;
+  if (d->workspace == nullptr || d->workspace_bytes < pl.ws_bytes)
+    return fail(MB_ERR_WORKSPACE, "workspace of %lld bytes required", (long long)pl.ws_bytes);
+  const bool gemv = pl.kind == PK_GEMV_COLS || pl.kind == PK_GEMV_ROWS;
+  const uintptr_t align = !gemv ? 16 : acc_is_8byte(d->dtype) ? 8 : 4;
+  if (reinterpret_cast<uintptr_t>(d->workspace) % align)
+    return fail(MB_ERR_WORKSPACE, "the workspace must start on a %d-byte boundary", (int)align);
+  return MB_OK;
+}
+
 // `query`: plan without a device if none is present (a B200's 148 SMs are
 // assumed), so the tile table can be inspected on a host without a GPU.
 int plan_for(const mb_gemm_desc *d, Plan &pl, Op &o, int &sms, bool query = false) {
@@ -1707,8 +1721,8 @@ int mb_gemm(const mb_gemm_desc *d, void *stream) {
   int rc = plan_for(d, pl, o, sms);
   if (rc) return rc;
   if (pl.kind == PK_EMPTY) return MB_OK;
-  if (pl.ws_bytes > 0 && (d->workspace == nullptr || d->workspace_bytes < pl.ws_bytes))
-    return fail(MB_ERR_WORKSPACE, "workspace of %lld bytes required", (long long)pl.ws_bytes);
+  rc = check_workspace(d, pl);
+  if (rc) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const EpiScalars e = make_epi(d);
   return by_dtype(d->dtype, [&](auto *tag) -> int {
@@ -1764,8 +1778,8 @@ int mb_gemm_peer(const mb_gemm_desc *d, const mb_peer_targets *peers, void *stre
     rc = plan_for(&q, pl, o, sms);
     if (rc) return rc;
   }
-  if (pl.ws_bytes > 0 && (d->workspace == nullptr || d->workspace_bytes < pl.ws_bytes))
-    return fail(MB_ERR_WORKSPACE, "workspace of %lld bytes required", (long long)pl.ws_bytes);
+  rc = check_workspace(d, pl);
+  if (rc) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const EpiScalars e = make_epi(d);
   return by_dtype(d->dtype, [&](auto *tag) -> int {
