@@ -790,15 +790,22 @@ __global__ static void __launch_bounds__(256, 4) scaled_pack_kernel(const PackAr
   }
 }
 
-// K = 0: the sum is empty.
+// K = 0: the sum is empty.  (Offsets that are not ascending name no groups, as
+// in the other kernels.)
 template <class TO>
 __global__ void __launch_bounds__(256) scaled_empty_kernel(const SgParams p) {
   pdl_trigger();
   pdl_wait();
+  int wrong = 0;
+  if (p.offsets)
+    for (int e = threadIdx.x + 1; e < p.groups; e += 256)
+      wrong |= min(max(p.offsets[e + 1], 0), p.M) < min(max(p.offsets[e], 0), p.M);
+  wrong = __syncthreads_or(wrong);
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)p.M * p.N; i += (int64_t)gridDim.x * 256) {
     const int64_t m = i / p.N, n = i - m * p.N;
     int e = 0;
     if (p.offsets) {
+      if (wrong) e = p.groups;
       while (e < p.groups && m >= p.offsets[e + 1]) ++e;
     }
     float v = 0.f;
