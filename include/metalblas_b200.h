@@ -270,7 +270,8 @@ int mb_quantize(int32_t dtype, int64_t rows, int64_t cols, const void *x, int64_
  *     they are not ascending, every row is set to zero.
  * Operands with a unit stride, a 16-byte aligned base and 16-byte multiples in
  * the other strides are read in place; others are copied into the workspace
- * first.  K <= 131071, so that no sum leaves 32 bits. */
+ * first.  K <= 131071, so that no sum leaves 32 bits.  No two elements of C may
+ * have one address. */
 typedef struct mb_scaled_desc {
     int32_t out_dtype, bias_dtype;       /* bias_dtype: out_dtype or MB_F32      */
     int64_t M, N, K, groups;

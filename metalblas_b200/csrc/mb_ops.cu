@@ -6,6 +6,7 @@
 #include <atomic>
 #include <cmath>
 #include <cstring>
+#include <numeric>
 #include <type_traits>
 
 #include "mb_host.cuh"
@@ -155,6 +156,17 @@ int launch_quantize(const RouteParams &p, cudaStream_t st, const char *what) {
 }
 
 // ------------------------------------------------------------- int8 products with scales
+// Whether two elements of a rows x cols matrix have one address: i rs + j cs = 0
+// for some |i| < rows and |j| < cols, not both 0.  The least such pair is the
+// strides over their greatest common divisor.
+bool share_memory(int64_t rows, int64_t cols, int64_t rs, int64_t cs) {
+  if (rows <= 1) return cols > 1 && cs == 0;
+  if (cols <= 1) return rs == 0;
+  rs = std::abs(rs);
+  cs = std::abs(cs);
+  const int64_t g = std::gcd(rs, cs);
+  return g == 0 || (cs / g < rows && rs / g < cols);
+}
 int scaled_check(const mb_scaled_desc *d) {
   if (!d) return fail(MB_ERR_INVALID, "null descriptor");
   if (!is_float(d->out_dtype)) return fail(MB_ERR_UNSUPPORTED, "out_dtype %d is not fp32, fp16 or bf16", d->out_dtype);
@@ -164,6 +176,8 @@ int scaled_check(const mb_scaled_desc *d) {
   if (d->groups > 1024) return fail(MB_ERR_INVALID, "more than 1024 groups");
   if (d->M == 0 || d->N == 0) return MB_OK;
   if (!d->C || !d->scale_a || !d->scale_b) return fail(MB_ERR_INVALID, "null C, scale_a or scale_b");
+  if (share_memory(d->M, d->N, d->c_rs, d->c_cs))
+    return fail(MB_ERR_INVALID, "elements of C share memory (strides %lld, %lld)", (long long)d->c_rs, (long long)d->c_cs);
   if (d->K > 0 && (!d->A || !d->B)) return fail(MB_ERR_INVALID, "null A or B");
   if (d->groups > 0 && !d->offsets) return fail(MB_ERR_INVALID, "groups need offsets");
   if (d->bias && d->bias_dtype != d->out_dtype && d->bias_dtype != MB_F32)

@@ -170,7 +170,8 @@ def scaled_mm(a, b, scale_a, scale_b, *, bias=None, out_dtype=None, out=None, _p
     ``scale_a`` has a's leading shape (one scale per token) and ``scale_b [N]`` one scale per
     output channel; either may also be any shape that broadcasts to that, such as a single
     scale.  ``out_dtype`` is bf16 (default), fp16 or fp32; ``bias [N]`` has that type or fp32.
-    The sum over K is exact, so K is at most 131071.
+    The sum over K is exact, so K is at most 131071.  ``out`` may have any strides that give
+    every element a place of its own.
 
     ``b`` is read in place when it is row- or column-major (a transposed ``[N, K]`` weight) on
     a 16-byte aligned base and pitch, as is ``a`` with contiguous aligned rows; other layouts
