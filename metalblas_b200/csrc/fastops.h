@@ -46,7 +46,10 @@ inline int float_code(at::ScalarType t) {
 }
 inline bool here(const at::Tensor &t, int dev) { return t.is_cuda() && t.get_device() == dev && !t.is_neg(); }
 inline void *stream_of(int dev) { return reinterpret_cast<void *>(c10::cuda::getCurrentCUDAStream(dev).stream()); }
-inline bool grad_of(const at::Tensor &t) { return t.requires_grad() && at::GradMode::is_enabled(); }
+// A derivative to record or, with a tangent, to refuse: not a plain call.
+inline bool grad_of(const at::Tensor &t) {
+  return (t.requires_grad() && at::GradMode::is_enabled()) || t._fw_grad(/*level=*/0).defined();
+}
 
 // A matrix with contiguous, non-overlapping rows; its row stride.
 inline bool rows_of(const at::Tensor &t, int dev, int64_t &ld) {

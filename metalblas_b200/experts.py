@@ -11,14 +11,17 @@ the router's weights.  Nothing here reads a count back to the host.
     y = grouped_scaled_mm(q, w, s, sw, order.offsets)
     out = expert_combine(y, weights, order)
 
-``expert_gather`` and ``expert_combine`` take part in autograd;
-``expert_gather_backward`` and ``expert_combine_backward`` are the gradients by themselves.
+``expert_gather`` and ``expert_combine`` take part in reverse-mode autograd, once: a tangent
+(forward mode) raises NotImplementedError, and so does differentiating their gradients again
+(RuntimeError).  ``expert_gather_backward`` and ``expert_combine_backward`` are the gradients by
+themselves; what they and ``expert_gather_quantize`` return carries no gradient.
 """
 from __future__ import annotations
 
 from typing import NamedTuple
 
 import torch
+import torch.autograd.forward_ad as fwd
 
 from . import _lib
 from .dispatch import FLOATS, _plain, _stream_of
@@ -132,6 +135,12 @@ def _combine(rows, weights, order):
     return out
 
 
+def _no_tangent(*tensors):
+    for t in tensors:
+        if t is not None and fwd.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("expert_gather, expert_combine and their gradients have no forward-mode derivative")
+
+
 class _Gather(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, order, position, offsets):
@@ -141,6 +150,7 @@ class _Gather(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        _no_tangent(grad)
         return expert_gather_backward(grad, ExpertOrder(*ctx.saved_tensors)), None, None, None
 
 
@@ -154,28 +164,32 @@ class _Combine(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         rows, weights, *order = ctx.saved_tensors
+        _no_tangent(grad)
         return (*expert_combine_backward(grad, rows, weights, ExpertOrder(*order)), None, None, None)
 
 
 def expert_gather(x, order):
-    """The rows of ``x [T, cols]`` in ``order``: ``[T * k, cols]``, zero rows for dropped entries."""
+    """The rows of ``x [T, cols]`` in ``order``: ``[T * k, cols]``, zero rows for dropped entries.
+    Takes part in reverse-mode autograd."""
     out = _try_gather(x, order.position, order.offsets)
     if out is not None:
         return out
+    _no_tangent(x)
     if x.requires_grad and torch.is_grad_enabled():
         return _Gather.apply(x, *order)
     return _gather(x, order)
 
 
 def expert_gather_backward(grad, order):
-    """Gradient of ``expert_gather`` by x: each token's rows of ``grad [T * k, cols]`` summed."""
+    """Gradient of ``expert_gather`` by x: each token's rows of ``grad [T * k, cols]`` summed.
+    The result carries no gradient."""
     out = _try_combine(grad, None, order.position, order.offsets)
     return out if out is not None else _combine(grad, None, order)
 
 
 def expert_gather_quantize(x, order):
     """``quantize(expert_gather(x, order))`` without the rows in between: int8 ``[T * k, cols]``
-    and fp32 ``[T * k]``; dropped entries have q 0 and scale 0."""
+    and fp32 ``[T * k]``; dropped entries have q 0 and scale 0.  The result carries no gradient."""
     return _try_gather_quantize(x, order.position, order.offsets) or _gather_quantize(x, order)
 
 
@@ -198,10 +212,12 @@ def _gather_quantize(x, order):
 def expert_combine(rows, weights, order):
     """``out[t] = sum_j weights[t, j] * rows[position[t, j]]``: ``[T, cols]`` from the experts'
     ``rows [T * k, cols]``, dropped entries left out, summed in fp32 in the order of j.
-    ``weights [T, k]`` have the rows' type or fp32; None stands for ones."""
+    ``weights [T, k]`` have the rows' type or fp32; None stands for ones.  Takes part in
+    reverse-mode autograd."""
     out = _try_combine(rows, weights, order.position, order.offsets)
     if out is not None:
         return out
+    _no_tangent(rows, weights)
     if torch.is_grad_enabled():
         if weights is None:
             if rows.requires_grad:
@@ -215,7 +231,8 @@ def expert_combine(rows, weights, order):
 def expert_combine_backward(grad, rows, weights, order):
     """Gradients of ``expert_combine`` by rows and by weights: ``drows[position[t, j]] =
     weights[t, j] * grad[t]`` (zero for dropped entries) and ``dweights[t, j] = <grad[t],
-    rows[position[t, j]]>`` (zero likewise), in the types of rows and weights."""
+    rows[position[t, j]]>`` (zero likewise), in the types of rows and weights.  The results carry
+    no gradient."""
     return _try_combine_backward(grad, rows, weights, order.position, order.offsets) or \
         _combine_backward(grad, rows, weights, order)
 

@@ -68,7 +68,7 @@ def quantize(x):
     ``scale = max|x| / 127`` of the row and ``q = round(127 x / max|x|)``, halves to even.  A
     row of zeros has scale 0.  A row with an infinity or a NaN has scale NaN and q 0.  The
     rows of a 2-D ``q`` start on 16-byte boundaries: with a number of columns that is no
-    multiple of 16, ``q`` is a view of a wider matrix.
+    multiple of 16, ``q`` is a view of a wider matrix.  Neither carries a gradient.
     """
     return _try_quantize(x) or _quantize(x)
 
