@@ -254,13 +254,19 @@ inline Pair try_combine_backward(const at::Tensor &grad, const at::Tensor &rows,
 
 inline void bind(pybind11::module &m) {
   m.def("set_ops", &set_ops);
-  m.def("try_quantize", &try_quantize);
-  m.def("try_scaled", &try_scaled);
-  m.def("try_sort", &try_sort);
-  m.def("try_gather", &try_gather);
-  m.def("try_gather_quantize", &try_gather_quantize);
-  m.def("try_combine", &try_combine);
-  m.def("try_combine_backward", &try_combine_backward);
+  // Arguments of other kinds (a scale that is no tensor) take the second form of
+  // each name, so that the Python path's checks refuse them.
+  auto def = [&](const char *name, auto fn) {
+    m.def(name, fn);
+    m.def(name, [](const pybind11::args &) { return pybind11::none(); });
+  };
+  def("try_quantize", &try_quantize);
+  def("try_scaled", &try_scaled);
+  def("try_sort", &try_sort);
+  def("try_gather", &try_gather);
+  def("try_gather_quantize", &try_gather_quantize);
+  def("try_combine", &try_combine);
+  def("try_combine_backward", &try_combine_backward);
 }
 
 }  // namespace fastops

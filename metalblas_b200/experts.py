@@ -85,6 +85,7 @@ def _check_order(order, dev):
 
 
 def _check_rows(t, shape, name):
+    assert isinstance(t, torch.Tensor), f"{name} must be a tensor"
     if t.dtype not in FLOATS:
         raise NotImplementedError(f"{name} must be fp32, fp16 or bf16, got {t.dtype}")
     assert tuple(t.shape) == tuple(shape), f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}"
@@ -92,6 +93,7 @@ def _check_rows(t, shape, name):
 
 
 def _check_weights(weights, pos, dtype):
+    assert isinstance(weights, torch.Tensor), "weights must be a tensor"
     assert weights.device == pos.device and tuple(weights.shape) == tuple(pos.shape), \
         f"weights have shape {tuple(weights.shape)}, expected {tuple(pos.shape)}"
     if weights.dtype is not dtype and weights.dtype is not torch.float32:
@@ -137,8 +139,9 @@ def _combine(rows, weights, order):
 
 def _no_tangent(*tensors):
     for t in tensors:
-        if t is not None and fwd.unpack_dual(t).tangent is not None:
-            raise NotImplementedError("expert_gather, expert_combine and their gradients have no forward-mode derivative")
+        if isinstance(t, torch.Tensor) and fwd.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("expert_gather, expert_combine and their gradients have no forward-mode "
+                                      "derivative")
 
 
 class _Gather(torch.autograd.Function):
@@ -175,7 +178,7 @@ def expert_gather(x, order):
     if out is not None:
         return out
     _no_tangent(x)
-    if x.requires_grad and torch.is_grad_enabled():
+    if isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled():
         return _Gather.apply(x, *order)
     return _gather(x, order)
 
@@ -218,13 +221,10 @@ def expert_combine(rows, weights, order):
     if out is not None:
         return out
     _no_tangent(rows, weights)
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (rows, weights)):
         if weights is None:
-            if rows.requires_grad:
-                weights = torch.ones(order.position.shape, dtype=torch.float32, device=rows.device)
-                return _Combine.apply(rows, weights, *order)
-        elif rows.requires_grad or weights.requires_grad:
-            return _Combine.apply(rows, weights, *order)
+            weights = torch.ones(order.position.shape, dtype=torch.float32, device=rows.device)
+        return _Combine.apply(rows, weights, *order)
     return _combine(rows, weights, order)
 
 
@@ -242,6 +242,7 @@ def _combine_backward(grad, rows, weights, order):
     pos, off = _check_order(order, grad.device)
     T, k = pos.shape
     H = grad.shape[-1]
+    assert isinstance(rows, torch.Tensor), "rows must be a tensor"
     if grad.dtype is not rows.dtype:
         raise NotImplementedError(f"grad is {grad.dtype}, rows are {rows.dtype}")
     assert rows.device == grad.device, "grad and rows on different devices"

@@ -31,7 +31,7 @@ _try_scaled = _lib.fast_op("try_scaled")
 def _on_device(fn):
     """Run fn with the device of its first argument current."""
     def call(t, *args, **kw):
-        assert t.is_cuda, "CUDA tensors expected"
+        assert isinstance(t, torch.Tensor) and t.is_cuda, "CUDA tensors expected"
         if torch.cuda.current_device() != t.device.index:
             with torch.cuda.device(t.device):
                 return fn(t, *args, **kw)
@@ -144,6 +144,7 @@ def _check_int8(a, b):
 
 def _check_out(out_dtype, out, shape, device):
     if out is not None:
+        assert isinstance(out, torch.Tensor), "out must be a tensor"
         assert out.device == device and tuple(out.shape) == tuple(shape), \
             f"out has shape {tuple(out.shape)} on {out.device}, expected {tuple(shape)} on {device}"
         if out_dtype is not None and out.dtype is not out_dtype:
@@ -158,6 +159,7 @@ def _check_out(out_dtype, out, shape, device):
 def _check_bias(bias, N, out_dtype, device):
     if bias is None:
         return None
+    assert isinstance(bias, torch.Tensor), "bias must be a tensor"
     assert bias.device == device and tuple(bias.shape) == (N,), f"bias has shape {tuple(bias.shape)}, not ({N},)"
     if bias.dtype is not out_dtype and bias.dtype is not torch.float32:
         raise NotImplementedError(f"bias must be {out_dtype} or fp32, got {bias.dtype}")
@@ -186,7 +188,7 @@ def scaled_mm(a, b, scale_a, scale_b, *, bias=None, out_dtype=None, out=None, _p
 
 @_on_device
 def _scaled_mm(a, b, scale_a, scale_b, bias, out_dtype, out, _plan):
-    assert b.dim() == 2 and a.dim() >= 1, "scaled_mm takes a [..., K] and b [K, N]"
+    assert isinstance(b, torch.Tensor) and b.dim() == 2 and a.dim() >= 1, "scaled_mm takes a [..., K] and b [K, N]"
     _check_int8(a, b)
     K, N = b.shape
     assert a.shape[-1] == K, f"inner dimensions differ: {tuple(a.shape)} @ {tuple(b.shape)}"
@@ -225,7 +227,8 @@ def grouped_scaled_mm(a, b, scale_a, scale_b, offsets, *, out_dtype=None, out=No
 
 @_on_device
 def _grouped_scaled_mm(a, b, scale_a, scale_b, offsets, out_dtype, out, _plan):
-    assert a.dim() == 2 and b.dim() == 3, "grouped_scaled_mm takes a [M, K] and b [E, K, N]"
+    assert isinstance(b, torch.Tensor) and a.dim() == 2 and b.dim() == 3, \
+        "grouped_scaled_mm takes a [M, K] and b [E, K, N]"
     _check_int8(a, b)
     M, K = a.shape
     E, Kb, N = b.shape
@@ -233,6 +236,7 @@ def _grouped_scaled_mm(a, b, scale_a, scale_b, offsets, out_dtype, out, _plan):
     if not 1 <= E <= MAX_GROUPS:
         raise ValueError(f"{E} groups: 1 to {MAX_GROUPS} expected")
     dev = a.device
+    assert isinstance(offsets, torch.Tensor), "offsets must be a tensor"
     assert offsets.device == dev and tuple(offsets.shape) == (E + 1,), \
         f"offsets has shape {tuple(offsets.shape)} on {offsets.device}, expected ({E + 1},) on {dev}"
     if offsets.dtype is not torch.int32:
