@@ -173,7 +173,7 @@ def scaled_mm(a, b, scale_a, scale_b, *, bias=None, out_dtype=None, out=None, _p
     output channel; either may also be any shape that broadcasts to that, such as a single
     scale.  ``out_dtype`` is bf16 (default), fp16 or fp32; ``bias [N]`` has that type or fp32.
     The sum over K is exact, so K is at most 131071.  ``out`` may have any strides that give
-    every element a place of its own.
+    every element a place of its own and fold its leading dimensions into one.
 
     ``b`` is read in place when it is row- or column-major (a transposed ``[N, K]`` weight) on
     a 16-byte aligned base and pitch, as is ``a`` with contiguous aligned rows; other layouts
@@ -203,7 +203,11 @@ def _scaled_mm(a, b, scale_a, scale_b, bias, out_dtype, out, _plan):
     sa = sa.reshape(M) if sa.dim() != 1 else sa
     if out is None:
         out = torch.empty((*lead, N), dtype=out_dtype, device=dev)
-    c = out if out.dim() == 2 else out.view(M, N)
+    try:
+        c = out if out.dim() == 2 else out.view(M, N)
+    except RuntimeError:
+        raise AssertionError(f"out of shape {tuple(out.shape)} and strides {out.stride()} is no matrix of "
+                             "rows") from None
     _product(a2, b, sa, sb, M, N, K, 0, None, bias, out_dtype, c, _plan)
     return out
 

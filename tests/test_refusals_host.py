@@ -49,3 +49,11 @@ def test_the_argument_is_named_by_group():
         experts._combine.__wrapped__(ROWS, [1.0], ORDER)
     with pytest.raises(AssertionError, match="rows"):
         experts._combine_backward.__wrapped__(ROWS[:4], [1.0], IDS.float(), ORDER)
+
+
+@pytest.mark.parametrize("out", [torch.zeros(3, 2, 4).transpose(0, 1), torch.zeros(2, 5, 4)[:, :3]])
+def test_an_output_that_is_no_matrix_of_rows(out):
+    """Leading dimensions of out that do not fold into one stride."""
+    a, b = torch.zeros(2, 3, 16, dtype=torch.int8), torch.zeros(16, 4, dtype=torch.int8)
+    with pytest.raises(AssertionError, match="out"):
+        quantized._scaled_mm.__wrapped__(a, b, torch.ones(2, 3), torch.ones(4), None, torch.float32, out, None)
