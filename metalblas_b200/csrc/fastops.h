@@ -163,7 +163,8 @@ inline One try_scaled(const at::Tensor &a, const at::Tensor &b, const at::Tensor
 inline Triple try_sort(const at::Tensor &ids, int64_t experts) {
   if (!g_ops.sort || !ids.is_cuda()) return c10::nullopt;
   const int dev = c10::cuda::current_device();
-  if (!here(ids, dev) || ids.dim() != 2 || !ids.is_contiguous() || experts < 1) return c10::nullopt;
+  if (!here(ids, dev) || ids.dim() != 2 || !ids.is_contiguous()) return c10::nullopt;
+  if (experts < 1 || experts > 1024) return c10::nullopt;  // mb_expert_sort's limit, before the allocation
   const bool wide = ids.scalar_type() == at::kLong;
   if (!wide && ids.scalar_type() != at::kInt) return c10::nullopt;
   const int64_t n = ids.numel();
