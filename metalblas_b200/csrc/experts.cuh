@@ -218,9 +218,10 @@ struct RouteParams {
   float *scale;
 };
 
-// The kernels run blocks of 256 threads, `lanes` (32, 128 or 256) of them to a
-// token, so that short rows still fill warps and long ones have a block; a
-// token's columns are shared out over blockIdx.y as well.
+// The kernels run blocks of 256 threads, `lanes` (16, 32, 128 or 256; whole warps
+// in combine's gradient) of them to a token, so that short rows still fill warps
+// and long ones have a block; a token's columns are shared out over blockIdx.y
+// as well.
 constexpr int kRouteThreads = 256;
 // A token's entries are worked on NE (2, 4 or 8) at a time: the rows of a batch
 // are in flight together, a batch wider than k is spent on nothing (k = 2 in

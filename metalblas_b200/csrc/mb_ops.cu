@@ -1,5 +1,5 @@
-// C ABI of the int8 products with scales (quantize.cuh, scaled_gemm.cuh) and of
-// the expert routing (experts.cuh).
+// C ABI of the int8 products with scales (quantize.cuh, scaled_tc.cuh,
+// scaled_gemv.cuh) and of the expert routing (experts.cuh).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -524,8 +524,8 @@ int mb_scaled_plan(const mb_scaled_desc *d, char *buf, int buflen) {
   if (pl.gemv) return snprintf(buf, room, "rows in one pass over the weights");
   if (pl.thin) return snprintf(buf, room, "rows in one pass over the weights, MMA, %d blocks an SM", pl.thin);
   if (pl.bn == 0) return snprintf(buf, room, pl.empty ? "empty" : "no sum");
-  return snprintf(buf, room, "%s bn=%d pair=%d split=%d a_mn=%d b_mn=%d pack_a=%d pack_b=%d ws=%lld",
-                  pl.swap ? "channels" : "tokens", pl.bn, pl.pair, pl.split, 0, pl.w_mn, pl.pk_a, pl.pk_b,
+  return snprintf(buf, room, "%s bn=%d pair=%d split=%d w_mn=%d pack_a=%d pack_b=%d ws=%lld",
+                  pl.swap ? "channels" : "tokens", pl.bn, pl.pair, pl.split, pl.w_mn, pl.pk_a, pl.pk_b,
                   (long long)pl.ws_bytes);
 }
 

@@ -74,14 +74,14 @@ __device__ __forceinline__ uint4 bytes_at(const uint4 &w0, const uint4 &w1, uint
 // destination pitch `ld` is a multiple of 16 bytes; the group past the end of a
 // row spills into its padding, which the tensor maps never read.
 template <class U>
-__device__ __forceinline__ void pack_rows16(const PackArgs &a, int64_t block, int64_t blocks) {
+__global__ void __launch_bounds__(256) pack_rows16_kernel(const PackArgs a) {
   constexpr int G = 16 / (int)sizeof(U);
   const U *src = static_cast<const U *>(a.src);
   U *dst = static_cast<U *>(a.dst);
   const int64_t groups = (a.cols + G - 1) / G;
   const int64_t per_batch = a.rows * groups;
   const int64_t total = a.batch * per_batch;
-  for (int64_t i = block * blockDim.x + threadIdx.x; i < total; i += blocks * blockDim.x) {
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t b = i / per_batch;
     const int64_t rem = i - b * per_batch;
     const int64_t r = rem / groups;
@@ -100,10 +100,6 @@ __device__ __forceinline__ void pack_rows16(const PackArgs &a, int64_t block, in
     }
     *reinterpret_cast<uint4 *>(dst + (b * a.rows + r) * a.ld + c0) = v.q;
   }
-}
-template <class U>
-__global__ void __launch_bounds__(256) pack_rows16_kernel(const PackArgs a) {
-  pack_rows16<U>(a, blockIdx.x, gridDim.x);
 }
 
 }  // namespace mb

@@ -89,6 +89,7 @@ struct SgParams {
 template <int BN, int PAIR, bool SWAP, class TO>
 struct SgCfg {
   using B = tc::Cfg<BN, 1, PAIR>;
+  static_assert(B::NMMA == 1, "one MMA per K-step");
   static constexpr int TROWS = SWAP ? BN : BM * PAIR;   // token rows per tile
   static constexpr int TCOLS = SWAP ? BM : BN;          // channels per tile
   static constexpr int STAGE_BYTES = B::A_BYTES + B::B_BYTES;
@@ -149,13 +150,6 @@ __device__ __forceinline__ float scaled_sum(int sum, float scale_a, float scale_
 
 // Four sums of one row, two to an instruction: the same roundings.
 __device__ __forceinline__ void scaled_sums(const int *sum, float scale_a, const float4 &scale_b, float *v) {
-  auto mul2 = [](float2 a, float2 b) {
-    float2 o;
-    asm("mul.rn.f32x2 %0, %1, %2;"
-        : "=l"(reinterpret_cast<unsigned long long &>(o))
-        : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
-    return o;
-  };
   const float2 sa = make_float2(scale_a, scale_a);
 #pragma unroll
   for (int i = 0; i < 4; i += 2) {
@@ -363,18 +357,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
           };
           if (SWAP && p.a_mn) load(sa, &p.tmA, a0, kb * BK, ag);
           else load(sa, &p.tmA, kb * BK, a0, ag);
-          // this CTA's share of each MMA's columns (see tc_gemm.cuh)
+          // this CTA's share of the MMA's columns (see tc_gemm.cuh)
           constexpr int SH = B_::UMMA_N / PAIR;
+          const int col = b0 + prank * SH;
+          if (!SWAP && p.b_mn) {
 #pragma unroll
-          for (int h = 0; h < B_::NMMA; ++h) {
-            const int col = b0 + h * B_::UMMA_N + prank * SH;
-            if (!SWAP && p.b_mn) {
-#pragma unroll
-              for (int j = 0; j < SH / 128; ++j)
-                load(sb + h * SH * 128 + j * (BK * 128), &p.tmB, col + j * 128, kb * BK, bg);
-            } else {
-              load(sb + h * SH * 128, &p.tmB, kb * BK, col, bg);
-            }
+            for (int j = 0; j < SH / 128; ++j) load(sb + j * (BK * 128), &p.tmB, col + j * 128, kb * BK, bg);
+          } else {
+            load(sb, &p.tmB, kb * BK, col, bg);
           }
           issued_stage = stage;
           issued_phase = phase;
@@ -413,12 +403,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
           const uint32_t sa = ring_u32 + stage * STAGE_BYTES, sb = sa + A_BYTES;
 #pragma unroll
           for (int ks = 0; ks < B_::KSTEPS; ++ks) {
-            const uint64_t ad = sdesc(sa + ks * a_kstep, a_lbo, 1024);
-#pragma unroll
-            for (int h = 0; h < B_::NMMA; ++h) {
-              const uint64_t bd = sdesc(sb + h * (B_::UMMA_N / PAIR) * 128 + ks * b_kstep, b_lbo, 1024);
-              umma_g<1, PAIR>(d_tmem + h * B_::UMMA_N, ad, bd, idesc, (kb > kb0 || ks > 0) ? 1u : 0u);
-            }
+            const uint64_t ad = sdesc(sa + ks * a_kstep, a_lbo, 1024), bd = sdesc(sb + ks * b_kstep, b_lbo, 1024);
+            umma_g<1, PAIR>(d_tmem, ad, bd, idesc, (kb > kb0 || ks > 0) ? 1u : 0u);
           }
           issued_any = true;
           umma_commit_g<PAIR>(empty_bar(stage));
