@@ -509,10 +509,10 @@ __global__ void __launch_bounds__(kRouteThreads) expert_combine_backward_kernel(
 // or, with position == null, to row t.  TPR threads hold a row's vectors, up to
 // HELD each, in registers between the maximum and the rounding; longer rows are
 // read again (from L2).  It is bound by how much of its loads an SM can keep in
-// flight between the barriers and roundings, and by HBM behind that: 16384 x 8192
-// bf16 72.8 us (5.5 TB/s) with four vectors a thread, 87 with two and twice the
-// threads, 79 with eight and half of them; copies into shared memory ahead of a
-// persistent block gave 79.
+// flight between the barriers and roundings (issue slots 77 % in use), and by HBM
+// behind that: 16384 x 8192 bf16 72.8 us (5.5 TB/s) with four vectors a thread,
+// 87 with two and twice the threads, 79 with eight and half of them; copies into
+// shared memory ahead of a persistent block gave 79.
 template <class T, bool AL, int TPR, int HELD>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, (HELD > 4 ? 768 : HELD > 2 || !AL ? 1280 : 2048) / (TPR < 256 ? 256 : TPR)) quantize_rows_kernel(const RouteParams p, int q_vec) {
   constexpr int V = Vec<T>::V, THREADS = TPR < 256 ? 256 : TPR;

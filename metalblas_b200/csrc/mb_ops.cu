@@ -142,7 +142,10 @@ int launch_quantize(const RouteParams &p, cudaStream_t st, const char *what) {
   // Threads to a row and vectors they hold, by the row's vectors, measured on B200
   // with 2, 4 and 8 held: many rows want them held by few threads (16384 x 4096
   // bf16 41.5 us by 128, 44.3 by 256; 8192 x 14336 70 us by 256, 88 by 512), few
-  // rows want many threads (1024 x 4096 3.9 us by 256, 4.5 by 128).
+  // rows want many threads (1024 x 4096 3.9 us by 256, 4.5 by 128).  A row between
+  // two sizes leaves slots empty whose instructions are issued all the same: 7601 x
+  // 5408, 676 vectors of 1024, 30.2 us, 141 warp instructions for 256 elements (116
+  // at 16384 x 8192) with the issue slots 73 % in use.
   if (vecs <= 16) return go(integral_constant<int, 8>(), integral_constant<int, 2>());
   if (vecs <= 64) return go(integral_constant<int, 32>(), integral_constant<int, 2>());
   if (vecs <= 128) return go(integral_constant<int, 32>(), integral_constant<int, 4>());
@@ -298,10 +301,19 @@ int sg_plan(const mb_scaled_desc *d, SgPlan &pl) {
   const bool forced = d->tile_n || d->cta_pair || d->split_k || d->swap_ab;
   if (!forced && !pl.pk_a && !pl.pk_b && !pl.w_mn) {
     // Few rows: one of the single-pass kernels of scaled_gemv.cuh, by the weights'
-    // bytes.  The MMA one starts first (4 x 2048 x 1536 3.5 us, tcgen05 5.1; 4 x 4096 x
-    // 4096 6.0 and 8.8; 16 x 4096 x 4096 7.5 and 8.7) but streams at 4.5 TB/s (4 x 4096 x
-    // 14336 14.7 and 14.0; 16 rows 17.3 and 14.3); the dp4a one streams two rows
-    // faster (2 x 4096 x 14336 13.4, MMA 14.7) and starts later (2 x 2048 x 1536 4.2, 3.3).
+    // bytes.  The MMA one starts first (4 x 2048 x 1536 3.5 us, tcgen05 5.1) but streams
+    // at 4.5 TB/s; the dp4a one streams two rows faster and starts later.  MMA kernel
+    // against what runs otherwise (two rows: dp4a, more: tcgen05), us at so many MiB:
+    //   K = 4096   2 rows   16: 5.7, 5.7    20: 7.1, 6.3    24: 8.0, 7.7
+    //              4 rows   32: 8.9, 11.4   40: 12.2, 13.2  48: 13.4, 13.6  64: 16.4, 15.0
+    //              16 rows  16: 7.5, 8.8    20: 8.9, 10.3   24: 9.8, 10.3   40: 14.1, 13.5
+    //   K = 1024   2 rows   8: 4.3, 3.5     16: 6.3, 4.4
+    //              4 rows   8: 4.3, 5.3     16: 6.5, 6.4    24: 8.8, 8.0    40: 13.2, 11.0
+    //              16 rows  8: 4.9, 5.3     16: 7.3, 6.5    20: 9.0, 7.8
+    //   K = 12288  2 rows   8: 10.5, 5.1    16: 12.0, 5.9
+    //              4 rows   8: 10.9, 7.7    40: 19.6, 13.6
+    // The limits fit K near 4096.  With rows of 1 KB the MMA kernel's range ends
+    // earlier, and at K = 12288 it is slower at every size: the bytes alone do not tell.
     const int64_t weights = d->K * d->N, small = (d->M > 8 || d->M == 2 ? 20ll : 40ll) << 20;
     if (!d->groups && d->M > 1 && d->M <= sg::THIN_ROWS && weights <= small) {
       pl.thin = thin_smem(d, 2) <= kThinSmem / 2 ? 2 : thin_smem(d, 1) <= kThinSmem ? 1 : 0;

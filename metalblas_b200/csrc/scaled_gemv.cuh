@@ -8,8 +8,8 @@
 // through whole rows but for the first and the last of its share.  The
 // tensor-core kernel hands out 128 channels at a time, which leaves 36 of 148
 // SMs idle at N = 14336, and starts later (TMEM, pipeline).  Measured on B200,
-// one row: K x N = 4096 x 14336 12.9 us against 14.3, 8192 x 28672 39.4
-// (5.96 TB/s) against 47.9.  With four rows the dp4a work and the rows' reads from shared
+// one row: K x N = 4096 x 14336 11.5 us against 13.8, 8192 x 28672 40.0
+// (5.9 TB/s) against 45.8.  With four rows the dp4a work and the rows' reads from shared
 // memory bind it (17.6 us against 14.6), so it takes two at most.
 //
 // By group (GROUPED) every row of A is a product of its own with its group's
@@ -19,8 +19,8 @@
 // Rows of up to 2048 bytes leave most of a warp's eight loads unused, and a row's
 // wait, sum and reduction follow one another.  So with more rows than warps a warp
 // takes several whole rows at a time (ROWSTEPS: the 512-byte steps of a row): one
-// row, K x N = 432 x 32768 4.3 us against 10.6, 1024 x 32768 6.9 against 12.0, 2048 x
-// 8192 4.0 against 6.4; eight rows with an expert each, 512 x 8192 10.1 against 23.0.
+// row, K x N = 432 x 32768 3.8 us against 10.6, 1024 x 32768 5.9 against 12.0, 2048 x
+// 8192 3.8 against 6.4; eight rows with an expert each, 512 x 8192 9.8 against 23.0.
 //
 // A lane multiplies its 16 weight bytes by dp4a with the rows of A, which lie in
 // shared memory, padded with zeros to whole vectors.  A run's 32-bit sums are
@@ -264,7 +264,7 @@ scaled_gemv_kernel(const __grid_constant__ SgParams p, const GemvArgs g) {
 // the instruction stands for, as long as A's words, read from shared memory the
 // same way, agree.  What counts here is that every SM reads the same bytes and
 // starts at once: the tcgen05 kernel, which hands out 128 channels at a time and
-// sets up TMEM and a pipeline first, took 8.8 us for 4 x 4096 x 4096 against 6.0.
+// sets up TMEM and a pipeline first, takes 8.7 us for 4 x 4096 x 4096 against 6.0.
 // Its eight-row reads stream at 4.5 TB/s, so products of more weights go there.
 //
 // A block's warps share K (KS slices) and pairs of eight weight rows.

@@ -35,16 +35,22 @@
 // by cluster rank i * split / 8, and the other ranks send it their s32 partial
 // sums through distributed shared memory.
 //
-// What bounds it, measured on B200 (twice the bf16 GEMM rate 1650 TFLOP/s is
-// taken as the int8 rate, 6.54 TB/s is a copy's):
-//   8192^3 bf16 out                331 us, 3320 TOPS: the tensor pipe;
-//   4096^3                         48.6 us, 2830 TOPS: operands into shared memory,
+// What bounds it, measured on B200 by graph replay (twice the bf16 GEMM rate 1650
+// TFLOP/s is taken as the int8 rate, 6.54 TB/s is a copy's):
+//   8192^3 bf16 out                333 us, 3300 TOPS: the tensor pipe;
+//   4096^3                         49.6 us, 2770 TOPS: operands into shared memory,
 //                                  and 256 tiles over 74 pairs;
-//   16384 rows by 8 experts of 4096 x 14336   650 us, 2960 TOPS: the same, and
+//   16384 rows by 8 experts of 4096 x 14336   662 us, 2910 TOPS: the same, and
 //                                  tiles that end with their group;
-//   8192 x 512 x 8192              45 to 49 us: the epilogue (134 MB out);
-//   16 rows by 8 experts of 4096 x 14336      65.8 us, 6.2 TB/s: the weights' bytes;
-//   16 x 4096 x 14336              14.3 us, 4.1 TB/s: 112 tiles keep 112 SMs busy.
+//   8192 x 512 x 8192              49 us, 2.9 TB/s: latency of the epilogue, whose eight
+//                                  warps an SM wait for one TMEM load, conversion and
+//                                  store after another (issue slots 36 % in use, tensor
+//                                  pipe 30 %, L2 29 %);
+//   16 rows by 7 experts of 4096 x 14336      69.5 us, 5.9 TB/s: the weights' bytes;
+//   16 x 4096 x 14336              14.2 us, 4.2 TB/s: 112 tiles keep 112 SMs busy;
+//   17 to 1000 rows, one wave of tiles or less: the start, one tile's K loop and its
+//                                  epilogue, one after another (1024 x 4096 x 2048 14.0
+//                                  us: tensor pipe 22 %, DRAM 9 %, issue slots 13 %).
 // The tile is chosen by sg_cost (mb_ops.cu), a model of such times; TROWS, TCOLS
 // and split change no result.
 #pragma once
@@ -208,7 +214,7 @@ template <class TO> __device__ __forceinline__ void pack4(const float *v, uint32
 }
 
 // RUNS: rows of C are contiguous but off 16 bytes (a kernel of its own: the shifts
-// cost the others 10% where the epilogue binds, 5551 x 512 x 9312 37.8 us).
+// cost the others 10% where the epilogue binds, 5551 x 512 x 9312 39.8 us).
 template <int BN, int PAIR, bool SWAP, bool RUNS, class TO>
 __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __grid_constant__ SgParams p) {
   using C_ = SgCfg<BN, PAIR, SWAP, TO>;
@@ -603,7 +609,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) scaled_gemm_kernel(const __gri
               // C that hold them, with the last chunk's rest before them.  What is left
               // over at either end of the warp's columns goes out by itself.  (5551 x 512 x
               // 9315 bf16 53 us; an element a lane 85, with chunks cut out of the staged
-              // rows 87: instructions bind it; rows of 9312 40.)
+              // rows 87; rows of 9312 40.)
               TO *own = C + m * p.c_rs + nn;
               const uint32_t past = (uint32_t)(reinterpret_cast<uintptr_t>(own) & 15);
               char *chunk = reinterpret_cast<char *>(own) - past;
