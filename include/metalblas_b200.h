@@ -328,6 +328,89 @@ int mb_expert_combine_backward(int32_t dtype, int32_t weights_dtype, int64_t tok
                                const int32_t *position, const int32_t *kept, void *dsorted, int64_t ldds,
                                void *dweights, void *stream);
 
+/* ---------------------------------------------------------------------------
+ * 4-bit weights with group scales.  The reference has no counterpart of the
+ * functions down to mb_last_error_string.
+ *
+ * A row of `cols` weights is (cols + 1) / 2 bytes of two values u in 0..15 each,
+ * the even column in the low half, and for each group of `group` (32, 64, 128 or
+ * 256) consecutive columns a scale and, where zero points are given, a zero
+ * point (uint8): weight = (u - zero) scale, zero 8 without zero points. */
+
+/* scale = amax / 7 rounded to scale_dtype, amax the largest |x| of the group;
+ * u = 8 + rint(x / scale), halves to even, within 1..15.  A group of zeros has
+ * scale 0, one that holds an infinity or a NaN scale NaN, both u = 8. */
+int mb_int4_quantize(int32_t dtype, int32_t scale_dtype, int64_t rows, int64_t cols, int32_t group, const void *x,
+                     int64_t ldx, uint8_t *q, int64_t ldq, void *scale, int64_t lds, void *stream);
+/* out = the weights, rounded once to dtype; zero may be null. */
+int mb_int4_dequantize(int32_t dtype, int32_t scale_dtype, int64_t rows, int64_t cols, int32_t group, const uint8_t *q,
+                       int64_t ldq, const void *scale, int64_t lds, const uint8_t *zero, int64_t ldz, void *out,
+                       int64_t ldo, void *stream);
+
+/* out[m, n] = sum_k x[m, k] w_e[n, k] + bias[n] for fp16 or bf16 x and out; the
+ * weights are not rounded and the sums are fp32.
+ *   groups == 0: one weight matrix for every row; offsets unused.
+ *   groups >= 1: `groups` matrices; offsets is a device array of groups + 1
+ *     ascending row numbers starting at 0; rows offsets[e] .. offsets[e+1]-1 use
+ *     matrix e, rows at or past offsets[groups] are set to zero.  Values outside
+ *     0..M are taken as the nearest of the two; if they are not ascending, every
+ *     row is set to zero.
+ * Columns are contiguous; strides are in elements (w: bytes). */
+typedef struct mb_int4_desc {
+    int32_t dtype, scale_dtype, bias_dtype, group;  /* scales and bias: dtype or MB_F32 */
+    int64_t M, N, K, groups;
+    const void *x;
+    int64_t x_rs;
+    const uint8_t *w;
+    int64_t w_rs, w_e;                   /* from row to row, from matrix to matrix */
+    const void *scale;
+    int64_t scale_rs, scale_e;
+    const uint8_t *zero;                 /* or null */
+    int64_t zero_rs, zero_e;
+    const void *bias;                    /* N values, or null */
+    const int32_t *offsets;
+    void *out;
+    int64_t out_rs;
+    int32_t plan[4];                     /* 0: chosen; see mb_int4_plan */
+    void *workspace;
+    int64_t workspace_bytes;
+} mb_int4_desc;
+
+void mb_int4_desc_init(mb_int4_desc *d);
+int mb_int4_gemm(const mb_int4_desc *d, void *stream);
+/* Bytes of scratch mb_int4_gemm needs for this descriptor (0 for operands read
+ * in place), on a 16-byte boundary.  The contents need not be kept or cleared. */
+int64_t mb_int4_workspace_size(const mb_int4_desc *d);
+/* One line on the plan the descriptor gets; its length, or a negative status. */
+int mb_int4_plan(const mb_int4_desc *d, char *buf, int buflen);
+
+/* ---------------------------------------------------------------------------
+ * Router and balance loss of a mixture-of-experts layer.  logits[tokens, experts]
+ * are of a float type, ldl apart; experts <= 1024.
+ *
+ * ids[t, j] = the k largest scores of a row, descending, ties to the lower
+ * number; weights[t, j] = softmax(row) there, with normalize divided by their sum.
+ * Scores of -inf are never chosen: entries for which no other is left have the
+ * number -1 and weight 0.  k <= 64. */
+int mb_expert_route(int32_t dtype, int64_t tokens, int64_t experts, int64_t k, int32_t normalize, const void *logits,
+                    int64_t ldl, float *weights, int32_t *ids, void *stream);
+/* dlogits [tokens, experts] of the weights' gradient grad [tokens, k]. */
+int mb_expert_route_backward(int32_t dtype, int64_t tokens, int64_t experts, int64_t k, int32_t normalize,
+                             const float *grad, const void *logits, int64_t ldl, const int32_t *ids, void *dlogits,
+                             void *stream);
+/* counts[e] = entries ids[t, j] = e (numbers outside 0..experts-1 count for none)
+ * of the tokens with mask[t] != 0 (null: all), counted = their number, and
+ * loss = experts * sum_e (counts[e] / sum counts) * (sum_t softmax(logits[t])[e] / counted),
+ * 0 when there is none.  The workspace (4-byte boundary) need not be cleared. */
+int64_t mb_expert_balance_workspace_size(int64_t tokens, int64_t experts);
+int mb_expert_balance(int32_t dtype, int64_t tokens, int64_t experts, int64_t k, const void *logits, int64_t ldl,
+                      const int32_t *ids, const uint8_t *mask, float *loss, int32_t *counts, int32_t *counted,
+                      void *workspace, int64_t workspace_bytes, void *stream);
+/* dlogits [tokens, experts] = grad[0] * d loss / d logits. */
+int mb_expert_balance_backward(int32_t dtype, int64_t tokens, int64_t experts, const float *grad, const void *logits,
+                               int64_t ldl, const int32_t *counts, const int32_t *counted, const uint8_t *mask,
+                               void *dlogits, void *stream);
+
 /* Text of the last error raised on this thread. */
 const char *mb_last_error_string(void);
 

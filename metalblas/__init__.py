@@ -19,15 +19,24 @@ from metalblas_b200 import (  # noqa: F401
     vdot,
 )
 from metalblas_b200 import (  # noqa: F401
+    ExpertBalance,
     ExpertOrder,
+    dequantize_int4,
+    expert_balance,
+    expert_balance_backward,
     expert_combine,
     expert_combine_backward,
     expert_gather,
     expert_gather_backward,
     expert_gather_quantize,
+    expert_route,
+    expert_route_backward,
     expert_sort,
+    grouped_int4_mm,
     grouped_scaled_mm,
+    int4_mm,
     quantize,
+    quantize_int4,
     scaled_mm,
 )
 from metalblas_b200 import __all__  # noqa: F401

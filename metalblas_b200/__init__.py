@@ -33,7 +33,15 @@ from .experts import (  # noqa: F401
     expert_gather_quantize,
     expert_sort,
 )
+from .int4 import dequantize_int4, grouped_int4_mm, int4_mm, quantize_int4  # noqa: F401
 from .quantized import grouped_scaled_mm, quantize, scaled_mm  # noqa: F401
+from .router import (  # noqa: F401
+    ExpertBalance,
+    expert_balance,
+    expert_balance_backward,
+    expert_route,
+    expert_route_backward,
+)
 
 __all__ = [
     "matmul", "gemm", "addmm", "bmm", "baddbmm", "addbmm",

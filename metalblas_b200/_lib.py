@@ -42,6 +42,9 @@ EXPORTS = (
     "mb_quantize", "mb_scaled_desc_init", "mb_scaled_gemm", "mb_scaled_workspace_size", "mb_scaled_plan",
     "mb_expert_sort", "mb_expert_gather", "mb_expert_gather_quantize", "mb_expert_combine",
     "mb_expert_combine_backward",
+    "mb_int4_quantize", "mb_int4_dequantize", "mb_int4_desc_init", "mb_int4_gemm", "mb_int4_workspace_size",
+    "mb_int4_plan", "mb_expert_route", "mb_expert_route_backward", "mb_expert_balance_workspace_size",
+    "mb_expert_balance", "mb_expert_balance_backward",
 )
 
 MB_MAX_PEERS = 7
@@ -106,6 +109,24 @@ class ScaledDesc(ctypes.Structure):
         ("bias", ctypes.c_void_p), ("bias_s", ctypes.c_int64), ("offsets", ctypes.c_void_p),
         ("tile_n", ctypes.c_int32), ("split_k", ctypes.c_int32), ("swap_ab", ctypes.c_int32),
         ("cta_pair", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
+class Int4Desc(ctypes.Structure):
+    """Mirror of ``mb_int4_desc`` (field order and C types must match)."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("scale_dtype", ctypes.c_int32), ("bias_dtype", ctypes.c_int32),
+        ("group", ctypes.c_int32),
+        ("M", ctypes.c_int64), ("N", ctypes.c_int64), ("K", ctypes.c_int64), ("groups", ctypes.c_int64),
+        ("x", ctypes.c_void_p), ("x_rs", ctypes.c_int64),
+        ("w", ctypes.c_void_p), ("w_rs", ctypes.c_int64), ("w_e", ctypes.c_int64),
+        ("scale", ctypes.c_void_p), ("scale_rs", ctypes.c_int64), ("scale_e", ctypes.c_int64),
+        ("zero", ctypes.c_void_p), ("zero_rs", ctypes.c_int64), ("zero_e", ctypes.c_int64),
+        ("bias", ctypes.c_void_p), ("offsets", ctypes.c_void_p),
+        ("out", ctypes.c_void_p), ("out_rs", ctypes.c_int64),
+        ("plan", ctypes.c_int32 * 4),
         ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64),
     ]
 
@@ -205,6 +226,24 @@ def _bind_ops(lib) -> None:
             ("mb_expert_gather_quantize", [I32, I64, I64, I64, V, I64, V, V, V, I64, V, V]),
             ("mb_expert_combine", [I32, I32, I64, I64, I64, V, I64, V, V, V, V, I64, V]),
             ("mb_expert_combine_backward", [I32, I32, I64, I64, I64, V, I64, V, I64, V, V, V, V, I64, V, V])):
+        fn = getattr(lib, name)
+        fn.argtypes, fn.restype = args, ctypes.c_int
+    if not hasattr(lib, "mb_int4_gemm"):
+        return
+    D = ctypes.POINTER(Int4Desc)
+    lib.mb_int4_desc_init.argtypes, lib.mb_int4_desc_init.restype = [D], None
+    lib.mb_int4_workspace_size.argtypes, lib.mb_int4_workspace_size.restype = [D], I64
+    lib.mb_expert_balance_workspace_size.argtypes = [I64, I64]
+    lib.mb_expert_balance_workspace_size.restype = I64
+    for name, args in (
+            ("mb_int4_quantize", [I32, I32, I64, I64, I32, V, I64, V, I64, V, I64, V]),
+            ("mb_int4_dequantize", [I32, I32, I64, I64, I32, V, I64, V, I64, V, I64, V, I64, V]),
+            ("mb_int4_gemm", [D, V]),
+            ("mb_int4_plan", [D, ctypes.c_char_p, ctypes.c_int]),
+            ("mb_expert_route", [I32, I64, I64, I64, I32, V, I64, V, V, V]),
+            ("mb_expert_route_backward", [I32, I64, I64, I64, I32, V, V, I64, V, V, V]),
+            ("mb_expert_balance", [I32, I64, I64, I64, V, I64, V, V, V, V, V, V, I64, V]),
+            ("mb_expert_balance_backward", [I32, I64, I64, V, V, I64, V, V, V, V, V])):
         fn = getattr(lib, name)
         fn.argtypes, fn.restype = args, ctypes.c_int
 

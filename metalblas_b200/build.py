@@ -1,8 +1,9 @@
 """Build the sm_100a shared library in-tree (nvcc, no JIT cache).
 
-The library is two CUDA translation units, compiled side by side: ``csrc/mb_abi.cu``
-(the products of one element type) and ``csrc/mb_ops.cu`` (int8 products with scales,
-expert routing), exporting the C ABI declared in ``include/metalblas_b200.h``; a small torch C++ extension
+The library is four CUDA translation units, compiled side by side: ``csrc/mb_abi.cu``
+(the products of one element type), ``csrc/mb_ops.cu`` (int8 products with scales,
+expert routing), ``csrc/mb_int4.cu`` (4-bit weights) and ``csrc/mb_router.cu`` (a router
+and its balance loss), exporting the C ABI declared in ``include/metalblas_b200.h``; a small torch C++ extension
 (``csrc/fastpath.cpp``) holds the host fast paths.  The library links the CUDA runtime statically
 so it does not depend on which libcudart torch happened to load, and reaches the
 driver (for cuTensorMapEncodeTiled) through cudaGetDriverEntryPoint, so it needs
@@ -20,7 +21,7 @@ import sys
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(PKG_DIR)
-UNITS = ("mb_abi", "mb_ops")
+UNITS = ("mb_abi", "mb_ops", "mb_int4", "mb_router")
 LIB = os.path.join(PKG_DIR, "libmetalblas_b200.so")
 ARCH = "-gencode=arch=compute_100a,code=sm_100a"
 

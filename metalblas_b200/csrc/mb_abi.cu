@@ -2066,6 +2066,7 @@ int mb_device_status(void) {
   rc = cuda_check(cudaMemcpyFromSymbol(&v, g_mb_status, sizeof(int)), "read status");
   if (rc) return rc;
   if (v == 0) rc = ops_status_read(&v);
+  if (!rc && v == 0) rc = int4_status_read(&v);
   if (rc) return rc;
   return v;
 }
@@ -2074,6 +2075,7 @@ void mb_device_status_clear(void) {
   int z = 0;
   cudaMemcpyToSymbol(g_mb_status, &z, sizeof(int));
   ops_status_clear();
+  int4_status_clear();
 }
 
 int mb_debug_wait_timeout(int64_t limit_us, void *stream) {

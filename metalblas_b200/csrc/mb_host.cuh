@@ -1,4 +1,5 @@
-// Host helpers shared by the library's translation units (mb_abi.cu, mb_ops.cu):
+// Host helpers shared by the library's translation units (mb_abi.cu,
+// mb_ops.cu, mb_int4.cu, mb_router.cu):
 // the thread's error text, status mapping, launches and tensor maps.
 #pragma once
 #include <cuda.h>
@@ -151,9 +152,11 @@ int device_sms();
 
 }  // namespace host
 
-// Device status word of the second translation unit (mb_ops.cu keeps its own,
-// since each unit's kernels write the word of their module).
+// Device status words of the other translation units with bounded waits (mb_ops.cu,
+// mb_int4.cu; each unit's kernels write the word of their module).
 int ops_status_read(int *v);
 void ops_status_clear();
+int int4_status_read(int *v);
+void int4_status_clear();
 
 }  // namespace mb
