@@ -36,42 +36,64 @@ template <class T> __device__ __forceinline__ float scale_at(const GemmArgs &a, 
   return a.scale_f32 ? static_cast<const float *>(a.scale)[i] : to_f32(static_cast<const T *>(a.scale)[i]);
 }
 
-template <class T>
-__global__ void __launch_bounds__(256) int4_simple_kernel(const GemmArgs a) {
-  const int lane = threadIdx.x & 31;
-  pdl_trigger();
-  pdl_wait();
-  bool wrong = false;
-  if (a.offsets)
-    for (int e = 0; e < a.groups; ++e) wrong |= min(max(a.offsets[e + 1], 0), a.M) < (e ? min(max(a.offsets[e], 0), a.M) : 0);
-  const int64_t tasks = (int64_t)a.M * a.N;
-  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < tasks; i += (int64_t)gridDim.x * 8) {
-    const int64_t m = i / a.N, n = i - m * a.N;
-    int e = 0;
-    if (a.offsets) {
-      if (wrong) e = a.groups;
-      while (e < a.groups && m >= a.offsets[e + 1]) ++e;
-    }
-    T *dst = static_cast<T *>(a.out) + m * a.out_rs + n;
-    if (a.offsets && e == a.groups) {
-      if (lane == 0) *dst = Elem<T>::store(0.f);
-      continue;
-    }
-    const T *x = static_cast<const T *>(a.x) + m * a.x_rs;
-    const uint8_t *w = a.w + e * a.w_e + n * a.w_rs;
-    float y = 0.f;
-    for (int g = 0; g << a.group_log2 < a.K; ++g) {
-      const float z = a.zero ? (float)a.zero[e * a.z_e + n * a.z_rs + g] : 8.f;
-      float s = 0.f;
-      const int k1 = min(a.K, (g + 1) << a.group_log2);
-      for (int k = (g << a.group_log2) + lane; k < k1; k += 32)
-        s = fmaf(to_f32(x[k]), (float)((w[k >> 1] >> (4 * (k & 1))) & 15) - z, s);
-      y = fmaf(s, scale_at<T>(a, e * a.s_e + n * a.s_rs + g), y);
-    }
+template <class T> __device__ __forceinline__ float bias_at(const GemmArgs &a, int64_t n) {
+  return a.bias_f32 ? static_cast<const float *>(a.bias)[n] : to_f32(static_cast<const T *>(a.bias)[n]);
+}
+
+// The groups' rows and units of `tokens` rows each: row0[e] and first_unit[e] for e <=
+// groups, by the whole block; the number of units.  `scan` has a word per warp.  Offsets
+// that are not ascending name no groups: every row comes out as zeros (and no count
+// can leave the range that the host has checked).
+__device__ __forceinline__ int unit_table(const GemmArgs &a, int tokens, int *first_unit, int *row0, int *scan) {
+  const int G = a.groups, tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5;
+  for (int e = tid; e <= G; e += threads) row0[e] = e ? min(max(a.offsets[e], 0), a.M) : 0;
+  __syncthreads();
+  int wrong = 0;
+  for (int e = tid; e < G; e += threads) wrong |= row0[e + 1] < row0[e];
+  if (__syncthreads_or(wrong)) {
+    for (int e = tid; e <= G; e += threads) row0[e] = 0;
+    __syncthreads();
+  }
+  // each thread sums `per` consecutive groups, then a scan over threads
+  const int per = (G + threads - 1) / threads;
+  const int e0 = min(G, tid * per), e1 = min(G, e0 + per);
+  auto units_of = [&](int e) { return (row0[e + 1] - row0[e] + tokens - 1) / tokens; };
+  int sum = 0;
+  for (int e = e0; e < e1; ++e) sum += units_of(e);
+  int upto = sum;
 #pragma unroll
-    for (int d = 16; d; d >>= 1) y += __shfl_xor_sync(0xffffffffu, y, d);
-    if (a.bias) y += a.bias_f32 ? static_cast<const float *>(a.bias)[n] : to_f32(static_cast<const T *>(a.bias)[n]);
-    if (lane == 0) *dst = Elem<T>::store(y);
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += o;
+  }
+  if (lane == 31) scan[warp] = upto;
+  __syncthreads();
+  int at = upto - sum;
+  for (int w = 0; w < warp; ++w) at += scan[w];
+  for (int e = e0; e < e1; ++e) {
+    first_unit[e] = at;
+    at += units_of(e);
+  }
+  if (tid == threads - 1) first_unit[G] = at;
+  __syncthreads();
+  return first_unit[G];
+}
+__device__ __forceinline__ int group_of_unit(const int *first_unit, int groups, int u) {
+  int lo = 0, hi = groups;  // first_unit[lo] <= u < first_unit[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first_unit[mid] <= u) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// Zeros for the rows from `first` on, shared out over the grid; thread `tid` of `threads`.
+template <class T> __device__ __forceinline__ void zero_rest(const GemmArgs &a, int64_t first, int tid, int threads) {
+  const int64_t n = (a.M - first) * (int64_t)a.N;
+  for (int64_t i = (int64_t)blockIdx.x * threads + tid; i < n; i += (int64_t)gridDim.x * threads) {
+    const int64_t m = i / a.N;
+    static_cast<T *>(a.out)[(first + m) * a.out_rs + (i - m * a.N)] = Elem<T>::store(0.f);
   }
 }
 

@@ -10,6 +10,8 @@
 #include "mb_common.cuh"
 #include "int4.cuh"
 #include "int4_gemm.cuh"
+#include "int4_few.cuh"
+#include "scaled_tc.cuh"
 
 using namespace mb;
 using namespace mb::host;
@@ -104,11 +106,81 @@ i4::GemmArgs gemm_args(const mb_int4_desc *d) {
   return a;
 }
 
+// Lets a kernel use `bytes` of dynamic shared memory; once per kernel and device.
+template <auto Kernel>
+int allow_smem(int bytes) {
+  static std::atomic<bool> done[64];
+  int dev = 0;
+  int rc = cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
+  if (rc) return rc;
+  const bool keep = dev >= 0 && dev < 64;
+  if (keep && done[dev].load(std::memory_order_acquire)) return MB_OK;
+  rc = cuda_check(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute");
+  if (!rc && keep) done[dev].store(true, std::memory_order_release);
+  return rc;
+}
+
+template <class T, int LW, int NT, bool ZERO>
+int few_launch_as(const i4::GemmArgs &a, cudaStream_t st) {
+  constexpr auto kern = i4::int4_few_kernel<T, LW, NT, ZERO>;
+  const int rc = allow_smem<kern>(i4::FewCfg<NT>::smem(i4::kMaxGroups));
+  if (rc) return rc;
+  const int x_aligned = rows16(a.x, a.M, a.x_rs, 2);
+  return launch_pdl(kern, dim3((unsigned)device_sms()), dim3(i4::FEW_THREADS), i4::FewCfg<NT>::smem(a.groups), st, 1,
+                    "int4_gemm", a, x_aligned);
+}
+template <class T, int LW, int NT>
+int few_launch_lw(const i4::GemmArgs &a, cudaStream_t st) {
+  return a.zero ? few_launch_as<T, LW, NT, true>(a, st) : few_launch_as<T, LW, NT, false>(a, st);
+}
+template <class T, int NT>
+int few_launch(const i4::GemmArgs &a, cudaStream_t st) {
+  if (a.group_log2 == 5) return few_launch_lw<T, 1, NT>(a, st);
+  return a.group_log2 == 6 ? few_launch_lw<T, 2, NT>(a, st) : few_launch_lw<T, 4, NT>(a, st);
+}
+
+struct Plan {
+  int few = 0;                 // tokens of a unit / 8 of the one-pass kernel, or 0
+  int pk_x = 0, pk_w = 0;      // operand copied into the workspace first
+  int64_t x_rs = 0, w_rs = 0, w_e = 0;
+  int64_t w_off = 0, ws_bytes = 0;
+};
+
+int int4_plan(const mb_int4_desc *d, Plan &pl) {
+  pl.x_rs = d->x_rs;
+  pl.w_rs = d->w_rs;
+  pl.w_e = d->w_e;
+  if (d->M == 0 || d->N == 0) return MB_OK;
+  const int64_t E = std::max<int64_t>(d->groups, 1), bytes = (d->K + 1) / 2;
+  pl.few = d->plan[0] ? d->plan[0] : (d->groups ? d->M > 8 * d->groups : d->M > 8) ? 2 : 1;
+  int64_t at = 0;
+  if (d->K > 0 && !(rows16(d->w, d->N, d->w_rs, 1) && (E == 1 || d->w_e % 16 == 0))) {
+    pl.pk_w = 1;
+    pl.w_off = at;
+    pl.w_rs = round_up(bytes, 16);
+    pl.w_e = d->w_e == 0 ? 0 : d->N * pl.w_rs;
+    at = round_up(at + (d->w_e == 0 ? 1 : E) * d->N * pl.w_rs, 256);
+  }
+  pl.ws_bytes = at;
+  return MB_OK;
+}
+
 template <class T>
-int gemm_launch(const mb_int4_desc *d, cudaStream_t st) {
-  const i4::GemmArgs a = gemm_args(d);
-  const int64_t blocks = std::min<int64_t>(ceil_div(d->M * d->N, 8), (int64_t)device_sms() * 64);
-  return launch_pdl(i4::int4_simple_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, 1, "int4_gemm", a);
+int gemm_launch(const mb_int4_desc *d, const Plan &pl, cudaStream_t st) {
+  i4::GemmArgs a = gemm_args(d);
+  if (pl.pk_w) {
+    uint8_t *w = static_cast<uint8_t *>(d->workspace) + pl.w_off;
+    const int64_t E = d->w_e == 0 ? 1 : std::max<int64_t>(d->groups, 1);
+    const PackArgs pw{d->w, w, d->N, (d->K + 1) / 2, d->w_rs, 1, d->w_e, E, pl.w_rs}, none{};
+    const int64_t blocks = std::min<int64_t>(ceil_div(E * d->N * ceil_div(pw.cols, 512), 8), (int64_t)device_sms() * 4);
+    const int rc = launch_pdl(sg::scaled_pack_kernel, dim3((unsigned)blocks), dim3(256), 0, st, 1, "int4_gemm: operand copy",
+                              none, pw, 0, d->w_e == 0 ? nullptr : a.offsets, a.M);
+    if (rc) return rc;
+    a.w = w;
+    a.w_rs = pl.w_rs;
+    a.w_e = pl.w_e;
+  }
+  return pl.few == 2 ? few_launch<T, 2>(a, st) : few_launch<T, 1>(a, st);
 }
 
 }  // namespace
@@ -151,18 +223,34 @@ void mb_int4_desc_init(mb_int4_desc *d) {
   if (d) memset(d, 0, sizeof(*d));
 }
 
-int64_t mb_int4_workspace_size(const mb_int4_desc *d) { return int4_check(d) ? 0 : 0; }
+int64_t mb_int4_workspace_size(const mb_int4_desc *d) {
+  Plan pl;
+  if (int4_check(d) || int4_plan(d, pl)) return 0;
+  return pl.ws_bytes;
+}
 
 int mb_int4_plan(const mb_int4_desc *d, char *buf, int buflen) {
-  const int rc = int4_check(d);
+  Plan pl;
+  int rc = int4_check(d);
+  if (!rc) rc = int4_plan(d, pl);
   if (rc) return -rc;
-  return snprintf(buf, buf ? (size_t)std::max(buflen, 0) : 0, "simple");
+  const size_t room = buf ? (size_t)std::max(buflen, 0) : 0;
+  if (d->M == 0 || d->N == 0) return snprintf(buf, room, "empty");
+  return snprintf(buf, room, "units of %d tokens in one pass over the weights, pack_w=%d ws=%lld", 8 * pl.few, pl.pk_w,
+                  (long long)pl.ws_bytes);
 }
 
 int mb_int4_gemm(const mb_int4_desc *d, void *stream) {
-  const int rc = int4_check(d);
+  Plan pl;
+  int rc = int4_check(d);
+  if (!rc) rc = int4_plan(d, pl);
   if (rc || d->M == 0 || d->N == 0) return rc;
-  return d->dtype == MB_F16 ? gemm_launch<__half>(d, (cudaStream_t)stream) : gemm_launch<__nv_bfloat16>(d, (cudaStream_t)stream);
+  if (pl.ws_bytes > 0 && (!d->workspace || d->workspace_bytes < pl.ws_bytes))
+    return fail(MB_ERR_WORKSPACE, "workspace of %lld bytes required", (long long)pl.ws_bytes);
+  if (pl.ws_bytes > 0 && !aligned16(d->workspace))  // operand copies are stored and loaded 16 bytes at a time
+    return fail(MB_ERR_WORKSPACE, "the workspace must start on a 16-byte boundary");
+  return d->dtype == MB_F16 ? gemm_launch<__half>(d, pl, (cudaStream_t)stream)
+                            : gemm_launch<__nv_bfloat16>(d, pl, (cudaStream_t)stream);
 }
 
 }  // extern "C"
