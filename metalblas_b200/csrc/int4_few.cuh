@@ -9,9 +9,11 @@
 // inside, are cut into one run per warp.  So a warp keeps to one or two slices,
 // whose tokens it holds in registers as MMA fragments while the weights stream by:
 // tokens pass through no shared memory and are read once per block.  Each warp
-// copies its items ahead into a ring of its own (cp.async, no barrier but the
-// warp's), and adds its 16 x 8 NT sums of a tile to its own place in shared
+// has its items brought into a ring of its own by TMA (one lane issues, no barrier but
+// the warp's), and adds its 16 x 8 NT sums of a tile to its own place in shared
 // memory; at the end the warps' sums are added in order.  Results repeat bit for bit.
+// The rows' scales lie in shared memory as fp32: loaded item by item, even one item
+// ahead, they were a third of the time (1 x 4096 x 14336: 22.1 us, 13.9 without them).
 //
 // m16n8k16 with weights as the rows.  A lane needs K positions in an order of the
 // instruction's, but the sum does not mind which columns they stand for as long as
@@ -20,28 +22,25 @@
 // the pair (128 + u0, 128 + u4) in bf16; subtracting 128 + z is exact.
 #pragma once
 #include "int4_gemm.cuh"
+#include "tc_gemm.cuh"
 
 namespace mb {
 namespace i4 {
 
-constexpr int FEW_WARPS = 16;
-constexpr int FEW_THREADS = FEW_WARPS * 32;
-constexpr int FEW_SLICE = 256;              // columns of an item
+constexpr int FEW_SLICE = 256;                // columns of an item
 constexpr int FEW_ITEM = 16 * FEW_SLICE / 2;  // its bytes
-constexpr int FEW_STAGES = 4;
 template <int NT> struct FewCfg {
-  static constexpr int TILES = NT == 1 ? 10 : 5;   // row tiles of a block at a time
-  static constexpr int RING = FEW_WARPS * FEW_STAGES * FEW_ITEM;
-  static constexpr int SUMS = FEW_WARPS * TILES * NT * 512;
-  static constexpr int smem(int groups) { return RING + SUMS + (2 * (groups + 1) + 32) * 4; }
-  static_assert(RING + SUMS + (2 * (kMaxGroups + 1) + 32) * 4 <= 232448, "shared memory");
+  static constexpr int WARPS = NT == 1 ? 16 : 8;   // (two fragments of tokens take 64 registers)
+  static constexpr int THREADS = WARPS * 32;
+  static constexpr int STAGES = NT == 1 ? 3 : 6;
+  static constexpr int TILES = 7;                  // row tiles of a block at a time
+  static constexpr int RING = WARPS * STAGES * FEW_ITEM;
+  static constexpr int SUMS = WARPS * TILES * NT * 512;
+  static constexpr int SCALES = 15360;             // fp32 words of scales (and zero points)
+  static constexpr int BARS = (WARPS * STAGES + 1) * 8;
+  static constexpr int smem(int groups) { return 1024 + RING + SUMS + SCALES * 4 + BARS + (2 * (groups + 1) + 32) * 4; }
+  static_assert(1024 + RING + SUMS + SCALES * 4 + BARS + (2 * (kMaxGroups + 1) + 32) * 4 <= 232448, "shared memory");
 };
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 template <class T>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -122,30 +121,45 @@ __device__ __forceinline__ void token_pairs(const T *row, int k, int K, bool ali
 // LW: words that a lane takes of a row at a time, so that four lanes' words lie in
 // one group (1: groups of 32 columns, 2: 64, 4: 128 and 256).
 template <class T, int LW, int NT, bool ZERO>
-__global__ void __launch_bounds__(FEW_THREADS, 1) int4_few_kernel(const __grid_constant__ GemmArgs a, int x_aligned) {
+__global__ void __launch_bounds__(FewCfg<NT>::THREADS, 1)
+    int4_few_kernel(const __grid_constant__ GemmArgs a, const __grid_constant__ CUtensorMap weights, int x_aligned,
+                    unsigned long long timeout_ns) {
   using Cfg = FewCfg<NT>;
   constexpr int TOKENS = 8 * NT, SUB = 32 * LW, SUBS = FEW_SLICE / SUB;  // columns scaled together, and such in a slice
-  constexpr int HELD = SUBS > 4 ? 2 : 1;                                 // scales of a row that a lane fetches
-  extern __shared__ __align__(1024) uint8_t smem[];
+  constexpr int WORDS = ZERO ? 2 : 1;                                    // a scale, or a scale and a zero point
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float *sums = reinterpret_cast<float *>(smem + Cfg::RING);
-  int *first_unit = reinterpret_cast<int *>(smem + Cfg::RING + Cfg::SUMS);
+  float *scales = reinterpret_cast<float *>(smem + Cfg::RING + Cfg::SUMS);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(scales + Cfg::SCALES);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + Cfg::WARPS * Cfg::STAGES);
+  int *first_unit = reinterpret_cast<int *>(bars + Cfg::WARPS * Cfg::STAGES + 1);
   int *row0 = first_unit + a.groups + 1, *scan = row0 + a.groups + 1;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t4 = lane & 3;
   const int wrow = ((g & 1) << 2) | (g & 2) | (g >> 2);   // the weight row of MMA row g (shared-memory banks)
-  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * (FEW_STAGES * FEW_ITEM);
-  const int row_bytes = (a.K + 1) / 2, slices = (a.K + FEW_SLICE - 1) / FEW_SLICE;
-  const int scales = (a.K + (1 << a.group_log2) - 1) >> a.group_log2;
+  const uint32_t ring = tc::smem_u32(smem) + warp * (Cfg::STAGES * FEW_ITEM);
+  const uint32_t bar = tc::smem_u32(bars) + warp * (Cfg::STAGES * 8);
+  const int slices = (a.K + FEW_SLICE - 1) / FEW_SLICE, groups = (a.K + (1 << a.group_log2) - 1) >> a.group_log2;
 
+  if (lane == 0) {
+    for (int i = 0; i < Cfg::STAGES; ++i) tc::mbar_init(bar + 8 * i, 1);
+    tc::fence_mbar_init();
+  }
+  if (tid == 0) {
+    *abort_flag = 0;
+    tc::prefetch_tmap(&weights);
+  }
   int units = (a.M + TOKENS - 1) / TOKENS;
   if (!a.offsets) {
     // this block's rows are known: as much of them as may matter starts its way into L2
     // (with one unit; more units' rows are the same ones again)
     const int64_t r0 = (int64_t)a.N * blockIdx.x / gridDim.x, rows = (int64_t)a.N * (blockIdx.x + 1) / gridDim.x - r0;
-    const int bytes = (int)min((int64_t)row_bytes, (int64_t)(96 << 10) / max((int64_t)1, rows)) & ~15;
+    const int bytes = (int)min((int64_t)(a.K + 1) / 2, (int64_t)(96 << 10) / max((int64_t)1, rows)) & ~15;
     if (bytes && units == 1)
-      for (int i = tid; i < rows; i += FEW_THREADS) prefetch_l2_bulk(a.w + (r0 + i) * a.w_rs, (uint32_t)bytes);
+      for (int i = tid; i < rows; i += Cfg::THREADS) prefetch_l2_bulk(a.w + (r0 + i) * a.w_rs, (uint32_t)bytes);
     pdl_wait();
+    __syncthreads();
   } else {
     pdl_wait();
     units = unit_table(a, TOKENS, first_unit, row0, scan);
@@ -153,6 +167,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) int4_few_kernel(const __grid_c
   const int64_t total = (int64_t)units * a.N;
   int64_t at = total * blockIdx.x / gridDim.x;
   const int64_t end = total * (blockIdx.x + 1) / gridDim.x;
+  int st = 0;            // the ring's next stage and its phase: the same for copies and reads
+  uint32_t phase = 0;
 
   while (at < end) {
     // up to TILES row tiles of one unit
@@ -165,160 +181,170 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) int4_few_kernel(const __grid_c
       m1 = row0[e + 1];
     }
     m1 = min(m1, m0 + TOKENS);
-    const int tiles = (rows + 15) / 16, items = slices * tiles;
-    const int i0 = items * warp / FEW_WARPS, i1 = items * (warp + 1) / FEW_WARPS;
-    const uint8_t *w = a.w + e * a.w_e + (int64_t)n0 * a.w_rs;
+    const int tiles = (rows + 15) / 16, we = a.w_e == 0 ? 0 : e;
 
-    // item i of the block to stage st of the ring: 128 bytes of 16 rows, a lane 16 bytes of
-    // rows lane / 8, + 4, + 8, + 12; chunks are exchanged by row so that reads meet no bank twice
-    const int crow = lane >> 3, chunk = lane & 7;
-    int fs = i0 / tiles, ft = i0 - fs * tiles;   // the next item to fetch
-    int fetched = i0;
-    auto fetch = [&](int st) {
-      if (fetched < i1) {
-        const int off = fs * (FEW_SLICE / 2) + chunk * 16;
-        const int bytes = min(max(row_bytes - off, 0), 16);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = crow + 4 * i, row = ft * 16 + r;
-          const bool on = row < rows && bytes > 0;
-          cp_async16(ring + st * FEW_ITEM + r * 128 + ((chunk ^ (r & 7)) << 4),
-                     on ? w + (int64_t)row * a.w_rs + off : a.w, on ? bytes : 0);
-        }
-        ++fetched;
-        if (++ft == tiles) { ft = 0; ++fs; }
-      }
-      cp_async_commit();
-    };
-#pragma unroll
-    for (int st = 0; st < FEW_STAGES; ++st) fetch(st);
-
-    // scales and zero points of the warp's next item: rows wrow and wrow + 8, sums t4 and t4 + 4
-    float sc[2][HELD], zc[2][HELD];
-    auto fetch_scales = [&](int s, int t) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = t * 16 + h * 8 + wrow;
-#pragma unroll
-        for (int j = 0; j < HELD; ++j) {
-          const int q = (s * FEW_SLICE + (t4 + 4 * j) * SUB) >> a.group_log2;
-          const bool on = row < rows && t4 + 4 * j < SUBS && q < scales;
-          sc[h][j] = on ? scale_at<T>(a, e * a.s_e + (int64_t)(n0 + row) * a.s_rs + q) : 0.f;
-          if constexpr (ZERO) zc[h][j] = on ? (float)a.zero[e * a.z_e + (int64_t)(n0 + row) * a.z_rs + q] : 0.f;
-        }
-      }
-    };
-
-    float *own = sums + (size_t)warp * (Cfg::TILES * NT * 128) + lane * 4;
+    float *own = sums + warp * (Cfg::TILES * NT * 128) + lane * 4;
     for (int i = 0; i < tiles * NT; ++i) *reinterpret_cast<float4 *>(own + i * 128) = make_float4(0.f, 0.f, 0.f, 0.f);
 
-    uint32_t x[NT][8][4];
-    int s = i0 / tiles, t = i0 - s * tiles, held = -1, st = 0;
-    if (i0 < i1) fetch_scales(s, t);
-    for (int i = i0; i < i1; ++i) {
-      if (s != held) {
-        held = s;
+    // the slices whose scales fit, at a time (all of them, with groups of 128 columns and K up to 30000)
+    const int per_slice = max(1, FEW_SLICE >> a.group_log2);
+    const int fit = max(1, (Cfg::SCALES / WORDS / (tiles * 16) - 1) / per_slice);
+    for (int s0 = 0; s0 < slices; s0 += fit) {
+      const int s1 = min(slices, s0 + fit), items = (s1 - s0) * tiles;
+      const int i0 = items * warp / Cfg::WARPS, i1 = items * (warp + 1) / Cfg::WARPS;
+      int fs = s0 + i0 / tiles, ft = i0 % tiles, fetched = i0;   // the next item to fetch
+      auto fetch = [&](int stage) {   // (by lane 0)
+        if (fetched >= i1) return;
+        tc::mbar_arrive_expect_tx(bar + 8 * stage, FEW_ITEM);
+        tc::tma_load_3d(ring + stage * FEW_ITEM, &weights, bar + 8 * stage, fs * (FEW_SLICE / 2), n0 + ft * 16, we);
+        ++fetched;
+        if (++ft == tiles) { ft = 0; ++fs; }
+      };
+      if (lane == 0) {
+        int stage = st;
+        for (int i = 0; i < Cfg::STAGES; ++i) {
+          fetch(stage);
+          stage = stage + 1 == Cfg::STAGES ? 0 : stage + 1;
+        }
+      }
+      // scales of the rows, fp32; an odd pitch, so that eight rows meet eight banks
+      // and zeros for groups past the end, whose sums are zeros
+      const int q0 = (s0 * FEW_SLICE) >> a.group_log2, qn = (s1 - s0) * per_slice, pitch = qn | 1;
+      // (a row a warp, and eight loads on their way at a time: one after another they were 4 of 19 us)
+      for (int q = lane; q < qn; q += 32) {
+        const bool on = q0 + q < groups;
+        const int64_t i_s = e * a.s_e + (int64_t)n0 * a.s_rs + q0 + q, i_z = e * a.z_e + (int64_t)n0 * a.z_rs + q0 + q;
+        for (int r0 = warp; r0 < rows; r0 += 8 * Cfg::WARPS) {
+          uint32_t v[8];
+          uint8_t z[8];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const int m = m0 + n * 8 + g;
-          const T *row = static_cast<const T *>(a.x) + (int64_t)m * a.x_rs;
+          for (int j = 0; j < 8; ++j) {
+            const int r = r0 + j * Cfg::WARPS;
+            const bool load = on && r < rows;
+            v[j] = load ? scale_bits<T>(a, i_s + r * a.s_rs) : 0u;
+            if constexpr (ZERO) z[j] = load ? a.zero[i_z + r * a.z_rs] : 0;
+          }
 #pragma unroll
-          for (int v = 0; v < 8; ++v) {
-            const int k = s * FEW_SLICE + (v / LW) * SUB + t4 * (8 * LW) + (v % LW) * 8;
-            if (m < m1) token_pairs(row, k, a.K, x_aligned, x[n][v]);
-            else x[n][v][0] = x[n][v][1] = x[n][v][2] = x[n][v][3] = 0;
+          for (int j = 0; j < 8; ++j) {
+            const int r = r0 + j * Cfg::WARPS;
+            if (r >= rows) break;
+            const float f = scale_of<T>(a, v[j]);
+            if constexpr (ZERO) reinterpret_cast<float2 *>(scales)[r * pitch + q] = make_float2(f, (float)z[j]);
+            else scales[r * pitch + q] = f;
           }
         }
       }
-      float sn[2][HELD], zn[2][HELD];
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int j = 0; j < HELD; ++j) {
-          sn[h][j] = sc[h][j];
-          if constexpr (ZERO) zn[h][j] = zc[h][j];
-        }
-      const int this_t = t;
-      if (++t == tiles) { t = 0; ++s; }
-      if (i + 1 < i1) fetch_scales(s, t);
+      __syncthreads();
 
-      cp_async_wait<FEW_STAGES - 1>();
-      __syncwarp();
-      // this lane's words of rows wrow and wrow + 8
-      uint32_t q[2][8];
+      uint32_t x[NT][8][4];
+      int s = s0 + i0 / tiles, t = i0 % tiles, held = -1, i = i0;
+      for (; i < i1; ++i) {
+        if (s != held) {
+          held = s;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t base = ring + st * FEW_ITEM + (h * 8 + wrow) * 128;
+          for (int n = 0; n < NT; ++n) {
+            const int m = m0 + n * 8 + g;
+            const T *row = static_cast<const T *>(a.x) + (int64_t)m * a.x_rs;
+#pragma unroll
+            for (int v = 0; v < 8; ++v) {
+              const int k = s * FEW_SLICE + (v / LW) * SUB + t4 * (8 * LW) + (v % LW) * 8;
+              if (m < m1) token_pairs(row, k, a.K, x_aligned, x[n][v]);
+              else x[n][v][0] = x[n][v][1] = x[n][v][2] = x[n][v][3] = 0;
+            }
+          }
+        }
+        if (!__all_sync(0xffffffffu, tc::mbar_wait(bar + 8 * st, phase, abort_flag, timeout_ns))) break;
+        // this lane's words of rows wrow and wrow + 8
+        uint32_t q[2][8];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t base = ring + st * FEW_ITEM + (h * 8 + wrow) * 128;
+#pragma unroll
+          for (int j = 0; j < SUBS; ++j) {
+            const int byte = j * (SUB / 2) + t4 * (4 * LW);
+            const uint32_t p = base + ((((byte >> 4) ^ wrow) << 4) | (byte & 15));
+            if constexpr (LW == 4)
+              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(q[h][4 * j]), "=r"(q[h][4 * j + 1]), "=r"(q[h][4 * j + 2]), "=r"(q[h][4 * j + 3]) : "r"(p));
+            else if constexpr (LW == 2)
+              asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(q[h][2 * j]), "=r"(q[h][2 * j + 1]) : "r"(p));
+            else
+              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(q[h][j]) : "r"(p));
+          }
+        }
+        __syncwarp();
+        if (lane == 0) fetch(st);
+        if (++st == Cfg::STAGES) { st = 0; phase ^= 1u; }
+
+        // (rows past the end have any numbers for scales: their sums are not stored)
+        const float *sc = scales + WORDS * ((t * 16 + wrow) * pitch + (((s - s0) * FEW_SLICE) >> a.group_log2));
+        float acc[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
 #pragma unroll
         for (int j = 0; j < SUBS; ++j) {
-          const int byte = j * (SUB / 2) + t4 * (4 * LW);
-          const uint32_t p = base + ((((byte >> 4) ^ wrow) << 4) | (byte & 15));
-          if constexpr (LW == 4)
-            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(q[h][4 * j]), "=r"(q[h][4 * j + 1]), "=r"(q[h][4 * j + 2]), "=r"(q[h][4 * j + 3]) : "r"(p));
-          else if constexpr (LW == 2)
-            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(q[h][2 * j]), "=r"(q[h][2 * j + 1]) : "r"(p));
-          else
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(q[h][j]) : "r"(p));
-        }
-      }
-      __syncwarp();
-      fetch(st);
-      if (++st == FEW_STAGES) st = 0;
-
-      float acc[NT][4];
+          // groups of 256 columns are two sums of 128
+          const int c = LW == 4 ? (a.group_log2 == 8 ? 0 : j) : j;
+          float sv0, sv1, z0 = 8.f, z1 = 8.f;
+          if constexpr (ZERO) {
+            const float2 v0 = *reinterpret_cast<const float2 *>(sc + 2 * c), v1 = *reinterpret_cast<const float2 *>(sc + 2 * (8 * pitch + c));
+            sv0 = v0.x; z0 = v0.y;
+            sv1 = v1.x; z1 = v1.y;
+          } else {
+            sv0 = sc[c];
+            sv1 = sc[8 * pitch + c];
+          }
+          const Decode<T, ZERO> d0(z0), d1(z1);
+          float d[NT][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+          for (int n = 0; n < NT; ++n) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.f;
 #pragma unroll
-      for (int j = 0; j < SUBS; ++j) {
-        const int src = (lane & ~3) | (j & 3);
-        const float s0 = __shfl_sync(0xffffffffu, sn[0][j / 4], src), s1 = __shfl_sync(0xffffffffu, sn[1][j / 4], src);
-        float z0 = 8.f, z1 = 8.f;
-        if constexpr (ZERO) {
-          z0 = __shfl_sync(0xffffffffu, zn[0][j / 4], src);
-          z1 = __shfl_sync(0xffffffffu, zn[1][j / 4], src);
-        }
-        const Decode<T, ZERO> d0(z0), d1(z1);
-        float d[NT][4];
+          for (int v = j * LW; v < (j + 1) * LW; ++v) {
+            uint32_t p0[4], p1[4];
+            d0(q[0][v], p0);
+            d1(q[1][v], p1);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.f;
+            for (int h = 0; h < 4; h += 2) {
+              const uint32_t f[4] = {p0[h], p1[h], p0[h + 1], p1[h + 1]};
 #pragma unroll
-        for (int v = j * LW; v < (j + 1) * LW; ++v) {
-          uint32_t p0[4], p1[4];
-          d0(q[0][v], p0);
-          d1(q[1][v], p1);
+              for (int n = 0; n < NT; ++n) mma16816<T>(d[n], f, x[n][v][h], x[n][v][h + 1]);
+            }
+          }
 #pragma unroll
-          for (int h = 0; h < 4; h += 2) {
-            const uint32_t f[4] = {p0[h], p1[h], p0[h + 1], p1[h + 1]};
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma16816<T>(d[n], f, x[n][v][h], x[n][v][h + 1]);
+          for (int n = 0; n < NT; ++n) {
+            acc[n][0] = fmaf(d[n][0], sv0, acc[n][0]);
+            acc[n][1] = fmaf(d[n][1], sv0, acc[n][1]);
+            acc[n][2] = fmaf(d[n][2], sv1, acc[n][2]);
+            acc[n][3] = fmaf(d[n][3], sv1, acc[n][3]);
           }
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          acc[n][0] = fmaf(d[n][0], s0, acc[n][0]);
-          acc[n][1] = fmaf(d[n][1], s0, acc[n][1]);
-          acc[n][2] = fmaf(d[n][2], s1, acc[n][2]);
-          acc[n][3] = fmaf(d[n][3], s1, acc[n][3]);
+          float4 *o = reinterpret_cast<float4 *>(own + (t * NT + n) * 128);
+          const float4 v = *o;
+          *o = make_float4(v.x + acc[n][0], v.y + acc[n][1], v.z + acc[n][2], v.w + acc[n][3]);
+        }
+        if (++t == tiles) { t = 0; ++s; }
+      }
+      if (i < i1 && lane == 0) {
+        // given up: the copies on their way land before the block can leave
+        volatile int no_abort = 0;
+        for (; i < fetched; ++i) {
+          tc::mbar_wait(bar + 8 * st, phase, &no_abort, timeout_ns);
+          if (++st == Cfg::STAGES) { st = 0; phase ^= 1u; }
         }
       }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float4 *o = reinterpret_cast<float4 *>(own + (this_t * NT + n) * 128);
-        const float4 v = *o;
-        *o = make_float4(v.x + acc[n][0], v.y + acc[n][1], v.z + acc[n][2], v.w + acc[n][3]);
-      }
+      if (s1 == slices && end - at == rows) pdl_trigger();
+      if (__syncthreads_or(*abort_flag)) return;
     }
-    cp_async_wait<0>();
-    if (end - at == rows) pdl_trigger();
-    __syncthreads();
+    if (slices == 0) __syncthreads();
     // four results of a tile: rows r and r + 8, tokens c and c + 1
-    for (int i = tid; i < tiles * NT * 32; i += FEW_THREADS) {
+    for (int i = tid; i < tiles * NT * 32; i += Cfg::THREADS) {
       const int l = i & 31, tn = i >> 5, tile = tn / NT, n = tn - tile * NT;
       float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int k = 0; k < FEW_WARPS; ++k) {
-        const float4 v = *reinterpret_cast<const float4 *>(sums + (size_t)k * (Cfg::TILES * NT * 128) + tn * 128 + l * 4);
+      for (int k = 0; k < Cfg::WARPS; ++k) {
+        const float4 v = *reinterpret_cast<const float4 *>(sums + k * (Cfg::TILES * NT * 128) + tn * 128 + l * 4);
         y.x += v.x; y.y += v.y; y.z += v.z; y.w += v.w;
       }
       const int lg = l >> 2, r = tile * 16 + (((lg & 1) << 2) | (lg & 2) | (lg >> 2)), m = m0 + n * 8 + (l & 3) * 2;
@@ -336,7 +362,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) int4_few_kernel(const __grid_c
     __syncthreads();
     at += rows;
   }
-  if (a.offsets) zero_rest<T>(a, row0[a.groups], tid, FEW_THREADS);
+  if (a.offsets) zero_rest<T>(a, row0[a.groups], tid, Cfg::THREADS);
 }
 
 }  // namespace i4

@@ -32,8 +32,14 @@ struct GemmArgs {
   int64_t out_rs;
 };
 
-template <class T> __device__ __forceinline__ float scale_at(const GemmArgs &a, int64_t i) {
-  return a.scale_f32 ? static_cast<const float *>(a.scale)[i] : to_f32(static_cast<const T *>(a.scale)[i]);
+// A scale as it lies in memory, and its value: apart, so that several can be on their way.
+template <class T> __device__ __forceinline__ uint32_t scale_bits(const GemmArgs &a, int64_t i) {
+  return a.scale_f32 ? static_cast<const uint32_t *>(a.scale)[i] : static_cast<const uint16_t *>(a.scale)[i];
+}
+template <class T> __device__ __forceinline__ float scale_of(const GemmArgs &a, uint32_t bits) {
+  if (a.scale_f32) return __uint_as_float(bits);
+  const uint16_t h = (uint16_t)bits;
+  return to_f32(reinterpret_cast<const T &>(h));
 }
 
 template <class T> __device__ __forceinline__ float bias_at(const GemmArgs &a, int64_t n) {

@@ -123,11 +123,18 @@ int allow_smem(int bytes) {
 template <class T, int LW, int NT, bool ZERO>
 int few_launch_as(const i4::GemmArgs &a, cudaStream_t st) {
   constexpr auto kern = i4::int4_few_kernel<T, LW, NT, ZERO>;
-  const int rc = allow_smem<kern>(i4::FewCfg<NT>::smem(i4::kMaxGroups));
+  using Cfg = i4::FewCfg<NT>;
+  int rc = allow_smem<kern>(Cfg::smem(i4::kMaxGroups));
+  if (rc) return rc;
+  CUtensorMap w{};
+  const int64_t bytes = (a.K + 1) / 2;
+  if (a.K > 0)   // boxes of 16 rows x 256 columns
+    rc = encode_map(&w, MB_U8, a.w, bytes, a.N, a.w_e == 0 ? 1 : std::max(a.groups, 1), a.N == 1 ? round_up(bytes, 16) : a.w_rs, a.w_e,
+                    i4::FEW_SLICE / 2, 16);
   if (rc) return rc;
   const int x_aligned = rows16(a.x, a.M, a.x_rs, 2);
-  return launch_pdl(kern, dim3((unsigned)device_sms()), dim3(i4::FEW_THREADS), i4::FewCfg<NT>::smem(a.groups), st, 1,
-                    "int4_gemm", a, x_aligned);
+  return launch_pdl(kern, dim3((unsigned)device_sms()), dim3(Cfg::THREADS), Cfg::smem(a.groups), st, 1, "int4_gemm", a, w,
+                    x_aligned, wait_timeout_ns());
 }
 template <class T, int LW, int NT>
 int few_launch_lw(const i4::GemmArgs &a, cudaStream_t st) {
