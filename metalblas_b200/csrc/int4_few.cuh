@@ -30,9 +30,9 @@ namespace i4 {
 constexpr int FEW_SLICE = 256;                // columns of an item
 constexpr int FEW_ITEM = 16 * FEW_SLICE / 2;  // its bytes
 template <int NT> struct FewCfg {
-  static constexpr int WARPS = NT == 1 ? 16 : 8;   // (two fragments of tokens take 64 registers)
+    static constexpr int WARPS = NT == 1 ? 12 : 8;   // (two fragments of tokens take 64 registers)
   static constexpr int THREADS = WARPS * 32;
-  static constexpr int STAGES = NT == 1 ? 3 : 6;
+  static constexpr int STAGES = 48 / WARPS;
   static constexpr int TILES = 7;                  // row tiles of a block at a time
   static constexpr int RING = WARPS * STAGES * FEW_ITEM;
   static constexpr int SUMS = WARPS * TILES * NT * 512;
@@ -100,18 +100,16 @@ template <bool ZERO> struct Decode<__half, ZERO> {
   }
 };
 
-// The 8 columns of a token from k on, as the pairs (0, 4), (1, 5), (2, 6), (3, 7); zeros past K.
+// The 8 columns of a token from k on, zeros past K; and as the pairs (0, 4), (1, 5), (2, 6), (3, 7).
 template <class T>
-__device__ __forceinline__ void token_pairs(const T *row, int k, int K, bool aligned, uint32_t (&o)[4]) {
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (aligned && k + 8 <= K) {
-    v = *reinterpret_cast<const uint4 *>(row + k);
-  } else {
-    uint16_t t[8];
+__device__ __forceinline__ uint4 token_word(const T *row, int k, int K, bool aligned) {
+  if (aligned && k + 8 <= K) return *reinterpret_cast<const uint4 *>(row + k);
+  uint16_t t[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = k + i < K ? reinterpret_cast<const uint16_t *>(row)[k + i] : 0;
-    v = make_uint4(t[0] | t[1] << 16, t[2] | t[3] << 16, t[4] | t[5] << 16, t[6] | t[7] << 16);
-  }
+  for (int i = 0; i < 8; ++i) t[i] = k + i < K ? reinterpret_cast<const uint16_t *>(row)[k + i] : 0;
+  return make_uint4(t[0] | t[1] << 16, t[2] | t[3] << 16, t[4] | t[5] << 16, t[6] | t[7] << 16);
+}
+__device__ __forceinline__ void token_pairs(const uint4 &v, uint32_t (&o)[4]) {
   o[0] = __byte_perm(v.x, v.z, 0x5410);
   o[1] = __byte_perm(v.x, v.z, 0x7632);
   o[2] = __byte_perm(v.y, v.w, 0x5410);
@@ -150,30 +148,33 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 1)
     *abort_flag = 0;
     tc::prefetch_tmap(&weights);
   }
+  pdl_trigger();
   int units = (a.M + TOKENS - 1) / TOKENS;
   if (!a.offsets) {
     // this block's rows are known: as much of them as may matter starts its way into L2
     // (with one unit; more units' rows are the same ones again)
-    const int64_t r0 = (int64_t)a.N * blockIdx.x / gridDim.x, rows = (int64_t)a.N * (blockIdx.x + 1) / gridDim.x - r0;
-    const int bytes = (int)min((int64_t)(a.K + 1) / 2, (int64_t)(96 << 10) / max((int64_t)1, rows)) & ~15;
+    const uint32_t share = a.N / gridDim.x, over = a.N % gridDim.x, rows = share + (blockIdx.x < over ? 1 : 0);
+    const uint8_t *w = a.w + (int64_t)(blockIdx.x * share + min(blockIdx.x, over)) * a.w_rs;
+    const uint32_t bytes = min((uint32_t)(a.K + 1) / 2, (96u << 10) / max(1u, rows)) & ~15u;
     if (bytes && units == 1)
-      for (int i = tid; i < rows; i += Cfg::THREADS) prefetch_l2_bulk(a.w + (r0 + i) * a.w_rs, (uint32_t)bytes);
+      for (uint32_t i = tid; i < rows; i += Cfg::THREADS) prefetch_l2_bulk(w + i * a.w_rs, bytes);
     pdl_wait();
     __syncthreads();
   } else {
     pdl_wait();
     units = unit_table(a, TOKENS, first_unit, row0, scan);
   }
-  const int64_t total = (int64_t)units * a.N;
-  int64_t at = total * blockIdx.x / gridDim.x;
-  const int64_t end = total * (blockIdx.x + 1) / gridDim.x;
+  // this block's share of the units' rows (units * N stays below 2^32: checked by the host)
+  const uint32_t total = (uint32_t)units * (uint32_t)a.N, share = total / gridDim.x, over = total % gridDim.x;
+  uint32_t at = blockIdx.x * share + min(blockIdx.x, over);
+  const uint32_t end = at + share + (blockIdx.x < over ? 1 : 0);
   int st = 0;            // the ring's next stage and its phase: the same for copies and reads
   uint32_t phase = 0;
 
   while (at < end) {
     // up to TILES row tiles of one unit
-    const int u = (int)(at / a.N), n0 = (int)(at - (int64_t)u * a.N);
-    const int rows = (int)min(min(end - at, (int64_t)(a.N - n0)), (int64_t)(16 * Cfg::TILES));
+    const int u = (int)(at / (uint32_t)a.N), n0 = (int)(at - (uint32_t)u * (uint32_t)a.N);
+    const int rows = (int)min(min(end - at, (uint32_t)(a.N - n0)), (uint32_t)(16 * Cfg::TILES));
     int e = 0, m0 = u * TOKENS, m1 = a.M;
     if (a.offsets) {
       e = group_of_unit(first_unit, a.groups, u);
@@ -207,6 +208,22 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 1)
           stage = stage + 1 == Cfg::STAGES ? 0 : stage + 1;
         }
       }
+      // the first slice's tokens
+      const int last = i0 < i1 ? s0 + (i1 - 1) / tiles : -1;
+      uint4 raw[NT][8];
+      auto fetch_tokens = [&](int s) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const int m = m0 + n * 8 + g;
+          const T *row = static_cast<const T *>(a.x) + (int64_t)m * a.x_rs;
+#pragma unroll
+          for (int v = 0; v < 8; ++v) {
+            const int k = s * FEW_SLICE + (v / LW) * SUB + t4 * (8 * LW) + (v % LW) * 8;
+            raw[n][v] = m < m1 ? token_word(row, k, a.K, x_aligned) : make_uint4(0, 0, 0, 0);
+          }
+        }
+      };
+      if (i0 < i1) fetch_tokens(s0 + i0 / tiles);
       // scales of the rows, fp32; an odd pitch, so that eight rows meet eight banks
       // and zeros for groups past the end, whose sums are zeros
       const int q0 = (s0 * FEW_SLICE) >> a.group_log2, qn = (s1 - s0) * per_slice, pitch = qn | 1;
@@ -242,16 +259,10 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 1)
         if (s != held) {
           held = s;
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const int m = m0 + n * 8 + g;
-            const T *row = static_cast<const T *>(a.x) + (int64_t)m * a.x_rs;
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int v = 0; v < 8; ++v) {
-              const int k = s * FEW_SLICE + (v / LW) * SUB + t4 * (8 * LW) + (v % LW) * 8;
-              if (m < m1) token_pairs(row, k, a.K, x_aligned, x[n][v]);
-              else x[n][v][0] = x[n][v][1] = x[n][v][2] = x[n][v][3] = 0;
-            }
-          }
+            for (int v = 0; v < 8; ++v) token_pairs(raw[n][v], x[n][v]);
+          if (s < last) fetch_tokens(s + 1);
         }
         if (!__all_sync(0xffffffffu, tc::mbar_wait(bar + 8 * st, phase, abort_flag, timeout_ns))) break;
         // this lane's words of rows wrow and wrow + 8
@@ -334,7 +345,6 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 1)
           if (++st == Cfg::STAGES) { st = 0; phase ^= 1u; }
         }
       }
-      if (s1 == slices && end - at == rows) pdl_trigger();
       if (__syncthreads_or(*abort_flag)) return;
     }
     if (slices == 0) __syncthreads();

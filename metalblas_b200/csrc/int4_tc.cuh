@@ -1,0 +1,442 @@
+// Products of many tokens with 4-bit weights on tcgen05.
+//
+// A tile is 128 weight rows (UMMA rows, TMEM lanes) x BN tokens (UMMA columns).
+// Weights come by TMA as they are, 128 rows x 256 columns (16 KB) a stage, are
+// decoded to whole numbers u - z by four warps, a thread a row, and stored to TMEM,
+// from where the MMA reads its A operand: they never pass through shared memory as
+// 16-bit values, whose writes and reads would bind it (the MMA of 128 x 128 takes its
+// 128 bytes a cycle already).  Tokens come by TMA, BN x 64 columns a stage.
+//
+// The MMA sums 128 columns (a group, where groups are smaller) into one of two
+// accumulators in TMEM; eight warps read it, multiply it by the row's scale, one
+// number a lane, and add it to fp32 sums in registers.  So scales are applied in
+// fp32 to exact products, the weights are not rounded, and the tensor core's own
+// fp32 sums are short.
+//
+// Roles: warp 0 TMA, warp 1 the MMA issuer, warps 2..5 decode, 6..13 sums and
+// output; two warps of sums per TMEM lane quarter, half of the columns each.
+// Persistent over units (matrix, token tile, row tile); units of groups are found
+// in a table made from the device's offsets (int4_gemm.cuh).  A tile of tokens may
+// hold rows of the next group: they are columns of their own and are not stored.
+//
+// split > 1 (few units): the CTAs of a cluster share a unit, each a range of
+// columns of K; the warps' pieces of the tile are finished by rank piece * split / 8,
+// which gets the other ranks' sums through distributed shared memory and adds
+// them to its own in the order of the ranks.
+#pragma once
+#include "int4_few.cuh"
+
+namespace mb {
+namespace i4 {
+
+using namespace mb::tc;
+
+constexpr int TC_WARPS = 14;
+constexpr int TC_THREADS = TC_WARPS * 32;
+constexpr int TC_W_BYTES = 128 * 128;    // weights of a stage: 128 rows x 256 columns
+constexpr int TC_A_STAGES = 8;           // decoded K-blocks in TMEM, 32 columns each
+constexpr int TC_A_COL = 256;            // their first TMEM column
+
+struct TcArgs {
+  CUtensorMap w, x;
+  GemmArgs g;
+  int tiles_n, split, kb_total;          // K-blocks of 64 columns
+  unsigned long long timeout_ns;
+};
+
+template <int BN> struct TcCfg {
+  static constexpr int X_BYTES = BN * 128;
+  static constexpr int W_STAGES = BN == 128 ? 3 : 6;
+  static constexpr int X_STAGES = BN == 128 ? 6 : BN == 64 ? 8 : 12;
+  static constexpr int CW = BN / 2;                 // columns of a warp of sums
+  static constexpr int PIECE = 32 * CW * 4;
+  static __host__ __device__ constexpr int red_bytes(int split) { return (split - 1) * (8 / split) * PIECE; }
+  static constexpr int NBARS = 2 * W_STAGES + 2 * X_STAGES + 2 * TC_A_STAGES + 7;
+  static constexpr int smem(int split, int groups) {
+    return 1024 + W_STAGES * TC_W_BYTES + X_STAGES * X_BYTES + red_bytes(split) + (NBARS + 2) * 8 + (2 * (groups + 1) + 32) * 4;
+  }
+  static_assert(smem(8, kMaxGroups) <= SMEM_LIMIT, "shared memory");
+};
+
+// D (+)= A B with A in TMEM.
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(idesc), "r"(accum)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// The columns of a word in their order, (0, 1), (2, 3), (4, 5), (6, 7): a byte b holds
+// two neighbours, and (b * 0x1001) & 0x000f000f is the pair (the multiplication
+// runs beside the logic pipe, which binds the decoding).
+__device__ __forceinline__ uint32_t byte_pair(uint32_t w, int i) {
+  const uint32_t b = i == 0 ? w & 0xffu : i == 3 ? w >> 24 : (w >> (8 * i)) & 0xffu;
+  return (b * 0x1001u) & 0x000f000fu;
+}
+template <class T, bool ZERO> struct InOrder;
+template <bool ZERO> struct InOrder<__nv_bfloat16, ZERO> {
+  uint32_t z2;
+  __device__ __forceinline__ explicit InOrder(uint32_t z) {
+    if constexpr (ZERO) {
+      const uint32_t b = __float_as_uint((float)z) >> 16;   // a whole number up to 255
+      z2 = b | (b << 16);
+    }
+  }
+  __device__ __forceinline__ void operator()(uint32_t w, uint32_t *o) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t v = byte_pair(w, i) | 0x43004300u, c = ZERO ? 0x43004300u : 0x43084308u;
+      __nv_bfloat162 x = __hsub2(reinterpret_cast<const __nv_bfloat162 &>(v), reinterpret_cast<const __nv_bfloat162 &>(c));
+      if constexpr (ZERO) x = __hsub2(x, reinterpret_cast<const __nv_bfloat162 &>(z2));   // 128 + z may take nine bits
+      o[i] = reinterpret_cast<uint32_t &>(x);
+    }
+  }
+};
+template <bool ZERO> struct InOrder<__half, ZERO> {
+  __half2 z;
+  __device__ __forceinline__ explicit InOrder(uint32_t zero) {
+    z = __float2half2_rn(1024.f + (ZERO ? (float)zero : 8.f));
+  }
+  __device__ __forceinline__ void operator()(uint32_t w, uint32_t *o) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t v = byte_pair(w, i) | 0x64006400u;
+      const __half2 x = __hsub2(reinterpret_cast<const __half2 &>(v), z);
+      o[i] = reinterpret_cast<const uint32_t &>(x);
+    }
+  }
+};
+
+struct TcTile {
+  int e, r0, rend, n0;   // matrix, first token row, end of the group's rows, first weight row
+};
+
+template <class T, int BN, bool ZERO>
+__global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_constant__ TcArgs p) {
+  using Cfg = TcCfg<BN>;
+  constexpr int WS = Cfg::W_STAGES, XS = Cfg::X_STAGES, AS = TC_A_STAGES, CW = Cfg::CW;
+  const GemmArgs &a = p.g;
+  const int split = p.split;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *xring = smem + WS * TC_W_BYTES, *red = xring + XS * Cfg::X_BYTES;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(red + Cfg::red_bytes(split));
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + Cfg::NBARS);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  int *first_unit = reinterpret_cast<int *>(bars + Cfg::NBARS + 2);
+  int *row0 = first_unit + a.groups + 1, *scan = row0 + a.groups + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t bar0 = smem_u32(bars);
+  auto bar = [&](int i) { return bar0 + 8u * i; };
+  // barriers: weights full, empty; tokens full, empty; A full, empty; D full, empty; drain, exchange
+  constexpr int W_FULL = 0, W_EMPTY = WS, X_FULL = 2 * WS, X_EMPTY = X_FULL + XS, A_FULL = X_FULL + 2 * XS,
+                A_EMPTY = A_FULL + AS, D_FULL = A_FULL + 2 * AS, D_EMPTY = D_FULL + 2, DRAIN = D_FULL + 4,
+                RED_FULL = DRAIN + 1, RED_FREE = DRAIN + 2;
+  static_assert(RED_FREE < Cfg::NBARS, "barriers");
+  const uint32_t rank = split > 1 ? cluster_rank() : 0u;
+  const int cid = blockIdx.x / split, ncl = gridDim.x / split;
+
+  pdl_trigger();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < WS; ++s) { mbar_init(bar(W_FULL + s), 1); mbar_init(bar(W_EMPTY + s), 4); }
+    for (int s = 0; s < XS; ++s) { mbar_init(bar(X_FULL + s), 1); mbar_init(bar(X_EMPTY + s), 1); }
+    for (int s = 0; s < AS; ++s) { mbar_init(bar(A_FULL + s), 4); mbar_init(bar(A_EMPTY + s), 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(bar(D_FULL + s), 1); mbar_init(bar(D_EMPTY + s), 8); }
+    mbar_init(bar(DRAIN), 1);
+    if (split > 1) {   // lane 0 of each sending warp; of each finishing warp
+      mbar_init(bar(RED_FULL), (split - 1) * (8 / split));
+      mbar_init(bar(RED_FREE), (split - 1) * (8 / split));
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tmap(&p.w);
+    prefetch_tmap(&p.x);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (split > 1) cluster_sync_all();   // every CTA's barriers are initialised before any remote arrival
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  int units;   // token tiles of all groups
+  if (a.offsets) {
+    units = unit_table(a, BN, first_unit, row0, scan);
+  } else {
+    units = (a.M + BN - 1) / BN;
+  }
+  const int num_units = units * p.tiles_n;
+  auto unit_at = [&](int u) {
+    // groups in order; within one row tiles outside, up to 16 token tiles inside (concurrent
+    // CTAs share weight tiles in L2, and with many token tiles their panels too)
+    TcTile t;
+    int tiles_m = units, first = 0;
+    t.e = 0;
+    t.r0 = 0;
+    t.rend = a.M;
+    if (a.offsets) {
+      const int g = group_of_unit(first_unit, a.groups, u / p.tiles_n);
+      t.e = g;
+      first = first_unit[g];
+      tiles_m = first_unit[g + 1] - first;
+      t.r0 = row0[g];
+      t.rend = row0[g + 1];
+    }
+    const int v = u - first * p.tiles_n, per = 16 * p.tiles_n, grp = v / per, w = v - grp * per;
+    const int gsz = min(tiles_m - grp * 16, 16);
+    t.r0 += (grp * 16 + w % gsz) * BN;
+    t.n0 = (w / gsz) * 128;
+    return t;
+  };
+  // this rank's K-blocks: whole stages of weights
+  const int stages = (p.kb_total + 3) / 4;
+  const int kb0 = (int)((int64_t)rank * stages / split) * 4, kb1 = min(p.kb_total, (int)((int64_t)(rank + 1) * stages / split) * 4);
+  // K-blocks of a sum (1 or 2), or sums of a K-block
+  const bool half = a.group_log2 == 5;
+  const int kb_sum = a.group_log2 >= 7 ? 2 : 1;
+  auto all = [](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      int ws = 0, xs = 0, last_w = -1, last_x = -1;
+      uint32_t wp = 0, xp = 0, last_wp = 0, last_xp = 0;
+      bool ok = true;
+      for (int u = cid; u < num_units && ok; u += ncl) {
+        const TcTile t = unit_at(u);
+        const int we = a.w_e == 0 ? 0 : t.e;
+        for (int kb = kb0; kb < kb1 && ok; ++kb) {
+          if ((kb & 3) == 0) {
+            if (!mbar_wait(bar(W_EMPTY + ws), wp ^ 1u, abort_flag, p.timeout_ns)) { ok = false; break; }
+            mbar_arrive_expect_tx(bar(W_FULL + ws), TC_W_BYTES);
+            tma_load_3d(smem_u32(smem) + ws * TC_W_BYTES, &p.w, bar(W_FULL + ws), kb * 32, t.n0, we);
+            last_w = ws;
+            last_wp = wp;
+            if (++ws == WS) { ws = 0; wp ^= 1u; }
+          }
+          if (!mbar_wait(bar(X_EMPTY + xs), xp ^ 1u, abort_flag, p.timeout_ns)) { ok = false; break; }
+          mbar_arrive_expect_tx(bar(X_FULL + xs), Cfg::X_BYTES);
+          tma_load_3d(smem_u32(xring) + xs * Cfg::X_BYTES, &p.x, bar(X_FULL + xs), kb * 64, t.r0, 0);
+          last_x = xs;
+          last_xp = xp;
+          if (++xs == XS) { xs = 0; xp ^= 1u; }
+        }
+      }
+      // the last copies must land before the CTA can exit
+      volatile int no_abort = 0;
+      if (last_w >= 0) mbar_wait(bar(W_FULL + last_w), last_wp, &no_abort, p.timeout_ns);
+      if (last_x >= 0) mbar_wait(bar(X_FULL + last_x), last_xp, &no_abort, p.timeout_ns);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      const uint32_t idesc = make_idesc<T, BN>(0, 0);
+      int xs = 0, as = 0, d = 0;
+      uint32_t xp = 0, ap = 0, dp = 0;
+      bool ok = true, issued = false;
+      for (int u = cid; u < num_units && ok; u += ncl) {
+        int in_sum = 0;   // K-blocks of the current sum
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(bar(X_FULL + xs), xp, abort_flag, p.timeout_ns) ||
+              !mbar_wait(bar(A_FULL + as), ap, abort_flag, p.timeout_ns)) { ok = false; break; }
+          if (in_sum == 0 && !mbar_wait(bar(D_EMPTY + d), dp ^ 1u, abort_flag, p.timeout_ns)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t at = tmem + TC_A_COL + as * 32, xb = smem_u32(xring) + xs * Cfg::X_BYTES;
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) {
+            if (half && ks == 2) {   // the second group of the K-block
+              umma_commit(bar(D_FULL + d));
+              if (++d == 2) { d = 0; dp ^= 1u; }
+              if (!mbar_wait(bar(D_EMPTY + d), dp ^ 1u, abort_flag, p.timeout_ns)) { ok = false; break; }
+              tc_fence_after();
+            }
+            umma_ts(tmem + d * BN, at + ks * 8, sdesc(xb + ks * 32, 16, 1024), idesc,
+                    (in_sum > 0 || (half ? ks & 1 : ks) > 0) ? 1u : 0u);
+          }
+          issued = true;
+          if (!ok) break;
+          umma_commit(bar(X_EMPTY + xs));
+          umma_commit(bar(A_EMPTY + as));
+          if (++xs == XS) { xs = 0; xp ^= 1u; }
+          if (++as == AS) { as = 0; ap ^= 1u; }
+          if (++in_sum == kb_sum || kb + 1 == kb1) {
+            umma_commit(bar(D_FULL + d));
+            if (++d == 2) { d = 0; dp ^= 1u; }
+            in_sum = 0;
+          }
+        }
+      }
+      if (*abort_flag && issued) {
+        umma_commit(bar(DRAIN));
+        volatile int no_abort = 0;
+        mbar_wait(bar(DRAIN), 0, &no_abort, p.timeout_ns);
+      }
+    }
+  } else if (warp < 6) {
+    // ------------------------------------------------------------ decoding
+    const int q = warp & 3, r = q * 32 + lane;   // this thread's row of the tile, its TMEM lane
+    const uint32_t at = tmem + TC_A_COL + ((uint32_t)(q * 32) << 16);
+    const uint32_t src = smem_u32(smem) + r * 128;
+    int ws = 0, as = 0;
+    uint32_t wp = 0, ap = 0;
+    bool ok = true;
+    for (int u = cid; u < num_units && ok; u += ncl) {
+      const TcTile t = unit_at(u);
+      const int n = min(t.n0 + r, a.N - 1);
+      const uint8_t *zero = ZERO ? a.zero + t.e * a.z_e + (int64_t)n * a.z_rs : nullptr;
+      uint32_t zn0 = 8, zn1 = 8;   // zero points, one K-block ahead
+      auto fetch_zero = [&](int kb) {
+        if constexpr (ZERO) {
+          zn0 = zero[(kb * 64) >> a.group_log2];
+          zn1 = half && kb * 64 + 32 < a.K ? zero[kb * 2 + 1] : zn0;
+        }
+      };
+      if (kb0 < kb1) fetch_zero(kb0);
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const uint32_t z0 = zn0, z1 = zn1;
+        if (kb + 1 < kb1) fetch_zero(kb + 1);
+        if ((kb & 3) == 0 && !all(mbar_wait(bar(W_FULL + ws), wp, abort_flag, p.timeout_ns))) { ok = false; break; }
+        const uint32_t row = src + ws * TC_W_BYTES;
+        const uint4 lo = ld_shared_v4(row + ((((kb & 3) * 2) ^ (r & 7)) << 4));
+        const uint4 hi = ld_shared_v4(row + ((((kb & 3) * 2 + 1) ^ (r & 7)) << 4));
+        if ((kb & 3) == 3 || kb + 1 == kb1) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(W_EMPTY + ws));
+          if (++ws == WS) { ws = 0; wp ^= 1u; }
+        }
+        uint32_t o[32];
+        const InOrder<T, ZERO> d0(z0), d1(z1);
+        d0(lo.x, o); d0(lo.y, o + 4); d0(lo.z, o + 8); d0(lo.w, o + 12);
+        d1(hi.x, o + 16); d1(hi.y, o + 20); d1(hi.z, o + 24); d1(hi.w, o + 28);
+        if (!all(mbar_wait(bar(A_EMPTY + as), ap ^ 1u, abort_flag, p.timeout_ns))) { ok = false; break; }
+        tc_fence_after();
+        tmem_st_x32(at + as * 32, o);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(A_FULL + as));
+        if (++as == AS) { as = 0; ap ^= 1u; }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ sums and output
+    const int q = warp & 3, hf = (warp - 6) >> 2, r = q * 32 + lane;
+    T *out = static_cast<T *>(a.out);
+    const int piece = q * 2 + hf, per_rank = 8 / split, owner = piece / per_rank;
+    const uint32_t red_u32 = smem_u32(red) + (uint32_t)(piece % per_rank) * Cfg::PIECE + lane * 16u;
+    const uint32_t red_step = (uint32_t)(per_rank * Cfg::PIECE);   // from one source rank to the next
+    const int sum_log2 = min(a.group_log2, 7), k1 = min(a.K, kb1 * 64);
+    int d = 0;
+    uint32_t dp = 0, rphase = 0;
+    bool first = true, ok = true;
+    for (int u = cid; u < num_units && ok; u += ncl) {
+      const TcTile t = unit_at(u);
+      const int64_t n = t.n0 + r;
+      const int64_t i_s = t.e * a.s_e + min(n, (int64_t)a.N - 1) * a.s_rs;
+      float acc[CW];
+#pragma unroll
+      for (int j = 0; j < CW; ++j) acc[j] = 0.f;
+      uint32_t bits = kb0 < kb1 ? scale_bits<T>(a, i_s + ((kb0 * 64) >> a.group_log2)) : 0u;
+      for (int k = kb0 * 64; k < kb1 * 64; k += 1 << sum_log2) {
+        const float s = k < k1 ? scale_of<T>(a, bits) : 0.f;
+        const int next = k + (1 << sum_log2);
+        if (next < k1) bits = scale_bits<T>(a, i_s + (next >> a.group_log2));
+        if (!all(mbar_wait(bar(D_FULL + d), dp, abort_flag, p.timeout_ns))) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + d * BN + hf * CW;
+        constexpr int CH = CW < 32 ? CW : 32;
+#pragma unroll
+        for (int c = 0; c < CW; c += CH) {
+          uint32_t v[32];
+          tmem_ld<CH>(from + c, v);
+          tmem_wait_ld();
+          if (c + CH >= CW) {   // the accumulator is read
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(D_EMPTY + d));
+          }
+#pragma unroll
+          for (int j = 0; j < CH; j += 2) {
+            const float2 o = fma2(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), make_float2(s, s),
+                                  make_float2(acc[c + j], acc[c + j + 1]));
+            acc[c + j] = o.x;
+            acc[c + j + 1] = o.y;
+          }
+        }
+        if (++d == 2) { d = 0; dp ^= 1u; }
+      }
+      if (!ok) break;
+      if (split > 1) {
+        if (owner != (int)rank) {
+          // what this CTA sent for the last unit has been read
+          if (!first && !all(mbar_wait_cluster(bar(RED_FREE), rphase ^ 1u, abort_flag, p.timeout_ns))) break;
+          const uint32_t dst = mapa_shared(red_u32 + (uint32_t)((int)rank - ((int)rank > owner ? 1 : 0)) * red_step, (uint32_t)owner);
+#pragma unroll
+          for (int j = 0; j < CW; j += 4)
+            st_cluster_v4(dst + (uint32_t)(j >> 2) * 512u, __float_as_uint(acc[j]), __float_as_uint(acc[j + 1]),
+                          __float_as_uint(acc[j + 2]), __float_as_uint(acc[j + 3]));
+          __syncwarp();   // the lanes' stores come before lane 0's release
+          if (lane == 0) mbar_arrive_cluster(mapa_shared(bar(RED_FULL), (uint32_t)owner));
+        } else {
+          if (!all(mbar_wait_cluster(bar(RED_FULL), rphase, abort_flag, p.timeout_ns))) break;
+          // to this rank's own sums, in the order of the ranks
+#pragma unroll 1
+          for (int s = 0; s < split - 1; ++s) {
+#pragma unroll
+            for (int j = 0; j < CW; j += 4) {
+              const uint4 v = ld_shared_v4(red_u32 + s * red_step + (uint32_t)(j >> 2) * 512u);
+              acc[j] += __uint_as_float(v.x);
+              acc[j + 1] += __uint_as_float(v.y);
+              acc[j + 2] += __uint_as_float(v.z);
+              acc[j + 3] += __uint_as_float(v.w);
+            }
+          }
+          __syncwarp();
+          if (lane < split && lane != (int)rank) mbar_arrive_cluster(mapa_shared(bar(RED_FREE), (uint32_t)lane));
+        }
+        rphase ^= 1u;
+        first = false;
+      }
+      if (split == 1 || owner == (int)rank) {
+        const float b = a.bias && n < a.N ? bias_at<T>(a, n) : 0.f;
+        if (n < a.N) {
+          const int64_t m = t.r0 + hf * CW;
+          const int live = (int)min((int64_t)CW, t.rend - m);
+          T *dst = out + m * a.out_rs + n;
+#pragma unroll
+          for (int j = 0; j < CW; ++j)
+            if (j < live) dst[j * a.out_rs] = Elem<T>::store(acc[j] + b);
+        }
+      }
+    }
+    if (a.offsets) zero_rest<T>(a, row0[a.groups], threadIdx.x - 6 * 32, 8 * 32);
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (split > 1) cluster_sync_all();   // no CTA leaves while others still reach its shared memory
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_g<1>(tmem, 512);
+  }
+}
+
+}  // namespace i4
+}  // namespace mb

@@ -11,6 +11,7 @@
 #include "int4.cuh"
 #include "int4_gemm.cuh"
 #include "int4_few.cuh"
+#include "int4_tc.cuh"
 #include "scaled_tc.cuh"
 
 using namespace mb;
@@ -146,11 +147,29 @@ int few_launch(const i4::GemmArgs &a, cudaStream_t st) {
   return a.group_log2 == 6 ? few_launch_lw<T, 2, NT>(a, st) : few_launch_lw<T, 4, NT>(a, st);
 }
 
+template <class T, int BN, bool ZERO>
+int tc_launch_as(i4::TcArgs &p, int split, int64_t units, cudaStream_t st) {
+  constexpr auto kern = i4::int4_tc_kernel<T, BN, ZERO>;
+  using Cfg = i4::TcCfg<BN>;
+  const int rc = allow_smem<kern>(Cfg::smem(8, i4::kMaxGroups));
+  if (rc) return rc;
+  p.split = split;
+  const int64_t clusters = std::min<int64_t>(units, device_sms() / split);
+  return launch_pdl(kern, dim3((unsigned)(clusters * split)), dim3(i4::TC_THREADS), Cfg::smem(split, p.g.groups), st, split,
+                    "int4_gemm", p);
+}
+template <class T, int BN>
+int tc_launch_bn(i4::TcArgs &p, int split, int64_t units, cudaStream_t st) {
+  return p.g.zero ? tc_launch_as<T, BN, true>(p, split, units, st) : tc_launch_as<T, BN, false>(p, split, units, st);
+}
+
 struct Plan {
   int few = 0;                 // tokens of a unit / 8 of the one-pass kernel, or 0
+  int bn = 0, split = 1;       // tokens of a tile and CTAs that share it of the tcgen05 kernel
+  int64_t units = 0;           // its units, at most
   int pk_x = 0, pk_w = 0;      // operand copied into the workspace first
   int64_t x_rs = 0, w_rs = 0, w_e = 0;
-  int64_t w_off = 0, ws_bytes = 0;
+  int64_t x_off = 0, w_off = 0, ws_bytes = 0;
 };
 
 int int4_plan(const mb_int4_desc *d, Plan &pl) {
@@ -159,8 +178,43 @@ int int4_plan(const mb_int4_desc *d, Plan &pl) {
   pl.w_e = d->w_e;
   if (d->M == 0 || d->N == 0) return MB_OK;
   const int64_t E = std::max<int64_t>(d->groups, 1), bytes = (d->K + 1) / 2;
-  pl.few = d->plan[0] ? d->plan[0] : (d->groups ? d->M > 8 * d->groups : d->M > 8) ? 2 : 1;
+  const int64_t active = d->groups ? std::min(E, d->M) : 1;
+  const double rows = (double)d->M / active;
+  const int want = d->plan[0];
+  if (want != 0 && want != 1 && want != 2 && want != 16 && want != 32 && want != 64 && want != 128)
+    return fail(MB_ERR_INVALID, "no plan %d", want);
+  // the one-pass kernel counts rows of units in 32 bits
+  auto few_fits = [&](int nt) { return (ceil_div(d->M, 8 * nt) + (d->groups ? E : 0)) * d->N < (1ll << 32); };
+  if (want == 1 || want == 2) {
+    pl.few = want;
+  } else if (!want && (d->K == 0 || rows <= 16)) {
+    pl.few = rows <= 8 ? 1 : 2;
+  }
+  if (pl.few && !few_fits(pl.few)) {
+    if (want || d->K == 0) return fail(MB_ERR_INVALID, "too many rows");
+    pl.few = 0;
+  }
+  if (!pl.few) {
+    pl.bn = want >= 16 ? want : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    const int64_t tiles_n = ceil_div(d->N, 128), stages = ceil_div(d->K, 256);
+    pl.units = (ceil_div(d->M, pl.bn) + (d->groups ? active : 0)) * tiles_n;
+    if (pl.units >= (1ll << 31)) return fail(MB_ERR_INVALID, "too many tiles");
+    const int sms = device_sms();
+    if (d->plan[1]) {
+      pl.split = d->plan[1];
+      if (pl.split != 1 && pl.split != 2 && pl.split != 4 && pl.split != 8) return fail(MB_ERR_INVALID, "a split is 1, 2, 4 or 8");
+      if (pl.split > stages) return fail(MB_ERR_INVALID, "a split of %d exceeds the columns", pl.split);
+    } else {
+      while (pl.split < 8 && pl.units * pl.split * 2 <= sms && pl.split * 2 <= stages) pl.split *= 2;
+    }
+  }
   int64_t at = 0;
+  if (!pl.few && !rows16(d->x, d->M, d->x_rs, 2)) {
+    pl.pk_x = 1;
+    pl.x_off = at;
+    pl.x_rs = round_up(d->K, 8);
+    at = round_up(at + d->M * pl.x_rs * 2, 256);
+  }
   if (d->K > 0 && !(rows16(d->w, d->N, d->w_rs, 1) && (E == 1 || d->w_e % 16 == 0))) {
     pl.pk_w = 1;
     pl.w_off = at;
@@ -175,19 +229,43 @@ int int4_plan(const mb_int4_desc *d, Plan &pl) {
 template <class T>
 int gemm_launch(const mb_int4_desc *d, const Plan &pl, cudaStream_t st) {
   i4::GemmArgs a = gemm_args(d);
+  PackArgs px{}, pw{};
+  const int64_t nw = d->w_e == 0 ? 1 : std::max<int64_t>(d->groups, 1);
+  if (pl.pk_x) {   // rows as bytes
+    px = PackArgs{d->x, static_cast<uint8_t *>(d->workspace) + pl.x_off, d->M, d->K * 2, d->x_rs * 2, 1, 0, 1, pl.x_rs * 2};
+    a.x = px.dst;
+    a.x_rs = pl.x_rs;
+  }
   if (pl.pk_w) {
-    uint8_t *w = static_cast<uint8_t *>(d->workspace) + pl.w_off;
-    const int64_t E = d->w_e == 0 ? 1 : std::max<int64_t>(d->groups, 1);
-    const PackArgs pw{d->w, w, d->N, (d->K + 1) / 2, d->w_rs, 1, d->w_e, E, pl.w_rs}, none{};
-    const int64_t blocks = std::min<int64_t>(ceil_div(E * d->N * ceil_div(pw.cols, 512), 8), (int64_t)device_sms() * 4);
-    const int rc = launch_pdl(sg::scaled_pack_kernel, dim3((unsigned)blocks), dim3(256), 0, st, 1, "int4_gemm: operand copy",
-                              none, pw, 0, d->w_e == 0 ? nullptr : a.offsets, a.M);
-    if (rc) return rc;
-    a.w = w;
+    pw = PackArgs{d->w, static_cast<uint8_t *>(d->workspace) + pl.w_off, d->N, (d->K + 1) / 2, d->w_rs, 1, d->w_e, nw, pl.w_rs};
+    a.w = static_cast<uint8_t *>(pw.dst);
     a.w_rs = pl.w_rs;
     a.w_e = pl.w_e;
   }
-  return pl.few == 2 ? few_launch<T, 2>(a, st) : few_launch<T, 1>(a, st);
+  if (pl.pk_x || pl.pk_w) {
+    auto blocks = [&](const PackArgs &m) {
+      return m.dst ? std::min<int64_t>(ceil_div(m.batch * m.rows * ceil_div(m.cols, 512), 8), (int64_t)device_sms() * 4) : 0;
+    };
+    const int rc = launch_pdl(sg::scaled_pack_kernel, dim3((unsigned)(blocks(px) + blocks(pw))), dim3(256), 0, st, 1,
+                              "int4_gemm: operand copy", px, pw, (int)blocks(px), d->w_e == 0 ? nullptr : a.offsets, a.M);
+    if (rc) return rc;
+  }
+  if (pl.few) return pl.few == 2 ? few_launch<T, 2>(a, st) : few_launch<T, 1>(a, st);
+  i4::TcArgs p{};
+  p.g = a;
+  p.tiles_n = (int)ceil_div(d->N, 128);
+  p.kb_total = (int)ceil_div(d->K, 64);
+  p.timeout_ns = wait_timeout_ns();
+  const int64_t bytes = (d->K + 1) / 2;
+  int rc = encode_map(&p.w, MB_U8, a.w, bytes, d->N, nw, d->N == 1 ? round_up(bytes, 16) : a.w_rs, a.w_e, 128, 128);
+  if (!rc) rc = encode_map(&p.x, d->dtype, a.x, d->K, d->M, 1, d->M == 1 ? round_up(d->K, 8) : a.x_rs, 0, 64, pl.bn);
+  if (rc) return rc;
+  switch (pl.bn) {
+    case 16: return tc_launch_bn<T, 16>(p, pl.split, pl.units, st);
+    case 32: return tc_launch_bn<T, 32>(p, pl.split, pl.units, st);
+    case 64: return tc_launch_bn<T, 64>(p, pl.split, pl.units, st);
+    default: return tc_launch_bn<T, 128>(p, pl.split, pl.units, st);
+  }
 }
 
 }  // namespace
@@ -243,8 +321,11 @@ int mb_int4_plan(const mb_int4_desc *d, char *buf, int buflen) {
   if (rc) return -rc;
   const size_t room = buf ? (size_t)std::max(buflen, 0) : 0;
   if (d->M == 0 || d->N == 0) return snprintf(buf, room, "empty");
-  return snprintf(buf, room, "units of %d tokens in one pass over the weights, pack_w=%d ws=%lld", 8 * pl.few, pl.pk_w,
-                  (long long)pl.ws_bytes);
+  if (pl.few)
+    return snprintf(buf, room, "units of %d tokens in one pass over the weights, pack_w=%d ws=%lld", 8 * pl.few, pl.pk_w,
+                    (long long)pl.ws_bytes);
+  return snprintf(buf, room, "tiles of 128 rows x %d tokens, split=%d pack_x=%d pack_w=%d ws=%lld", pl.bn, pl.split, pl.pk_x,
+                  pl.pk_w, (long long)pl.ws_bytes);
 }
 
 int mb_int4_gemm(const mb_int4_desc *d, void *stream) {
