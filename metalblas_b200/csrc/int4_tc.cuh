@@ -1,20 +1,24 @@
 // Products of many tokens with 4-bit weights on tcgen05.
 //
-// A tile is 128 weight rows (UMMA rows, TMEM lanes) x BN tokens (UMMA columns).
-// Weights come by TMA as they are, 128 rows x 256 columns (16 KB) a stage, are
-// decoded to whole numbers u - z by four warps, a thread a row, and stored to TMEM,
-// from where the MMA reads its A operand: they never pass through shared memory as
-// 16-bit values, whose writes and reads would bind it (the MMA of 128 x 128 takes its
-// 128 bytes a cycle already).  Tokens come by TMA, BN x 64 columns a stage.
+// A tile is 128 weight rows (UMMA rows, TMEM lanes) x BN tokens (UMMA columns), and
+// a step 128 columns of K.  Weights come by TMA as they are, 128 rows x 256 columns
+// (16 KB) a stage, are decoded to whole numbers u - z by eight warps, a thread a row
+// and 64 columns, and stored to TMEM, from where the MMA reads its A operand: they
+// never pass through shared memory as 16-bit values, whose writes and reads would
+// bind it (the MMA of 128 x 128 takes its 128 bytes a cycle already).  Tokens come
+// by TMA, BN x 128 columns a step.
 //
-// The MMA sums 128 columns (a group, where groups are smaller) into one of two
+// The MMA sums a step (a group, where groups are smaller) into one of two
 // accumulators in TMEM; eight warps read it, multiply it by the row's scale, one
 // number a lane, and add it to fp32 sums in registers.  So scales are applied in
 // fp32 to exact products, the weights are not rounded, and the tensor core's own
-// fp32 sums are short.
+// fp32 sums are short.  One tcgen05.commit a step tells the copies, the decoding and
+// the sums at once (steps of 64 columns with a commit for each of them took 600 cycles
+// in barriers alone).
 //
-// Roles: warp 0 TMA, warp 1 the MMA issuer, warps 2..5 decode, 6..13 sums and
-// output; two warps of sums per TMEM lane quarter, half of the columns each.
+// Roles, by warpgroup: warp 0 TMA, warp 1 the MMA issuer; warps 4..11 decode; warps
+// 12..19 sums and output, two to a TMEM lane quarter, half of the columns each.  The
+// registers go where the sums are (setmaxnreg).
 // Persistent over units (matrix, token tile, row tile); units of groups are found
 // in a table made from the device's offsets (int4_gemm.cuh).  A tile of tokens may
 // hold rows of the next group: they are columns of their own and are not stored.
@@ -31,33 +35,44 @@ namespace i4 {
 
 using namespace mb::tc;
 
-constexpr int TC_WARPS = 14;
+constexpr int TC_WARPS = 20;
 constexpr int TC_THREADS = TC_WARPS * 32;
 constexpr int TC_W_BYTES = 128 * 128;    // weights of a stage: 128 rows x 256 columns
-constexpr int TC_A_STAGES = 8;           // decoded K-blocks in TMEM, 32 columns each
-constexpr int TC_A_COL = 256;            // their first TMEM column
+constexpr int TC_STEP = 128;             // columns of K of a step
+constexpr int TC_STEPS = 4;              // steps held: tokens in shared memory, decoded weights in TMEM
+constexpr int TC_A_COL = 256;            // first TMEM column of the weights, 64 columns a step
+// Registers of a thread: 128 x 40 + 256 x 72 + 256 x 144 of the 640 x 96 at launch.
+constexpr int TC_REGS_ISSUE = 40, TC_REGS_DECODE = 72, TC_REGS_SUM = 144;
+static_assert(128 * TC_REGS_ISSUE + 256 * TC_REGS_DECODE + 256 * TC_REGS_SUM <= TC_THREADS * 96, "registers at launch");
 
 struct TcArgs {
   CUtensorMap w, x;
   GemmArgs g;
-  int tiles_n, split, kb_total;          // K-blocks of 64 columns
+  int tiles_n, split, steps;             // steps of the whole of K
   unsigned long long timeout_ns;
 };
 
 template <int BN> struct TcCfg {
-  static constexpr int X_BYTES = BN * 128;
-  static constexpr int W_STAGES = BN == 128 ? 3 : 6;
-  static constexpr int X_STAGES = BN == 128 ? 6 : BN == 64 ? 8 : 12;
+  static constexpr int X_BYTES = BN * 256;          // two boxes of 64 columns
+  static constexpr int W_STAGES = BN == 128 ? 2 : 6;
   static constexpr int CW = BN / 2;                 // columns of a warp of sums
   static constexpr int PIECE = 32 * CW * 4;
   static __host__ __device__ constexpr int red_bytes(int split) { return (split - 1) * (8 / split) * PIECE; }
-  static constexpr int NBARS = 2 * W_STAGES + 2 * X_STAGES + 2 * TC_A_STAGES + 7;
+  static constexpr int NBARS = 2 * W_STAGES + 3 * TC_STEPS + 7;
   static constexpr int smem(int split, int groups) {
-    return 1024 + W_STAGES * TC_W_BYTES + X_STAGES * X_BYTES + red_bytes(split) + (NBARS + 2) * 8 + (2 * (groups + 1) + 32) * 4;
+    return 1024 + W_STAGES * TC_W_BYTES + TC_STEPS * X_BYTES + red_bytes(split) + (NBARS + 2) * 8 + (2 * (groups + 1) + 32) * 4;
   }
   static_assert(smem(8, kMaxGroups) <= SMEM_LIMIT, "shared memory");
 };
 
+template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+// One lane of the warp, the same at every call.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
 // D (+)= A B with A in TMEM.
 __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
   asm volatile(
@@ -127,34 +142,34 @@ struct TcTile {
 template <class T, int BN, bool ZERO>
 __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_constant__ TcArgs p) {
   using Cfg = TcCfg<BN>;
-  constexpr int WS = Cfg::W_STAGES, XS = Cfg::X_STAGES, AS = TC_A_STAGES, CW = Cfg::CW;
+  constexpr int WS = Cfg::W_STAGES, ST = TC_STEPS, CW = Cfg::CW;
   const GemmArgs &a = p.g;
   const int split = p.split;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t *xring = smem + WS * TC_W_BYTES, *red = xring + XS * Cfg::X_BYTES;
+  uint8_t *xring = smem + WS * TC_W_BYTES, *red = xring + ST * Cfg::X_BYTES;
   uint64_t *bars = reinterpret_cast<uint64_t *>(red + Cfg::red_bytes(split));
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + Cfg::NBARS);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   int *first_unit = reinterpret_cast<int *>(bars + Cfg::NBARS + 2);
   int *row0 = first_unit + a.groups + 1, *scan = row0 + a.groups + 1;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // (from lane 0, so that the compiler knows it is the same for the whole warp)
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t bar0 = smem_u32(bars);
   auto bar = [&](int i) { return bar0 + 8u * i; };
-  // barriers: weights full, empty; tokens full, empty; A full, empty; D full, empty; drain, exchange
-  constexpr int W_FULL = 0, W_EMPTY = WS, X_FULL = 2 * WS, X_EMPTY = X_FULL + XS, A_FULL = X_FULL + 2 * XS,
-                A_EMPTY = A_FULL + AS, D_FULL = A_FULL + 2 * AS, D_EMPTY = D_FULL + 2, DRAIN = D_FULL + 4,
-                RED_FULL = DRAIN + 1, RED_FREE = DRAIN + 2;
+  // barriers: weights full, empty; a step's tokens full, its weights decoded, its MMA done;
+  // an accumulator's sum done (groups below a step), read; drain, exchange
+  constexpr int W_FULL = 0, W_EMPTY = WS, X_FULL = 2 * WS, A_FULL = X_FULL + ST, DONE = A_FULL + ST, D_FULL = DONE + ST,
+                D_EMPTY = D_FULL + 2, DRAIN = D_EMPTY + 2, RED_FULL = DRAIN + 1, RED_FREE = DRAIN + 2;
   static_assert(RED_FREE < Cfg::NBARS, "barriers");
   const uint32_t rank = split > 1 ? cluster_rank() : 0u;
   const int cid = blockIdx.x / split, ncl = gridDim.x / split;
 
   pdl_trigger();
   if (threadIdx.x == 0) {
-    for (int s = 0; s < WS; ++s) { mbar_init(bar(W_FULL + s), 1); mbar_init(bar(W_EMPTY + s), 4); }
-    for (int s = 0; s < XS; ++s) { mbar_init(bar(X_FULL + s), 1); mbar_init(bar(X_EMPTY + s), 1); }
-    for (int s = 0; s < AS; ++s) { mbar_init(bar(A_FULL + s), 4); mbar_init(bar(A_EMPTY + s), 1); }
+    for (int s = 0; s < WS; ++s) { mbar_init(bar(W_FULL + s), 1); mbar_init(bar(W_EMPTY + s), 8); }
+    for (int s = 0; s < ST; ++s) { mbar_init(bar(X_FULL + s), 1); mbar_init(bar(A_FULL + s), 8); mbar_init(bar(DONE + s), 1); }
     for (int s = 0; s < 2; ++s) { mbar_init(bar(D_FULL + s), 1); mbar_init(bar(D_EMPTY + s), 8); }
     mbar_init(bar(DRAIN), 1);
     if (split > 1) {   // lane 0 of each sending warp; of each finishing warp
@@ -174,15 +189,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
   __syncthreads();
   if (split > 1) cluster_sync_all();   // every CTA's barriers are initialised before any remote arrival
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   pdl_wait();
-  int units;   // token tiles of all groups
-  if (a.offsets) {
-    units = unit_table(a, BN, first_unit, row0, scan);
-  } else {
-    units = (a.M + BN - 1) / BN;
-  }
-  const int num_units = units * p.tiles_n;
+  // token tiles of all groups
+  const int units = a.offsets ? unit_table(a, BN, first_unit, row0, scan) : (a.M + BN - 1) / BN;
+  const int num_units = __shfl_sync(0xffffffffu, units * p.tiles_n, 0);
   auto unit_at = [&](int u) {
     // groups in order; within one row tiles outside, up to 16 token tiles inside (concurrent
     // CTAs share weight tiles in L2, and with many token tiles their panels too)
@@ -205,118 +216,127 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
     t.n0 = (w / gsz) * 128;
     return t;
   };
-  // this rank's K-blocks: whole stages of weights
-  const int stages = (p.kb_total + 3) / 4;
-  const int kb0 = (int)((int64_t)rank * stages / split) * 4, kb1 = min(p.kb_total, (int)((int64_t)(rank + 1) * stages / split) * 4);
-  // K-blocks of a sum (1 or 2), or sums of a K-block
-  const bool half = a.group_log2 == 5;
-  const int kb_sum = a.group_log2 >= 7 ? 2 : 1;
+  // this rank's steps: whole stages of weights
+  const int stages = (p.steps + 1) / 2;
+  const int k0 = (int)((int64_t)rank * stages / split) * 2, k1 = min(p.steps, (int)((int64_t)(rank + 1) * stages / split) * 2);
+  // sums of a step
+  const int sums_log2 = max(0, 7 - a.group_log2);
   auto all = [](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ producer
-    if (lane == 0) {
-      int ws = 0, xs = 0, last_w = -1, last_x = -1;
-      uint32_t wp = 0, xp = 0, last_wp = 0, last_xp = 0;
+  if (warp < 4) {
+    regs_dec<TC_REGS_ISSUE>();
+    // Whole warps run these loops and one lane issues: so everything an instruction names is
+    // known to be uniform (an MMA whose operands had to be moved to uniform registers first
+    // took 200 cycles to issue, whatever its size).
+    const bool one = elect_one();
+    if (warp == 0) {
+      // ---------------------------------------------------------- producer
+      int ws = 0, st = 0, last_w = -1, last_x = -1;
+      uint32_t wp = 0, sp = 0, last_wp = 0, last_xp = 0;
       bool ok = true;
       for (int u = cid; u < num_units && ok; u += ncl) {
         const TcTile t = unit_at(u);
-        const int we = a.w_e == 0 ? 0 : t.e;
-        for (int kb = kb0; kb < kb1 && ok; ++kb) {
-          if ((kb & 3) == 0) {
-            if (!mbar_wait(bar(W_EMPTY + ws), wp ^ 1u, abort_flag, p.timeout_ns)) { ok = false; break; }
-            mbar_arrive_expect_tx(bar(W_FULL + ws), TC_W_BYTES);
-            tma_load_3d(smem_u32(smem) + ws * TC_W_BYTES, &p.w, bar(W_FULL + ws), kb * 32, t.n0, we);
+        const int we = a.w_e == 0 ? 0 : __shfl_sync(0xffffffffu, t.e, 0);
+        const int r0 = __shfl_sync(0xffffffffu, t.r0, 0), n0 = __shfl_sync(0xffffffffu, t.n0, 0);
+        for (int k = k0; k < k1; ++k) {
+          if ((k & 1) == 0) {
+            if (!all(mbar_wait(bar(W_EMPTY + ws), wp ^ 1u, abort_flag, p.timeout_ns))) { ok = false; break; }
+            if (one) {
+              mbar_arrive_expect_tx(bar(W_FULL + ws), TC_W_BYTES);
+              tma_load_3d(smem_u32(smem) + ws * TC_W_BYTES, &p.w, bar(W_FULL + ws), k * (TC_STEP / 2), n0, we);
+            }
             last_w = ws;
             last_wp = wp;
             if (++ws == WS) { ws = 0; wp ^= 1u; }
           }
-          if (!mbar_wait(bar(X_EMPTY + xs), xp ^ 1u, abort_flag, p.timeout_ns)) { ok = false; break; }
-          mbar_arrive_expect_tx(bar(X_FULL + xs), Cfg::X_BYTES);
-          tma_load_3d(smem_u32(xring) + xs * Cfg::X_BYTES, &p.x, bar(X_FULL + xs), kb * 64, t.r0, 0);
-          last_x = xs;
-          last_xp = xp;
-          if (++xs == XS) { xs = 0; xp ^= 1u; }
+          if (!all(mbar_wait(bar(DONE + st), sp ^ 1u, abort_flag, p.timeout_ns))) { ok = false; break; }
+          if (one) {
+            mbar_arrive_expect_tx(bar(X_FULL + st), Cfg::X_BYTES);
+            const uint32_t to = smem_u32(xring) + st * Cfg::X_BYTES;
+            tma_load_3d(to, &p.x, bar(X_FULL + st), k * TC_STEP, r0, 0);
+            tma_load_3d(to + BN * 128, &p.x, bar(X_FULL + st), k * TC_STEP + 64, r0, 0);
+          }
+          last_x = st;
+          last_xp = sp;
+          if (++st == ST) { st = 0; sp ^= 1u; }
         }
       }
       // the last copies must land before the CTA can exit
       volatile int no_abort = 0;
       if (last_w >= 0) mbar_wait(bar(W_FULL + last_w), last_wp, &no_abort, p.timeout_ns);
       if (last_x >= 0) mbar_wait(bar(X_FULL + last_x), last_xp, &no_abort, p.timeout_ns);
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
+    } else if (warp == 1) {
+      // ---------------------------------------------------------- MMA issuer
       const uint32_t idesc = make_idesc<T, BN>(0, 0);
-      int xs = 0, as = 0, d = 0;
-      uint32_t xp = 0, ap = 0, dp = 0;
+      const int per_sum = 8 >> sums_log2;   // MMAs of 16 columns
+      int st = 0, d = 0;
+      uint32_t sp = 0, dp = 0;
       bool ok = true, issued = false;
       for (int u = cid; u < num_units && ok; u += ncl) {
-        int in_sum = 0;   // K-blocks of the current sum
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait(bar(X_FULL + xs), xp, abort_flag, p.timeout_ns) ||
-              !mbar_wait(bar(A_FULL + as), ap, abort_flag, p.timeout_ns)) { ok = false; break; }
-          if (in_sum == 0 && !mbar_wait(bar(D_EMPTY + d), dp ^ 1u, abort_flag, p.timeout_ns)) { ok = false; break; }
-          tc_fence_after();
-          const uint32_t at = tmem + TC_A_COL + as * 32, xb = smem_u32(xring) + xs * Cfg::X_BYTES;
+        for (int k = k0; k < k1 && ok; ++k) {
+          if (!all(mbar_wait(bar(X_FULL + st), sp, abort_flag, p.timeout_ns)) ||
+              !all(mbar_wait(bar(A_FULL + st), sp, abort_flag, p.timeout_ns))) { ok = false; break; }
+          const uint32_t at = tmem + TC_A_COL + st * 64;
+          const uint64_t xd = sdesc(smem_u32(xring) + st * Cfg::X_BYTES, 16, 1024);
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {
-            if (half && ks == 2) {   // the second group of the K-block
-              umma_commit(bar(D_FULL + d));
-              if (++d == 2) { d = 0; dp ^= 1u; }
-              if (!mbar_wait(bar(D_EMPTY + d), dp ^ 1u, abort_flag, p.timeout_ns)) { ok = false; break; }
+          for (int ks = 0; ks < 8; ++ks) {
+            if ((ks & (per_sum - 1)) == 0) {
+              if (!all(mbar_wait(bar(D_EMPTY + d), dp ^ 1u, abort_flag, p.timeout_ns))) { ok = false; break; }
               tc_fence_after();
             }
-            umma_ts(tmem + d * BN, at + ks * 8, sdesc(xb + ks * 32, 16, 1024), idesc,
-                    (in_sum > 0 || (half ? ks & 1 : ks) > 0) ? 1u : 0u);
+            // (a descriptor counts shared memory in 16 bytes)
+            if (one) umma_ts(tmem + d * BN, at + ks * 8, xd + ((ks >> 2) * (BN * 128) + (ks & 3) * 32) / 16, idesc,
+                             (ks & (per_sum - 1)) ? 1u : 0u);
+            issued = true;
+            if ((ks & (per_sum - 1)) == per_sum - 1) {
+              if (sums_log2 && one) umma_commit(bar(D_FULL + d));
+              if (++d == 2) { d = 0; dp ^= 1u; }
+            }
           }
-          issued = true;
           if (!ok) break;
-          umma_commit(bar(X_EMPTY + xs));
-          umma_commit(bar(A_EMPTY + as));
-          if (++xs == XS) { xs = 0; xp ^= 1u; }
-          if (++as == AS) { as = 0; ap ^= 1u; }
-          if (++in_sum == kb_sum || kb + 1 == kb1) {
-            umma_commit(bar(D_FULL + d));
-            if (++d == 2) { d = 0; dp ^= 1u; }
-            in_sum = 0;
-          }
+          if (one) umma_commit(bar(DONE + st));
+          if (++st == ST) { st = 0; sp ^= 1u; }
         }
       }
       if (*abort_flag && issued) {
-        umma_commit(bar(DRAIN));
+        if (one) umma_commit(bar(DRAIN));
         volatile int no_abort = 0;
         mbar_wait(bar(DRAIN), 0, &no_abort, p.timeout_ns);
       }
     }
-  } else if (warp < 6) {
+  } else if (warp < 12) {
     // ------------------------------------------------------------ decoding
-    const int q = warp & 3, r = q * 32 + lane;   // this thread's row of the tile, its TMEM lane
-    const uint32_t at = tmem + TC_A_COL + ((uint32_t)(q * 32) << 16);
+    regs_dec<TC_REGS_DECODE>();
+    const int q = warp & 3, hf = (warp - 4) >> 2, r = q * 32 + lane;   // this thread's row of the tile, its TMEM lane
+    const uint32_t at = tmem + TC_A_COL + hf * 32 + ((uint32_t)(q * 32) << 16);
     const uint32_t src = smem_u32(smem) + r * 128;
-    int ws = 0, as = 0;
-    uint32_t wp = 0, ap = 0;
+    int ws = 0, st = 0;
+    uint32_t wp = 0, sp = 0;
     bool ok = true;
     for (int u = cid; u < num_units && ok; u += ncl) {
-      const TcTile t = unit_at(u);
-      const int n = min(t.n0 + r, a.N - 1);
-      const uint8_t *zero = ZERO ? a.zero + t.e * a.z_e + (int64_t)n * a.z_rs : nullptr;
-      uint32_t zn0 = 8, zn1 = 8;   // zero points, one K-block ahead
-      auto fetch_zero = [&](int kb) {
+      uint32_t zn0 = 8, zn1 = 8;   // zero points of 32 columns each, one step ahead
+      const uint8_t *zero = nullptr;
+      auto fetch_zero = [&](int k) {
         if constexpr (ZERO) {
-          zn0 = zero[(kb * 64) >> a.group_log2];
-          zn1 = half && kb * 64 + 32 < a.K ? zero[kb * 2 + 1] : zn0;
+          const int c = k * TC_STEP + hf * 64;
+          zn0 = c < a.K ? zero[c >> a.group_log2] : 8u;
+          zn1 = c + 32 < a.K ? zero[(c + 32) >> a.group_log2] : 8u;
         }
       };
-      if (kb0 < kb1) fetch_zero(kb0);
-      for (int kb = kb0; kb < kb1; ++kb) {
+      if constexpr (ZERO) {
+        const TcTile t = unit_at(u);
+        zero = a.zero + t.e * a.z_e + (int64_t)min(t.n0 + r, a.N - 1) * a.z_rs;
+        if (k0 < k1) fetch_zero(k0);
+      }
+      for (int k = k0; k < k1; ++k) {
         const uint32_t z0 = zn0, z1 = zn1;
-        if (kb + 1 < kb1) fetch_zero(kb + 1);
-        if ((kb & 3) == 0 && !all(mbar_wait(bar(W_FULL + ws), wp, abort_flag, p.timeout_ns))) { ok = false; break; }
+        if (k + 1 < k1) fetch_zero(k + 1);
+        if ((k & 1) == 0 && !all(mbar_wait(bar(W_FULL + ws), wp, abort_flag, p.timeout_ns))) { ok = false; break; }
         const uint32_t row = src + ws * TC_W_BYTES;
-        const uint4 lo = ld_shared_v4(row + ((((kb & 3) * 2) ^ (r & 7)) << 4));
-        const uint4 hi = ld_shared_v4(row + ((((kb & 3) * 2 + 1) ^ (r & 7)) << 4));
-        if ((kb & 3) == 3 || kb + 1 == kb1) {
+        const int ch = (k & 1) * 4 + hf * 2;
+        const uint4 lo = ld_shared_v4(row + ((ch ^ (r & 7)) << 4));
+        const uint4 hi = ld_shared_v4(row + (((ch + 1) ^ (r & 7)) << 4));
+        if ((k & 1) || k + 1 == k1) {
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(W_EMPTY + ws));
           if (++ws == WS) { ws = 0; wp ^= 1u; }
@@ -325,26 +345,27 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
         const InOrder<T, ZERO> d0(z0), d1(z1);
         d0(lo.x, o); d0(lo.y, o + 4); d0(lo.z, o + 8); d0(lo.w, o + 12);
         d1(hi.x, o + 16); d1(hi.y, o + 20); d1(hi.z, o + 24); d1(hi.w, o + 28);
-        if (!all(mbar_wait(bar(A_EMPTY + as), ap ^ 1u, abort_flag, p.timeout_ns))) { ok = false; break; }
+        if (!all(mbar_wait(bar(DONE + st), sp ^ 1u, abort_flag, p.timeout_ns))) { ok = false; break; }
         tc_fence_after();
-        tmem_st_x32(at + as * 32, o);
+        tmem_st_x32(at + st * 64, o);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(A_FULL + as));
-        if (++as == AS) { as = 0; ap ^= 1u; }
+        if (lane == 0) mbar_arrive(bar(A_FULL + st));
+        if (++st == ST) { st = 0; sp ^= 1u; }
       }
     }
   } else {
     // ------------------------------------------------------------ sums and output
-    const int q = warp & 3, hf = (warp - 6) >> 2, r = q * 32 + lane;
+    regs_inc<TC_REGS_SUM>();
+    const int q = warp & 3, hf = (warp - 12) >> 2, r = q * 32 + lane;
     T *out = static_cast<T *>(a.out);
     const int piece = q * 2 + hf, per_rank = 8 / split, owner = piece / per_rank;
     const uint32_t red_u32 = smem_u32(red) + (uint32_t)(piece % per_rank) * Cfg::PIECE + lane * 16u;
     const uint32_t red_step = (uint32_t)(per_rank * Cfg::PIECE);   // from one source rank to the next
-    const int sum_log2 = min(a.group_log2, 7), k1 = min(a.K, kb1 * 64);
-    int d = 0;
-    uint32_t dp = 0, rphase = 0;
+    const int sum_log2 = min(a.group_log2, 7), end = min(a.K, k1 * TC_STEP);
+    int d = 0, st = 0;
+    uint32_t dp = 0, sp = 0, rphase = 0;
     bool first = true, ok = true;
     for (int u = cid; u < num_units && ok; u += ncl) {
       const TcTile t = unit_at(u);
@@ -353,12 +374,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
       float acc[CW];
 #pragma unroll
       for (int j = 0; j < CW; ++j) acc[j] = 0.f;
-      uint32_t bits = kb0 < kb1 ? scale_bits<T>(a, i_s + ((kb0 * 64) >> a.group_log2)) : 0u;
-      for (int k = kb0 * 64; k < kb1 * 64; k += 1 << sum_log2) {
-        const float s = k < k1 ? scale_of<T>(a, bits) : 0.f;
+      uint32_t bits = k0 < k1 ? scale_bits<T>(a, i_s + ((k0 * TC_STEP) >> a.group_log2)) : 0u;
+      for (int k = k0 * TC_STEP; k < k1 * TC_STEP; k += 1 << sum_log2) {
+        const float s = k < end ? scale_of<T>(a, bits) : 0.f;
         const int next = k + (1 << sum_log2);
-        if (next < k1) bits = scale_bits<T>(a, i_s + (next >> a.group_log2));
-        if (!all(mbar_wait(bar(D_FULL + d), dp, abort_flag, p.timeout_ns))) { ok = false; break; }
+        if (next < end) bits = scale_bits<T>(a, i_s + (next >> a.group_log2));
+        if (sums_log2) {
+          if (!all(mbar_wait(bar(D_FULL + d), dp, abort_flag, p.timeout_ns))) { ok = false; break; }
+        } else {
+          if (!all(mbar_wait(bar(DONE + st), sp, abort_flag, p.timeout_ns))) { ok = false; break; }
+          if (++st == ST) { st = 0; sp ^= 1u; }
+        }
         tc_fence_after();
         const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + d * BN + hf * CW;
         constexpr int CH = CW < 32 ? CW : 32;
@@ -426,7 +452,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
         }
       }
     }
-    if (a.offsets) zero_rest<T>(a, row0[a.groups], threadIdx.x - 6 * 32, 8 * 32);
+    if (a.offsets) zero_rest<T>(a, row0[a.groups], threadIdx.x - 12 * 32, 8 * 32);
   }
 
   tc_fence_before();
