@@ -225,83 +225,84 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
 
   if (warp < 4) {
     regs_dec<TC_REGS_ISSUE>();
-    // Whole warps run these loops and one lane issues: so everything an instruction names is
-    // known to be uniform (an MMA whose operands had to be moved to uniform registers first
-    // took 200 cycles to issue, whatever its size).
-    const bool one = elect_one();
+    // One elected lane runs these loops: the compiler then knows that all that an instruction
+    // names is uniform (with `lane == 0` every MMA had its operands moved to uniform registers
+    // first and took 200 cycles to issue, whatever its size).
     if (warp == 0) {
       // ---------------------------------------------------------- producer
-      int ws = 0, st = 0, last_w = -1, last_x = -1;
-      uint32_t wp = 0, sp = 0, last_wp = 0, last_xp = 0;
-      bool ok = true;
-      for (int u = cid; u < num_units && ok; u += ncl) {
-        const TcTile t = unit_at(u);
-        const int we = a.w_e == 0 ? 0 : __shfl_sync(0xffffffffu, t.e, 0);
-        const int r0 = __shfl_sync(0xffffffffu, t.r0, 0), n0 = __shfl_sync(0xffffffffu, t.n0, 0);
-        for (int k = k0; k < k1; ++k) {
-          if ((k & 1) == 0) {
-            if (!all(mbar_wait(bar(W_EMPTY + ws), wp ^ 1u, abort_flag, p.timeout_ns))) { ok = false; break; }
-            if (one) {
+      if (elect_one()) {
+        int ws = 0, st = 0, last_w = -1, last_x = -1;
+        uint32_t wp = 0, sp = 0, last_wp = 0, last_xp = 0;
+        bool ok = true;
+        for (int u = cid; u < num_units && ok; u += ncl) {
+          const TcTile t = unit_at(u);
+          const int we = a.w_e == 0 ? 0 : t.e;
+          for (int k = k0; k < k1; ++k) {
+            if ((k & 1) == 0) {
+              if (!mbar_wait(bar(W_EMPTY + ws), wp ^ 1u, abort_flag, p.timeout_ns)) { ok = false; break; }
               mbar_arrive_expect_tx(bar(W_FULL + ws), TC_W_BYTES);
-              tma_load_3d(smem_u32(smem) + ws * TC_W_BYTES, &p.w, bar(W_FULL + ws), k * (TC_STEP / 2), n0, we);
+              tma_load_3d(smem_u32(smem) + ws * TC_W_BYTES, &p.w, bar(W_FULL + ws), k * (TC_STEP / 2), t.n0, we);
+              last_w = ws;
+              last_wp = wp;
+              if (++ws == WS) { ws = 0; wp ^= 1u; }
             }
-            last_w = ws;
-            last_wp = wp;
-            if (++ws == WS) { ws = 0; wp ^= 1u; }
-          }
-          if (!all(mbar_wait(bar(DONE + st), sp ^ 1u, abort_flag, p.timeout_ns))) { ok = false; break; }
-          if (one) {
+            if (!mbar_wait(bar(DONE + st), sp ^ 1u, abort_flag, p.timeout_ns)) { ok = false; break; }
             mbar_arrive_expect_tx(bar(X_FULL + st), Cfg::X_BYTES);
             const uint32_t to = smem_u32(xring) + st * Cfg::X_BYTES;
-            tma_load_3d(to, &p.x, bar(X_FULL + st), k * TC_STEP, r0, 0);
-            tma_load_3d(to + BN * 128, &p.x, bar(X_FULL + st), k * TC_STEP + 64, r0, 0);
+            tma_load_3d(to, &p.x, bar(X_FULL + st), k * TC_STEP, t.r0, 0);
+            tma_load_3d(to + BN * 128, &p.x, bar(X_FULL + st), k * TC_STEP + 64, t.r0, 0);
+            last_x = st;
+            last_xp = sp;
+            if (++st == ST) { st = 0; sp ^= 1u; }
           }
-          last_x = st;
-          last_xp = sp;
-          if (++st == ST) { st = 0; sp ^= 1u; }
         }
+        // the last copies must land before the CTA can exit
+        volatile int no_abort = 0;
+        if (last_w >= 0) mbar_wait(bar(W_FULL + last_w), last_wp, &no_abort, p.timeout_ns);
+        if (last_x >= 0) mbar_wait(bar(X_FULL + last_x), last_xp, &no_abort, p.timeout_ns);
       }
-      // the last copies must land before the CTA can exit
-      volatile int no_abort = 0;
-      if (last_w >= 0) mbar_wait(bar(W_FULL + last_w), last_wp, &no_abort, p.timeout_ns);
-      if (last_x >= 0) mbar_wait(bar(X_FULL + last_x), last_xp, &no_abort, p.timeout_ns);
     } else if (warp == 1) {
       // ---------------------------------------------------------- MMA issuer
-      const uint32_t idesc = make_idesc<T, BN>(0, 0);
-      const int per_sum = 8 >> sums_log2;   // MMAs of 16 columns
-      int st = 0, d = 0;
-      uint32_t sp = 0, dp = 0;
-      bool ok = true, issued = false;
-      for (int u = cid; u < num_units && ok; u += ncl) {
-        for (int k = k0; k < k1 && ok; ++k) {
-          if (!all(mbar_wait(bar(X_FULL + st), sp, abort_flag, p.timeout_ns)) ||
-              !all(mbar_wait(bar(A_FULL + st), sp, abort_flag, p.timeout_ns))) { ok = false; break; }
-          const uint32_t at = tmem + TC_A_COL + st * 64;
-          const uint64_t xd = sdesc(smem_u32(xring) + st * Cfg::X_BYTES, 16, 1024);
+      if (elect_one()) {
+        const uint32_t idesc = make_idesc<T, BN>(0, 0);
+        int st = 0, d = 0;
+        uint32_t sp = 0, dp = 0;
+        bool issued = false;
+        // PER: MMAs of 16 columns in a sum.  Known here, so that a sum's MMAs follow one another: this
+        // warp shares its issue slots with busy ones, and 15 instructions an MMA were 125 cycles.
+        auto issue = [&](auto per) {
+          constexpr int PER = decltype(per)::value;
+          for (int u = cid; u < num_units; u += ncl) {
+            for (int k = k0; k < k1; ++k) {
+              const uint32_t at = tmem + TC_A_COL + st * 64;
+              const uint64_t xd = sdesc(smem_u32(xring) + st * Cfg::X_BYTES, 16, 1024);
+              if (!mbar_wait(bar(X_FULL + st), sp, abort_flag, p.timeout_ns) ||
+                  !mbar_wait(bar(A_FULL + st), sp, abort_flag, p.timeout_ns))
+                return;
 #pragma unroll
-          for (int ks = 0; ks < 8; ++ks) {
-            if ((ks & (per_sum - 1)) == 0) {
-              if (!all(mbar_wait(bar(D_EMPTY + d), dp ^ 1u, abort_flag, p.timeout_ns))) { ok = false; break; }
-              tc_fence_after();
-            }
-            // (a descriptor counts shared memory in 16 bytes)
-            if (one) umma_ts(tmem + d * BN, at + ks * 8, xd + ((ks >> 2) * (BN * 128) + (ks & 3) * 32) / 16, idesc,
-                             (ks & (per_sum - 1)) ? 1u : 0u);
-            issued = true;
-            if ((ks & (per_sum - 1)) == per_sum - 1) {
-              if (sums_log2 && one) umma_commit(bar(D_FULL + d));
-              if (++d == 2) { d = 0; dp ^= 1u; }
+              for (int s = 0; s < 8; s += PER) {
+                if (!mbar_wait(bar(D_EMPTY + d), dp ^ 1u, abort_flag, p.timeout_ns)) return;
+                tc_fence_after();
+                issued = true;
+#pragma unroll
+                for (int ks = s; ks < s + PER; ++ks)   // (a descriptor counts shared memory in 16 bytes)
+                  umma_ts(tmem + d * BN, at + ks * 8, xd + ((ks >> 2) * (BN * 128) + (ks & 3) * 32) / 16, idesc, ks > s ? 1u : 0u);
+                if (PER < 8) umma_commit(bar(D_FULL + d));
+                if (++d == 2) { d = 0; dp ^= 1u; }
+              }
+              umma_commit(bar(DONE + st));
+              if (++st == ST) { st = 0; sp ^= 1u; }
             }
           }
-          if (!ok) break;
-          if (one) umma_commit(bar(DONE + st));
-          if (++st == ST) { st = 0; sp ^= 1u; }
+        };
+        if (sums_log2 == 0) issue(std::integral_constant<int, 8>());
+        else if (sums_log2 == 1) issue(std::integral_constant<int, 4>());
+        else issue(std::integral_constant<int, 2>());
+        if (*abort_flag && issued) {
+          umma_commit(bar(DRAIN));
+          volatile int no_abort = 0;
+          mbar_wait(bar(DRAIN), 0, &no_abort, p.timeout_ns);
         }
-      }
-      if (*abort_flag && issued) {
-        if (one) umma_commit(bar(DRAIN));
-        volatile int no_abort = 0;
-        mbar_wait(bar(DRAIN), 0, &no_abort, p.timeout_ns);
       }
     }
   } else if (warp < 12) {
