@@ -41,24 +41,27 @@ constexpr int TC_W_BYTES = 128 * 128;    // weights of a stage: 128 rows x 256 c
 constexpr int TC_STEP = 128;             // columns of K of a step
 constexpr int TC_STEPS = 4;              // steps held: tokens in shared memory, decoded weights in TMEM
 constexpr int TC_A_COL = 256;            // first TMEM column of the weights, 64 columns a step
-// Registers of a thread: 128 x 40 + 256 x 72 + 256 x 144 of the 640 x 96 at launch.
-constexpr int TC_REGS_ISSUE = 40, TC_REGS_DECODE = 72, TC_REGS_SUM = 144;
+// Registers of a thread: 128 x 32 + 256 x 72 + 256 x 152 of the 640 x 96 at launch.
+constexpr int TC_REGS_ISSUE = 32, TC_REGS_DECODE = 72, TC_REGS_SUM = 152;
 static_assert(128 * TC_REGS_ISSUE + 256 * TC_REGS_DECODE + 256 * TC_REGS_SUM <= TC_THREADS * 96, "registers at launch");
 
 struct TcArgs {
   CUtensorMap w, x;
   GemmArgs g;
   int tiles_n, split, steps;             // steps of the whole of K
+  int out_vec;                           // rows of out start on 16 bytes
   unsigned long long timeout_ns;
 };
 
 template <int BN> struct TcCfg {
   static constexpr int X_BYTES = BN * 256;          // two boxes of 64 columns
   static constexpr int W_STAGES = BN == 128 ? 2 : 6;
+  static constexpr int D_BUFS = BN == 128 ? 2 : 4;  // accumulators
   static constexpr int CW = BN / 2;                 // columns of a warp of sums
-  static constexpr int PIECE = 32 * CW * 4;
-  static __host__ __device__ constexpr int red_bytes(int split) { return (split - 1) * (8 / split) * PIECE; }
-  static constexpr int NBARS = 2 * W_STAGES + 3 * TC_STEPS + 7;
+  static constexpr int PIECE = 32 * CW * 4;         // its sums; its results are half as many bytes
+  // sums from other ranks, or results on their way out
+  static __host__ __device__ constexpr int red_bytes(int split) { return split > 1 ? (split - 1) * (8 / split) * PIECE : 4 * PIECE; }
+  static constexpr int NBARS = 2 * W_STAGES + 3 * TC_STEPS + 2 * D_BUFS + 3;
   static constexpr int smem(int split, int groups) {
     return 1024 + W_STAGES * TC_W_BYTES + TC_STEPS * X_BYTES + red_bytes(split) + (NBARS + 2) * 8 + (2 * (groups + 1) + 32) * 4;
   }
@@ -98,7 +101,7 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 // two neighbours, and (b * 0x1001) & 0x000f000f is the pair (the multiplication
 // runs beside the logic pipe, which binds the decoding).
 __device__ __forceinline__ uint32_t byte_pair(uint32_t w, int i) {
-  const uint32_t b = i == 0 ? w & 0xffu : i == 3 ? w >> 24 : (w >> (8 * i)) & 0xffu;
+  const uint32_t b = i == 0 ? w & 0xffu : i == 3 ? w >> 24 : __byte_perm(w, 0, 0x4440 + i);
   return (b * 0x1001u) & 0x000f000fu;
 }
 template <class T, bool ZERO> struct InOrder;
@@ -142,7 +145,7 @@ struct TcTile {
 template <class T, int BN, bool ZERO>
 __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_constant__ TcArgs p) {
   using Cfg = TcCfg<BN>;
-  constexpr int WS = Cfg::W_STAGES, ST = TC_STEPS, CW = Cfg::CW;
+  constexpr int WS = Cfg::W_STAGES, ST = TC_STEPS, CW = Cfg::CW, DB = Cfg::D_BUFS;
   const GemmArgs &a = p.g;
   const int split = p.split;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -161,7 +164,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
   // barriers: weights full, empty; a step's tokens full, its weights decoded, its MMA done;
   // an accumulator's sum done (groups below a step), read; drain, exchange
   constexpr int W_FULL = 0, W_EMPTY = WS, X_FULL = 2 * WS, A_FULL = X_FULL + ST, DONE = A_FULL + ST, D_FULL = DONE + ST,
-                D_EMPTY = D_FULL + 2, DRAIN = D_EMPTY + 2, RED_FULL = DRAIN + 1, RED_FREE = DRAIN + 2;
+                D_EMPTY = D_FULL + DB, DRAIN = D_EMPTY + DB, RED_FULL = DRAIN + 1, RED_FREE = DRAIN + 2;
   static_assert(RED_FREE < Cfg::NBARS, "barriers");
   const uint32_t rank = split > 1 ? cluster_rank() : 0u;
   const int cid = blockIdx.x / split, ncl = gridDim.x / split;
@@ -170,7 +173,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
   if (threadIdx.x == 0) {
     for (int s = 0; s < WS; ++s) { mbar_init(bar(W_FULL + s), 1); mbar_init(bar(W_EMPTY + s), 8); }
     for (int s = 0; s < ST; ++s) { mbar_init(bar(X_FULL + s), 1); mbar_init(bar(A_FULL + s), 8); mbar_init(bar(DONE + s), 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(bar(D_FULL + s), 1); mbar_init(bar(D_EMPTY + s), 8); }
+    for (int s = 0; s < DB; ++s) { mbar_init(bar(D_FULL + s), 1); mbar_init(bar(D_EMPTY + s), 8); }
     mbar_init(bar(DRAIN), 1);
     if (split > 1) {   // lane 0 of each sending warp; of each finishing warp
       mbar_init(bar(RED_FULL), (split - 1) * (8 / split));
@@ -288,7 +291,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
                 for (int ks = s; ks < s + PER; ++ks)   // (a descriptor counts shared memory in 16 bytes)
                   umma_ts(tmem + d * BN, at + ks * 8, xd + ((ks >> 2) * (BN * 128) + (ks & 3) * 32) / 16, idesc, ks > s ? 1u : 0u);
                 if (PER < 8) umma_commit(bar(D_FULL + d));
-                if (++d == 2) { d = 0; dp ^= 1u; }
+                if (++d == DB) { d = 0; dp ^= 1u; }
               }
               umma_commit(bar(DONE + st));
               if (++st == ST) { st = 0; sp ^= 1u; }
@@ -313,40 +316,42 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
     const uint32_t src = smem_u32(smem) + r * 128;
     int ws = 0, st = 0;
     uint32_t wp = 0, sp = 0;
-    bool ok = true;
-    for (int u = cid; u < num_units && ok; u += ncl) {
-      uint32_t zn0 = 8, zn1 = 8;   // zero points of 32 columns each, one step ahead
-      const uint8_t *zero = nullptr;
-      auto fetch_zero = [&](int k) {
-        if constexpr (ZERO) {
-          const int c = k * TC_STEP + hf * 64;
-          zn0 = c < a.K ? zero[c >> a.group_log2] : 8u;
-          zn1 = c + 32 < a.K ? zero[(c + 32) >> a.group_log2] : 8u;
-        }
-      };
+    // this thread's words and zero points (of 32 columns each) of the next step
+    uint4 lo, hi;
+    uint32_t z0 = 8, z1 = 8;
+    const uint8_t *zero = nullptr;
+    auto fetch = [&](int u, int k) {
       if constexpr (ZERO) {
-        const TcTile t = unit_at(u);
-        zero = a.zero + t.e * a.z_e + (int64_t)min(t.n0 + r, a.N - 1) * a.z_rs;
-        if (k0 < k1) fetch_zero(k0);
-      }
-      for (int k = k0; k < k1; ++k) {
-        const uint32_t z0 = zn0, z1 = zn1;
-        if (k + 1 < k1) fetch_zero(k + 1);
-        if ((k & 1) == 0 && !all(mbar_wait(bar(W_FULL + ws), wp, abort_flag, p.timeout_ns))) { ok = false; break; }
-        const uint32_t row = src + ws * TC_W_BYTES;
-        const int ch = (k & 1) * 4 + hf * 2;
-        const uint4 lo = ld_shared_v4(row + ((ch ^ (r & 7)) << 4));
-        const uint4 hi = ld_shared_v4(row + (((ch + 1) ^ (r & 7)) << 4));
-        if ((k & 1) || k + 1 == k1) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(W_EMPTY + ws));
-          if (++ws == WS) { ws = 0; wp ^= 1u; }
+        if (k == k0) {
+          const TcTile t = unit_at(u);
+          zero = a.zero + t.e * a.z_e + (int64_t)min(t.n0 + r, a.N - 1) * a.z_rs;
         }
+        const int c = k * TC_STEP + hf * 64;
+        z0 = c < a.K ? zero[c >> a.group_log2] : 8u;
+        z1 = c + 32 < a.K ? zero[(c + 32) >> a.group_log2] : 8u;
+      }
+      if ((k & 1) == 0 && !all(mbar_wait(bar(W_FULL + ws), wp, abort_flag, p.timeout_ns))) return false;
+      const uint32_t row = src + ws * TC_W_BYTES;
+      const int ch = (k & 1) * 4 + hf * 2;
+      lo = ld_shared_v4(row + ((ch ^ (r & 7)) << 4));
+      hi = ld_shared_v4(row + (((ch + 1) ^ (r & 7)) << 4));
+      if ((k & 1) || k + 1 == k1) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(W_EMPTY + ws));
+        if (++ws == WS) { ws = 0; wp ^= 1u; }
+      }
+      return true;
+    };
+    bool ok = cid < num_units && k0 < k1 && fetch(cid, k0);
+    for (int u = cid; u < num_units && ok; u += ncl) {
+      for (int k = k0; k < k1; ++k) {
         uint32_t o[32];
         const InOrder<T, ZERO> d0(z0), d1(z1);
         d0(lo.x, o); d0(lo.y, o + 4); d0(lo.z, o + 8); d0(lo.w, o + 12);
         d1(hi.x, o + 16); d1(hi.y, o + 20); d1(hi.z, o + 24); d1(hi.w, o + 28);
-        if (!all(mbar_wait(bar(DONE + st), sp ^ 1u, abort_flag, p.timeout_ns))) { ok = false; break; }
+        if (k + 1 < k1) ok = fetch(u, k + 1);
+        else if (u + ncl < num_units) ok = fetch(u + ncl, k0);
+        if (!ok || !all(mbar_wait(bar(DONE + st), sp ^ 1u, abort_flag, p.timeout_ns))) { ok = false; break; }
         tc_fence_after();
         tmem_st_x32(at + st * 64, o);
         tmem_wait_st();
@@ -364,50 +369,66 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
     const int piece = q * 2 + hf, per_rank = 8 / split, owner = piece / per_rank;
     const uint32_t red_u32 = smem_u32(red) + (uint32_t)(piece % per_rank) * Cfg::PIECE + lane * 16u;
     const uint32_t red_step = (uint32_t)(per_rank * Cfg::PIECE);   // from one source rank to the next
-    const int sum_log2 = min(a.group_log2, 7), end = min(a.K, k1 * TC_STEP);
+    const int sum_log2 = min(a.group_log2, 7), end = min(a.K, k1 * TC_STEP), stop = k1 * TC_STEP;
     int d = 0, st = 0;
     uint32_t dp = 0, sp = 0, rphase = 0;
     bool first = true, ok = true;
+    // the row's scales of the next AHEAD sums, as they lie in memory (converted when they are
+    // used, or the first would be waited for at once)
+    constexpr int AHEAD = 4;
+    uint32_t next[AHEAD];
+    auto fetch = [&](int u, int k) {
+      const TcTile t = unit_at(u);
+      const int64_t i_s = t.e * a.s_e + (int64_t)min(t.n0 + r, a.N - 1) * a.s_rs;
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) next[i] = k + (i << sum_log2) < end ? scale_bits<T>(a, i_s + ((k + (i << sum_log2)) >> a.group_log2)) : 0u;
+    };
+    if (cid < num_units) fetch(cid, k0 * TC_STEP);
     for (int u = cid; u < num_units && ok; u += ncl) {
       const TcTile t = unit_at(u);
       const int64_t n = t.n0 + r;
-      const int64_t i_s = t.e * a.s_e + min(n, (int64_t)a.N - 1) * a.s_rs;
       float acc[CW];
 #pragma unroll
       for (int j = 0; j < CW; ++j) acc[j] = 0.f;
-      uint32_t bits = k0 < k1 ? scale_bits<T>(a, i_s + ((k0 * TC_STEP) >> a.group_log2)) : 0u;
-      for (int k = k0 * TC_STEP; k < k1 * TC_STEP; k += 1 << sum_log2) {
-        const float s = k < end ? scale_of<T>(a, bits) : 0.f;
-        const int next = k + (1 << sum_log2);
-        if (next < end) bits = scale_bits<T>(a, i_s + (next >> a.group_log2));
-        if (sums_log2) {
-          if (!all(mbar_wait(bar(D_FULL + d), dp, abort_flag, p.timeout_ns))) { ok = false; break; }
-        } else {
-          if (!all(mbar_wait(bar(DONE + st), sp, abort_flag, p.timeout_ns))) { ok = false; break; }
-          if (++st == ST) { st = 0; sp ^= 1u; }
-        }
-        tc_fence_after();
-        const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + d * BN + hf * CW;
-        constexpr int CH = CW < 32 ? CW : 32;
+      for (int k = k0 * TC_STEP; k < stop && ok;) {
+        float s[AHEAD];
 #pragma unroll
-        for (int c = 0; c < CW; c += CH) {
-          uint32_t v[32];
-          tmem_ld<CH>(from + c, v);
-          tmem_wait_ld();
-          if (c + CH >= CW) {   // the accumulator is read
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(D_EMPTY + d));
-          }
+        for (int i = 0; i < AHEAD; ++i) s[i] = scale_of<T>(a, next[i]);
+        if (k + (AHEAD << sum_log2) < stop) fetch(u, k + (AHEAD << sum_log2));
+        else if (u + ncl < num_units) fetch(u + ncl, k0 * TC_STEP);
 #pragma unroll
-          for (int j = 0; j < CH; j += 2) {
-            const float2 o = fma2(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), make_float2(s, s),
-                                  make_float2(acc[c + j], acc[c + j + 1]));
-            acc[c + j] = o.x;
-            acc[c + j + 1] = o.y;
+        for (int i = 0; i < AHEAD; ++i, k += 1 << sum_log2) {
+          if (k >= stop) break;
+          if (sums_log2) {
+            if (!all(mbar_wait(bar(D_FULL + d), dp, abort_flag, p.timeout_ns))) { ok = false; break; }
+          } else {
+            if (!all(mbar_wait(bar(DONE + st), sp, abort_flag, p.timeout_ns))) { ok = false; break; }
+            if (++st == ST) { st = 0; sp ^= 1u; }
           }
+          tc_fence_after();
+          const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + d * BN + hf * CW;
+          constexpr int CH = CW < 32 ? CW : 32;
+          const float2 s2 = make_float2(s[i], s[i]);
+#pragma unroll
+          for (int c = 0; c < CW; c += CH) {
+            uint32_t v[32];
+            tmem_ld<CH>(from + c, v);
+            tmem_wait_ld();
+            if (c + CH >= CW) {   // the accumulator is read
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bar(D_EMPTY + d));
+            }
+#pragma unroll
+            for (int j = 0; j < CH; j += 2) {
+              const float2 o = fma2(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), s2,
+                                    make_float2(acc[c + j], acc[c + j + 1]));
+              acc[c + j] = o.x;
+              acc[c + j + 1] = o.y;
+            }
+          }
+          if (++d == DB) { d = 0; dp ^= 1u; }
         }
-        if (++d == 2) { d = 0; dp ^= 1u; }
       }
       if (!ok) break;
       if (split > 1) {
@@ -435,23 +456,34 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
               acc[j + 3] += __uint_as_float(v.w);
             }
           }
+        }
+      }
+      if (split == 1 || owner == (int)rank) {
+        // Lanes hold rows of the weights, columns of the output: transposed through this warp's own
+        // shared memory (its sums of the other ranks have been read), so that rows leave in
+        // whole 16 bytes where they lie on them.
+        const float b = a.bias && n < a.N ? bias_at<T>(a, n) : 0.f;
+        T *stage = reinterpret_cast<T *>(split > 1 ? red + (piece % per_rank) * Cfg::PIECE : red + piece * (Cfg::PIECE / 2));
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < CW; ++j) stage[j * 32 + lane] = Elem<T>::store(acc[j] + b);
+        __syncwarp();
+        const int64_t m = t.r0 + hf * CW, nw = t.n0 + q * 32;
+        const int live = (int)min((int64_t)CW, t.rend - m);
+        T *dst = out + m * a.out_rs + nw;
+        if (p.out_vec && nw + 32 <= a.N) {
+          for (int j = lane >> 2; j < live; j += 8)
+            *reinterpret_cast<uint4 *>(dst + j * a.out_rs + (lane & 3) * 8) = *reinterpret_cast<const uint4 *>(stage + j * 32 + (lane & 3) * 8);
+        } else if (n < a.N) {
+          for (int j = 0; j < live; ++j) dst[j * a.out_rs + lane] = stage[j * 32 + lane];
+        }
+        if (split > 1) {
           __syncwarp();
           if (lane < split && lane != (int)rank) mbar_arrive_cluster(mapa_shared(bar(RED_FREE), (uint32_t)lane));
         }
-        rphase ^= 1u;
-        first = false;
       }
-      if (split == 1 || owner == (int)rank) {
-        const float b = a.bias && n < a.N ? bias_at<T>(a, n) : 0.f;
-        if (n < a.N) {
-          const int64_t m = t.r0 + hf * CW;
-          const int live = (int)min((int64_t)CW, t.rend - m);
-          T *dst = out + m * a.out_rs + n;
-#pragma unroll
-          for (int j = 0; j < CW; ++j)
-            if (j < live) dst[j * a.out_rs] = Elem<T>::store(acc[j] + b);
-        }
-      }
+      rphase ^= 1u;
+      first = false;
     }
     if (a.offsets) zero_rest<T>(a, row0[a.groups], threadIdx.x - 12 * 32, 8 * 32);
   }

@@ -255,6 +255,7 @@ int gemm_launch(const mb_int4_desc *d, const Plan &pl, cudaStream_t st) {
   p.g = a;
   p.tiles_n = (int)ceil_div(d->N, 128);
   p.steps = (int)ceil_div(d->K, i4::TC_STEP);
+  p.out_vec = rows16(d->out, d->M, d->out_rs, 2);
   p.timeout_ns = wait_timeout_ns();
   const int64_t bytes = (d->K + 1) / 2;
   int rc = encode_map(&p.w, MB_U8, a.w, bytes, d->N, nw, d->N == 1 ? round_up(bytes, 16) : a.w_rs, a.w_e, 128, 128);
