@@ -377,15 +377,19 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
     // used, or the first would be waited for at once)
     constexpr int AHEAD = 4;
     uint32_t next[AHEAD];
-    auto fetch = [&](int u, int k) {
-      const TcTile t = unit_at(u);
+    auto fetch = [&](const TcTile &t, int k) {
       const int64_t i_s = t.e * a.s_e + (int64_t)min(t.n0 + r, a.N - 1) * a.s_rs;
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) next[i] = k + (i << sum_log2) < end ? scale_bits<T>(a, i_s + ((k + (i << sum_log2)) >> a.group_log2)) : 0u;
     };
-    if (cid < num_units) fetch(cid, k0 * TC_STEP);
+    TcTile t, following;
+    if (cid < num_units) {
+      following = unit_at(cid);
+      fetch(following, k0 * TC_STEP);
+    }
     for (int u = cid; u < num_units && ok; u += ncl) {
-      const TcTile t = unit_at(u);
+      t = following;
+      if (u + ncl < num_units) following = unit_at(u + ncl);
       const int64_t n = t.n0 + r;
       float acc[CW];
 #pragma unroll
@@ -394,8 +398,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
         float s[AHEAD];
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) s[i] = scale_of<T>(a, next[i]);
-        if (k + (AHEAD << sum_log2) < stop) fetch(u, k + (AHEAD << sum_log2));
-        else if (u + ncl < num_units) fetch(u + ncl, k0 * TC_STEP);
+        if (k + (AHEAD << sum_log2) < stop) fetch(t, k + (AHEAD << sum_log2));
+        else if (u + ncl < num_units) fetch(following, k0 * TC_STEP);
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i, k += 1 << sum_log2) {
           if (k >= stop) break;
