@@ -35,15 +35,9 @@ namespace i4 {
 
 using namespace mb::tc;
 
-constexpr int TC_WARPS = 20;
-constexpr int TC_THREADS = TC_WARPS * 32;
 constexpr int TC_W_BYTES = 128 * 128;    // weights of a stage: 128 rows x 256 columns
 constexpr int TC_STEP = 128;             // columns of K of a step
-constexpr int TC_STEPS = 4;              // steps held: tokens in shared memory, decoded weights in TMEM
 constexpr int TC_A_COL = 256;            // first TMEM column of the weights, 64 columns a step
-// Registers of a thread: 128 x 32 + 256 x 72 + 256 x 152 of the 640 x 96 at launch.
-constexpr int TC_REGS_ISSUE = 32, TC_REGS_DECODE = 72, TC_REGS_SUM = 152;
-static_assert(128 * TC_REGS_ISSUE + 256 * TC_REGS_DECODE + 256 * TC_REGS_SUM <= TC_THREADS * 96, "registers at launch");
 
 struct TcArgs {
   CUtensorMap w, x;
@@ -54,18 +48,30 @@ struct TcArgs {
 };
 
 template <int BN> struct TcCfg {
-  static constexpr int X_BYTES = BN * 256;          // two boxes of 64 columns
-  static constexpr int W_STAGES = BN == 128 ? 2 : 6;
-  static constexpr int D_BUFS = BN == 128 ? 2 : 4;  // accumulators
-  static constexpr int CW = BN / 2;                 // columns of a warp of sums
+  static constexpr int TILES = BN == 256 ? 2 : 1;   // MMAs that share a step's weights
+  static constexpr int UN = BN / TILES;             // their columns
+  static constexpr int STEPS = BN == 256 ? 2 : 4;   // steps held: tokens in shared memory, decoded weights in TMEM
+  static constexpr int DECODERS = BN == 256 ? 4 : 8;
+  static constexpr int SUM0 = 4 + DECODERS;         // first warp of the sums
+  static constexpr int THREADS = (SUM0 + 8) * 32;
+  // registers of a thread at launch (all of the SM's, in eights) and by role
+  static constexpr int REGS = 65536 / THREADS / 8 * 8;
+  static constexpr int REGS_ISSUE = 32, REGS_DECODE = BN == 256 ? 80 : 72, REGS_SUM = BN == 256 ? 192 : 152;
+  static_assert(128 * REGS_ISSUE + DECODERS * 32 * REGS_DECODE + 256 * REGS_SUM <= THREADS * REGS, "registers at launch");
+  static constexpr int X_TILE = UN * 128;           // a box of 64 columns
+  static constexpr int X_BYTES = TILES * 2 * X_TILE;
+  static constexpr int W_STAGES = BN >= 128 ? 2 : 6;
+  static constexpr int D_BUFS = UN == 128 ? 2 : 4;  // accumulators
+  static constexpr int CW = UN / 2;                 // columns of a warp of sums
   static constexpr int PIECE = 32 * CW * 4;         // its sums; its results are half as many bytes
   // sums from other ranks, or results on their way out
   static __host__ __device__ constexpr int red_bytes(int split) { return split > 1 ? (split - 1) * (8 / split) * PIECE : 4 * PIECE; }
-  static constexpr int NBARS = 2 * W_STAGES + 3 * TC_STEPS + 2 * D_BUFS + 3;
+  static constexpr int MAX_SPLIT = BN == 256 ? 1 : 8;
+  static constexpr int NBARS = 2 * W_STAGES + 3 * STEPS + 2 * D_BUFS + 3;
   static constexpr int smem(int split, int groups) {
-    return 1024 + W_STAGES * TC_W_BYTES + TC_STEPS * X_BYTES + red_bytes(split) + (NBARS + 2) * 8 + (2 * (groups + 1) + 32) * 4;
+    return 1024 + W_STAGES * TC_W_BYTES + STEPS * X_BYTES + red_bytes(split) + (NBARS + 2) * 8 + (2 * (groups + 1) + 32) * 4;
   }
-  static_assert(smem(8, kMaxGroups) <= SMEM_LIMIT, "shared memory");
+  static_assert(smem(MAX_SPLIT, kMaxGroups) <= SMEM_LIMIT, "shared memory");
 };
 
 template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -143,9 +149,9 @@ struct TcTile {
 };
 
 template <class T, int BN, bool ZERO>
-__global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_constant__ TcArgs p) {
+__global__ void __launch_bounds__(TcCfg<BN>::THREADS, 1) int4_tc_kernel(const __grid_constant__ TcArgs p) {
   using Cfg = TcCfg<BN>;
-  constexpr int WS = Cfg::W_STAGES, ST = TC_STEPS, CW = Cfg::CW, DB = Cfg::D_BUFS;
+  constexpr int WS = Cfg::W_STAGES, ST = Cfg::STEPS, CW = Cfg::CW, DB = Cfg::D_BUFS, TT = Cfg::TILES, UN = Cfg::UN, ND = Cfg::DECODERS;
   const GemmArgs &a = p.g;
   const int split = p.split;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -171,8 +177,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
 
   pdl_trigger();
   if (threadIdx.x == 0) {
-    for (int s = 0; s < WS; ++s) { mbar_init(bar(W_FULL + s), 1); mbar_init(bar(W_EMPTY + s), 8); }
-    for (int s = 0; s < ST; ++s) { mbar_init(bar(X_FULL + s), 1); mbar_init(bar(A_FULL + s), 8); mbar_init(bar(DONE + s), 1); }
+    for (int s = 0; s < WS; ++s) { mbar_init(bar(W_FULL + s), 1); mbar_init(bar(W_EMPTY + s), ND); }
+    for (int s = 0; s < ST; ++s) { mbar_init(bar(X_FULL + s), 1); mbar_init(bar(A_FULL + s), ND); mbar_init(bar(DONE + s), 1); }
     for (int s = 0; s < DB; ++s) { mbar_init(bar(D_FULL + s), 1); mbar_init(bar(D_EMPTY + s), 8); }
     mbar_init(bar(DRAIN), 1);
     if (split > 1) {   // lane 0 of each sending warp; of each finishing warp
@@ -227,7 +233,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
   auto all = [](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
 
   if (warp < 4) {
-    regs_dec<TC_REGS_ISSUE>();
+    regs_dec<Cfg::REGS_ISSUE>();
     // One elected lane runs these loops: the compiler then knows that all that an instruction
     // names is uniform (with `lane == 0` every MMA had its operands moved to uniform registers
     // first and took 200 cycles to issue, whatever its size).
@@ -252,8 +258,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
             if (!mbar_wait(bar(DONE + st), sp ^ 1u, abort_flag, p.timeout_ns)) { ok = false; break; }
             mbar_arrive_expect_tx(bar(X_FULL + st), Cfg::X_BYTES);
             const uint32_t to = smem_u32(xring) + st * Cfg::X_BYTES;
-            tma_load_3d(to, &p.x, bar(X_FULL + st), k * TC_STEP, t.r0, 0);
-            tma_load_3d(to + BN * 128, &p.x, bar(X_FULL + st), k * TC_STEP + 64, t.r0, 0);
+#pragma unroll
+            for (int i = 0; i < 2 * TT; ++i)   // (rows past the last token are filled with zeros)
+              tma_load_3d(to + i * Cfg::X_TILE, &p.x, bar(X_FULL + st), k * TC_STEP + (i & 1) * 64, t.r0 + (i >> 1) * UN, 0);
             last_x = st;
             last_xp = sp;
             if (++st == ST) { st = 0; sp ^= 1u; }
@@ -267,7 +274,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
     } else if (warp == 1) {
       // ---------------------------------------------------------- MMA issuer
       if (elect_one()) {
-        const uint32_t idesc = make_idesc<T, BN>(0, 0);
+        const uint32_t idesc = make_idesc<T, UN>(0, 0);
         int st = 0, d = 0;
         uint32_t sp = 0, dp = 0;
         bool issued = false;
@@ -284,14 +291,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
                 return;
 #pragma unroll
               for (int s = 0; s < 8; s += PER) {
-                if (!mbar_wait(bar(D_EMPTY + d), dp ^ 1u, abort_flag, p.timeout_ns)) return;
-                tc_fence_after();
-                issued = true;
 #pragma unroll
-                for (int ks = s; ks < s + PER; ++ks)   // (a descriptor counts shared memory in 16 bytes)
-                  umma_ts(tmem + d * BN, at + ks * 8, xd + ((ks >> 2) * (BN * 128) + (ks & 3) * 32) / 16, idesc, ks > s ? 1u : 0u);
-                if (PER < 8) umma_commit(bar(D_FULL + d));
-                if (++d == DB) { d = 0; dp ^= 1u; }
+                for (int i = 0; i < TT; ++i) {
+                  if (!mbar_wait(bar(D_EMPTY + d), dp ^ 1u, abort_flag, p.timeout_ns)) return;
+                  tc_fence_after();
+                  issued = true;
+#pragma unroll
+                  for (int ks = s; ks < s + PER; ++ks)   // (a descriptor counts shared memory in 16 bytes)
+                    umma_ts(tmem + d * UN, at + ks * 8, xd + ((i * 2 + (ks >> 2)) * Cfg::X_TILE + (ks & 3) * 32) / 16, idesc, ks > s ? 1u : 0u);
+                  if (PER < 8 || TT > 1) umma_commit(bar(D_FULL + d));
+                  if (++d == DB) { d = 0; dp ^= 1u; }
+                }
               }
               umma_commit(bar(DONE + st));
               if (++st == ST) { st = 0; sp ^= 1u; }
@@ -308,17 +318,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
         }
       }
     }
-  } else if (warp < 12) {
+  } else if (warp < Cfg::SUM0) {
     // ------------------------------------------------------------ decoding
-    regs_dec<TC_REGS_DECODE>();
-    const int q = warp & 3, hf = (warp - 4) >> 2, r = q * 32 + lane;   // this thread's row of the tile, its TMEM lane
+    regs_dec<Cfg::REGS_DECODE>();
+    constexpr int HALVES = 8 / ND;   // of a step, 64 columns each, that a thread decodes
+    const int q = warp & 3, hf = ND == 8 ? (warp - 4) >> 2 : 0, r = q * 32 + lane;   // this thread's row of the tile, its TMEM lane
     const uint32_t at = tmem + TC_A_COL + hf * 32 + ((uint32_t)(q * 32) << 16);
     const uint32_t src = smem_u32(smem) + r * 128;
     int ws = 0, st = 0;
     uint32_t wp = 0, sp = 0;
     // this thread's words and zero points (of 32 columns each) of the next step
-    uint4 lo, hi;
-    uint32_t z0 = 8, z1 = 8;
+    uint4 w[2 * HALVES];
+    uint32_t z[2 * HALVES];
     const uint8_t *zero = nullptr;
     auto fetch = [&](int u, int k) {
       if constexpr (ZERO) {
@@ -326,15 +337,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
           const TcTile t = unit_at(u);
           zero = a.zero + t.e * a.z_e + (int64_t)min(t.n0 + r, a.N - 1) * a.z_rs;
         }
-        const int c = k * TC_STEP + hf * 64;
-        z0 = c < a.K ? zero[c >> a.group_log2] : 8u;
-        z1 = c + 32 < a.K ? zero[(c + 32) >> a.group_log2] : 8u;
+#pragma unroll
+        for (int i = 0; i < 2 * HALVES; ++i) {
+          const int c = k * TC_STEP + hf * 64 + i * 32;
+          z[i] = c < a.K ? zero[c >> a.group_log2] : 8u;
+        }
       }
       if ((k & 1) == 0 && !all(mbar_wait(bar(W_FULL + ws), wp, abort_flag, p.timeout_ns))) return false;
       const uint32_t row = src + ws * TC_W_BYTES;
-      const int ch = (k & 1) * 4 + hf * 2;
-      lo = ld_shared_v4(row + ((ch ^ (r & 7)) << 4));
-      hi = ld_shared_v4(row + (((ch + 1) ^ (r & 7)) << 4));
+#pragma unroll
+      for (int i = 0; i < 2 * HALVES; ++i) w[i] = ld_shared_v4(row + ((((k & 1) * 4 + hf * 2 + i) ^ (r & 7)) << 4));
       if ((k & 1) || k + 1 == k1) {
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(W_EMPTY + ws));
@@ -345,15 +357,25 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
     bool ok = cid < num_units && k0 < k1 && fetch(cid, k0);
     for (int u = cid; u < num_units && ok; u += ncl) {
       for (int k = k0; k < k1; ++k) {
-        uint32_t o[32];
-        const InOrder<T, ZERO> d0(z0), d1(z1);
-        d0(lo.x, o); d0(lo.y, o + 4); d0(lo.z, o + 8); d0(lo.w, o + 12);
-        d1(hi.x, o + 16); d1(hi.y, o + 20); d1(hi.z, o + 24); d1(hi.w, o + 28);
-        if (k + 1 < k1) ok = fetch(u, k + 1);
-        else if (u + ncl < num_units) ok = fetch(u + ncl, k0);
-        if (!ok || !all(mbar_wait(bar(DONE + st), sp ^ 1u, abort_flag, p.timeout_ns))) { ok = false; break; }
-        tc_fence_after();
-        tmem_st_x32(at + st * 64, o);
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+          uint32_t o[32];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const InOrder<T, ZERO> d(ZERO ? z[2 * h + i] : 8u);
+            const uint4 &v = w[2 * h + i];
+            d(v.x, o + 16 * i); d(v.y, o + 16 * i + 4); d(v.z, o + 16 * i + 8); d(v.w, o + 16 * i + 12);
+          }
+          if (h == HALVES - 1) {
+            if (k + 1 < k1) ok = fetch(u, k + 1);
+            else if (u + ncl < num_units) ok = fetch(u + ncl, k0);
+          }
+          if (h == 0) ok = ok && all(mbar_wait(bar(DONE + st), sp ^ 1u, abort_flag, p.timeout_ns));
+          if (!ok) break;
+          if (h == 0) tc_fence_after();
+          tmem_st_x32(at + st * 64 + h * 32, o);
+        }
+        if (!ok) break;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -363,8 +385,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
     }
   } else {
     // ------------------------------------------------------------ sums and output
-    regs_inc<TC_REGS_SUM>();
-    const int q = warp & 3, hf = (warp - 12) >> 2, r = q * 32 + lane;
+    regs_inc<Cfg::REGS_SUM>();
+    const int q = warp & 3, hf = (warp - Cfg::SUM0) >> 2, r = q * 32 + lane;
     T *out = static_cast<T *>(a.out);
     const int piece = q * 2 + hf, per_rank = 8 / split, owner = piece / per_rank;
     const uint32_t red_u32 = smem_u32(red) + (uint32_t)(piece % per_rank) * Cfg::PIECE + lane * 16u;
@@ -391,59 +413,63 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
       t = following;
       if (u + ncl < num_units) following = unit_at(u + ncl);
       const int64_t n = t.n0 + r;
-      float acc[CW];
+      float acc[TT][CW];
 #pragma unroll
-      for (int j = 0; j < CW; ++j) acc[j] = 0.f;
+      for (int j = 0; j < TT * CW; ++j) acc[j / CW][j % CW] = 0.f;
       for (int k = k0 * TC_STEP; k < stop && ok;) {
         float s[AHEAD];
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) s[i] = scale_of<T>(a, next[i]);
         if (k + (AHEAD << sum_log2) < stop) fetch(t, k + (AHEAD << sum_log2));
         else if (u + ncl < num_units) fetch(following, k0 * TC_STEP);
+        // (not unrolled: four copies of the body missed the instruction cache)
+#pragma unroll 1
+        for (int i = 0; i < AHEAD && k < stop && ok; ++i, k += 1 << sum_log2) {
+          const float si = i & 2 ? (i & 1 ? s[3] : s[2]) : (i & 1 ? s[1] : s[0]);
+          const float2 s2 = make_float2(si, si);
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i, k += 1 << sum_log2) {
-          if (k >= stop) break;
-          if (sums_log2) {
-            if (!all(mbar_wait(bar(D_FULL + d), dp, abort_flag, p.timeout_ns))) { ok = false; break; }
-          } else {
-            if (!all(mbar_wait(bar(DONE + st), sp, abort_flag, p.timeout_ns))) { ok = false; break; }
-            if (++st == ST) { st = 0; sp ^= 1u; }
-          }
-          tc_fence_after();
-          const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + d * BN + hf * CW;
-          constexpr int CH = CW < 32 ? CW : 32;
-          const float2 s2 = make_float2(s[i], s[i]);
-#pragma unroll
-          for (int c = 0; c < CW; c += CH) {
-            uint32_t v[32];
-            tmem_ld<CH>(from + c, v);
-            tmem_wait_ld();
-            if (c + CH >= CW) {   // the accumulator is read
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(bar(D_EMPTY + d));
+          for (int tt = 0; tt < TT; ++tt) {
+            if (sums_log2 || TT > 1) {
+              if (!all(mbar_wait(bar(D_FULL + d), dp, abort_flag, p.timeout_ns))) { ok = false; break; }
+            } else {
+              if (!all(mbar_wait(bar(DONE + st), sp, abort_flag, p.timeout_ns))) { ok = false; break; }
+              if (++st == ST) { st = 0; sp ^= 1u; }
             }
+            tc_fence_after();
+            const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + d * UN + hf * CW;
+            constexpr int CH = CW < 32 ? CW : 32;
 #pragma unroll
-            for (int j = 0; j < CH; j += 2) {
-              const float2 o = fma2(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), s2,
-                                    make_float2(acc[c + j], acc[c + j + 1]));
-              acc[c + j] = o.x;
-              acc[c + j + 1] = o.y;
+            for (int c = 0; c < CW; c += CH) {
+              uint32_t v[32];
+              tmem_ld<CH>(from + c, v);
+              tmem_wait_ld();
+              if (c + CH >= CW) {   // the accumulator is read
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(D_EMPTY + d));
+              }
+#pragma unroll
+              for (int j = 0; j < CH; j += 2) {
+                const float2 o = fma2(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), s2,
+                                      make_float2(acc[tt][c + j], acc[tt][c + j + 1]));
+                acc[tt][c + j] = o.x;
+                acc[tt][c + j + 1] = o.y;
+              }
             }
+            if (++d == DB) { d = 0; dp ^= 1u; }
           }
-          if (++d == DB) { d = 0; dp ^= 1u; }
         }
       }
       if (!ok) break;
-      if (split > 1) {
+      if (Cfg::MAX_SPLIT > 1 && split > 1) {
         if (owner != (int)rank) {
           // what this CTA sent for the last unit has been read
           if (!first && !all(mbar_wait_cluster(bar(RED_FREE), rphase ^ 1u, abort_flag, p.timeout_ns))) break;
           const uint32_t dst = mapa_shared(red_u32 + (uint32_t)((int)rank - ((int)rank > owner ? 1 : 0)) * red_step, (uint32_t)owner);
 #pragma unroll
           for (int j = 0; j < CW; j += 4)
-            st_cluster_v4(dst + (uint32_t)(j >> 2) * 512u, __float_as_uint(acc[j]), __float_as_uint(acc[j + 1]),
-                          __float_as_uint(acc[j + 2]), __float_as_uint(acc[j + 3]));
+            st_cluster_v4(dst + (uint32_t)(j >> 2) * 512u, __float_as_uint(acc[0][j]), __float_as_uint(acc[0][j + 1]),
+                          __float_as_uint(acc[0][j + 2]), __float_as_uint(acc[0][j + 3]));
           __syncwarp();   // the lanes' stores come before lane 0's release
           if (lane == 0) mbar_arrive_cluster(mapa_shared(bar(RED_FULL), (uint32_t)owner));
         } else {
@@ -454,10 +480,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
 #pragma unroll
             for (int j = 0; j < CW; j += 4) {
               const uint4 v = ld_shared_v4(red_u32 + s * red_step + (uint32_t)(j >> 2) * 512u);
-              acc[j] += __uint_as_float(v.x);
-              acc[j + 1] += __uint_as_float(v.y);
-              acc[j + 2] += __uint_as_float(v.z);
-              acc[j + 3] += __uint_as_float(v.w);
+              acc[0][j] += __uint_as_float(v.x);
+              acc[0][j + 1] += __uint_as_float(v.y);
+              acc[0][j + 2] += __uint_as_float(v.z);
+              acc[0][j + 3] += __uint_as_float(v.w);
             }
           }
         }
@@ -468,18 +494,22 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
         // whole 16 bytes where they lie on them.
         const float b = a.bias && n < a.N ? bias_at<T>(a, n) : 0.f;
         T *stage = reinterpret_cast<T *>(split > 1 ? red + (piece % per_rank) * Cfg::PIECE : red + piece * (Cfg::PIECE / 2));
-        __syncwarp();
+        const int64_t nw = t.n0 + q * 32;
 #pragma unroll
-        for (int j = 0; j < CW; ++j) stage[j * 32 + lane] = Elem<T>::store(acc[j] + b);
-        __syncwarp();
-        const int64_t m = t.r0 + hf * CW, nw = t.n0 + q * 32;
-        const int live = (int)min((int64_t)CW, t.rend - m);
-        T *dst = out + m * a.out_rs + nw;
-        if (p.out_vec && nw + 32 <= a.N) {
-          for (int j = lane >> 2; j < live; j += 8)
-            *reinterpret_cast<uint4 *>(dst + j * a.out_rs + (lane & 3) * 8) = *reinterpret_cast<const uint4 *>(stage + j * 32 + (lane & 3) * 8);
-        } else if (n < a.N) {
-          for (int j = 0; j < live; ++j) dst[j * a.out_rs + lane] = stage[j * 32 + lane];
+        for (int tt = 0; tt < TT; ++tt) {
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < CW; ++j) stage[j * 32 + lane] = Elem<T>::store(acc[tt][j] + b);
+          __syncwarp();
+          const int64_t m = t.r0 + tt * UN + hf * CW;
+          const int live = (int)max((int64_t)0, min((int64_t)CW, t.rend - m));
+          T *dst = out + m * a.out_rs + nw;
+          if (p.out_vec && nw + 32 <= a.N) {
+            for (int j = lane >> 2; j < live; j += 8)
+              *reinterpret_cast<uint4 *>(dst + j * a.out_rs + (lane & 3) * 8) = *reinterpret_cast<const uint4 *>(stage + j * 32 + (lane & 3) * 8);
+          } else if (n < a.N) {
+            for (int j = 0; j < live; ++j) dst[j * a.out_rs + lane] = stage[j * 32 + lane];
+          }
         }
         if (split > 1) {
           __syncwarp();
@@ -489,7 +519,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) int4_tc_kernel(const __grid_con
       rphase ^= 1u;
       first = false;
     }
-    if (a.offsets) zero_rest<T>(a, row0[a.groups], threadIdx.x - 12 * 32, 8 * 32);
+    if (a.offsets) zero_rest<T>(a, row0[a.groups], threadIdx.x - Cfg::SUM0 * 32, 8 * 32);
   }
 
   tc_fence_before();

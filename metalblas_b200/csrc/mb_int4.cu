@@ -151,11 +151,11 @@ template <class T, int BN, bool ZERO>
 int tc_launch_as(i4::TcArgs &p, int split, int64_t units, cudaStream_t st) {
   constexpr auto kern = i4::int4_tc_kernel<T, BN, ZERO>;
   using Cfg = i4::TcCfg<BN>;
-  const int rc = allow_smem<kern>(Cfg::smem(8, i4::kMaxGroups));
+  const int rc = allow_smem<kern>(std::max(Cfg::smem(1, i4::kMaxGroups), Cfg::smem(Cfg::MAX_SPLIT, i4::kMaxGroups)));
   if (rc) return rc;
   p.split = split;
   const int64_t clusters = std::min<int64_t>(units, device_sms() / split);
-  return launch_pdl(kern, dim3((unsigned)(clusters * split)), dim3(i4::TC_THREADS), Cfg::smem(split, p.g.groups), st, split,
+  return launch_pdl(kern, dim3((unsigned)(clusters * split)), dim3(Cfg::THREADS), Cfg::smem(split, p.g.groups), st, split,
                     "int4_gemm", p);
 }
 template <class T, int BN>
@@ -181,7 +181,7 @@ int int4_plan(const mb_int4_desc *d, Plan &pl) {
   const int64_t active = d->groups ? std::min(E, d->M) : 1;
   const double rows = (double)d->M / active;
   const int want = d->plan[0];
-  if (want != 0 && want != 1 && want != 2 && want != 16 && want != 32 && want != 64 && want != 128)
+  if (want != 0 && want != 1 && want != 2 && want != 16 && want != 32 && want != 64 && want != 128 && want != 256)
     return fail(MB_ERR_INVALID, "no plan %d", want);
   // the one-pass kernel counts rows of units in 32 bits
   auto few_fits = [&](int nt) { return (ceil_div(d->M, 8 * nt) + (d->groups ? E : 0)) * d->N < (1ll << 32); };
@@ -195,7 +195,7 @@ int int4_plan(const mb_int4_desc *d, Plan &pl) {
     pl.few = 0;
   }
   if (!pl.few) {
-    pl.bn = want >= 16 ? want : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    pl.bn = want >= 16 ? want : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 256 ? 128 : 256;
     const int64_t tiles_n = ceil_div(d->N, 128), stages = ceil_div(d->K, 256);
     pl.units = (ceil_div(d->M, pl.bn) + (d->groups ? active : 0)) * tiles_n;
     if (pl.units >= (1ll << 31)) return fail(MB_ERR_INVALID, "too many tiles");
@@ -203,9 +203,9 @@ int int4_plan(const mb_int4_desc *d, Plan &pl) {
     if (d->plan[1]) {
       pl.split = d->plan[1];
       if (pl.split != 1 && pl.split != 2 && pl.split != 4 && pl.split != 8) return fail(MB_ERR_INVALID, "a split is 1, 2, 4 or 8");
-      if (pl.split > stages) return fail(MB_ERR_INVALID, "a split of %d exceeds the columns", pl.split);
+      if (pl.split > (pl.bn == 256 ? 1 : stages)) return fail(MB_ERR_INVALID, "a split of %d exceeds the columns", pl.split);
     } else {
-      while (pl.split < 8 && pl.units * pl.split * 2 <= sms && pl.split * 2 <= stages) pl.split *= 2;
+      while (pl.bn < 256 && pl.split < 8 && pl.units * pl.split * 2 <= sms && pl.split * 2 <= stages) pl.split *= 2;
     }
   }
   int64_t at = 0;
@@ -259,13 +259,14 @@ int gemm_launch(const mb_int4_desc *d, const Plan &pl, cudaStream_t st) {
   p.timeout_ns = wait_timeout_ns();
   const int64_t bytes = (d->K + 1) / 2;
   int rc = encode_map(&p.w, MB_U8, a.w, bytes, d->N, nw, d->N == 1 ? round_up(bytes, 16) : a.w_rs, a.w_e, 128, 128);
-  if (!rc) rc = encode_map(&p.x, d->dtype, a.x, d->K, d->M, 1, d->M == 1 ? round_up(d->K, 8) : a.x_rs, 0, 64, pl.bn);
+  if (!rc) rc = encode_map(&p.x, d->dtype, a.x, d->K, d->M, 1, d->M == 1 ? round_up(d->K, 8) : a.x_rs, 0, 64, std::min(pl.bn, 128));
   if (rc) return rc;
   switch (pl.bn) {
     case 16: return tc_launch_bn<T, 16>(p, pl.split, pl.units, st);
     case 32: return tc_launch_bn<T, 32>(p, pl.split, pl.units, st);
     case 64: return tc_launch_bn<T, 64>(p, pl.split, pl.units, st);
-    default: return tc_launch_bn<T, 128>(p, pl.split, pl.units, st);
+    case 128: return tc_launch_bn<T, 128>(p, pl.split, pl.units, st);
+    default: return tc_launch_bn<T, 256>(p, pl.split, pl.units, st);
   }
 }
 
