@@ -10,9 +10,13 @@
 // group, and u = 8 + rint(x / s), halves to even, within 1..15.  A group of zeros
 // has scale 0, one with an infinity or a NaN scale NaN; both have u = 8.
 //
-// rint(x / s) is decided exactly: t = x (1 / s) is close enough that the half h
+// rint(x / s) is decided exactly, halves included.  16-bit x have so many of them that
+// they are decided without a branch or a residual (Quant16 below); for fp32 x, and
+// scales below the normal range, t = x (1 / s) is close enough that the half h
 // nearest to it is the one next to the true quotient, and the sign of x - h s, which
 // one fused multiply-add gives without error, says on which side of h that lies.
+//
+// Both directions are bound by HBM, with as many loads on their way as registers allow.
 #pragma once
 #include "mb_common.cuh"
 #include "quantize.cuh"
@@ -44,92 +48,171 @@ __device__ __forceinline__ float rounded_quotient(float x, float s, float inv) {
   return __fsub_rn(__fadd_rn(y, kMagic), kMagic);
 }
 
-// A lane takes 8 consecutive columns, so a group has G / 8 neighbouring lanes and a
-// warp 256 columns of one row.
-template <class T, class S, bool AL>
+// Eight quotients of 16-bit x as the nibbles 8 + rint(x / s).
+//
+// x (hi + lo), hi + lo being the inverse of the scale to 2^-42, is the quotient
+// rounded once to fp32.  With a scale of 16 bits too a quotient that is a half comes out
+// exactly, and another one differs from it by more than that rounding.  A scale of
+// fp32 is amax / 7 rounded: then 7 x / amax, which is a half or 2^-18.7 of it away from
+// one at least (x and amax have 11 bits at most and lie within 4 binades where the
+// quotient reaches 1/2), is taken instead and moved by 2^-21 of itself to the side
+// that x / s lies on: all ties of a group go one way, the way that the scale was rounded.
+struct Quant16 {
+  float hi, lo;
+  // num / den, and the way that quotients move
+  __device__ __forceinline__ Quant16(float num, float den, float move) {
+    const float h = __fdividef(num, den);
+    hi = h;
+    lo = fmaf(fmaf(-h, den, num), __fdividef(1.f, den), h * move);
+  }
+  __device__ __forceinline__ uint32_t operator()(const float (&x)[8]) const {
+    constexpr float kMagic = 12582912.f;   // 1.5 * 2^23: adding it rounds to an integer
+    const float2 h = make_float2(hi, hi), l = make_float2(lo, lo), m = make_float2(kMagic, kMagic), n = make_float2(-kMagic, -kMagic);
+    float2 q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = make_float2(x[i], x[i + 4]);
+      q[i] = add2(add2(fma2(v, h, mul2(v, l)), m), n);
+    }
+    // four nibbles are a whole number below 2^16
+    float2 f = fma2(q[1], make_float2(16.f, 16.f), q[0]);
+    f = fma2(q[2], make_float2(256.f, 256.f), f);
+    f = fma2(q[3], make_float2(4096.f, 4096.f), f);
+    f = add2(f, make_float2(kMagic + 34952.f, kMagic + 34952.f));   // 8 in each
+    return __byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x5410);
+  }
+};
+
+// A lane takes 8 consecutive columns at a time, so a group has G / 8 neighbouring lanes
+// and a warp 256 columns of one row.  A task is B times that, next to one another.
+template <class T, class S, bool AL, int B>
 __global__ void __launch_bounds__(256) quantize_int4_kernel(const ConvertArgs a) {
   const int lane = threadIdx.x & 31;
-  const int64_t per_row = (a.cols + 255) / 256, tasks = a.rows * per_row;
+  const uint32_t per_row = (a.cols + 256 * B - 1) / (256 * B);
+  const int64_t tasks = a.rows * (int64_t)per_row;
   pdl_trigger();
   pdl_wait();
+  constexpr int V = Vec<T>::V, NV = 8 / V;
   for (int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < tasks; w += (int64_t)gridDim.x * 8) {
-    const int64_t r = w / per_row;
-    const int c = (int)(w - r * per_row) * 256 + lane * 8;
-    const T *row = static_cast<const T *>(a.src) + r * a.ld_src;
-    constexpr int V = Vec<T>::V;
-    float x[8];
-    MaxAbs<T> m;
+    const int64_t r = tasks < (1ll << 32) ? (uint32_t)w / per_row : w / per_row;
+    const int c0 = (int)(w - r * per_row) * (256 * B) + lane * 8;
+    const T *src = static_cast<const T *>(a.src) + r * a.ld_src;
+    Vec<T> v[B][NV];
 #pragma unroll
-    for (int i = 0; i < 8; i += V) {
-      const Vec<T> v = load_vec<T, AL>(row, c + i, a.cols);
-      m.add(v);
+    for (int b = 0; b < B; ++b)
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[i + j] = v.f(j);
-    }
-    uint32_t bits = m.bits();
-    for (int d = 1; d < (1 << a.group_log2) / 8; d <<= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, d));
-    // the scale as it is stored
-    const bool finite = bits < 0x7f800000u;
-    const S stored = Elem<S>::store(finite ? __fdiv_rn(__uint_as_float(bits), 7.f) : __uint_as_float(0x7fc00000u));
-    const float s0 = to_f32(stored);
-    if (c < a.cols && (c & ((1 << a.group_log2) - 1)) == 0)
-      static_cast<S *>(a.scale)[r * a.ld_scale + (c >> a.group_log2)] = stored;
-    // groups of tiny values are moved by a power of two, so that 1 / s and h s stay in range
-    const float pre = s0 < 0x1p-90f ? 0x1p100f : 1.f, s = s0 * pre;
-    const float inv = __fdividef(1.f, s);
-    uint32_t word = 0;
+      for (int i = 0; i < NV; ++i) v[b][i] = load_vec<T, AL>(src, c0 + b * 256 + i * V, a.cols);
+    uint8_t *row = static_cast<uint8_t *>(a.dst) + r * a.ld_dst;
+    S *scales = static_cast<S *>(a.scale) + r * a.ld_scale;
+    const bool words = (reinterpret_cast<uintptr_t>(row) & 3) == 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float q = rounded_quotient(x[i] * pre, s, inv);
-      q = fminf(fmaxf(q, -7.f), 7.f);   // a scale that rounded down to a subnormal
-      const uint32_t u = !finite || s0 == 0.f ? 8u : (uint32_t)((int)q + 8);
-      word |= u << (4 * i);
-    }
-    if (c >= a.cols) continue;
-    uint8_t *dst = static_cast<uint8_t *>(a.dst) + r * a.ld_dst + c / 2;
-    const int bytes = (min(8, a.cols - c) + 1) / 2;
-    if (bytes == 4 && (reinterpret_cast<uintptr_t>(dst) & 3) == 0) {
-      *reinterpret_cast<uint32_t *>(dst) = word;
-    } else {
-      for (int i = 0; i < bytes; ++i) dst[i] = (uint8_t)(word >> (8 * i));
+    for (int b = 0; b < B; ++b) {
+      const int c = c0 + b * 256;
+      if (c - lane * 8 >= a.cols) break;
+      float x[8];
+      MaxAbs<T> m;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        m.add(v[b][i]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[i * V + j] = v[b][i].f(j);
+      }
+      uint32_t bits = m.bits();
+      for (int d = 1; d < (1 << a.group_log2) / 8; d <<= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, d));
+      // the scale as it is stored
+      const bool finite = bits < 0x7f800000u;
+      const float amax = __uint_as_float(bits);
+      const float exact7 = __fdiv_rn(amax, 7.f);
+      const S stored = Elem<S>::store(finite ? exact7 : __uint_as_float(0x7fc00000u));
+      const float s0 = to_f32(stored);
+      if (c < a.cols && (c & ((1 << a.group_log2) - 1)) == 0)
+        scales[c >> a.group_log2] = stored;
+      uint32_t word = 0x88888888u;
+      // (scales of fp16 are normal numbers from 2^-14 on)
+      constexpr bool F32 = sizeof(S) == 4;
+      if (sizeof(T) == 2 && s0 >= (std::is_same_v<S, __half> ? 0x1p-14f : 0x1p-100f) && s0 < 0x1p100f) {
+        // x / s lies above 7 x / amax where s was rounded down: s - amax / 7 has the sign of 7 s - amax
+        const float over = F32 ? fmaf(7.f, s0, -amax) : 0.f;
+        const float move = over == 0.f ? 0.f : copysignf(0x1p-21f, -over);
+        word = Quant16(F32 ? 7.f : 1.f, F32 ? amax : s0, move)(x);
+      } else if (finite && s0 != 0.f) {
+        // groups of tiny values are moved by a power of two, so that 1 / s and h s stay in range
+        const float pre = s0 < 0x1p-90f ? 0x1p100f : 1.f, s = s0 * pre, inv = __fdividef(1.f, s);
+        word = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float q = fminf(fmaxf(rounded_quotient(x[i] * pre, s, inv), -7.f), 7.f);   // (a scale that rounded down to a subnormal)
+          word |= (uint32_t)((int)q + 8) << (4 * i);
+        }
+      }
+      if (c >= a.cols) continue;
+      if (words && c + 7 <= a.cols) {
+        *reinterpret_cast<uint32_t *>(row + c / 2) = word;
+      } else {
+        for (int i = 0; i < (min(8, a.cols - c) + 1) / 2; ++i) row[c / 2 + i] = (uint8_t)(word >> (8 * i));
+      }
     }
   }
 }
 
-template <class T, class S, bool AL>
+template <class T, class S, bool AL, int B>
 __global__ void __launch_bounds__(256) dequantize_int4_kernel(const ConvertArgs a) {
   const int lane = threadIdx.x & 31;
-  const int64_t per_row = (a.cols + 255) / 256, tasks = a.rows * per_row;
+  const uint32_t per_row = (a.cols + 256 * B - 1) / (256 * B);
+  const int64_t tasks = a.rows * (int64_t)per_row;
   pdl_trigger();
   pdl_wait();
   for (int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < tasks; w += (int64_t)gridDim.x * 8) {
-    const int64_t r = w / per_row;
-    const int c = (int)(w - r * per_row) * 256 + lane * 8;
-    if (c >= a.cols) continue;
-    const uint8_t *src = static_cast<const uint8_t *>(a.src) + r * a.ld_src + c / 2;
-    const int n = min(8, a.cols - c);
-    uint32_t word = 0;
-    if (n >= 7 && (reinterpret_cast<uintptr_t>(src) & 3) == 0) {
-      word = *reinterpret_cast<const uint32_t *>(src);
-    } else {
-      for (int i = 0; i < (n + 1) / 2; ++i) word |= (uint32_t)src[i] << (8 * i);
-    }
-    const int g = c >> a.group_log2;
-    const float s = to_f32(static_cast<const S *>(a.scale)[r * a.ld_scale + g]);
-    const float z = a.zero ? (float)a.zero[r * a.ld_zero + g] : 8.f;
-    T *dst = static_cast<T *>(a.dst) + r * a.ld_dst + c;
-    constexpr int V = Vec<T>::V;
+    const int64_t r = tasks < (1ll << 32) ? (uint32_t)w / per_row : w / per_row;
+    const int c0 = (int)(w - r * per_row) * (256 * B) + lane * 8;
+    const uint8_t *row = static_cast<const uint8_t *>(a.src) + r * a.ld_src;
+    const S *scales = static_cast<const S *>(a.scale) + r * a.ld_scale;
+    const bool words = (reinterpret_cast<uintptr_t>(row) & 3) == 0;
+    uint32_t word[B], zero[B];
+    S scale[B];
 #pragma unroll
-    for (int i = 0; i < 8; i += V) {
-      Vec<T> v;
-#pragma unroll
-      for (int j = 0; j < V; ++j) v.set(j, ((float)((word >> (4 * (i + j))) & 15) - z) * s);
-      if (AL && n >= i + V) {
-        *reinterpret_cast<uint4 *>(dst + i) = v.u.q;
+    for (int b = 0; b < B; ++b) {
+      const int c = c0 + b * 256;
+      word[b] = 0;
+      zero[b] = 8;
+      scale[b] = S();
+      if (c >= a.cols) continue;
+      if (words && c + 7 <= a.cols) {
+        word[b] = *reinterpret_cast<const uint32_t *>(row + c / 2);
       } else {
+        for (int i = 0; i < (min(8, a.cols - c) + 1) / 2; ++i) word[b] |= (uint32_t)row[c / 2 + i] << (8 * i);
+      }
+      scale[b] = scales[c >> a.group_log2];
+      if (a.zero) zero[b] = a.zero[r * a.ld_zero + (c >> a.group_log2)];
+    }
+    T *out = static_cast<T *>(a.dst) + r * a.ld_dst;
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (i + j < n) dst[i + j] = v.u.t[j];
+    for (int b = 0; b < B; ++b) {
+      const int c = c0 + b * 256, n = min(8, a.cols - c);
+      if (n <= 0) break;
+      const float s = to_f32(scale[b]);
+      const float2 s2 = make_float2(s, s);
+      const float off = -(8388608.f + (float)zero[b]);   // 2^23 + u - (2^23 + z)
+      const float2 o2 = make_float2(off, off);
+      constexpr int V = Vec<T>::V;
+#pragma unroll
+      for (int i = 0; i < 8; i += V) {
+        Vec<T> v;
+#pragma unroll
+        for (int j = 0; j < V; j += 2) {
+          const uint32_t u = word[b] >> (4 * (i + j));
+          const float2 f = make_float2(__uint_as_float((u & 15) | 0x4b000000u), __uint_as_float(((u >> 4) & 15) | 0x4b000000u));
+          const float2 y = mul2(add2(f, o2), s2);
+          v.set(j, y.x);
+          v.set(j + 1, y.y);
+        }
+        if (AL && n >= i + V) {
+          *reinterpret_cast<uint4 *>(out + c + i) = v.u.q;
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (i + j < n) out[c + i + j] = v.u.t[j];
+        }
       }
     }
   }

@@ -64,8 +64,15 @@ int check_convert(const char *what, int dtype, int scale_dtype, int64_t rows, in
     return fail(MB_ERR_INVALID, "%s: rows overlap", what);
   return MB_OK;
 }
-unsigned convert_grid(int64_t rows, int64_t cols) {
-  return (unsigned)std::min<int64_t>(ceil_div(rows * ceil_div(cols, 256), 8), (int64_t)device_sms() * 64);
+// Spans of 256 columns that a warp of a conversion takes at a time, f(it, blocks): several where
+// rows have them and there is work for every SM.
+template <class F>
+int by_spans(int64_t rows, int64_t cols, F &&f) {
+  using std::integral_constant;
+  const int64_t sms = device_sms(), most = sms * 32;
+  auto blocks = [&](int b) { return (unsigned)std::min<int64_t>(ceil_div(rows * ceil_div(cols, 256 * b), 8), most); };
+  if (cols > 512 && rows * ceil_div(cols, 1024) >= sms * 32) return f(integral_constant<int, 4>(), blocks(4));
+  return f(integral_constant<int, 1>(), blocks(1));
 }
 
 int int4_check(const mb_int4_desc *d) {
@@ -283,8 +290,11 @@ int mb_int4_quantize(int32_t dtype, int32_t scale_dtype, int64_t rows, int64_t c
     return by_float(scale_dtype, [&](auto *s) {
       using T = std::remove_pointer_t<decltype(t)>;
       using S = std::remove_pointer_t<decltype(s)>;
-      auto kern = rows16(x, rows, ldx, sizeof(T)) ? i4::quantize_int4_kernel<T, S, true> : i4::quantize_int4_kernel<T, S, false>;
-      return launch_pdl(kern, dim3(convert_grid(rows, cols)), dim3(256), 0, (cudaStream_t)stream, 1, "int4_quantize", a);
+      return by_spans(rows, cols, [&](auto b, unsigned blocks) {
+        constexpr int B = decltype(b)::value;
+        auto kern = rows16(x, rows, ldx, sizeof(T)) ? i4::quantize_int4_kernel<T, S, true, B> : i4::quantize_int4_kernel<T, S, false, B>;
+        return launch_pdl(kern, dim3(blocks), dim3(256), 0, (cudaStream_t)stream, 1, "int4_quantize", a);
+      });
     });
   });
 }
@@ -300,8 +310,11 @@ int mb_int4_dequantize(int32_t dtype, int32_t scale_dtype, int64_t rows, int64_t
     return by_float(scale_dtype, [&](auto *s) {
       using T = std::remove_pointer_t<decltype(t)>;
       using S = std::remove_pointer_t<decltype(s)>;
-      auto kern = rows16(out, rows, ldo, sizeof(T)) ? i4::dequantize_int4_kernel<T, S, true> : i4::dequantize_int4_kernel<T, S, false>;
-      return launch_pdl(kern, dim3(convert_grid(rows, cols)), dim3(256), 0, (cudaStream_t)stream, 1, "int4_dequantize", a);
+      return by_spans(rows, cols, [&](auto b, unsigned blocks) {
+        constexpr int B = decltype(b)::value;
+        auto kern = rows16(out, rows, ldo, sizeof(T)) ? i4::dequantize_int4_kernel<T, S, true, B> : i4::dequantize_int4_kernel<T, S, false, B>;
+        return launch_pdl(kern, dim3(blocks), dim3(256), 0, (cudaStream_t)stream, 1, "int4_dequantize", a);
+      });
     });
   });
 }
