@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -102,6 +103,20 @@ int launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaS
   cfg.attrs = attr;
   cfg.numAttrs = n;
   return cuda_check(cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...), what);
+}
+
+// Lets a kernel use `bytes` of dynamic shared memory; once per kernel and device.
+template <auto Kernel>
+int allow_smem(int bytes) {
+  static std::atomic<bool> done[64];
+  int dev = 0;
+  int rc = cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
+  if (rc) return rc;
+  const bool keep = dev >= 0 && dev < 64;
+  if (keep && done[dev].load(std::memory_order_acquire)) return MB_OK;
+  rc = cuda_check(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute");
+  if (!rc && keep) done[dev].store(true, std::memory_order_release);
+  return rc;
 }
 
 inline PFN_cuTensorMapEncodeTiled_v12000 get_encode() {

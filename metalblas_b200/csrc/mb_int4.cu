@@ -114,20 +114,6 @@ i4::GemmArgs gemm_args(const mb_int4_desc *d) {
   return a;
 }
 
-// Lets a kernel use `bytes` of dynamic shared memory; once per kernel and device.
-template <auto Kernel>
-int allow_smem(int bytes) {
-  static std::atomic<bool> done[64];
-  int dev = 0;
-  int rc = cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
-  if (rc) return rc;
-  const bool keep = dev >= 0 && dev < 64;
-  if (keep && done[dev].load(std::memory_order_acquire)) return MB_OK;
-  rc = cuda_check(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute");
-  if (!rc && keep) done[dev].store(true, std::memory_order_release);
-  return rc;
-}
-
 template <class T, int LW, int NT, bool ZERO>
 int few_launch_as(const i4::GemmArgs &a, cudaStream_t st) {
   constexpr auto kern = i4::int4_few_kernel<T, LW, NT, ZERO>;

@@ -113,20 +113,6 @@ int sort_setup(int &max_ranks) {
   return MB_OK;
 }
 
-// Lets a kernel use `bytes` of dynamic shared memory; once per kernel and device.
-template <auto Kernel>
-int allow_smem(int bytes) {
-  static std::atomic<bool> done[64];
-  int dev = 0;
-  int rc = cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
-  if (rc) return rc;
-  const bool keep = dev >= 0 && dev < 64;
-  if (keep && done[dev].load(std::memory_order_acquire)) return MB_OK;
-  rc = cuda_check(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute");
-  if (!rc && keep) done[dev].store(true, std::memory_order_release);
-  return rc;
-}
-
 template <class T>
 int launch_quantize(const RouteParams &p, cudaStream_t st, const char *what) {
   constexpr int V = Vec<T>::V;

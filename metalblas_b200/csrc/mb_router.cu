@@ -52,9 +52,19 @@ int by_shape(int dtype, int64_t E, const void *p, int64_t ld, const void *p2, F 
   }
 }
 
-unsigned row_grid(int64_t T) { return (unsigned)std::min<int64_t>(ceil_div(T, WARPS), (int64_t)device_sms() * 8); }
-// Blocks that sum up the balance of T tokens.
-int64_t parts_of(int64_t T) { return std::max<int64_t>(1, std::min<int64_t>(ceil_div(T, 4 * WARPS), MAX_PARTS)); }
+// Rows that a warp takes at once (Rows in router.cuh), by the experts.
+int rows_at_once(int64_t E) { return E <= 128 ? 4 : E <= 256 ? 2 : 1; }
+// Blocks of T rows: resident ones, each through its share.
+unsigned row_grid(int64_t T, int rows) {
+  return (unsigned)std::min<int64_t>(ceil_div(T, WARPS * rows), (int64_t)device_sms() * 6);
+}
+// Clusters that sum up the balance of T tokens.  One makes the loss in the same launch;
+// measured at 64 experts: @@
+int64_t parts_of(int64_t T, int64_t E) {
+  const int64_t rows = (int64_t)CLUSTER * WARPS * rows_at_once(E);
+  if (T <= 4 * rows) return 1;
+  return std::min<int64_t>(ceil_div(T, rows), device_sms() * 4 / CLUSTER);
+}
 
 }  // namespace
 
@@ -70,7 +80,13 @@ int mb_expert_route(int32_t dtype, int64_t tokens, int64_t experts, int64_t k, i
   RouteArgs a{logits, ldl, (int)tokens, (int)experts, (int)k, normalize, weights, ids, nullptr, nullptr};
   return by_shape(dtype, experts, logits, ldl, nullptr, [&](auto *t, auto nv, auto v, auto al) {
     using T = std::remove_pointer_t<decltype(t)>;
-    return launch_pdl(route_kernel<T, decltype(nv)::value, decltype(v)::value, decltype(al)::value>, dim3(row_grid(tokens)), dim3(THREADS), 0,
+    constexpr int NV = decltype(nv)::value, V = decltype(v)::value;
+    constexpr bool AL = decltype(al)::value;
+    if constexpr (NV > 1)
+      if (k > 32)
+        return launch_pdl(route_kernel<T, NV, V, AL, true>, dim3(row_grid(tokens, 1)), dim3(THREADS), 0, (cudaStream_t)stream, 1,
+                          "expert_route", a);
+    return launch_pdl(route_kernel<T, NV, V, AL, false>, dim3(row_grid(tokens, rows_at_once(experts))), dim3(THREADS), 0,
                       (cudaStream_t)stream, 1, "expert_route", a);
   });
 }
@@ -79,19 +95,26 @@ int mb_expert_route_backward(int32_t dtype, int64_t tokens, int64_t experts, int
                              const float *grad, const void *logits, int64_t ldl, const int32_t *ids, void *dlogits,
                              void *stream) {
   const int rc = check("expert_route_backward", dtype, tokens, experts, k, ldl, logits);
-  if (rc || tokens == 0) return rc;
+  if (rc) return rc;
+  if (k > MAX_K) return fail(MB_ERR_INVALID, "expert_route_backward: k = %lld (at most %d)", (long long)k, MAX_K);
+  if (tokens == 0) return MB_OK;
   if (!dlogits || (k && (!grad || !ids))) return fail(MB_ERR_INVALID, "expert_route_backward: null pointer");
   RouteArgs a{logits, ldl, (int)tokens, (int)experts, (int)k, normalize, nullptr, const_cast<int32_t *>(ids), grad, dlogits};
   return by_shape(dtype, experts, logits, ldl, dlogits, [&](auto *t, auto nv, auto v, auto al) {
     using T = std::remove_pointer_t<decltype(t)>;
-    return launch_pdl(route_backward_kernel<T, decltype(nv)::value, decltype(v)::value, decltype(al)::value>, dim3(row_grid(tokens)),
-                      dim3(THREADS), 0, (cudaStream_t)stream, 1, "expert_route_backward", a);
+    constexpr int NV = decltype(nv)::value;
+    constexpr auto kern = route_backward_kernel<T, NV, decltype(v)::value, decltype(al)::value>;
+    constexpr int smem = WARPS * Rows<NV>::R * 32 * NV * 8;   // 64 KB at most
+    const int rc = allow_smem<kern>(smem);
+    if (rc) return rc;
+    return launch_pdl(kern, dim3(row_grid(tokens, Rows<NV>::R)), dim3(THREADS), smem, (cudaStream_t)stream, 1,
+                      "expert_route_backward", a);
   });
 }
 
 int64_t mb_expert_balance_workspace_size(int64_t tokens, int64_t experts) {
   if (tokens < 0 || experts < 1 || experts > MAX_EXPERTS) return 0;
-  return parts_of(tokens) * (2 * experts + 1) * 4;
+  return parts_of(tokens, experts) * (2 * experts + 1) * 4;
 }
 
 int mb_expert_balance(int32_t dtype, int64_t tokens, int64_t experts, int64_t k, const void *logits, int64_t ldl,
@@ -103,7 +126,7 @@ int mb_expert_balance(int32_t dtype, int64_t tokens, int64_t experts, int64_t k,
   const int64_t need = mb_expert_balance_workspace_size(tokens, experts);
   if (!workspace || workspace_bytes < need) return fail(MB_ERR_WORKSPACE, "expert_balance: workspace of %lld bytes required", (long long)need);
   if (reinterpret_cast<uintptr_t>(workspace) & 3) return fail(MB_ERR_WORKSPACE, "expert_balance: the workspace must start on a 4-byte boundary");
-  const int64_t parts = parts_of(tokens);
+  const int64_t parts = parts_of(tokens, experts);
   BalanceArgs a{};
   a.logits = logits; a.ld = ldl; a.T = (int)tokens; a.E = (int)experts; a.k = (int)k;
   a.experts = ids; a.mask = mask;
@@ -114,10 +137,10 @@ int mb_expert_balance(int32_t dtype, int64_t tokens, int64_t experts, int64_t k,
   const int r = by_shape(dtype, experts, logits, ldl, nullptr, [&](auto *t, auto nv, auto v, auto al) {
     using T = std::remove_pointer_t<decltype(t)>;
     const size_t smem = (size_t)(WARPS * experts + experts + 1) * 4;   // 36 KB at 1024 experts
-    return launch_pdl(balance_kernel<T, decltype(nv)::value, decltype(v)::value, decltype(al)::value>, dim3((unsigned)parts), dim3(THREADS), smem,
-                      (cudaStream_t)stream, 1, "expert_balance", a);
+    return launch_pdl(balance_kernel<T, decltype(nv)::value, decltype(v)::value, decltype(al)::value>, dim3((unsigned)parts * CLUSTER), dim3(THREADS),
+                      smem, (cudaStream_t)stream, CLUSTER, "expert_balance", a);
   });
-  if (r) return r;
+  if (r || parts == 1) return r;
   return launch_pdl(balance_finish_kernel, dim3(1), dim3(1024), 0, (cudaStream_t)stream, 1, "expert_balance", a);
 }
 
@@ -133,7 +156,8 @@ int mb_expert_balance_backward(int32_t dtype, int64_t tokens, int64_t experts, c
   a.grad = grad; a.dlogits = dlogits;
   return by_shape(dtype, experts, logits, ldl, dlogits, [&](auto *t, auto nv, auto v, auto al) {
     using T = std::remove_pointer_t<decltype(t)>;
-    return launch_pdl(balance_backward_kernel<T, decltype(nv)::value, decltype(v)::value, decltype(al)::value>, dim3(row_grid(tokens)),
+    return launch_pdl(balance_backward_kernel<T, decltype(nv)::value, decltype(v)::value, decltype(al)::value>,
+                      dim3(row_grid(tokens, rows_at_once(experts))),
                       dim3(THREADS), 0, (cudaStream_t)stream, 1, "expert_balance_backward", a);
   });
 }

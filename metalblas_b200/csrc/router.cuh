@@ -19,10 +19,11 @@
 // the row's p NaN, as the formula does.  Scores as low as the type goes are
 // ordinary numbers.  Numbers outside 0..E-1 in `experts` mark dropped entries.
 //
-// One warp takes a row, NV scores a lane, in registers; exponentials, sums and
-// gradients are fp32.  Sums over tokens have a fixed order: a warp's rows, the
-// warps of a block, the blocks; the counts are integers.  Results repeat bit for
-// bit.
+// A warp takes a row, NV scores a lane, in registers, and several rows at once where
+// registers allow: a row is a chain of shuffles and reductions, and what it waits for
+// is latency.  Exponentials, sums and gradients are fp32.  Sums over tokens have a
+// fixed order (a warp's rows, the warps of a block, the blocks of a cluster, the
+// clusters); the counts are integers.  Results repeat bit for bit.
 #pragma once
 #include "mb_common.cuh"
 #include "quantize.cuh"
@@ -33,7 +34,7 @@ namespace router {
 constexpr int MAX_EXPERTS = 1024;
 constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
-constexpr int MAX_PARTS = 256;      // blocks that sum up the balance, at most
+constexpr int CLUSTER = 8;          // blocks that sum up the balance together
 constexpr int MAX_K = 64;
 
 struct RouteArgs {
@@ -52,7 +53,7 @@ struct BalanceArgs {
   int T, E, k;
   const int *experts;      // [T, k]
   const uint8_t *mask;     // [T] or null: 0 leaves a token out
-  float *part_p;           // [parts, E]
+  float *part_p;           // [parts, E], a part a cluster
   int *part_c;             // [parts, E + 1]: counts, tokens
   int parts;
   float *loss;
@@ -108,6 +109,21 @@ __device__ __forceinline__ void store_scores(T *row, int E, int lane, const floa
   }
 }
 
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// A word of shared memory of the cluster's block `rank`.
+__device__ __forceinline__ int ld_cluster_s32(const int *p, uint32_t rank) {
+  uint32_t a = static_cast<uint32_t>(__cvta_generic_to_shared(p)), r;
+  int v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(r) : "memory");
+  return v;
+}
+__device__ __forceinline__ float ld_cluster_f32(const float *p, uint32_t rank) {
+  return __int_as_float(ld_cluster_s32(reinterpret_cast<const int *>(p), rank));
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
@@ -145,133 +161,262 @@ template <int NV> __device__ __forceinline__ float exponentials(float (&x)[NV]) 
   return s == 0.f ? 0.f : __fdividef(1.f, s);
 }
 
-template <class T, int NV, int V, bool AL>
-__global__ void __launch_bounds__(THREADS) route_kernel(const RouteArgs a) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  pdl_trigger();
-  pdl_wait();
-  for (int64_t t = (int64_t)blockIdx.x * WARPS + warp; t < a.T; t += (int64_t)gridDim.x * WARPS) {
-    float x[NV];
-    load_scores<T, NV, V, AL>(static_cast<const T *>(a.logits) + t * a.ld, a.E, lane, x);
-    uint32_t key[NV];
+// Rows that a warp takes at once.
+template <int NV> struct Rows { static constexpr int R = NV <= 4 ? 4 : NV <= 8 ? 2 : 1; };
+
+// A lane's keys as a queue: the largest in front, equal ones in their order.  Short
+// lists are sorted once (neighbours exchanged, so equal keys keep their order), long
+// ones searched again when their front has gone.
+template <int NV> struct Queue {
+  static constexpr bool SORTED = NV <= 4;
+  uint32_t key[NV], best;
+  int at, place[SORTED ? NV : 1];
+  __device__ __forceinline__ void search() {
+    best = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (key[i] > best) { best = key[i]; at = i; }
+  }
+  __device__ __forceinline__ void init(const float (&x)[NV]) {
+    at = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) key[i] = order_bits(x[i]);
-    const float base = base_of(x);
-    float total = 0.f;
-    if (!a.normalize) {
+    if constexpr (SORTED) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) total += expf(x[i] - base);
-      total = warp_sum(total);
-    }
-    // k rounds: the largest key, the lowest expert that has it
-    float chosen = 0.f;      // of round `lane` (and 32 + lane): exp(score - base)
-    float chosen2 = 0.f, sum = 0.f;
-    int id = -1, id2 = -1;
-    uint32_t best = 0;
-    int at = 0;
-    auto scan = [&]() {
-      best = 0;
+      for (int i = 0; i < NV; ++i) place[i] = i;
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (key[i] > best) { best = key[i]; at = i; }
-    };
-    scan();
-    for (int j = 0; j < a.k; ++j) {
-      const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-      if (top <= kNever) break;
-      const uint32_t e = __reduce_min_sync(0xffffffffu, best == top ? (uint32_t)slot<V>(at, lane) : 0xffffffffu);
-      const float w = expf(from_order_bits(top) - base);
-      sum += w;
-      if (lane == (j & 31)) {
-        if (j < 32) { chosen = w; id = (int)e; }
-        else { chosen2 = w; id2 = (int)e; }
-      }
-      if (best == top && (uint32_t)slot<V>(at, lane) == e) {
+      for (int r = 0; r < NV; ++r)
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if (i == at) key[i] = 0;
-        scan();
-      }
-    }
-    const float all = a.normalize ? sum : total;
-    const float inv = all == 0.f ? 0.f : __fdividef(1.f, all);
-    if (lane < a.k) {
-      a.weights[t * a.k + lane] = chosen * inv;
-      a.experts[t * a.k + lane] = id;
-    }
-    if (lane + 32 < a.k) {
-      a.weights[t * a.k + 32 + lane] = chosen2 * inv;
-      a.experts[t * a.k + 32 + lane] = id2;
+        for (int i = r & 1; i + 1 < NV; i += 2) {
+          const bool swap = key[i + 1] > key[i];
+          const uint32_t a = key[i], b = key[i + 1];
+          const int p = place[i], q = place[i + 1];
+          key[i] = swap ? b : a;
+          key[i + 1] = swap ? a : b;
+          place[i] = swap ? q : p;
+          place[i + 1] = swap ? p : q;
+        }
+      best = key[0];
+      at = place[0];
+    } else {
+      search();
     }
   }
-}
+  __device__ __forceinline__ void pop(bool mine) {
+    if constexpr (SORTED) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        key[i] = mine ? (i + 1 < NV ? key[i + 1 < NV ? i + 1 : i] : 0u) : key[i];
+        place[i] = mine && i + 1 < NV ? place[i + 1 < NV ? i + 1 : i] : place[i];
+      }
+      best = key[0];
+      at = place[0];
+    } else if (mine) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (i == at) key[i] = 0;
+      search();
+    }
+  }
+};
 
-template <class T, int NV, int V, bool AL>
-__global__ void __launch_bounds__(THREADS) route_backward_kernel(const RouteArgs a) {
+// MANY: k above 32, a second result a lane.
+template <class T, int NV, int V, bool AL, bool MANY>
+__global__ void __launch_bounds__(THREADS) route_kernel(const RouteArgs a) {
+  constexpr int R = MANY ? 1 : Rows<NV>::R;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_trigger();
   pdl_wait();
-  for (int64_t t = (int64_t)blockIdx.x * WARPS + warp; t < a.T; t += (int64_t)gridDim.x * WARPS) {
-    float x[NV], d[NV];
-    load_scores<T, NV, V, AL>(static_cast<const T *>(a.logits) + t * a.ld, a.E, lane, x);
-    const float inv = exponentials(x);
+  for (int64_t t0 = ((int64_t)blockIdx.x * WARPS + warp) * R; t0 < a.T; t0 += (int64_t)gridDim.x * WARPS * R) {
+    float x[R][NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) d[i] = 0.f;
-    // each entry's exponential and gradient go to the lane that holds its expert
-    float total = 0.f, dot = 0.f;   // of this lane's entries
-    for (int j0 = 0; j0 < a.k; j0 += 32) {
-      const bool on = j0 + lane < a.k;
-      const int mine = on ? a.experts[t * a.k + j0 + lane] : -1;
-      const float g = on ? a.grad[t * a.k + j0 + lane] : 0.f;
-      const int n = min(32, a.k - j0);
-      for (int j = 0; j < n; ++j) {
-        const int e = __shfl_sync(0xffffffffu, mine, j);
-        const float gj = __shfl_sync(0xffffffffu, g, j);
-        if ((unsigned)e >= (unsigned)a.E) continue;
+    for (int r = 0; r < R; ++r)   // (rows past the last are the last again)
+      load_scores<T, NV, V, AL>(static_cast<const T *>(a.logits) + min(t0 + r, (int64_t)a.T - 1) * a.ld, a.E, lane, x[r]);
+    float base[R], total[R];
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if (slot<V>(i, lane) == e) {
-            d[i] += x[i] * gj;
-            dot += x[i] * gj;
-            total += x[i];
+    for (int r = 0; r < R; ++r) {
+      base[r] = base_of(x[r]);
+      total[r] = 0.f;
+    }
+    if (!a.normalize) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) total[r] += expf(x[r][i] - base[r]);
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) total[r] = warp_sum(total[r]);
+    }
+    // k rounds: the largest key, the lowest expert that has it; lane j keeps round j's
+    // (its exponential is taken once at the end, not by every lane in every round).
+    Queue<NV> q[R];
+    uint32_t top[R], top2 = 0;
+    int id[R], id2 = -1;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      q[r].init(x[r]);
+      top[r] = kNever;
+      id[r] = -1;
+    }
+    for (int j = 0; j < a.k; ++j) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const uint32_t m = __reduce_max_sync(0xffffffffu, q[r].best);
+        const uint32_t own = (uint32_t)slot<V>(q[r].at, lane);
+        const uint32_t e = __reduce_min_sync(0xffffffffu, q[r].best == m ? own : 0xffffffffu);
+        if (m > kNever) {
+          if constexpr (MANY) {
+            if (lane == j) { top[r] = m; id[r] = (int)e; }
+            if (lane + 32 == j) { top2 = m; id2 = (int)e; }
+          } else {
+            top[r] = lane == j ? m : top[r];
+            id[r] = lane == j ? (int)e : id[r];
           }
+        }
+        q[r].pop(q[r].best == m && own == e);
       }
     }
-    dot = warp_sum(dot);
-    if (a.normalize) {
-      // w_j = x_j / total over the entries; an expert named twice counts twice
-      total = warp_sum(total);
-      const float r = total == 0.f ? 0.f : __fdividef(1.f, total);
-      const float mean = dot * r;
-      float c[NV];
 #pragma unroll
-      for (int i = 0; i < NV; ++i) c[i] = 0.f;
-      for (int j0 = 0; j0 < a.k; j0 += 32) {
-        const int mine = j0 + lane < a.k ? a.experts[t * a.k + j0 + lane] : -1;
-        const int n = min(32, a.k - j0);
-        for (int j = 0; j < n; ++j) {
-          const int e = __shfl_sync(0xffffffffu, mine, j);
-#pragma unroll
-          for (int i = 0; i < NV; ++i) c[i] += slot<V>(i, lane) == e ? 1.f : 0.f;
+    for (int r = 0; r < R; ++r) {
+      // exp(-inf) for entries that name no expert
+      float w = id[r] < 0 ? 0.f : expf(from_order_bits(top[r]) - base[r]), w2 = 0.f;
+      if constexpr (MANY) w2 = id2 < 0 ? 0.f : expf(from_order_bits(top2) - base[r]);
+      const float all = a.normalize ? warp_sum(w + w2) : total[r];
+      const float inv = all == 0.f ? 0.f : __fdividef(1.f, all);
+      const int64_t at = (t0 + r) * a.k + lane;
+      if (t0 + r < a.T) {
+        if (lane < a.k) {
+          a.weights[at] = w * inv;
+          a.experts[at] = id[r];
+        }
+        if (MANY && lane + 32 < a.k) {
+          a.weights[at + 32] = w2 * inv;
+          a.experts[at + 32] = id2;
         }
       }
-#pragma unroll
-      for (int i = 0; i < NV; ++i) d[i] = c[i] == 0.f ? 0.f : (d[i] - c[i] * x[i] * mean) * r;
-    } else {
-      const float mean = dot * inv;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) d[i] = (d[i] - x[i] * mean) * inv;
     }
-    store_scores<T, NV, V, AL>(static_cast<T *>(a.dlogits) + t * a.E, a.E, lane, d);
   }
 }
 
-// Sums of probabilities and counts of a block's tokens.
+// An expert's entries' gradients and their number go through shared memory, {G, n} a
+// place, E places a row: lanes write their entries and read their experts.  Two
+// entries with one number (each writes its lane and reads it back) are added one
+// after another instead.
+template <class T, int NV, int V, bool AL>
+__global__ void __launch_bounds__(THREADS) route_backward_kernel(const RouteArgs a) {
+  constexpr int R = Rows<NV>::R;
+  extern __shared__ float2 places[];   // [WARPS][R][32 NV]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float2 *own = places + warp * (R * 32 * NV);
+  pdl_trigger();
+  pdl_wait();
+  for (int64_t t0 = ((int64_t)blockIdx.x * WARPS + warp) * R; t0 < a.T; t0 += (int64_t)gridDim.x * WARPS * R) {
+    float x[R][NV];
+#pragma unroll
+    for (int r = 0; r < R; ++r)   // (rows past the last are the last again)
+      load_scores<T, NV, V, AL>(static_cast<const T *>(a.logits) + min(t0 + r, (int64_t)a.T - 1) * a.ld, a.E, lane, x[r]);
+    int e[R], e2[R];
+    float g[R], g2[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t at = min(t0 + r, (int64_t)a.T - 1) * a.k + lane;
+      e[r] = lane < a.k ? a.experts[at] : -1;
+      g[r] = lane < a.k ? a.grad[at] : 0.f;
+      e2[r] = lane + 32 < a.k ? a.experts[at + 32] : -1;
+      g2[r] = lane + 32 < a.k ? a.grad[at + 32] : 0.f;
+    }
+    __syncwarp();   // the last rows' places have been read
+#pragma unroll
+    for (int i = 0; i < R * NV; ++i) own[i * 32 + lane] = make_float2(0.f, 0.f);
+    __syncwarp();
+    auto put = [&](int r, int e, float g) {   // by the whole warp
+      float2 *p = own + r * 32 * NV;
+      const bool on = (unsigned)e < (unsigned)a.E;
+      const float before = on ? p[e].y : 0.f;
+      __syncwarp();
+      if (on) p[e].y = (float)(lane + 1);
+      __syncwarp();
+      const bool alone = !on || (before == 0.f && p[e].y == (float)(lane + 1));
+      if (__all_sync(0xffffffffu, alone)) {
+        if (on) p[e] = make_float2(g, 1.f);
+        __syncwarp();
+        return;
+      }
+      if (on) p[e].y = before;
+      __syncwarp();
+      for (int l = 0; l < 32; ++l) {
+        if (lane == l && on) p[e] = make_float2(p[e].x + g, p[e].y + 1.f);
+        __syncwarp();
+      }
+    };
+#pragma unroll
+    for (int r = 0; r < R; ++r) put(r, e[r], g[r]);
+    if (a.k > 32) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) put(r, e2[r], g2[r]);
+    }
+    float inv[R], total[R], dot[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) inv[r] = exponentials(x[r]);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      total[r] = dot[r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const float2 p = own[r * 32 * NV + slot<V>(i, lane)];
+        dot[r] = fmaf(x[r][i], p.x, dot[r]);
+        total[r] = fmaf(x[r][i], p.y, total[r]);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      dot[r] = warp_sum(dot[r]);
+      if (a.normalize) {
+        total[r] = warp_sum(total[r]);
+        inv[r] = total[r] == 0.f ? 0.f : __fdividef(1.f, total[r]);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float mean = dot[r] * inv[r];
+      float d[NV];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const float2 p = own[r * 32 * NV + slot<V>(i, lane)];
+        // normalize: the sum goes over the entries, an expert named twice counts twice
+        if (a.normalize) d[i] = p.y == 0.f ? 0.f : x[r][i] * (p.x - p.y * mean) * inv[r];
+        else d[i] = x[r][i] * (p.x - mean) * inv[r];
+      }
+      if (t0 + r < a.T) store_scores<T, NV, V, AL>(static_cast<T *>(a.dlogits) + (t0 + r) * a.E, a.E, lane, d);
+    }
+  }
+}
+
+// A block's sum of integers, the same in every thread.
+__device__ __forceinline__ int block_sum(int v, int *red) {
+  v = __reduce_add_sync(0xffffffffu, v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  const int warps = blockDim.x / 32, lane = threadIdx.x & 31;
+  return __reduce_add_sync(0xffffffffu, lane < warps ? red[lane] : 0);
+}
+__device__ __forceinline__ float balance_loss(int E, float dot, int total, int n) {
+  return n == 0 || total == 0 ? 0.f : (float)((double)E * dot / ((double)total * n));
+}
+
+// Sums of probabilities and counts of a cluster's tokens; with one cluster the loss too.
 template <class T, int NV, int V, bool AL>
 __global__ void __launch_bounds__(THREADS) balance_kernel(const BalanceArgs a) {
-  extern __shared__ float sums[];                            // [WARPS][E]
+  constexpr int R = Rows<NV>::R;
+  extern __shared__ float sums[];                            // [WARPS][E], then the block's in the first E
   int *hist = reinterpret_cast<int *>(sums + WARPS * a.E);   // [E + 1], the last one the tokens
+  __shared__ int red[WARPS];
+  __shared__ float dots[CLUSTER];
+  __shared__ int totals[CLUSTER];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t rank;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   for (int e = threadIdx.x; e <= a.E; e += THREADS) hist[e] = 0;
   __syncthreads();
   pdl_trigger();
@@ -280,18 +425,35 @@ __global__ void __launch_bounds__(THREADS) balance_kernel(const BalanceArgs a) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) p[i] = 0.f;
   int tokens = 0;
-  for (int64_t t = (int64_t)blockIdx.x * WARPS + warp; t < a.T; t += (int64_t)gridDim.x * WARPS) {
-    if (a.mask && !a.mask[t]) continue;
-    float x[NV];
-    load_scores<T, NV, V, AL>(static_cast<const T *>(a.logits) + t * a.ld, a.E, lane, x);
-    for (int j = lane; j < a.k; j += 32) {
-      const int e = a.experts[t * a.k + j];
-      if ((unsigned)e < (unsigned)a.E) atomicAdd(hist + e, 1);
-    }
-    const float inv = exponentials(x);
+  for (int64_t t0 = ((int64_t)blockIdx.x * WARPS + warp) * R; t0 < a.T; t0 += (int64_t)gridDim.x * WARPS * R) {
+    float x[R][NV], inv[R];
+    bool on[R];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) p[i] = fmaf(x[i], inv, p[i]);
-    ++tokens;
+    for (int r = 0; r < R; ++r) {
+      on[r] = t0 + r < a.T && (!a.mask || a.mask[t0 + r]);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) x[r][i] = -INFINITY;
+      if (on[r]) {
+        load_scores<T, NV, V, AL>(static_cast<const T *>(a.logits) + (t0 + r) * a.ld, a.E, lane, x[r]);
+        ++tokens;
+      }
+    }
+    for (int j = lane; j < R * a.k; j += 32) {
+      // entry j of the rows' R k
+      int r = 0, i = j;
+      while (i >= a.k) { i -= a.k; ++r; }
+      const int64_t t = t0 + r;
+      if (t < a.T && (!a.mask || a.mask[t])) {
+        const int e = a.experts[t * a.k + i];
+        if ((unsigned)e < (unsigned)a.E) atomicAdd(hist + e, 1);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) inv[r] = exponentials(x[r]);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int i = 0; i < NV; ++i) p[i] = on[r] ? fmaf(x[r][i], inv[r], p[i]) : p[i];
   }
   if (lane == 0 && tokens) atomicAdd(hist + a.E, tokens);
 #pragma unroll
@@ -302,55 +464,122 @@ __global__ void __launch_bounds__(THREADS) balance_kernel(const BalanceArgs a) {
     float s = 0.f;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) s += sums[w * a.E + e];
-    a.part_p[(int64_t)blockIdx.x * a.E + e] = s;
+    sums[e] = s;   // (this thread alone reads column e)
   }
-  for (int e = threadIdx.x; e <= a.E; e += THREADS) a.part_c[(int64_t)blockIdx.x * (a.E + 1) + e] = hist[e];
+  cluster_barrier();
+  // each rank adds up its share of the experts, in the order of the ranks
+  const int part = blockIdx.x / CLUSTER;
+  int total = 0, n = 0;
+  float dot = 0.f;
+  for (int e = threadIdx.x * CLUSTER + rank; e <= a.E; e += THREADS * CLUSTER) {
+    float s = 0.f;
+    int c = 0;
+#pragma unroll
+    for (int w = 0; w < CLUSTER; ++w) {
+      if (e < a.E) s += ld_cluster_f32(sums + e, w);
+      c += ld_cluster_s32(hist + e, w);
+    }
+    if (a.parts > 1) {
+      if (e < a.E) a.part_p[(int64_t)part * a.E + e] = s;
+      a.part_c[(int64_t)part * (a.E + 1) + e] = c;
+    } else if (e < a.E) {
+      a.counts[e] = c;
+      total += c;
+      dot = fmaf((float)c, s, dot);
+    }
+  }
+  if (a.parts > 1) {
+    cluster_barrier();   // no block leaves while others still read its sums
+    return;
+  }
+  if (threadIdx.x < CLUSTER) n = ld_cluster_s32(hist + a.E, threadIdx.x);
+  n = block_sum(n, red);
+  total = block_sum(total, red);
+  // the dot products of a block's warps and of the blocks, in order
+  dot = warp_sum(dot);
+  __shared__ float warp_dot[WARPS];
+  if (lane == 0) warp_dot[warp] = dot;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    dot = 0.f;
+    for (int w = 0; w < WARPS; ++w) dot += warp_dot[w];
+    dots[0] = dot;
+    totals[0] = total;
+  }
+  cluster_barrier();
+  if (rank == 0 && threadIdx.x == 0) {
+    dot = 0.f;
+    total = 0;
+    for (int w = 0; w < CLUSTER; ++w) {
+      dot += ld_cluster_f32(dots, w);
+      total += ld_cluster_s32(totals, w);
+    }
+    *a.tokens = n;
+    *a.loss = balance_loss(a.E, dot, total, n);
+  }
+  cluster_barrier();
 }
 
-// The blocks' sums to counts, tokens and loss: one block, in the order of the blocks.
+// The clusters' sums to counts, tokens and loss: one block, in the order of the clusters.
 __global__ static void __launch_bounds__(1024) balance_finish_kernel(const BalanceArgs a) {
-  __shared__ float red[32];
-  __shared__ int redi[32];
+  __shared__ float ps[1024];
+  __shared__ int cs[1024], red[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_trigger();
   pdl_wait();
+  // threads share an expert's parts where there are fewer experts than threads
+  const int E1 = a.E + 1, share = max(1, 1024 / E1), mine = threadIdx.x / E1;
   float dot = 0.f;
   int total = 0, n = 0;
-  for (int i = threadIdx.x; i < a.parts; i += 1024) n += a.part_c[(int64_t)i * (a.E + 1) + a.E];
-  for (int e = threadIdx.x; e < a.E; e += 1024) {
+  for (int e0 = 0; e0 < E1; e0 += 1024) {
+    const int e = share > 1 ? threadIdx.x % E1 : e0 + threadIdx.x;
     float s = 0.f;
     int c = 0;
-    for (int i = 0; i < a.parts; ++i) {
-      s += a.part_p[(int64_t)i * a.E + e];
-      c += a.part_c[(int64_t)i * (a.E + 1) + e];
+    if (e < E1 && (share == 1 || mine < share)) {
+      const int i0 = share > 1 ? a.parts * mine / share : 0, i1 = share > 1 ? a.parts * (mine + 1) / share : a.parts;
+#pragma unroll 8
+      for (int i = i0; i < i1; ++i) {
+        if (e < a.E) s += a.part_p[(int64_t)i * a.E + e];
+        c += a.part_c[(int64_t)i * E1 + e];
+      }
     }
-    a.counts[e] = c;
-    total += c;
-    dot = fmaf((float)c, s, dot);
+    if (share > 1) {
+      ps[threadIdx.x] = s;
+      cs[threadIdx.x] = c;
+      __syncthreads();
+      if (threadIdx.x < E1)
+        for (int w = 1; w < share; ++w) {
+          s += ps[w * E1 + threadIdx.x];
+          c += cs[w * E1 + threadIdx.x];
+        }
+    }
+    if (e < E1 && (share == 1 || mine == 0)) {
+      if (e < a.E) {
+        a.counts[e] = c;
+        total += c;
+        dot = fmaf((float)c, s, dot);
+      } else {
+        n += c;
+      }
+    }
   }
-  auto block_int = [&](int v) {
-    v = __reduce_add_sync(0xffffffffu, v);
-    __syncthreads();
-    if (lane == 0) redi[warp] = v;
-    __syncthreads();
-    return __reduce_add_sync(0xffffffffu, redi[lane]);
-  };
-  n = block_int(n);
-  total = block_int(total);
+  n = block_sum(n, red);
+  total = block_sum(total, red);
   dot = warp_sum(dot);
-  if (lane == 0) red[warp] = dot;
   __syncthreads();
-  if (warp == 0) {
-    dot = warp_sum(red[lane]);
-    if (lane == 0) {
-      *a.tokens = n;
-      *a.loss = n == 0 || total == 0 ? 0.f : (float)((double)a.E * dot / ((double)total * n));
-    }
+  if (lane == 0) ps[warp] = dot;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    dot = 0.f;
+    for (int w = 0; w < 32; ++w) dot += ps[w];
+    *a.tokens = n;
+    *a.loss = balance_loss(a.E, dot, total, n);
   }
 }
 
 template <class T, int NV, int V, bool AL>
 __global__ void __launch_bounds__(THREADS) balance_backward_kernel(const BalanceArgs a) {
+  constexpr int R = Rows<NV>::R;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_trigger();
   pdl_wait();
@@ -368,25 +597,35 @@ __global__ void __launch_bounds__(THREADS) balance_backward_kernel(const Balance
   const float f = n == 0 || total == 0 ? 0.f : (float)((double)*a.grad * a.E / ((double)total * n));
 #pragma unroll
   for (int i = 0; i < NV; ++i) s[i] *= f;
-  for (int64_t t = (int64_t)blockIdx.x * WARPS + warp; t < a.T; t += (int64_t)gridDim.x * WARPS) {
-    float x[NV];
-    if (a.mask && !a.mask[t]) {
+  for (int64_t t0 = ((int64_t)blockIdx.x * WARPS + warp) * R; t0 < a.T; t0 += (int64_t)gridDim.x * WARPS * R) {
+    float x[R][NV], inv[R], dot[R];
+    bool on[R];
 #pragma unroll
-      for (int i = 0; i < NV; ++i) x[i] = 0.f;
-    } else {
-      load_scores<T, NV, V, AL>(static_cast<const T *>(a.logits) + t * a.ld, a.E, lane, x);
-      const float inv = exponentials(x);
-      float dot = 0.f;
+    for (int r = 0; r < R; ++r) {
+      on[r] = t0 + r < a.T && (!a.mask || a.mask[t0 + r]);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) x[r][i] = -INFINITY;   // of a token left out: no probabilities, no gradient
+      if (on[r]) load_scores<T, NV, V, AL>(static_cast<const T *>(a.logits) + (t0 + r) * a.ld, a.E, lane, x[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) inv[r] = exponentials(x[r]);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      dot[r] = 0.f;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        x[i] *= inv;
-        dot = fmaf(x[i], s[i], dot);
+        x[r][i] *= inv[r];
+        dot[r] = fmaf(x[r][i], s[i], dot[r]);
       }
-      dot = warp_sum(dot);
-#pragma unroll
-      for (int i = 0; i < NV; ++i) x[i] *= s[i] - dot;
     }
-    store_scores<T, NV, V, AL>(static_cast<T *>(a.dlogits) + t * a.E, a.E, lane, x);
+#pragma unroll
+    for (int r = 0; r < R; ++r) dot[r] = warp_sum(dot[r]);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) x[r][i] *= s[i] - dot[r];
+      if (t0 + r < a.T) store_scores<T, NV, V, AL>(static_cast<T *>(a.dlogits) + (t0 + r) * a.E, a.E, lane, x[r]);
+    }
   }
 }
 
