@@ -250,7 +250,10 @@ def _bind_ops(lib) -> None:
 
 # What csrc/fastops.h calls, in its order.
 _FAST_OPS = ("mb_quantize", "mb_scaled_gemm", "mb_scaled_workspace_size", "mb_expert_sort", "mb_expert_gather",
-             "mb_expert_gather_quantize", "mb_expert_combine", "mb_expert_combine_backward")
+             "mb_expert_gather_quantize", "mb_expert_combine", "mb_expert_combine_backward", "mb_int4_quantize",
+             "mb_int4_dequantize", "mb_int4_gemm", "mb_int4_workspace_size", "mb_expert_route",
+             "mb_expert_route_backward", "mb_expert_balance", "mb_expert_balance_workspace_size",
+             "mb_expert_balance_backward")
 _fast = None
 _fast_tried = False
 
@@ -283,8 +286,11 @@ def fast():
                 raise RuntimeError("_mbfast was built against a different mb_gemm_desc; rebuild the package")
             fn = ctypes.cast(lib.mb_gemm, ctypes.c_void_p).value
             mod.set_gemm(fn)
-            if hasattr(mod, "set_ops") and hasattr(lib, "mb_scaled_gemm"):
-                mod.set_ops([ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _FAST_OPS])
+            if hasattr(mod, "set_ops") and all(hasattr(lib, name) for name in _FAST_OPS):
+                try:
+                    mod.set_ops([ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _FAST_OPS])
+                except RuntimeError:
+                    pass  # built for another list: serves none of them, so that the builder can run
         _fast = mod
         _fast_tried = True
         return _fast

@@ -1,5 +1,5 @@
-// Host fast path of the int8 products with scales and the expert routing, part
-// of the torch C++ extension of fastpath.cpp.
+// Host fast path of the int8 and 4-bit products, the expert routing and the router,
+// part of the torch C++ extension of fastpath.cpp.
 //
 // These operators are a few microseconds of GPU time in a decode step, less than
 // checking their arguments and allocating their results costs in Python.  Each
@@ -25,14 +25,26 @@ struct Ops {
   decltype(&mb_expert_gather_quantize) gather_quantize = nullptr;
   decltype(&mb_expert_combine) combine = nullptr;
   decltype(&mb_expert_combine_backward) combine_backward = nullptr;
+  decltype(&mb_int4_quantize) int4_quantize = nullptr;
+  decltype(&mb_int4_dequantize) int4_dequantize = nullptr;
+  decltype(&mb_int4_gemm) int4_gemm = nullptr;
+  decltype(&mb_int4_workspace_size) int4_ws = nullptr;
+  decltype(&mb_expert_route) route = nullptr;
+  decltype(&mb_expert_route_backward) route_backward = nullptr;
+  decltype(&mb_expert_balance) balance = nullptr;
+  decltype(&mb_expert_balance_workspace_size) balance_ws = nullptr;
+  decltype(&mb_expert_balance_backward) balance_backward = nullptr;
 };
 inline Ops g_ops;
 
 inline void set_ops(const std::vector<int64_t> &fn) {
-  TORCH_CHECK(fn.size() == 8, "set_ops: eight addresses expected");
+  TORCH_CHECK(fn.size() == 17, "set_ops: 17 addresses expected");
   auto set = [&](auto &f, int i) { f = reinterpret_cast<std::remove_reference_t<decltype(f)>>(fn[i]); };
   set(g_ops.quantize, 0); set(g_ops.scaled_gemm, 1); set(g_ops.scaled_ws, 2); set(g_ops.sort, 3);
   set(g_ops.gather, 4); set(g_ops.gather_quantize, 5); set(g_ops.combine, 6); set(g_ops.combine_backward, 7);
+  set(g_ops.int4_quantize, 8); set(g_ops.int4_dequantize, 9); set(g_ops.int4_gemm, 10); set(g_ops.int4_ws, 11);
+  set(g_ops.route, 12); set(g_ops.route_backward, 13);
+  set(g_ops.balance, 14); set(g_ops.balance_ws, 15); set(g_ops.balance_backward, 16);
 }
 
 // mb_dtype of a float tensor, or -1.
@@ -253,6 +265,190 @@ inline Pair try_combine_backward(const at::Tensor &grad, const at::Tensor &rows,
   return std::make_tuple(drows, dw);
 }
 
+// ------------------------------------------------------------------ 4-bit weights
+inline bool group_of(int64_t g) { return g == 32 || g == 64 || g == 128 || g == 256; }
+
+inline Pair try_int4_quantize(const at::Tensor &w, int64_t group, at::ScalarType scale_type) {
+  if (!g_ops.int4_quantize || !w.is_cuda() || !group_of(group)) return c10::nullopt;
+  const int dev = c10::cuda::current_device();
+  int64_t ld;
+  const int code = float_code(w.scalar_type()), sc = float_code(scale_type);
+  if (code < 0 || sc < 0 || !rows_of(w, dev, ld)) return c10::nullopt;
+  const int64_t rows = w.size(0), cols = w.size(1), bytes = (cols + 1) / 2, pitch = (bytes + 15) / 16 * 16;
+  at::Tensor q = at::empty({rows, pitch}, plain_options(dev, at::kByte));
+  at::Tensor scale = at::empty({rows, (cols + group - 1) / group}, plain_options(dev, scale_type));
+  if (g_ops.int4_quantize(code, sc, rows, cols, (int32_t)group, w.data_ptr(), ld, q.data_ptr<uint8_t>(), pitch,
+                          scale.data_ptr(), scale.size(1), stream_of(dev)) != MB_OK)
+    return c10::nullopt;
+  return std::make_tuple(pitch == bytes ? q : q.narrow(1, 0, bytes), scale);
+}
+
+// Rows of packed weights, their scales and zero points: [rows, .] matrices with contiguous rows.
+inline bool weight_of(const at::Tensor &q, const at::Tensor &scale, const c10::optional<at::Tensor> &zero, int64_t cols,
+                      int64_t group, int dim, int dev) {
+  if (q.dim() != dim || scale.dim() != dim || !here(q, dev) || !here(scale, dev) || q.scalar_type() != at::kByte) return false;
+  const int64_t bytes = (cols + 1) / 2, groups = (cols + group - 1) / group;
+  auto fits = [&](const at::Tensor &t, int64_t n) {
+    if (t.size(dim - 1) != n || (n > 1 && t.stride(dim - 1) != 1)) return false;
+    if (t.size(dim - 2) != q.size(dim - 2) || (dim == 3 && t.size(0) != q.size(0))) return false;
+    return (t.size(dim - 2) <= 1 || t.stride(dim - 2) >= n) && (dim < 3 || t.stride(0) >= 0);
+  };
+  if (!fits(q, bytes) || !fits(scale, groups)) return false;
+  return !zero.has_value() || (here(*zero, dev) && zero->dim() == dim && zero->scalar_type() == at::kByte && fits(*zero, groups));
+}
+
+inline One try_int4_dequantize(const at::Tensor &q, const at::Tensor &scale, const c10::optional<at::Tensor> &zero,
+                               int64_t cols, int64_t group, at::ScalarType out_type) {
+  if (!g_ops.int4_dequantize || !q.is_cuda() || !group_of(group) || cols < 0) return c10::nullopt;
+  const int dev = c10::cuda::current_device();
+  const int code = float_code(out_type), sc = float_code(scale.scalar_type());
+  if (code < 0 || sc < 0 || !weight_of(q, scale, zero, cols, group, 2, dev)) return c10::nullopt;
+  const int64_t rows = q.size(0);
+  at::Tensor out = at::empty({rows, cols}, plain_options(dev, out_type));
+  if (g_ops.int4_dequantize(code, sc, rows, cols, (int32_t)group, q.data_ptr<uint8_t>(), q.stride(0), scale.data_ptr(),
+                            scale.stride(0), zero.has_value() ? zero->data_ptr<uint8_t>() : nullptr,
+                            zero.has_value() ? zero->stride(0) : 0, out.data_ptr(), cols, stream_of(dev)) != MB_OK)
+    return c10::nullopt;
+  return out;
+}
+
+// x [M, K]; weights [N, .], or [E, N, .] with offsets [E + 1].
+inline One try_int4(const at::Tensor &x, const at::Tensor &q, const at::Tensor &scale, const c10::optional<at::Tensor> &zero,
+                    int64_t group, const c10::optional<at::Tensor> &offsets, const c10::optional<at::Tensor> &bias) {
+  if (!g_ops.int4_gemm || !x.is_cuda() || grad_of(x) || !group_of(group)) return c10::nullopt;
+  const int dev = c10::cuda::current_device(), g = offsets.has_value() ? 1 : 0;
+  int64_t ld;
+  const at::ScalarType type = x.scalar_type();
+  if ((type != at::kHalf && type != at::kBFloat16) || !rows_of(x, dev, ld)) return c10::nullopt;
+  const int64_t M = x.size(0), K = x.size(1);
+  if (!weight_of(q, scale, zero, K, group, 2 + g, dev) || (scale.scalar_type() != type && scale.scalar_type() != at::kFloat))
+    return c10::nullopt;
+  mb_int4_desc d;
+  memset(&d, 0, sizeof(d));
+  d.dtype = d.bias_dtype = float_code(type);
+  d.scale_dtype = float_code(scale.scalar_type());
+  d.group = (int32_t)group;
+  d.M = M; d.N = q.size(g); d.K = K;
+  d.x = x.data_ptr(); d.x_rs = ld;
+  d.w = q.data_ptr<uint8_t>(); d.w_rs = q.stride(g);
+  d.scale = scale.data_ptr(); d.scale_rs = scale.stride(g);
+  if (zero.has_value()) {
+    d.zero = zero->data_ptr<uint8_t>();
+    d.zero_rs = zero->stride(g);
+  }
+  if (g) {
+    const int64_t E = q.size(0);
+    if (E < 1 || !here(*offsets, dev) || offsets->scalar_type() != at::kInt || offsets->dim() != 1 ||
+        offsets->size(0) != E + 1 || !offsets->is_contiguous())
+      return c10::nullopt;
+    d.groups = E;
+    d.offsets = offsets->data_ptr<int32_t>();
+    d.w_e = q.stride(0);
+    d.scale_e = scale.stride(0);
+    if (zero.has_value()) d.zero_e = zero->stride(0);
+  }
+  if (bias.has_value()) {
+    if (!here(*bias, dev) || bias->dim() != 1 || bias->size(0) != d.N || (d.N > 1 && bias->stride(0) != 1) ||
+        (bias->scalar_type() != type && bias->scalar_type() != at::kFloat))
+      return c10::nullopt;
+    d.bias = bias->data_ptr();
+    d.bias_dtype = float_code(bias->scalar_type());
+  }
+  at::Tensor out = at::empty({M, d.N}, plain_options(dev, type)), ws;
+  d.out = out.data_ptr();
+  d.out_rs = d.N;
+  const int64_t need = g_ops.int4_ws(&d);
+  if (need > 0) {
+    ws = at::empty({need}, plain_options(dev, at::kByte));
+    d.workspace = ws.data_ptr();
+    d.workspace_bytes = need;
+  }
+  if (g_ops.int4_gemm(&d, stream_of(dev)) != MB_OK) return c10::nullopt;
+  return out;
+}
+
+// ------------------------------------------------------------------ router
+// Scores [T, E] of a float type; their row stride.
+inline bool scores_of(const at::Tensor &x, int dev, int &code, int64_t &ld) {
+  code = float_code(x.scalar_type());
+  return code >= 0 && rows_of(x, dev, ld) && x.size(1) >= 1 && x.size(1) <= 1024;
+}
+// int32 expert numbers [T, k].
+inline bool ids_of(const at::Tensor &ids, const at::Tensor &x, int dev) {
+  return here(ids, dev) && ids.scalar_type() == at::kInt && ids.dim() == 2 && ids.size(0) == x.size(0) && ids.is_contiguous();
+}
+inline bool mask_of(const c10::optional<at::Tensor> &mask, const at::Tensor &x, int dev, const uint8_t *&p) {
+  p = nullptr;
+  if (!mask.has_value()) return true;
+  if (!here(*mask, dev) || mask->scalar_type() != at::kBool || mask->dim() != 1 || mask->size(0) != x.size(0) || !mask->is_contiguous())
+    return false;
+  p = static_cast<const uint8_t *>(mask->data_ptr());
+  return true;
+}
+
+inline Pair try_route(const at::Tensor &x, int64_t k, bool normalize) {
+  if (!g_ops.route || !x.is_cuda() || grad_of(x)) return c10::nullopt;
+  const int dev = c10::cuda::current_device();
+  int code;
+  int64_t ld;
+  if (!scores_of(x, dev, code, ld) || k < 1 || k > x.size(1) || k > 64) return c10::nullopt;
+  const int64_t T = x.size(0);
+  at::Tensor w = at::empty({T, k}, plain_options(dev, at::kFloat)), ids = at::empty({T, k}, plain_options(dev, at::kInt));
+  if (g_ops.route(code, T, x.size(1), k, normalize, x.data_ptr(), ld, w.data_ptr<float>(), ids.data_ptr<int32_t>(),
+                  stream_of(dev)) != MB_OK)
+    return c10::nullopt;
+  return std::make_tuple(w, ids);
+}
+
+inline One try_route_backward(const at::Tensor &x, const at::Tensor &grad, const at::Tensor &ids, bool normalize) {
+  if (!g_ops.route_backward || !x.is_cuda()) return c10::nullopt;
+  const int dev = c10::cuda::current_device();
+  int code;
+  int64_t ld;
+  if (!scores_of(x, dev, code, ld) || !ids_of(ids, x, dev)) return c10::nullopt;
+  if (!here(grad, dev) || grad.scalar_type() != at::kFloat || grad.sizes() != ids.sizes() || !grad.is_contiguous()) return c10::nullopt;
+  at::Tensor out = at::empty({x.size(0), x.size(1)}, plain_options(dev, x.scalar_type()));
+  if (g_ops.route_backward(code, x.size(0), x.size(1), ids.size(1), normalize, grad.data_ptr<float>(), x.data_ptr(), ld,
+                           ids.data_ptr<int32_t>(), out.data_ptr(), stream_of(dev)) != MB_OK)
+    return c10::nullopt;
+  return out;
+}
+
+inline Triple try_balance(const at::Tensor &x, const at::Tensor &ids, const c10::optional<at::Tensor> &mask) {
+  if (!g_ops.balance || !x.is_cuda() || grad_of(x)) return c10::nullopt;
+  const int dev = c10::cuda::current_device();
+  int code;
+  int64_t ld;
+  const uint8_t *m;
+  if (!scores_of(x, dev, code, ld) || !ids_of(ids, x, dev) || !mask_of(mask, x, dev, m)) return c10::nullopt;
+  const int64_t T = x.size(0), E = x.size(1), need = g_ops.balance_ws(T, E);
+  at::Tensor loss = at::empty({}, plain_options(dev, at::kFloat)), counts = at::empty({E}, plain_options(dev, at::kInt)),
+             tokens = at::empty({}, plain_options(dev, at::kInt)), ws = at::empty({need}, plain_options(dev, at::kByte));
+  if (g_ops.balance(code, T, E, ids.size(1), x.data_ptr(), ld, ids.data_ptr<int32_t>(), m, loss.data_ptr<float>(),
+                    counts.data_ptr<int32_t>(), tokens.data_ptr<int32_t>(), ws.data_ptr(), need, stream_of(dev)) != MB_OK)
+    return c10::nullopt;
+  return std::make_tuple(loss, counts, tokens);
+}
+
+inline One try_balance_backward(const at::Tensor &x, const at::Tensor &grad, const at::Tensor &counts,
+                                const at::Tensor &tokens, const c10::optional<at::Tensor> &mask) {
+  if (!g_ops.balance_backward || !x.is_cuda()) return c10::nullopt;
+  const int dev = c10::cuda::current_device();
+  int code;
+  int64_t ld;
+  const uint8_t *m;
+  if (!scores_of(x, dev, code, ld) || !mask_of(mask, x, dev, m)) return c10::nullopt;
+  if (!here(grad, dev) || grad.scalar_type() != at::kFloat || grad.dim() != 0 || !here(counts, dev) ||
+      counts.scalar_type() != at::kInt || counts.dim() != 1 || counts.size(0) != x.size(1) || !counts.is_contiguous() ||
+      !here(tokens, dev) || tokens.scalar_type() != at::kInt || tokens.dim() != 0)
+    return c10::nullopt;
+  at::Tensor out = at::empty({x.size(0), x.size(1)}, plain_options(dev, x.scalar_type()));
+  if (g_ops.balance_backward(code, x.size(0), x.size(1), grad.data_ptr<float>(), x.data_ptr(), ld, counts.data_ptr<int32_t>(),
+                             tokens.data_ptr<int32_t>(), m, out.data_ptr(), stream_of(dev)) != MB_OK)
+    return c10::nullopt;
+  return out;
+}
+
 inline void bind(pybind11::module &m) {
   m.def("set_ops", &set_ops);
   // Arguments of other kinds (a scale that is no tensor) take the second form of
@@ -268,6 +464,13 @@ inline void bind(pybind11::module &m) {
   def("try_gather_quantize", &try_gather_quantize);
   def("try_combine", &try_combine);
   def("try_combine_backward", &try_combine_backward);
+  def("try_int4_quantize", &try_int4_quantize);
+  def("try_int4_dequantize", &try_int4_dequantize);
+  def("try_int4", &try_int4);
+  def("try_route", &try_route);
+  def("try_route_backward", &try_route_backward);
+  def("try_balance", &try_balance);
+  def("try_balance_backward", &try_balance_backward);
 }
 
 }  // namespace fastops

@@ -28,6 +28,10 @@ GROUP_SIZES = (32, 64, 128, 256)
 TOKENS = (torch.float16, torch.bfloat16)
 
 _byref = ctypes.byref
+# The host fast path (csrc/fastops.h): the result of a plain call, or None.
+_try_quantize = _lib.fast_op("try_int4_quantize")
+_try_dequantize = _lib.fast_op("try_int4_dequantize")
+_try_int4 = _lib.fast_op("try_int4")
 
 
 def _group(group_size):
@@ -59,7 +63,7 @@ def quantize_int4(w, group_size=128, *, scale_dtype=torch.float32):
     be shorter.  The rows of ``q`` start on 16-byte boundaries: with a number of columns that is
     no multiple of 32, ``q`` is a view of a wider tensor.  Neither carries a gradient.
     """
-    return _quantize(w, group_size, scale_dtype)
+    return _try_quantize(w, group_size, scale_dtype) or _quantize(w, group_size, scale_dtype)
 
 
 @_on_device
@@ -114,6 +118,10 @@ def dequantize_int4(q, scale, group_size=128, *, zero=None, cols=None, out_dtype
     ``out_dtype`` (fp32, fp16 or bf16), rounded once.  ``scale`` and the optional uint8 ``zero``
     are ``[..., ceil(cols / group_size)]``; ``cols`` is twice the bytes of a row unless given (an
     odd number of columns has to be)."""
+    if isinstance(q, torch.Tensor) and q.dim() == 2:
+        out = _try_dequantize(q, scale, zero, 2 * q.shape[1] if cols is None else cols, group_size, out_dtype)
+        if out is not None:
+            return out
     return _dequantize(q, scale, group_size, zero, cols, out_dtype)
 
 
@@ -217,6 +225,10 @@ def int4_mm(x, weight, scale, group_size=128, *, zero=None, bias=None, out=None,
     Weights are read in place when their rows start on 16-byte boundaries (``quantize_int4``'s
     do); others are copied into scratch in every call.
     """
+    if out is None and _plan is None:
+        y = _try_int4(x, weight, scale, zero, group_size, None, bias)
+        if y is not None:
+            return y
     return _int4_mm(x, weight, scale, group_size, zero, bias, out, _plan)
 
 
@@ -253,6 +265,10 @@ def grouped_int4_mm(x, weight, scale, offsets, group_size=128, *, zero=None, out
     groups cost nothing, and E is at most 1024.  Numbers that are not ascending name no groups:
     every row comes out as zeros.
     """
+    if out is None and _plan is None and offsets is not None:
+        y = _try_int4(x, weight, scale, zero, group_size, offsets, None)
+        if y is not None:
+            return y
     return _grouped_int4_mm(x, weight, scale, offsets, group_size, zero, out, _plan)
 
 

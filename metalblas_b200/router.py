@@ -23,6 +23,12 @@ from .quantized import _ld, _on_device, _rows
 
 MAX_K = 64
 
+# The host fast path (csrc/fastops.h): the result of a plain call, or None.
+_try_route = _lib.fast_op("try_route")
+_try_route_backward = _lib.fast_op("try_route_backward")
+_try_balance = _lib.fast_op("try_balance")
+_try_balance_backward = _lib.fast_op("try_balance_backward")
+
 
 class ExpertBalance(NamedTuple):
     """loss    fp32 scalar
@@ -114,6 +120,9 @@ def expert_route(logits, k, *, normalize=True):
     number -1 (``expert_sort`` drops it) and weight 0.  A NaN counts as the largest score; it
     and +inf make the token's weights NaN.  The weights take part in reverse-mode autograd.
     """
+    fast = _try_route(logits, k, normalize)
+    if fast is not None:
+        return fast
     _no_tangent(logits)
     if isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled():
         return _Route.apply(logits, k, normalize)
@@ -124,7 +133,8 @@ def expert_route_backward(grad, logits, experts, *, normalize=True):
     """Gradient of ``expert_route`` by the logits, of their type, from fp32 ``grad [T, k]`` and the
     call's own logits and experts.  Entries outside 0..E-1 contribute nothing.  The result
     carries no gradient."""
-    return _route_backward(logits, grad, experts, normalize)
+    out = _try_route_backward(logits, grad, experts, normalize)
+    return out if out is not None else _route_backward(logits, grad, experts, normalize)
 
 
 @_on_device
@@ -185,6 +195,9 @@ def expert_balance(logits, experts, mask=None):
     alone has no probabilities and adds nothing.  The loss takes part in reverse-mode autograd
     (the counts are constants).
     """
+    fast = _try_balance(logits, experts, mask)
+    if fast is not None:
+        return ExpertBalance(*fast)
     _no_tangent(logits)
     if isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled():
         return ExpertBalance(*_Balance.apply(logits, experts, mask))
@@ -194,7 +207,8 @@ def expert_balance(logits, experts, mask=None):
 def expert_balance_backward(grad, logits, balance, mask=None):
     """Gradient of ``expert_balance``'s loss by the logits, of their type, from the fp32 scalar
     ``grad`` and the call's own logits, mask and result.  The result carries no gradient."""
-    return _balance_backward(logits, grad, balance, mask)
+    out = _try_balance_backward(logits, grad, balance.counts, balance.tokens, mask)
+    return out if out is not None else _balance_backward(logits, grad, balance, mask)
 
 
 @_on_device
