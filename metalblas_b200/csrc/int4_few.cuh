@@ -45,15 +45,22 @@ template <int NT> struct FewCfg {
 template <class T>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (std::is_same_v<T, __half>)
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// One lane of the warp, the same at every call.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
 }
 
 // What a row's zero point is to the decoding of its nibbles.
@@ -133,7 +140,8 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 1)
   volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + Cfg::WARPS * Cfg::STAGES);
   int *first_unit = reinterpret_cast<int *>(bars + Cfg::WARPS * Cfg::STAGES + 1);
   int *row0 = first_unit + a.groups + 1, *scan = row0 + a.groups + 1;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const bool one = elect_one();
   const int g = lane >> 2, t4 = lane & 3;
   const int wrow = ((g & 1) << 2) | (g & 2) | (g >> 2);   // the weight row of MMA row g (shared-memory banks)
   const uint32_t ring = tc::smem_u32(smem) + warp * (Cfg::STAGES * FEW_ITEM);
@@ -184,77 +192,81 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 1)
     m1 = min(m1, m0 + TOKENS);
     const int tiles = (rows + 15) / 16, we = a.w_e == 0 ? 0 : e;
 
-    float *own = sums + warp * (Cfg::TILES * NT * 128) + lane * 4;
-    for (int i = 0; i < tiles * NT; ++i) *reinterpret_cast<float4 *>(own + i * 128) = make_float4(0.f, 0.f, 0.f, 0.f);
-
     // the slices whose scales fit, at a time (all of them, with groups of 128 columns and K up to 30000)
+    float *own = sums + warp * (Cfg::TILES * NT * 128) + lane * 4;
     const int per_slice = max(1, FEW_SLICE >> a.group_log2);
     const int fit = max(1, (Cfg::SCALES / WORDS / (tiles * 16) - 1) / per_slice);
     for (int s0 = 0; s0 < slices; s0 += fit) {
       const int s1 = min(slices, s0 + fit), items = (s1 - s0) * tiles;
       const int i0 = items * warp / Cfg::WARPS, i1 = items * (warp + 1) / Cfg::WARPS;
-      int fs = s0 + i0 / tiles, ft = i0 % tiles, fetched = i0;   // the next item to fetch
-      auto fetch = [&](int stage) {   // (by lane 0)
+      const int q_first = i0 / tiles, first = s0 + q_first, t_first = i0 - q_first * tiles;
+      const int last = i0 < i1 ? s0 + (i1 - 1) / tiles : -1;
+      int fs = first, ft = t_first, fetched = i0;   // the next item to fetch
+      auto fetch = [&](int stage) {   // (by one lane)
         if (fetched >= i1) return;
         tc::mbar_arrive_expect_tx(bar + 8 * stage, FEW_ITEM);
         tc::tma_load_3d(ring + stage * FEW_ITEM, &weights, bar + 8 * stage, fs * (FEW_SLICE / 2), n0 + ft * 16, we);
         ++fetched;
         if (++ft == tiles) { ft = 0; ++fs; }
       };
-      if (lane == 0) {
+      if (one) {
         int stage = st;
+#pragma unroll 1
         for (int i = 0; i < Cfg::STAGES; ++i) {
           fetch(stage);
           stage = stage + 1 == Cfg::STAGES ? 0 : stage + 1;
         }
       }
-      // the first slice's tokens
-      const int last = i0 < i1 ? s0 + (i1 - 1) / tiles : -1;
+      // a slice's tokens
       uint4 raw[NT][8];
       auto fetch_tokens = [&](int s) {
+        const int k0 = s * FEW_SLICE + t4 * (8 * LW);
+        const bool whole = x_aligned && (s + 1) * FEW_SLICE <= a.K;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           const int m = m0 + n * 8 + g;
-          const T *row = static_cast<const T *>(a.x) + (int64_t)m * a.x_rs;
+          const T *row = static_cast<const T *>(a.x) + (int64_t)m * a.x_rs + k0;
 #pragma unroll
           for (int v = 0; v < 8; ++v) {
-            const int k = s * FEW_SLICE + (v / LW) * SUB + t4 * (8 * LW) + (v % LW) * 8;
-            raw[n][v] = m < m1 ? token_word(row, k, a.K, x_aligned) : make_uint4(0, 0, 0, 0);
+            const int k = (v / LW) * SUB + (v % LW) * 8;
+            raw[n][v] = make_uint4(0, 0, 0, 0);
+            if (m < m1) raw[n][v] = whole ? *reinterpret_cast<const uint4 *>(row + k) : token_word(row - k0, k0 + k, a.K, x_aligned);
           }
         }
       };
-      if (i0 < i1) fetch_tokens(s0 + i0 / tiles);
-      // scales of the rows, fp32; an odd pitch, so that eight rows meet eight banks
+      if (i0 < i1) fetch_tokens(first);
+      if (s0 == 0)
+        for (int i = 0; i < tiles * NT; ++i) *reinterpret_cast<float4 *>(own + i * 128) = make_float4(0.f, 0.f, 0.f, 0.f);
+      // scales of the rows, fp32; an odd pitch, so that eight rows meet eight banks;
       // and zeros for groups past the end, whose sums are zeros
       const int q0 = (s0 * FEW_SLICE) >> a.group_log2, qn = (s1 - s0) * per_slice, pitch = qn | 1;
-      // (a row a warp, and eight loads on their way at a time: one after another they were 4 of 19 us)
+      // (a row a warp, and all of a warp's rows on their way at a time: one after another they were
+      // 4 of 19 us)
+      constexpr int BATCH = (16 * Cfg::TILES + Cfg::WARPS - 1) / Cfg::WARPS;
       for (int q = lane; q < qn; q += 32) {
         const bool on = q0 + q < groups;
-        const int64_t i_s = e * a.s_e + (int64_t)n0 * a.s_rs + q0 + q, i_z = e * a.z_e + (int64_t)n0 * a.z_rs + q0 + q;
-        for (int r0 = warp; r0 < rows; r0 += 8 * Cfg::WARPS) {
-          uint32_t v[8];
-          uint8_t z[8];
+        const int64_t i_s = e * a.s_e + (int64_t)(n0 + warp) * a.s_rs + q0 + q, i_z = e * a.z_e + (int64_t)(n0 + warp) * a.z_rs + q0 + q;
+        uint32_t v[BATCH];
+        uint8_t z[BATCH];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int r = r0 + j * Cfg::WARPS;
-            const bool load = on && r < rows;
-            v[j] = load ? scale_bits<T>(a, i_s + r * a.s_rs) : 0u;
-            if constexpr (ZERO) z[j] = load ? a.zero[i_z + r * a.z_rs] : 0;
-          }
+        for (int j = 0; j < BATCH; ++j) {
+          const bool load = on && warp + j * Cfg::WARPS < rows;
+          v[j] = load ? scale_bits<T>(a, i_s + j * Cfg::WARPS * a.s_rs) : 0u;
+          if constexpr (ZERO) z[j] = load ? a.zero[i_z + j * Cfg::WARPS * a.z_rs] : 0;
+        }
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int r = r0 + j * Cfg::WARPS;
-            if (r >= rows) break;
-            const float f = scale_of<T>(a, v[j]);
-            if constexpr (ZERO) reinterpret_cast<float2 *>(scales)[r * pitch + q] = make_float2(f, (float)z[j]);
-            else scales[r * pitch + q] = f;
-          }
+        for (int j = 0; j < BATCH; ++j) {
+          const int r = warp + j * Cfg::WARPS;
+          if (r >= rows) break;
+          const float f = scale_of<T>(a, v[j]);
+          if constexpr (ZERO) reinterpret_cast<float2 *>(scales)[r * pitch + q] = make_float2(f, (float)z[j]);
+          else scales[r * pitch + q] = f;
         }
       }
       __syncthreads();
 
       uint32_t x[NT][8][4];
-      int s = s0 + i0 / tiles, t = i0 % tiles, held = -1, i = i0;
+      int s = first, t = t_first, held = -1, i = i0;
       for (; i < i1; ++i) {
         if (s != held) {
           held = s;
@@ -284,7 +296,7 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 1)
           }
         }
         __syncwarp();
-        if (lane == 0) fetch(st);
+        if (one) fetch(st);
         if (++st == Cfg::STAGES) { st = 0; phase ^= 1u; }
 
         // (rows past the end have any numbers for scales: their sums are not stored)
@@ -337,7 +349,7 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 1)
         }
         if (++t == tiles) { t = 0; ++s; }
       }
-      if (i < i1 && lane == 0) {
+      if (i < i1 && one) {
         // given up: the copies on their way land before the block can leave
         volatile int no_abort = 0;
         for (; i < fetched; ++i) {
@@ -347,7 +359,10 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 1)
       }
       if (__syncthreads_or(*abort_flag)) return;
     }
-    if (slices == 0) __syncthreads();
+    if (slices == 0) {
+      for (int i = 0; i < tiles * NT; ++i) *reinterpret_cast<float4 *>(own + i * 128) = make_float4(0.f, 0.f, 0.f, 0.f);
+      __syncthreads();
+    }
     // four results of a tile: rows r and r + 8, tokens c and c + 1
     for (int i = tid; i < tiles * NT * 32; i += Cfg::THREADS) {
       const int l = i & 31, tn = i >> 5, tile = tn / NT, n = tn - tile * NT;
