@@ -107,15 +107,7 @@ template <bool ZERO> struct Decode<__half, ZERO> {
   }
 };
 
-// The 8 columns of a token from k on, zeros past K; and as the pairs (0, 4), (1, 5), (2, 6), (3, 7).
-template <class T>
-__device__ __forceinline__ uint4 token_word(const T *row, int k, int K, bool aligned) {
-  if (aligned && k + 8 <= K) return *reinterpret_cast<const uint4 *>(row + k);
-  uint16_t t[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) t[i] = k + i < K ? reinterpret_cast<const uint16_t *>(row)[k + i] : 0;
-  return make_uint4(t[0] | t[1] << 16, t[2] | t[3] << 16, t[4] | t[5] << 16, t[6] | t[7] << 16);
-}
+// 8 columns of a token as the pairs (0, 4), (1, 5), (2, 6), (3, 7).
 __device__ __forceinline__ void token_pairs(const uint4 &v, uint32_t (&o)[4]) {
   o[0] = __byte_perm(v.x, v.z, 0x5410);
   o[1] = __byte_perm(v.x, v.z, 0x7632);
@@ -127,7 +119,7 @@ __device__ __forceinline__ void token_pairs(const uint4 &v, uint32_t (&o)[4]) {
 // one group (1: groups of 32 columns, 2: 64, 4: 128 and 256).
 template <class T, int LW, int NT, bool ZERO>
 __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 1)
-    int4_few_kernel(const __grid_constant__ GemmArgs a, const __grid_constant__ CUtensorMap weights, int x_aligned,
+    int4_few_kernel(const __grid_constant__ GemmArgs a, const __grid_constant__ CUtensorMap weights,
                     unsigned long long timeout_ns) {
   using Cfg = FewCfg<NT>;
   constexpr int TOKENS = 8 * NT, SUB = 32 * LW, SUBS = FEW_SLICE / SUB;  // columns scaled together, and such in a slice
@@ -209,6 +201,34 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 1)
         ++fetched;
         if (++ft == tiles) { ft = 0; ++fs; }
       };
+      // a slice's tokens
+      uint4 raw[NT][8];
+      auto fetch_tokens = [&](int s) {
+        const int k0 = s * FEW_SLICE + t4 * (8 * LW);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const int m = m0 + n * 8 + g;
+          const T *row = static_cast<const T *>(a.x) + (int64_t)m * a.x_rs + k0;
+          const bool on = m < m1;
+          if ((s + 1) * FEW_SLICE <= a.K) {
+#pragma unroll
+            for (int v = 0; v < 8; ++v) {
+              raw[n][v] = make_uint4(0, 0, 0, 0);
+              if (on) raw[n][v] = *reinterpret_cast<const uint4 *>(row + (v / LW) * SUB + (v % LW) * 8);
+            }
+          } else {   // (rows hold whole 16 bytes: the host has copied others)
+#pragma unroll
+            for (int v = 0; v < 8; ++v) {
+              const int k = (v / LW) * SUB + (v % LW) * 8, left = a.K - k0 - k;
+              Vec<T> w;
+              w.zero();
+              if (on && left > 0) w.u.q = *reinterpret_cast<const uint4 *>(row + k);
+              keep_first(w, max(left, 0));
+              raw[n][v] = w.u.q;
+            }
+          }
+        }
+      };
       if (one) {
         int stage = st;
 #pragma unroll 1
@@ -217,47 +237,33 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 1)
           stage = stage + 1 == Cfg::STAGES ? 0 : stage + 1;
         }
       }
-      // a slice's tokens
-      uint4 raw[NT][8];
-      auto fetch_tokens = [&](int s) {
-        const int k0 = s * FEW_SLICE + t4 * (8 * LW);
-        const bool whole = x_aligned && (s + 1) * FEW_SLICE <= a.K;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const int m = m0 + n * 8 + g;
-          const T *row = static_cast<const T *>(a.x) + (int64_t)m * a.x_rs + k0;
-#pragma unroll
-          for (int v = 0; v < 8; ++v) {
-            const int k = (v / LW) * SUB + (v % LW) * 8;
-            raw[n][v] = make_uint4(0, 0, 0, 0);
-            if (m < m1) raw[n][v] = whole ? *reinterpret_cast<const uint4 *>(row + k) : token_word(row - k0, k0 + k, a.K, x_aligned);
-          }
-        }
-      };
       if (i0 < i1) fetch_tokens(first);
       if (s0 == 0)
         for (int i = 0; i < tiles * NT; ++i) *reinterpret_cast<float4 *>(own + i * 128) = make_float4(0.f, 0.f, 0.f, 0.f);
       // scales of the rows, fp32; an odd pitch, so that eight rows meet eight banks;
       // and zeros for groups past the end, whose sums are zeros
+      // (A row a warp, and all of its rows' loads on their way at a time or, where the block has few
+      // rows, spans of two: one after another they were 4 of 19 us.)
       const int q0 = (s0 * FEW_SLICE) >> a.group_log2, qn = (s1 - s0) * per_slice, pitch = qn | 1;
-      // (a row a warp, and all of a warp's rows on their way at a time: one after another they were
-      // 4 of 19 us)
       constexpr int BATCH = (16 * Cfg::TILES + Cfg::WARPS - 1) / Cfg::WARPS;
-      for (int q = lane; q < qn; q += 32) {
-        const bool on = q0 + q < groups;
-        const int64_t i_s = e * a.s_e + (int64_t)(n0 + warp) * a.s_rs + q0 + q, i_z = e * a.z_e + (int64_t)(n0 + warp) * a.z_rs + q0 + q;
+      const bool narrow = rows <= 2 * Cfg::WARPS;
+      const int64_t i_s = e * a.s_e + (int64_t)(n0 + warp) * a.s_rs + q0 + lane;
+      const int64_t i_z = e * a.z_e + (int64_t)(n0 + warp) * a.z_rs + q0 + lane;
+      const int64_t step_s = Cfg::WARPS * a.s_rs, step_z = Cfg::WARPS * a.z_rs;
+      for (int qb = 0; qb < qn; qb += narrow ? 32 * (BATCH / 2) : 32) {
         uint32_t v[BATCH];
         uint8_t z[BATCH];
 #pragma unroll
         for (int j = 0; j < BATCH; ++j) {
-          const bool load = on && warp + j * Cfg::WARPS < rows;
-          v[j] = load ? scale_bits<T>(a, i_s + j * Cfg::WARPS * a.s_rs) : 0u;
-          if constexpr (ZERO) z[j] = load ? a.zero[i_z + j * Cfg::WARPS * a.z_rs] : 0;
+          const int row = narrow ? j & 1 : j, q = qb + (narrow ? (j >> 1) * 32 : 0);
+          const bool load = warp + row * Cfg::WARPS < rows && q + lane < qn && q0 + q + lane < groups;
+          v[j] = load ? scale_bits<T>(a, i_s + row * step_s + q) : 0u;
+          if constexpr (ZERO) z[j] = load ? a.zero[i_z + row * step_z + q] : 0;
         }
 #pragma unroll
         for (int j = 0; j < BATCH; ++j) {
-          const int r = warp + j * Cfg::WARPS;
-          if (r >= rows) break;
+          const int row = narrow ? j & 1 : j, q = qb + (narrow ? (j >> 1) * 32 : 0) + lane, r = warp + row * Cfg::WARPS;
+          if (r >= rows || q >= qn) continue;
           const float f = scale_of<T>(a, v[j]);
           if constexpr (ZERO) reinterpret_cast<float2 *>(scales)[r * pitch + q] = make_float2(f, (float)z[j]);
           else scales[r * pitch + q] = f;

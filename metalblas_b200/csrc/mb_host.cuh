@@ -107,7 +107,7 @@ int launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaS
 
 // Lets a kernel use `bytes` of dynamic shared memory; once per kernel and device.
 template <auto Kernel>
-int allow_smem(int bytes) {
+static int allow_smem(int bytes) {
   static std::atomic<bool> done[64];
   int dev = 0;
   int rc = cuda_check(cudaGetDevice(&dev), "cudaGetDevice");

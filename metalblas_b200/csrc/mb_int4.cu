@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <cmath>
 #include <cstring>
 #include <type_traits>
 
@@ -126,9 +127,8 @@ int few_launch_as(const i4::GemmArgs &a, cudaStream_t st) {
     rc = encode_map(&w, MB_U8, a.w, bytes, a.N, a.w_e == 0 ? 1 : std::max(a.groups, 1), a.N == 1 ? round_up(bytes, 16) : a.w_rs, a.w_e,
                     i4::FEW_SLICE / 2, 16);
   if (rc) return rc;
-  const int x_aligned = rows16(a.x, a.M, a.x_rs, 2);
   return launch_pdl(kern, dim3((unsigned)device_sms()), dim3(Cfg::THREADS), Cfg::smem(a.groups), st, 1, "int4_gemm", a, w,
-                    x_aligned, wait_timeout_ns());
+                    wait_timeout_ns());
 }
 template <class T, int LW, int NT>
 int few_launch_lw(const i4::GemmArgs &a, cudaStream_t st) {
@@ -165,44 +165,84 @@ struct Plan {
   int64_t x_off = 0, w_off = 0, ws_bytes = 0;
 };
 
+// Tiles of `rows` tokens that the groups are expected to have, groups of equal size at even odds.
+// (They do not end on tiles' ends: half a tile more each.)
+double expected_tiles(const mb_int4_desc *d, int rows) {
+  if (!d->groups) return std::ceil((double)d->M / rows);
+  const double E = (double)d->groups, used = E * (1.0 - std::pow(1.0 - 1.0 / E, (double)d->M)), each = d->M / used;
+  return used * (each > rows / 2 ? each / rows + 0.5 : 1.0);
+}
+// A product's time in us by either kernel, fitted to times on B200 of each forced in turn
+// over 30 products, 20 of them dense, of 1 to 8192 rows and K of 512 to 14336 (within 15 %
+// but for three; the choice was the best or within 5 % of it in all).  The one-pass
+// kernel: start, weights, tokens that a warp takes anew for every slice of columns, passes of
+// 112 rows of a block.  4096 x 14336 by one row 15.5, by 16 rows 20.8; tcgen05 22.9 and
+// 22.9.  16 rows of 8192 x 2048: 22 and 15.5.
+double few_cost(const mb_int4_desc *d, int nt, int sms) {
+  const double units = expected_tiles(d, 8 * nt), rows = units * d->N / sms;
+  const double weight = (nt == 1 ? 0.178e-6 : 0.255e-6) * (d->group == 32 ? 1.36 : d->group == 64 ? 1.09 : 1.0);
+  const double again = 1.0 + (nt == 1 ? 0.5 : 0.9) * (1.0 / std::max(1.0, std::min(rows / 16, 7.0)) - 1.0 / 7.0);
+  return (nt == 1 ? 4.9 : 6.0) + units * d->N * (double)d->K * weight * again + 2.0 * std::max(0.0, rows / 112 - 1.0);
+}
+// The tcgen05 kernel: a step of 128 columns takes its MMA and decoding or, with several sums
+// a step, the way of each accumulator to the sums and back.
+double tc_cost(const mb_int4_desc *d, int bn, int split, int sms) {
+  const double steps = std::ceil(d->K / 128.0) / split;
+  const int sums = d->group < 128 ? 128 / d->group : 1;
+  const double step = std::max(bn == 256 ? 1.02 : bn == 128 ? 0.62 : bn == 64 ? 0.57 : 0.52,
+                               sums == 1 ? 0.0 : sums * (bn == 256 ? 0.65 : bn == 128 ? 0.4 : 0.36));
+  const double tile = bn == 256 ? 3.0 : bn == 128 ? 1.5 : 1.0;
+  // clusters of 4 and 8 leave SMs over in some GPCs
+  const double slots = std::floor((double)sms / split * (split == 8 ? 0.75 : split == 4 ? 0.9 : 1.0));
+  const double units = expected_tiles(d, bn) * (double)ceil_div(d->N, 128);
+  const double waves = d->groups ? std::max(1.0, units / slots + 0.5) : std::ceil(units / slots);
+  return 4.0 + waves * (tile + std::ceil(steps) * step) + 1.3 * std::log2((double)split);
+}
+
 int int4_plan(const mb_int4_desc *d, Plan &pl) {
   pl.x_rs = d->x_rs;
   pl.w_rs = d->w_rs;
   pl.w_e = d->w_e;
   if (d->M == 0 || d->N == 0) return MB_OK;
   const int64_t E = std::max<int64_t>(d->groups, 1), bytes = (d->K + 1) / 2;
-  const int64_t active = d->groups ? std::min(E, d->M) : 1;
-  const double rows = (double)d->M / active;
-  const int want = d->plan[0];
+  const int want = d->plan[0], split = d->plan[1], sms = device_sms();
   if (want != 0 && want != 1 && want != 2 && want != 16 && want != 32 && want != 64 && want != 128 && want != 256)
     return fail(MB_ERR_INVALID, "no plan %d", want);
-  // the one-pass kernel counts rows of units in 32 bits
-  auto few_fits = [&](int nt) { return (ceil_div(d->M, 8 * nt) + (d->groups ? E : 0)) * d->N < (1ll << 32); };
-  if (want == 1 || want == 2) {
-    pl.few = want;
-  } else if (!want && (d->K == 0 || rows <= 16)) {
-    pl.few = rows <= 8 ? 1 : 2;
-  }
-  if (pl.few && !few_fits(pl.few)) {
-    if (want || d->K == 0) return fail(MB_ERR_INVALID, "too many rows");
-    pl.few = 0;
-  }
-  if (!pl.few) {
-    pl.bn = want >= 16 ? want : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 256 ? 128 : 256;
-    const int64_t tiles_n = ceil_div(d->N, 128), stages = ceil_div(d->K, 256);
-    pl.units = (ceil_div(d->M, pl.bn) + (d->groups ? active : 0)) * tiles_n;
-    if (pl.units >= (1ll << 31)) return fail(MB_ERR_INVALID, "too many tiles");
-    const int sms = device_sms();
-    if (d->plan[1]) {
-      pl.split = d->plan[1];
-      if (pl.split != 1 && pl.split != 2 && pl.split != 4 && pl.split != 8) return fail(MB_ERR_INVALID, "a split is 1, 2, 4 or 8");
-      if (pl.split > (pl.bn == 256 ? 1 : stages)) return fail(MB_ERR_INVALID, "a split of %d exceeds the columns", pl.split);
-    } else {
-      while (pl.bn < 256 && pl.split < 8 && pl.units * pl.split * 2 <= sms && pl.split * 2 <= stages) pl.split *= 2;
+  if (split != 0 && split != 1 && split != 2 && split != 4 && split != 8) return fail(MB_ERR_INVALID, "a split is 1, 2, 4 or 8");
+  const int64_t stages = ceil_div(d->K, 256);
+  double best = 1e300;
+  for (const int nt : {1, 2}) {
+    if (want ? want != nt : d->K > 0 && split) continue;
+    // (the one-pass kernel counts rows of units in 32 bits)
+    if ((ceil_div(d->M, 8 * nt) + (d->groups ? E : 0)) * d->N >= (1ll << 32)) continue;
+    const double t = few_cost(d, nt, sms);
+    if (t < best) {
+      best = t;
+      pl.few = nt;
     }
   }
+  for (const int bn : {16, 32, 64, 128, 256}) {
+    if (want ? want != bn : d->K == 0) continue;
+    const int64_t units = (ceil_div(d->M, bn) + (d->groups ? std::min(E, d->M) : 0)) * ceil_div(d->N, 128);
+    if (units >= (1ll << 31)) continue;
+    for (const int sp : {1, 2, 4, 8}) {
+      if (split ? split != sp : (units * sp > 2 * sms && sp > 1)) continue;
+      if (sp > 1 && (bn == 256 || sp > stages)) continue;
+      const double t = tc_cost(d, bn, sp, sms);
+      if (t < best) {
+        best = t;
+        pl.few = 0;
+        pl.bn = bn;
+        pl.split = sp;
+        pl.units = units;
+      }
+    }
+  }
+  if (!pl.few && !pl.bn) return fail(MB_ERR_INVALID, want || split ? "no kernel has plan %d with split %d" : "too many rows", want, split);
   int64_t at = 0;
-  if (!pl.few && !rows16(d->x, d->M, d->x_rs, 2)) {
+  // tokens are read 16 bytes at a time; where their columns end inside these, only from rows that go on to
+  // their end
+  if (d->K > 0 && (!rows16(d->x, d->M, d->x_rs, 2) || (pl.few && d->K % 8))) {
     pl.pk_x = 1;
     pl.x_off = at;
     pl.x_rs = round_up(d->K, 8);

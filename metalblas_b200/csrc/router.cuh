@@ -140,12 +140,20 @@ __device__ __forceinline__ float from_order_bits(uint32_t o) {
   return __uint_as_float(o == 0xffffffffu ? 0x7fc00000u : (o & 0x80000000u ? o ^ 0x80000000u : ~o));
 }
 
+// exp(y) for y <= 0, within (|y| / 2 + 2) 2^-23 of it: what rounds is the exponent y / ln 2, and
+// where that is large the result is small against the row's sum.  (expf takes three times as
+// many instructions, a fifth of all in the kernels without a choice of experts.)
+__device__ __forceinline__ float exponential(float y) { return __expf(y); }
+
 // The row's largest score, or 0 when there is no number above -inf (a base of exponentials).
 template <int NV> __device__ __forceinline__ float base_of(const float (&x)[NV]) {
   float m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < NV; ++i) m = fmaxf(m, x[i]);
-  m = from_order_bits(__reduce_max_sync(0xffffffffu, order_bits(m)));
+  // signed integers in the order of the floats (NaN where a lane has nothing else: every
+  // exponential of it is NaN whatever the base)
+  auto flip = [](int b) { return b ^ ((b >> 31) & 0x7fffffff); };
+  m = __int_as_float(flip(__reduce_max_sync(0xffffffffu, flip(__float_as_int(m)))));
   return m == -INFINITY ? 0.f : m;
 }
 // exp(x - base) in place, and 1 / their sum over the row (0 for a sum of 0).
@@ -154,7 +162,7 @@ template <int NV> __device__ __forceinline__ float exponentials(float (&x)[NV]) 
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    x[i] = expf(x[i] - base);
+    x[i] = exponential(x[i] - base);
     s += x[i];
   }
   s = warp_sum(s);
@@ -242,7 +250,7 @@ __global__ void __launch_bounds__(THREADS) route_kernel(const RouteArgs a) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) total[r] += expf(x[r][i] - base[r]);
+        for (int i = 0; i < NV; ++i) total[r] += exponential(x[r][i] - base[r]);
       }
 #pragma unroll
       for (int r = 0; r < R; ++r) total[r] = warp_sum(total[r]);
@@ -279,8 +287,8 @@ __global__ void __launch_bounds__(THREADS) route_kernel(const RouteArgs a) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       // exp(-inf) for entries that name no expert
-      float w = id[r] < 0 ? 0.f : expf(from_order_bits(top[r]) - base[r]), w2 = 0.f;
-      if constexpr (MANY) w2 = id2 < 0 ? 0.f : expf(from_order_bits(top2) - base[r]);
+      float w = id[r] < 0 ? 0.f : exponential(from_order_bits(top[r]) - base[r]), w2 = 0.f;
+      if constexpr (MANY) w2 = id2 < 0 ? 0.f : exponential(from_order_bits(top2) - base[r]);
       const float all = a.normalize ? warp_sum(w + w2) : total[r];
       const float inv = all == 0.f ? 0.f : __fdividef(1.f, all);
       const int64_t at = (t0 + r) * a.k + lane;
@@ -438,22 +446,20 @@ __global__ void __launch_bounds__(THREADS) balance_kernel(const BalanceArgs a) {
         ++tokens;
       }
     }
-    for (int j = lane; j < R * a.k; j += 32) {
-      // entry j of the rows' R k
-      int r = 0, i = j;
-      while (i >= a.k) { i -= a.k; ++r; }
-      const int64_t t = t0 + r;
-      if (t < a.T && (!a.mask || a.mask[t])) {
-        const int e = a.experts[t * a.k + i];
-        if ((unsigned)e < (unsigned)a.E) atomicAdd(hist + e, 1);
-      }
+    const int *ids = a.experts + t0 * a.k;
+    const int entries = (int)min((int64_t)R, a.T - t0) * a.k;   // of the rows, next to one another
+    for (int j = lane; j < entries; j += 32) {
+      const int e = ids[j];
+      bool count = (unsigned)e < (unsigned)a.E;
+      if (a.mask) count = count && a.mask[t0 + j / a.k];
+      if (count) atomicAdd(hist + e, 1);
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) inv[r] = exponentials(x[r]);
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int i = 0; i < NV; ++i) p[i] = on[r] ? fmaf(x[r][i], inv[r], p[i]) : p[i];
+      for (int i = 0; i < NV; ++i) p[i] = fmaf(x[r][i], inv[r], p[i]);   // (of a token left out all are 0)
   }
   if (lane == 0 && tokens) atomicAdd(hist + a.E, tokens);
 #pragma unroll
@@ -569,11 +575,12 @@ __global__ static void __launch_bounds__(1024) balance_finish_kernel(const Balan
   __syncthreads();
   if (lane == 0) ps[warp] = dot;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    dot = 0.f;
-    for (int w = 0; w < 32; ++w) dot += ps[w];
-    *a.tokens = n;
-    *a.loss = balance_loss(a.E, dot, total, n);
+  if (warp == 0) {
+    dot = warp_sum(ps[lane]);
+    if (lane == 0) {
+      *a.tokens = n;
+      *a.loss = balance_loss(a.E, dot, total, n);
+    }
   }
 }
 
