@@ -58,11 +58,12 @@ int rows_at_once(int64_t E) { return E <= 128 ? 4 : E <= 256 ? 2 : 1; }
 unsigned row_grid(int64_t T, int rows) {
   return (unsigned)std::min<int64_t>(ceil_div(T, WARPS * rows), (int64_t)device_sms() * 6);
 }
-// Clusters that sum up the balance of T tokens.  One makes the loss in the same launch;
-// measured at 64 experts: @@
+// Clusters that sum up the balance of T tokens.  One makes the loss in the same launch: up to two
+// rounds of its rows it is as fast as several and a second launch (64 experts, 512 tokens 6.2 and 6.0 us,
+// 1000 tokens 9.5 and 5.8, 4096 tokens 28.7 and 7.1; 256 experts, 256 tokens 6.0 and 6.3).
 int64_t parts_of(int64_t T, int64_t E) {
   const int64_t rows = (int64_t)CLUSTER * WARPS * rows_at_once(E);
-  if (T <= 4 * rows) return 1;
+  if (T <= 2 * rows) return 1;
   return std::min<int64_t>(ceil_div(T, rows), device_sms() * 4 / CLUSTER);
 }
 
@@ -141,7 +142,10 @@ int mb_expert_balance(int32_t dtype, int64_t tokens, int64_t experts, int64_t k,
                       smem, (cudaStream_t)stream, CLUSTER, "expert_balance", a);
   });
   if (r || parts == 1) return r;
-  return launch_pdl(balance_finish_kernel, dim3(1), dim3(1024), 0, (cudaStream_t)stream, 1, "expert_balance", a);
+  // one block adds up a few sums, a cluster many (64 experts, 1000 tokens 5.8 and 6.8 us; 256 experts, 2048
+  // tokens 9.5 and 8.3; 128 experts, 65536 tokens 20.9 and 19.9)
+  const int blocks = parts * (experts + 1) <= 3 * FINISH_THREADS && experts < FINISH_THREADS ? 1 : CLUSTER;
+  return launch_pdl(balance_finish_kernel, dim3(blocks), dim3(FINISH_THREADS), 0, (cudaStream_t)stream, blocks, "expert_balance", a);
 }
 
 int mb_expert_balance_backward(int32_t dtype, int64_t tokens, int64_t experts, const float *grad, const void *logits,

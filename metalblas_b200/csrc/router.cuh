@@ -35,6 +35,7 @@ constexpr int MAX_EXPERTS = 1024;
 constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
 constexpr int CLUSTER = 8;          // blocks that sum up the balance together
+constexpr int FINISH_THREADS = 512;
 constexpr int MAX_K = 64;
 
 struct RouteArgs {
@@ -526,47 +527,45 @@ __global__ void __launch_bounds__(THREADS) balance_kernel(const BalanceArgs a) {
   cluster_barrier();
 }
 
-// The clusters' sums to counts, tokens and loss: one block, in the order of the clusters.
-__global__ static void __launch_bounds__(1024) balance_finish_kernel(const BalanceArgs a) {
-  __shared__ float ps[1024];
-  __shared__ int cs[1024], red[32];
+// The clusters' sums to counts, tokens and loss, in the order of the clusters: one block (E < FINISH_THREADS)
+// or one cluster, each of its blocks a share of the experts.
+__global__ static void __launch_bounds__(FINISH_THREADS) balance_finish_kernel(const BalanceArgs a) {
+  __shared__ float ps[FINISH_THREADS], dots[1];
+  __shared__ int cs[FINISH_THREADS], red[32], totals[2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t rank;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   pdl_trigger();
   pdl_wait();
-  // threads share an expert's parts where there are fewer experts than threads
-  const int E1 = a.E + 1, share = max(1, 1024 / E1), mine = threadIdx.x / E1;
+  // this block's experts (the last is the tokens' count), and threads that share each one's parts
+  const int E1 = a.E + 1, ranks = gridDim.x, per = (E1 + ranks - 1) / ranks, share = FINISH_THREADS / per;
+  const int mine = threadIdx.x / per, e = rank * per + (threadIdx.x - mine * per);
+  float s = 0.f;
+  int c = 0;
+  if (mine < share && e < E1) {
+    const int i0 = a.parts * mine / share, i1 = a.parts * (mine + 1) / share;
+#pragma unroll 4
+    for (int i = i0; i < i1; ++i) {
+      s += e < a.E ? a.part_p[(int64_t)i * a.E + e] : 0.f;
+      c += a.part_c[(int64_t)i * E1 + e];
+    }
+  }
+  ps[threadIdx.x] = s;
+  cs[threadIdx.x] = c;
+  __syncthreads();
   float dot = 0.f;
   int total = 0, n = 0;
-  for (int e0 = 0; e0 < E1; e0 += 1024) {
-    const int e = share > 1 ? threadIdx.x % E1 : e0 + threadIdx.x;
-    float s = 0.f;
-    int c = 0;
-    if (e < E1 && (share == 1 || mine < share)) {
-      const int i0 = share > 1 ? a.parts * mine / share : 0, i1 = share > 1 ? a.parts * (mine + 1) / share : a.parts;
-#pragma unroll 8
-      for (int i = i0; i < i1; ++i) {
-        if (e < a.E) s += a.part_p[(int64_t)i * a.E + e];
-        c += a.part_c[(int64_t)i * E1 + e];
-      }
+  if (threadIdx.x < per && e < E1) {
+    for (int w = 1; w < share; ++w) {
+      s += ps[w * per + threadIdx.x];
+      c += cs[w * per + threadIdx.x];
     }
-    if (share > 1) {
-      ps[threadIdx.x] = s;
-      cs[threadIdx.x] = c;
-      __syncthreads();
-      if (threadIdx.x < E1)
-        for (int w = 1; w < share; ++w) {
-          s += ps[w * E1 + threadIdx.x];
-          c += cs[w * E1 + threadIdx.x];
-        }
-    }
-    if (e < E1 && (share == 1 || mine == 0)) {
-      if (e < a.E) {
-        a.counts[e] = c;
-        total += c;
-        dot = fmaf((float)c, s, dot);
-      } else {
-        n += c;
-      }
+    if (e < a.E) {
+      a.counts[e] = c;
+      total = c;
+      dot = (float)c * s;
+    } else {
+      n = c;
     }
   }
   n = block_sum(n, red);
@@ -576,12 +575,26 @@ __global__ static void __launch_bounds__(1024) balance_finish_kernel(const Balan
   if (lane == 0) ps[warp] = dot;
   __syncthreads();
   if (warp == 0) {
-    dot = warp_sum(ps[lane]);
+    dot = warp_sum(lane < FINISH_THREADS / 32 ? ps[lane] : 0.f);
     if (lane == 0) {
-      *a.tokens = n;
-      *a.loss = balance_loss(a.E, dot, total, n);
+      dots[0] = dot;
+      totals[0] = total;
+      totals[1] = n;
     }
   }
+  cluster_barrier();
+  if (rank == 0 && threadIdx.x == 0) {
+    dot = 0.f;
+    total = n = 0;
+    for (int w = 0; w < ranks; ++w) {
+      dot += ld_cluster_f32(dots, w);
+      total += ld_cluster_s32(totals, w);
+      n += ld_cluster_s32(totals + 1, w);
+    }
+    *a.tokens = n;
+    *a.loss = balance_loss(a.E, dot, total, n);
+  }
+  cluster_barrier();   // no block leaves while its sums are read
 }
 
 template <class T, int NV, int V, bool AL>
