@@ -315,7 +315,8 @@ inline One try_int4_dequantize(const at::Tensor &q, const at::Tensor &scale, con
 // x [M, K]; weights [N, .], or [E, N, .] with offsets [E + 1].
 inline One try_int4(const at::Tensor &x, const at::Tensor &q, const at::Tensor &scale, const c10::optional<at::Tensor> &zero,
                     int64_t group, const c10::optional<at::Tensor> &offsets, const c10::optional<at::Tensor> &bias) {
-  if (!g_ops.int4_gemm || !x.is_cuda() || grad_of(x) || !group_of(group)) return c10::nullopt;
+  if (!g_ops.int4_gemm || !x.is_cuda() || grad_of(x) || grad_of(scale) || (bias.has_value() && grad_of(*bias)) || !group_of(group))
+    return c10::nullopt;
   const int dev = c10::cuda::current_device(), g = offsets.has_value() ? 1 : 0;
   int64_t ld;
   const at::ScalarType type = x.scalar_type();

@@ -212,7 +212,7 @@ int int4_plan(const mb_int4_desc *d, Plan &pl) {
   const int64_t stages = ceil_div(d->K, 256);
   double best = 1e300;
   for (const int nt : {1, 2}) {
-    if (want ? want != nt : d->K > 0 && split) continue;
+    if (want ? want != nt || split > 1 : d->K > 0 && split) continue;
     // (the one-pass kernel counts rows of units in 32 bits)
     if ((ceil_div(d->M, 8 * nt) + (d->groups ? E : 0)) * d->N >= (1ll << 32)) continue;
     const double t = few_cost(d, nt, sms);

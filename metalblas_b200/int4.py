@@ -10,8 +10,8 @@ weights of other tools (nibbles in the order of the columns, the even column low
 they are.  The integers are exact in the tokens' type and the scales are applied to fp32 sums:
 the weights are never rounded, whatever the number of rows.
 
-The products have no gradient: 4-bit weights are constants of a serving program.  Tokens that
-require one are refused.
+The products have no gradient: 4-bit weights are constants of a serving program.  Tokens, scales
+and biases that require one are refused.
 """
 from __future__ import annotations
 
@@ -117,7 +117,7 @@ def dequantize_int4(q, scale, group_size=128, *, zero=None, cols=None, out_dtype
     """The weights ``(u - zero) * scale`` of ``q [..., (cols + 1) // 2]`` as ``[..., cols]`` of
     ``out_dtype`` (fp32, fp16 or bf16), rounded once.  ``scale`` and the optional uint8 ``zero``
     are ``[..., ceil(cols / group_size)]``; ``cols`` is twice the bytes of a row unless given (an
-    odd number of columns has to be)."""
+    odd number of columns has to be).  The result carries no gradient."""
     if isinstance(q, torch.Tensor) and q.dim() == 2:
         out = _try_dequantize(q, scale, zero, 2 * q.shape[1] if cols is None else cols, group_size, out_dtype)
         if out is not None:
@@ -178,10 +178,16 @@ def _product(x, q, scale, zero, G, offsets, bias, out, plan):
 def _check_tokens(x):
     if x.dtype not in TOKENS:
         raise NotImplementedError(f"tokens must be fp16 or bf16, got {x.dtype}")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise NotImplementedError("products with 4-bit weights have no gradient; call under torch.no_grad()")
-    if fwd.unpack_dual(x).tangent is not None:
-        raise NotImplementedError("products with 4-bit weights have no forward-mode derivative")
+
+
+def _no_derivative(*operands):
+    for t in operands:
+        if t is None:
+            continue
+        if t.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError("products with 4-bit weights have no gradient; call under torch.no_grad()")
+        if fwd.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("products with 4-bit weights have no forward-mode derivative")
 
 
 def _check_scale_type(scale, x):
@@ -249,6 +255,7 @@ def _int4_mm(x, weight, scale, group_size, zero, bias, out, _plan):
         if bias.dtype is not x.dtype and bias.dtype is not torch.float32:
             raise NotImplementedError(f"bias must be {x.dtype} or fp32, got {bias.dtype}")
         bias = _plain(bias).contiguous()
+    _no_derivative(x, scale, bias)
     out = _check_out(out, (*lead, N), x)
     _product(_rows(x if x.dim() == 2 else x.reshape(M, K)), weight, scale, zero, G, None, bias, _out_rows(out, M, N),
              _plan)
@@ -289,6 +296,7 @@ def _grouped_int4_mm(x, weight, scale, offsets, group_size, zero, out, _plan):
         raise NotImplementedError(f"offsets must be int32, got {offsets.dtype}")
     _check_scale_type(scale, x)
     weight, scale, zero = _check_weight(weight, scale, zero, K, G, (E, N), dev)
+    _no_derivative(x, scale)
     out = _check_out(out, (M, N), x)
     _product(_rows(x), weight, scale, zero, G, offsets.contiguous(), None, _out_rows(out, M, N), _plan)
     return out
