@@ -1,8 +1,10 @@
 """The router and its balance loss, with gradients, against their formulas in 64 bits.
 
-Bounds: expf and a division are within 4 units of 2^-23 of their value (CUDA's bounds: 1 and 2
-units), a sum of n terms within n units of 2^-24 of their sizes; a probability is an exponential
-times the inverse of a sum of E of them: (E + 12) units of 2^-23 of it is more than all of it.
+Bounds: an exponential of y <= 0 is within |y| / 2 + 2 units of 2^-23 of its value and a division
+within 2, a sum of n terms within n units of 2^-24 of their sizes; a probability p is an exponential
+times the inverse of a sum of E of them.  Errors by |y| count with the size of what they belong to:
+p |y| / 2 with y no less than -20 is under 10 units of p, and in the sum, where p is the weight of
+each, under ln(E) / 2.  (E + 12) units of 2^-23 of p is more than all of it.
 Gradients are sums and products of such values, each of which adds its own unit; results of the
 scores' type round once.  The chosen experts and the counts are whole numbers and equal.
 """
