@@ -172,17 +172,18 @@ double expected_tiles(const mb_int4_desc *d, int rows) {
   const double E = (double)d->groups, used = E * (1.0 - std::pow(1.0 - 1.0 / E, (double)d->M)), each = d->M / used;
   return used * (each > rows / 2 ? each / rows + 0.5 : 1.0);
 }
-// A product's time in us by either kernel, fitted to times on B200 of each forced in turn
-// over 30 products, 20 of them dense, of 1 to 8192 rows and K of 512 to 14336 (within 15 %
-// but for three; the choice was the best or within 5 % of it in all).  The one-pass
-// kernel: start, weights, tokens that a warp takes anew for every slice of columns, passes of
-// 112 rows of a block.  4096 x 14336 by one row 15.5, by 16 rows 20.8; tcgen05 22.9 and
-// 22.9.  16 rows of 8192 x 2048: 22 and 15.5.
+// A product's time in us by either kernel, fitted to times on B200.  The one-pass kernel: start,
+// weights, and where units share blocks a second pass in most of them (a unit's slices of
+// columns and tokens anew); passes of 112 rows; tokens.  Within 22 % over 160 dense products of
+// 1 to 48 rows, K of 512 to 14336 and groups of 32 to 128 columns (7 % in the mean): 8 rows of 8192 x
+// 2048 9.5 us, 9 rows 18.1 in two units of 8, 11.3 in one of 16.  The choice was the best of all forced
+// plans or within 5 % of it in 69 of 73 products, 11 of them by group, 15 % over it at the worst.
 double few_cost(const mb_int4_desc *d, int nt, int sms) {
-  const double units = expected_tiles(d, 8 * nt), rows = units * d->N / sms;
-  const double weight = (nt == 1 ? 0.178e-6 : 0.255e-6) * (d->group == 32 ? 1.36 : d->group == 64 ? 1.09 : 1.0);
-  const double again = 1.0 + (nt == 1 ? 0.5 : 0.9) * (1.0 / std::max(1.0, std::min(rows / 16, 7.0)) - 1.0 / 7.0);
-  return (nt == 1 ? 4.9 : 6.0) + units * d->N * (double)d->K * weight * again + 2.0 * std::max(0.0, rows / 112 - 1.0);
+  const double units = expected_tiles(d, 8 * nt), rows = units * d->N / sms, k = d->K * 1e-3;
+  const double weight = (nt == 1 ? 0.169e-6 : 0.238e-6) * (d->group == 32 ? 1.36 : d->group == 64 ? 1.09 : 1.0);
+  double t = (nt == 1 ? 4.7 + 0.1 * k : 5.2) + units * d->N * (double)d->K * weight;
+  if (units > 1.0) t += nt == 1 ? 1.9 + 0.41 * k : 2.7 + 0.52 * k;
+  return t + 2.8 * std::max(0.0, rows / 112 - 1.0) + 0.032 * std::min(d->M / units, 8.0 * nt) * k;
 }
 // The tcgen05 kernel: a step of 128 columns takes its MMA and decoding or, with several sums
 // a step, the way of each accumulator to the sums and back.
