@@ -608,20 +608,21 @@ __global__ void __launch_bounds__(THREADS) balance_backward_kernel(const Balance
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_trigger();
   pdl_wait();
+  // a[e] less their mean over the experts, which cancels (the p of a row sum to 1): what is left of an
+  // even load is 0, not what rounding makes of equal numbers
   float s[NV];
-  int total = 0;
+  int c[NV], total = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int e = slot<V>(i, lane);
-    const int c = e < a.E ? a.counts[e] : 0;
-    total += c;
-    s[i] = (float)c;
+    c[i] = e < a.E ? a.counts[e] : 0;
+    total += c[i];
   }
   total = __reduce_add_sync(0xffffffffu, total);
   const int n = *a.tokens;
-  const float f = n == 0 || total == 0 ? 0.f : (float)((double)*a.grad * a.E / ((double)total * n));
+  const float f = n == 0 || total == 0 ? 0.f : (float)((double)*a.grad / ((double)total * n));
 #pragma unroll
-  for (int i = 0; i < NV; ++i) s[i] *= f;
+  for (int i = 0; i < NV; ++i) s[i] = (float)((long long)c[i] * a.E - total) * f;
   for (int64_t t0 = ((int64_t)blockIdx.x * WARPS + warp) * R; t0 < a.T; t0 += (int64_t)gridDim.x * WARPS * R) {
     float x[R][NV], inv[R], dot[R];
     bool on[R];

@@ -183,6 +183,17 @@ def test_balance_of_nothing():
     assert mb.expert_route_backward(torch.zeros(0, 2, device=DEV), x[:0], ids[:0]).shape == (0, 6)
 
 
+@pytest.mark.parametrize("E,k", [(4, 4), (1, 1), (60, 60), (300, 1)])
+def test_even_load_has_no_gradient(E, k):
+    """The probabilities of a row sum to 1, so equal counts leave nothing of the gradient."""
+    T = 3 * E
+    x = (torch.randn(T, E, generator=gen(E)) * 3).to(DEV)
+    ids = (torch.arange(T)[:, None] + torch.arange(k)[None]).remainder(E).to(DEV)
+    b = mb.expert_balance(x, ids)
+    assert b.counts.tolist() == [3 * k] * E
+    assert not bool(mb.expert_balance_backward(torch.ones((), device=DEV), x, b).any())
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_autograd(dtype):
     """Both losses through the graph, as a training step sums them."""
