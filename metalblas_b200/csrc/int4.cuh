@@ -18,8 +18,8 @@
 //
 // A warp takes a row's spans of 256 columns, four at a time where there is work for every
 // SM, so that as many loads are on their way as registers allow.  4096 x 14336 bf16 in
-// groups of 128: quantize 44.5 us (floor 22.5: 117 MB read, 31 MB written; issue slots bound
-// it, some 70 instructions a span of 8 columns), dequantize 27.4 us (5.4 TB/s).
+// groups of 128: quantize 36.8 us (floor 22.7: 117 MB read, 31 MB written; issue slots bound
+// it), dequantize 27.5 us (5.3 TB/s).
 #pragma once
 #include "mb_common.cuh"
 #include "quantize.cuh"
@@ -86,11 +86,52 @@ struct Quant16 {
   }
 };
 
+// A group's scale as it is stored, and what its columns are divided with.
+template <class T, class S> struct GroupScale {
+  S stored;
+  float s0;       // its value
+  Quant16 quant;  // of 16-bit x, where `direct`
+  bool direct;
+  __device__ __forceinline__ explicit GroupScale(uint32_t amax_bits) : quant(0.f, 1.f, 0.f) {
+    const float amax = __uint_as_float(amax_bits);
+    const float exact7 = __fdiv_rn(amax, 7.f);
+    stored = Elem<S>::store(amax_bits < 0x7f800000u ? exact7 : __uint_as_float(0x7fc00000u));
+    s0 = to_f32(stored);
+    constexpr bool F32 = sizeof(S) == 4;
+    // (scales of fp16 are normal numbers from 2^-14 on)
+    direct = sizeof(T) == 2 && s0 >= (std::is_same_v<S, __half> ? 0x1p-14f : 0x1p-100f) && s0 < 0x1p100f;
+    if constexpr (sizeof(T) == 2) {
+      // x / s lies above 7 x / amax where s was rounded down: s - amax / 7 has the sign of 7 s - amax
+      const float over = F32 ? fmaf(7.f, s0, -amax) : 0.f;
+      const float move = over == 0.f ? 0.f : copysignf(0x1p-21f, -over);
+      quant = Quant16(F32 ? 7.f : 1.f, F32 ? amax : s0, move);
+    }
+  }
+};
+// The nibbles of 8 columns by a scale of any kind.
+template <class T> __device__ __forceinline__ uint32_t nibbles(const float (&x)[8], float s0) {
+  if (!(s0 < INFINITY) || s0 == 0.f) return 0x88888888u;   // NaN, infinite, 0
+  // groups of tiny values are moved by a power of two, so that 1 / s and h s stay in range
+  const float pre = s0 < 0x1p-90f ? 0x1p100f : 1.f, s = s0 * pre, inv = __fdividef(1.f, s);
+  uint32_t word = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float q = fminf(fmaxf(rounded_quotient(x[i] * pre, s, inv), -7.f), 7.f);   // (a scale that rounded down to a subnormal)
+    word |= (uint32_t)((int)q + 8) << (4 * i);
+  }
+  return word;
+}
+
 // A lane takes 8 consecutive columns at a time, so a group has G / 8 neighbouring lanes
-// and a warp 256 columns of one row.  A task is B times that, next to one another.
+// and a warp 256 columns of one row, a span.  A task is B spans next to one another.  Of four
+// spans each lane reduces and divides for one, lane & 3, and the others get it from there
+// (with every lane at work on all four, 4096 x 14336 took 44.7 us in bf16 and 73.2 in fp32, now 36.8
+// and 65.5).  Rows off 16 bytes keep each lane's own columns: a column a lane with a warp's maximum
+// for every 32 was slower, 15.6 us for 1001 x 4099 fp32 instead of 13.7.
 template <class T, class S, bool AL, int B>
 __global__ void __launch_bounds__(256) quantize_int4_kernel(const ConvertArgs a) {
-  const int lane = threadIdx.x & 31;
+  static_assert(B == 1 || B == 4, "spans");
+  const int lane = threadIdx.x & 31, lanes = (1 << a.group_log2) / 8;   // of a group
   const uint32_t per_row = (a.cols + 256 * B - 1) / (256 * B);
   const int64_t tasks = a.rows * (int64_t)per_row;
   pdl_trigger();
@@ -98,7 +139,7 @@ __global__ void __launch_bounds__(256) quantize_int4_kernel(const ConvertArgs a)
   constexpr int V = Vec<T>::V, NV = 8 / V;
   for (int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < tasks; w += (int64_t)gridDim.x * 8) {
     const int64_t r = tasks < (1ll << 32) ? (uint32_t)w / per_row : w / per_row;
-    const int c0 = (int)(w - r * per_row) * (256 * B) + lane * 8;
+    const int cw = (int)(w - r * per_row) * (256 * B), c0 = cw + lane * 8;
     const T *src = static_cast<const T *>(a.src) + r * a.ld_src;
     Vec<T> v[B][NV];
 #pragma unroll
@@ -106,47 +147,49 @@ __global__ void __launch_bounds__(256) quantize_int4_kernel(const ConvertArgs a)
 #pragma unroll
       for (int i = 0; i < NV; ++i) v[b][i] = load_vec<T, AL>(src, c0 + b * 256 + i * V, a.cols);
     uint8_t *row = static_cast<uint8_t *>(a.dst) + r * a.ld_dst;
-    S *scales = static_cast<S *>(a.scale) + r * a.ld_scale;
     const bool words = (reinterpret_cast<uintptr_t>(row) & 3) == 0;
+    uint32_t m[B];
 #pragma unroll
     for (int b = 0; b < B; ++b) {
-      const int c = c0 + b * 256;
-      if (c - lane * 8 >= a.cols) break;
-      float x[8];
-      MaxAbs<T> m;
+      MaxAbs<T> most;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        m.add(v[b][i]);
+      for (int i = 0; i < NV; ++i) most.add(v[b][i]);
+      m[b] = most.bits();
+    }
+    uint32_t bits = m[0];
+    if constexpr (B == 4) {
+      const bool o1 = lane & 1, o2 = lane & 2;
+      const uint32_t m0 = max(o1 ? m[1] : m[0], __shfl_xor_sync(0xffffffffu, o1 ? m[0] : m[1], 1));   // span lane & 1
+      const uint32_t m2 = max(o1 ? m[3] : m[2], __shfl_xor_sync(0xffffffffu, o1 ? m[2] : m[3], 1));   // and 2 on
+      bits = max(o2 ? m2 : m0, __shfl_xor_sync(0xffffffffu, o2 ? m0 : m2, 2));
+    }
+    for (int d = B; d < lanes; d <<= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, d));
+    const GroupScale<T, S> g(bits);
+    const int own = cw + (lane & (B - 1)) * 256 + (lane & -lanes) * 8;   // the group's first column
+    if ((lane & (lanes - 1)) < B && own < a.cols)
+      static_cast<S *>(a.scale)[r * a.ld_scale + (own >> a.group_log2)] = g.stored;
+    const bool all = __all_sync(0xffffffffu, g.direct || own >= a.cols);
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      const int c = c0 + b * 256, from = (lane & ~3) | b;
+      if (cw + b * 256 >= a.cols) break;
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) x[i * V + j] = v[b][i].f(j);
+      uint32_t word;
+      Quant16 q = g.quant;
+      if constexpr (B == 4 && sizeof(T) == 2) {
+        q.hi = __shfl_sync(0xffffffffu, q.hi, from);
+        q.lo = __shfl_sync(0xffffffffu, q.lo, from);
       }
-      uint32_t bits = m.bits();
-      for (int d = 1; d < (1 << a.group_log2) / 8; d <<= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, d));
-      // the scale as it is stored
-      const bool finite = bits < 0x7f800000u;
-      const float amax = __uint_as_float(bits);
-      const float exact7 = __fdiv_rn(amax, 7.f);
-      const S stored = Elem<S>::store(finite ? exact7 : __uint_as_float(0x7fc00000u));
-      const float s0 = to_f32(stored);
-      if (c < a.cols && (c & ((1 << a.group_log2) - 1)) == 0)
-        scales[c >> a.group_log2] = stored;
-      uint32_t word = 0x88888888u;
-      // (scales of fp16 are normal numbers from 2^-14 on)
-      constexpr bool F32 = sizeof(S) == 4;
-      if (sizeof(T) == 2 && s0 >= (std::is_same_v<S, __half> ? 0x1p-14f : 0x1p-100f) && s0 < 0x1p100f) {
-        // x / s lies above 7 x / amax where s was rounded down: s - amax / 7 has the sign of 7 s - amax
-        const float over = F32 ? fmaf(7.f, s0, -amax) : 0.f;
-        const float move = over == 0.f ? 0.f : copysignf(0x1p-21f, -over);
-        word = Quant16(F32 ? 7.f : 1.f, F32 ? amax : s0, move)(x);
-      } else if (finite && s0 != 0.f) {
-        // groups of tiny values are moved by a power of two, so that 1 / s and h s stay in range
-        const float pre = s0 < 0x1p-90f ? 0x1p100f : 1.f, s = s0 * pre, inv = __fdividef(1.f, s);
-        word = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float q = fminf(fmaxf(rounded_quotient(x[i] * pre, s, inv), -7.f), 7.f);   // (a scale that rounded down to a subnormal)
-          word |= (uint32_t)((int)q + 8) << (4 * i);
-        }
+      if (sizeof(T) == 2 && all) {
+        word = q(x);
+      } else {
+        const float s0 = B == 4 ? __shfl_sync(0xffffffffu, g.s0, from) : g.s0;
+        const bool direct = B == 4 ? __shfl_sync(0xffffffffu, (int)g.direct, from) : g.direct;
+        word = direct ? q(x) : nibbles<T>(x, s0);
       }
       if (c >= a.cols) continue;
       if (words && c + 7 <= a.cols) {
