@@ -21,9 +21,9 @@
 // and its tokens' fragment is gathered to match.  (w & 0x000f000f) | 0x43004300 is
 // the pair (128 + u0, 128 + u4) in bf16; subtracting 128 + z is exact.
 //
-// 1 x 4096 x 14336: 15.1 us (floor 4.6, the weights at the copy's rate), 16 rows 20.9.
+// 1 x 4096 x 14336: 15.2 us (floor 4.6, the weights at the copy's rate), 16 rows 21.8.
 // Some 5 us are the start, the scales and the sums' end; then the logic pipe's half rate
-// binds (48 % in use over the launch, issue slots 46 %, DRAM 30 MB, each weight once).
+// binds (50 % in use over the launch, issue slots 49 %, DRAM 30 MB, each weight once).
 #pragma once
 #include "int4_gemm.cuh"
 #include "tc_gemm.cuh"

@@ -26,9 +26,9 @@
 // clusters); the counts are integers.  Results repeat bit for bit.
 //
 // 65536 x 128 fp32 scores, 8 experts each: route 32.2 us and its gradient 21.6, balance
-// 20.1 and 14.7 (33.5 MB of scores are 5.1 us).  The logic pipe, at half rate, is the
-// busiest (41 to 47 % in balance, issue slots 63 to 67 %): reductions over a warp and, for
-// the choice, k rounds of them.
+// 20.1 and 15.0 (33.5 MB of scores are 5.1 us).  The logic pipe, at half rate, binds the choice
+// (83 % in use: k rounds of reductions over a warp) and is the busiest of the others (40 to
+// 44 %, issue slots 60 to 62 %).
 #pragma once
 #include "mb_common.cuh"
 #include "quantize.cuh"
