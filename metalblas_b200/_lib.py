@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 import os
 import threading
+import warnings
 
 import torch
 
@@ -258,6 +259,26 @@ _fast = None
 _fast_tried = False
 
 
+def register_ops(mod, lib) -> None:
+    """Give the extension the functions of its operators.  One of another build serves none of them
+    and says so: it must not be an error, since the builder imports the package to replace it."""
+    why = None
+    missing = [name for name in _FAST_OPS if not hasattr(lib, name)]
+    if missing:
+        why = f"the library lacks {', '.join(missing)}"
+    elif not hasattr(mod, "set_ops"):
+        why = "it has none of the operators"
+    else:
+        try:
+            mod.set_ops([ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _FAST_OPS])
+        except RuntimeError as e:
+            why = str(e).split("\n")[0]
+    if why:
+        warnings.warn(f"_mbfast and libmetalblas_b200.so are of different builds ({why}): expert, int8 and 4-bit "
+                      "operators take the slower Python path; run python -m metalblas_b200.build", RuntimeWarning,
+                      stacklevel=2)
+
+
 def fast_op(name):
     """A function of the host fast path's operators, or one that never serves a call."""
     return getattr(fast(), name, None) or (lambda *a: None)
@@ -286,11 +307,7 @@ def fast():
                 raise RuntimeError("_mbfast was built against a different mb_gemm_desc; rebuild the package")
             fn = ctypes.cast(lib.mb_gemm, ctypes.c_void_p).value
             mod.set_gemm(fn)
-            if hasattr(mod, "set_ops") and all(hasattr(lib, name) for name in _FAST_OPS):
-                try:
-                    mod.set_ops([ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _FAST_OPS])
-                except RuntimeError:
-                    pass  # built for another list: serves none of them, so that the builder can run
+            register_ops(mod, lib)
         _fast = mod
         _fast_tried = True
         return _fast
