@@ -223,9 +223,10 @@ def _balance_backward(logits, grad, balance, mask):
         f"counts have shape {tuple(counts.shape)}, expected ({E},)"
     if counts.dtype is not torch.int32 or tokens.dtype is not torch.int32:
         raise NotImplementedError("ExpertBalance holds int32 counts")
+    counts = counts.contiguous()   # (named: a copy has to live until the launch)
     out = torch.empty((T, E), dtype=x.dtype, device=dev)
     _lib.raise_for(_lib.load().mb_expert_balance_backward(
-        _lib.DTYPE_CODE[x.dtype], T, E, grad.data_ptr(), x.data_ptr(), _ld(x), counts.contiguous().data_ptr(),
+        _lib.DTYPE_CODE[x.dtype], T, E, grad.data_ptr(), x.data_ptr(), _ld(x), counts.data_ptr(),
         tokens.data_ptr(), mask.data_ptr() if mask is not None else None, out.data_ptr(), _stream_of(dev)),
         "mb_expert_balance_backward")
     return out
