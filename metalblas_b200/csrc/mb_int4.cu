@@ -364,8 +364,8 @@ int mb_int4_plan(const mb_int4_desc *d, char *buf, int buflen) {
   const size_t room = buf ? (size_t)std::max(buflen, 0) : 0;
   if (d->M == 0 || d->N == 0) return snprintf(buf, room, "empty");
   if (pl.few)
-    return snprintf(buf, room, "units of %d tokens in one pass over the weights, pack_w=%d ws=%lld", 8 * pl.few, pl.pk_w,
-                    (long long)pl.ws_bytes);
+    return snprintf(buf, room, "units of %d tokens in one pass over the weights, pack_x=%d pack_w=%d ws=%lld", 8 * pl.few,
+                    pl.pk_x, pl.pk_w, (long long)pl.ws_bytes);
   return snprintf(buf, room, "tiles of 128 rows x %d tokens, split=%d pack_x=%d pack_w=%d ws=%lld", pl.bn, pl.split, pl.pk_x,
                   pl.pk_w, (long long)pl.ws_bytes);
 }
