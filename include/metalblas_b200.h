@@ -355,7 +355,8 @@ int mb_int4_dequantize(int32_t dtype, int32_t scale_dtype, int64_t rows, int64_t
  *     matrix e, rows at or past offsets[groups] are set to zero.  Values outside
  *     0..M are taken as the nearest of the two; if they are not ascending, every
  *     row is set to zero.
- * Columns are contiguous; strides are in elements (w: bytes). */
+ * Columns are contiguous; strides are in elements (w: bytes).  out shares no memory
+ * with an operand. */
 typedef struct mb_int4_desc {
     int32_t dtype, scale_dtype, bias_dtype, group;  /* scales and bias: dtype or MB_F32 */
     int64_t M, N, K, groups;

@@ -102,6 +102,46 @@ int int4_check(const mb_int4_desc *d) {
   return MB_OK;
 }
 
+// Rows of bytes that do not overlap one another.
+struct ByteRows {
+  uintptr_t at;
+  int64_t rows, pitch, size;
+  uintptr_t end() const { return at + (rows - 1) * pitch + size; }
+};
+bool share_bytes(ByteRows a, ByteRows b) {
+  if (a.at > b.at) std::swap(a, b);
+  if (b.at >= a.end()) return false;
+  if (a.rows > 1 && b.rows > 1 && a.pitch == b.pitch) {   // b starts in a row of a, or in the space behind one
+    const int64_t in = (int64_t)(b.at - a.at) % a.pitch;
+    return in < a.size || in + b.size > a.pitch;
+  }
+  for (int64_t i = a.rows > 1 ? (int64_t)(b.at - a.at) / a.pitch : 0, j = 0; i < a.rows && j < b.rows;) {
+    const uintptr_t p = a.at + i * a.pitch, q = b.at + j * b.pitch;
+    if (p < q + b.size && q < p + a.size) return true;
+    if (p < q) ++i;
+    else ++j;
+  }
+  return false;
+}
+// Blocks write results while others still read.  (Of weights, scales and zero points all that lies
+// between the first and the last counts.)
+int check_out_apart(const mb_int4_desc *d) {
+  auto at = [](const void *p) { return reinterpret_cast<uintptr_t>(p); };
+  const ByteRows out{at(d->out), d->M, 2 * d->out_rs, 2 * d->N};
+  const int64_t groups = ceil_div(d->K, d->group), last = d->groups > 1 ? d->groups - 1 : 0;
+  auto meets = [&](const void *p, int64_t rs, int64_t e, int64_t n, int esz) {
+    return p && d->K > 0 && share_bytes(out, ByteRows{at(p), 1, 0, (last * e + (d->N - 1) * rs + n) * esz});
+  };
+  const char *name = nullptr;
+  if (d->K > 0 && share_bytes(out, ByteRows{at(d->x), d->M, 2 * d->x_rs, 2 * d->K})) name = "x";
+  else if (meets(d->w, d->w_rs, d->w_e, (d->K + 1) / 2, 1)) name = "w";
+  else if (meets(d->scale, d->scale_rs, d->scale_e, groups, elem_size(d->scale_dtype))) name = "scale";
+  else if (meets(d->zero, d->zero_rs, d->zero_e, groups, 1)) name = "zero";
+  else if (d->bias && share_bytes(out, ByteRows{at(d->bias), 1, 0, d->N * elem_size(d->bias_dtype)})) name = "bias";
+  else if (d->groups && share_bytes(out, ByteRows{at(d->offsets), 1, 0, (d->groups + 1) * 4})) name = "offsets";
+  return name ? fail(MB_ERR_INVALID, "out and %s share memory", name) : MB_OK;
+}
+
 i4::GemmArgs gemm_args(const mb_int4_desc *d) {
   i4::GemmArgs a{};
   a.x = d->x; a.x_rs = d->x_rs;
@@ -375,6 +415,8 @@ int mb_int4_gemm(const mb_int4_desc *d, void *stream) {
   int rc = int4_check(d);
   if (!rc) rc = int4_plan(d, pl);
   if (rc || d->M == 0 || d->N == 0) return rc;
+  rc = check_out_apart(d);
+  if (rc) return rc;
   if (pl.ws_bytes > 0 && (!d->workspace || d->workspace_bytes < pl.ws_bytes))
     return fail(MB_ERR_WORKSPACE, "workspace of %lld bytes required", (long long)pl.ws_bytes);
   if (pl.ws_bytes > 0 && !aligned16(d->workspace))  // operand copies are stored and loaded 16 bytes at a time

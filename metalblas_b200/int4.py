@@ -226,7 +226,8 @@ def int4_mm(x, weight, scale, group_size=128, *, zero=None, bias=None, out=None,
     type or fp32, optional zero points ``zero`` (uint8, like scale), as ``quantize_int4`` makes
     them.  The result ``[..., N]`` has x's type; sums are fp32 and round once.  ``bias [N]`` has
     x's type or fp32.  ``out`` may be any tensor of that shape whose leading dimensions fold
-    into rows with contiguous columns that do not overlap.
+    into rows with contiguous columns that do not overlap; one that shares memory with an operand
+    that is read in place is a ValueError.
 
     Weights are read in place when their rows start on 16-byte boundaries (``quantize_int4``'s
     do); others are copied into scratch in every call.
