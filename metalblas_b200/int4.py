@@ -10,8 +10,8 @@ weights of other tools (nibbles in the order of the columns, the even column low
 they are.  The integers are exact in the tokens' type and the scales are applied to fp32 sums:
 the weights are never rounded, whatever the number of rows.
 
-The products have no gradient: 4-bit weights are constants of a serving program.  Tokens, scales
-and biases that require one are refused.
+The products have no gradient: 4-bit weights are constants of a serving program.  Tokens, scales,
+biases and an ``out`` that require one are refused.
 """
 from __future__ import annotations
 
@@ -256,8 +256,8 @@ def _int4_mm(x, weight, scale, group_size, zero, bias, out, _plan):
         if bias.dtype is not x.dtype and bias.dtype is not torch.float32:
             raise NotImplementedError(f"bias must be {x.dtype} or fp32, got {bias.dtype}")
         bias = _plain(bias).contiguous()
-    _no_derivative(x, scale, bias)
     out = _check_out(out, (*lead, N), x)
+    _no_derivative(x, scale, bias, out)
     _product(_rows(x if x.dim() == 2 else x.reshape(M, K)), weight, scale, zero, G, None, bias, _out_rows(out, M, N),
              _plan)
     return out
@@ -297,7 +297,7 @@ def _grouped_int4_mm(x, weight, scale, offsets, group_size, zero, out, _plan):
         raise NotImplementedError(f"offsets must be int32, got {offsets.dtype}")
     _check_scale_type(scale, x)
     weight, scale, zero = _check_weight(weight, scale, zero, K, G, (E, N), dev)
-    _no_derivative(x, scale)
     out = _check_out(out, (M, N), x)
+    _no_derivative(x, scale, out)
     _product(_rows(x), weight, scale, zero, G, offsets.contiguous(), None, _out_rows(out, M, N), _plan)
     return out
