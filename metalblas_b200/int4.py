@@ -220,6 +220,12 @@ def _out_rows(out, M, N):
     return o
 
 
+def _written(out):
+    """Tell autograd: a graph that saved out for its backward pass must not use what stands there now."""
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+
+
 def int4_mm(x, weight, scale, group_size=128, *, zero=None, bias=None, out=None, _plan=None):
     """``x @ w.t() + bias`` for ``x [..., K]`` (fp16 or bf16) and 4-bit weights of N rows of K
     columns: ``weight`` uint8 ``[N, (K + 1) // 2]``, ``scale [N, ceil(K / group_size)]`` of x's
@@ -260,6 +266,7 @@ def _int4_mm(x, weight, scale, group_size, zero, bias, out, _plan):
     _no_derivative(x, scale, bias, out)
     _product(_rows(x if x.dim() == 2 else x.reshape(M, K)), weight, scale, zero, G, None, bias, _out_rows(out, M, N),
              _plan)
+    _written(out)
     return out
 
 
@@ -300,4 +307,5 @@ def _grouped_int4_mm(x, weight, scale, offsets, group_size, zero, out, _plan):
     out = _check_out(out, (M, N), x)
     _no_derivative(x, scale, out)
     _product(_rows(x), weight, scale, zero, G, offsets.contiguous(), None, _out_rows(out, M, N), _plan)
+    _written(out)
     return out

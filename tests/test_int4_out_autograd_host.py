@@ -48,3 +48,16 @@ def test_an_out_that_wants_a_gradient(library, call):
     with torch.no_grad():
         assert call(leaf) is leaf
     assert library.launched == 1
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_a_backward_pass_learns_of_the_write(library, call):
+    """What a graph has saved is not the same after the call."""
+    buf = torch.ones(4, 8, dtype=torch.bfloat16)
+    leaf = torch.ones(4, 8, dtype=torch.bfloat16, requires_grad=True)
+    loss = (leaf * buf).sum()
+    call(buf)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        call(torch.empty(4, 8, dtype=torch.bfloat16))
