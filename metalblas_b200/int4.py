@@ -202,6 +202,8 @@ def _check_out(out, shape, x):
     assert isinstance(out, torch.Tensor), "out must be a tensor"
     assert out.device == x.device and tuple(out.shape) == tuple(shape), \
         f"out has shape {tuple(out.shape)} on {out.device}, expected {tuple(shape)} on {x.device}"
+    if out.is_neg():
+        raise NotImplementedError("out with a lazy negation")
     if out.dtype is not x.dtype:
         raise ValueError(f"out is {out.dtype}, the tokens are {x.dtype}")
     return out

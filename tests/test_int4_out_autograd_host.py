@@ -61,3 +61,11 @@ def test_a_backward_pass_learns_of_the_write(library, call):
         loss.backward()
     with torch.inference_mode():
         call(torch.empty(4, 8, dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_a_lazy_negation(library, call):
+    """The kernels write values, not their negatives."""
+    with pytest.raises(NotImplementedError, match="negation"):
+        call(torch.empty(4, 8, dtype=torch.bfloat16)._neg_view())
+    assert library.launched == 0
