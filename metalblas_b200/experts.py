@@ -137,11 +137,10 @@ def _combine(rows, weights, order):
     return out
 
 
-def _no_tangent(*tensors):
+def _no_tangent(*tensors, what="expert_gather, expert_combine"):
     for t in tensors:
         if isinstance(t, torch.Tensor) and fwd.unpack_dual(t).tangent is not None:
-            raise NotImplementedError("expert_gather, expert_combine and their gradients have no forward-mode "
-                                      "derivative")
+            raise NotImplementedError(f"{what} and their gradients have no forward-mode derivative")
 
 
 class _Gather(torch.autograd.Function):

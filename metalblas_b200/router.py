@@ -22,6 +22,7 @@ from .experts import MAX_EXPERTS, _no_tangent
 from .quantized import _ld, _on_device, _rows
 
 MAX_K = 64
+_WHAT = "expert_route, expert_balance"   # in messages
 
 # The host fast path (csrc/fastops.h): the result of a plain call, or None.
 _try_route = _lib.fast_op("try_route")
@@ -105,7 +106,7 @@ class _Route(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad, _):
-        _no_tangent(grad)
+        _no_tangent(grad, what=_WHAT)
         logits, experts = ctx.saved_tensors
         return expert_route_backward(grad, logits, experts, normalize=ctx.normalize), None, None
 
@@ -123,7 +124,7 @@ def expert_route(logits, k, *, normalize=True):
     fast = _try_route(logits, k, normalize)
     if fast is not None:
         return fast
-    _no_tangent(logits)
+    _no_tangent(logits, what=_WHAT)
     if isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled():
         return _Route.apply(logits, k, normalize)
     return _route(logits, k, normalize)
@@ -179,7 +180,7 @@ class _Balance(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad, _, __):
-        _no_tangent(grad)
+        _no_tangent(grad, what=_WHAT)
         logits, counts, tokens, mask = ctx.saved_tensors
         return expert_balance_backward(grad, logits, ExpertBalance(None, counts, tokens), mask=mask), None, None
 
@@ -198,7 +199,7 @@ def expert_balance(logits, experts, mask=None):
     fast = _try_balance(logits, experts, mask)
     if fast is not None:
         return ExpertBalance(*fast)
-    _no_tangent(logits)
+    _no_tangent(logits, what=_WHAT)
     if isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled():
         return ExpertBalance(*_Balance.apply(logits, experts, mask))
     return ExpertBalance(*_balance(logits, experts, mask))
