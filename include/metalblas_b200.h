@@ -337,12 +337,12 @@ int mb_expert_combine_backward(int32_t dtype, int32_t weights_dtype, int64_t tok
  * 256) consecutive columns a scale and, where zero points are given, a zero
  * point (uint8): weight = (u - zero) scale, zero 8 without zero points. */
 
-/* scale = amax / 7 rounded to scale_dtype, amax the largest |x| of the group;
+/* scale = amax / 7 in fp32, rounded to scale_dtype, amax the largest |x| of the group;
  * u = 8 + rint(x / scale), halves to even, within 1..15.  A group of zeros has
  * scale 0, one that holds an infinity or a NaN scale NaN, both u = 8. */
 int mb_int4_quantize(int32_t dtype, int32_t scale_dtype, int64_t rows, int64_t cols, int32_t group, const void *x,
                      int64_t ldx, uint8_t *q, int64_t ldq, void *scale, int64_t lds, void *stream);
-/* out = the weights, rounded once to dtype; zero may be null. */
+/* out = the weights in fp32, rounded to dtype; zero may be null. */
 int mb_int4_dequantize(int32_t dtype, int32_t scale_dtype, int64_t rows, int64_t cols, int32_t group, const uint8_t *q,
                        int64_t ldq, const void *scale, int64_t lds, const uint8_t *zero, int64_t ldz, void *out,
                        int64_t ldo, void *stream);

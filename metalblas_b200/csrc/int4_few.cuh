@@ -22,8 +22,10 @@
 // the pair (128 + u0, 128 + u4) in bf16; subtracting 128 + z is exact.
 //
 // 1 x 4096 x 14336: 15.2 us (floor 4.6, the weights at the copy's rate), 16 rows 21.8.
-// Some 5 us are the start, the scales and the sums' end; then the logic pipe's half rate
-// binds (50 % in use over the launch, issue slots 49 %, DRAM 30 MB, each weight once).
+// Some 5 us are the start, the scales and the sums' end.  DRAM 30 MB, each weight once; no
+// pipe is full (logic 50 % in use over the launch, issue slots 49 %, 19 % of the warps active).
+// A lane's word of 8 weights takes 35 instructions (8.1 M for 229,376 of a warp), of which
+// its decoding and MMA are 12; the others have not been counted.
 #pragma once
 #include "int4_gemm.cuh"
 #include "tc_gemm.cuh"
@@ -188,7 +190,8 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 1)
     m1 = min(m1, m0 + TOKENS);
     const int tiles = (rows + 15) / 16, we = a.w_e == 0 ? 0 : e;
 
-    // the slices whose scales fit, at a time (all of them, with groups of 128 columns and K up to 30000)
+    // the slices whose scales fit, at a time: with 7 row tiles K up to 17408 in groups of 128 (8448 with
+    // zero points) or 4352 in groups of 32 (2048), with 4 tiles up to 30464 (15104) or 7424 (3584)
     float *own = sums + warp * (Cfg::TILES * NT * 128) + lane * 4;
     const int per_slice = max(1, FEW_SLICE >> a.group_log2);
     const int fit = max(1, (Cfg::SCALES / WORDS / (tiles * 16) - 1) / per_slice);

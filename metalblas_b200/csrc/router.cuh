@@ -146,9 +146,9 @@ __device__ __forceinline__ float from_order_bits(uint32_t o) {
   return __uint_as_float(o == 0xffffffffu ? 0x7fc00000u : (o & 0x80000000u ? o ^ 0x80000000u : ~o));
 }
 
-// exp(y) for y <= 0, within (|y| / 2 + 2) 2^-23 of it: what rounds is the exponent y / ln 2, and
-// where that is large the result is small against the row's sum.  (expf takes three times as
-// many instructions, a fifth of all in the kernels without a choice of experts.)
+// exp(y) for y <= 0: CUDA states 2 + floor(1.173 |y|) units in the last place.  What rounds is the exponent
+// y / ln 2, and where that is large the result is small against the row's sum; below 2^-126 it is 0.
+// (expf takes three times as many instructions, a fifth of all in the kernels without a choice of experts.)
 __device__ __forceinline__ float exponential(float y) { return __expf(y); }
 
 // The row's largest score, or 0 when there is no number above -inf (a base of exponentials).
@@ -156,8 +156,8 @@ template <int NV> __device__ __forceinline__ float base_of(const float (&x)[NV])
   float m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < NV; ++i) m = fmaxf(m, x[i]);
-  // signed integers in the order of the floats (NaN where a lane has nothing else: every
-  // exponential of it is NaN whatever the base)
+  // signed integers in the order of the floats (fmaxf leaves NaN out: the exponential of one is NaN whatever
+  // the base)
   auto flip = [](int b) { return b ^ ((b >> 31) & 0x7fffffff); };
   m = __int_as_float(flip(__reduce_max_sync(0xffffffffu, flip(__float_as_int(m)))));
   return m == -INFINITY ? 0.f : m;

@@ -56,8 +56,8 @@ def quantize_int4(w, group_size=128, *, scale_dtype=torch.float32):
     """Rows of ``w [..., cols]`` (fp32, fp16 or bf16) as ``(q, scale)``: uint8 ``q [..., (cols + 1)
     // 2]`` with two values to a byte, and ``scale [..., ceil(cols / group_size)]``.
 
-    ``scale = max|w| / 7`` of a group, rounded to ``scale_dtype`` (fp32, fp16 or bf16; one that
-    the type cannot hold is infinite), and ``u = 8 + round(w / scale)``, halves to even, so that
+    ``scale = max|w| / 7`` of a group in fp32, rounded to ``scale_dtype`` (fp32, fp16 or bf16; one
+    that the type cannot hold is infinite), and ``u = 8 + round(w / scale)``, halves to even, so that
     ``w ~ (u - 8) * scale``.  A group of zeros has scale 0; one with an infinity or a NaN has
     scale NaN; both have u 8.  ``group_size`` is 32, 64, 128 or 256, the last group of a row may
     be shorter.  The rows of ``q`` start on 16-byte boundaries: with a number of columns that is
@@ -115,7 +115,8 @@ def _inner(t):
 
 def dequantize_int4(q, scale, group_size=128, *, zero=None, cols=None, out_dtype=torch.bfloat16):
     """The weights ``(u - zero) * scale`` of ``q [..., (cols + 1) // 2]`` as ``[..., cols]`` of
-    ``out_dtype`` (fp32, fp16 or bf16), rounded once.  ``scale`` and the optional uint8 ``zero``
+    ``out_dtype`` (fp32, fp16 or bf16): products in fp32, rounded to that type (16-bit scales make
+    them exact in fp32).  ``scale`` and the optional uint8 ``zero``
     are ``[..., ceil(cols / group_size)]``; ``cols`` is twice the bytes of a row unless given (an
     odd number of columns has to be).  The result carries no gradient."""
     if isinstance(q, torch.Tensor) and q.dim() == 2:
