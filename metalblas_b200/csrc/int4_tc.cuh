@@ -30,9 +30,10 @@
 //
 // 4096 x 4096 x 14336: 420 us with tiles of 256 tokens, which decode a weight half as often
 // (1.14 PFLOP/s; of 128 tokens 523 us; floor 292), 512 x 4096 x 4096 25.7 us.  The tensor
-// pipe is in use 26 % of the latter's launch (52 % of the former's), issue slots 55 %, the logic
-// pipe 45 %: decoding and sums share an SM's slots.  Groups of 64 or 32 columns have two or four sums a step, whose
-// way to the registers and back binds (512 x 4096 x 4096: 37.3 and 62.7 us).
+// pipe is in use 26 % of the latter's launch (51 % of the former's), issue slots 55 % (49 %), the logic
+// pipe 45 % (38 %): decoding and sums share an SM's slots.  Groups of 64 or 32 columns have two or four sums a step, whose
+// way to the registers and back binds (512 x 4096 x 4096: 37.3 and 62.7 us,
+// 4096 x 4096 x 14336: 630 and 1076).
 #pragma once
 #include "int4_few.cuh"
 
